@@ -45,6 +45,9 @@ extern "C" {
                                   and waits for the predecessor before touching x / A or
                                   writing y / C */
 #define MIORI_GEMV_EXACT 4u    /* fp32 dequantization for every M (what every launch does) */
+#define MIORI_ROPE_ADJACENT 8u     /* rope_kv: elements 2j and 2j + 1 are a pair (else j and j + rotary / 2) */
+#define MIORI_ROPE_F32 16u         /* rope_kv: qkv is fp32, as projections write it (else bf16) */
+#define MIORI_ATTENTION_FULL 32u   /* attention: every token sees all of its request's positions (else causal) */
 const char* miori_last_error(void);
 /* Library version string, e.g. "miori_b200 0.1 sm_100a". */
 const char* miori_version(void);
@@ -366,6 +369,64 @@ int miori_gemv4_rmsnorm(const void* q, const void* s, const void* b, const void*
 int miori_gemv8_rmsnorm(const void* q, const void* s, const void* b, const void* x, const void* gamma,
                         float eps, void* y, uint32_t N, uint32_t K, uint32_t M, uint32_t group,
                         uint32_t flags, void* stream);
+
+/* ---- attention: from the QKV projection to the input of the output projection ------------------
+ *
+ * The cache is paged: k_cache and v_cache [pages][kv_heads][page][dim] bf16 (strides free), a request's
+ * position p is in page table[request][p / page], at p % page; its slot is that page's number * page + p % page.
+ * Tokens of a step are packed: those of request r are rows cu[r] .. cu[r + 1] - 1 of q.  Lengths, tables and
+ * cu live on the device and are read there, so a recorded graph serves every step; lengths that contradict
+ * one another are cut off at the end of the tensors given, nothing beyond is read or written. */
+
+/* Positions, slots and new pages of a step's tokens.  Request r (1..16384 of them) holds held[r] positions and gets
+ * new_tokens[r] more: it then owns ceil((held + new) / page) pages, at most `width`.  New ones are
+ * pool[*taken], pool[*taken + 1], ..., in the order of the requests, and are written into table[r][..].  Out:
+ * cu[requests + 1], the first token of each request; held_after[r]; *taken_after; and for each of `tokens`
+ * tokens positions[t] and slots[t].  Where the table or the pool is too short slots are -1 (and new table entries -1 too):
+ * *taken_after > pool_size tells.  tokens behind cu[requests] get slot -1 and position 0.  No output but
+ * the table may be an input too. */
+int miori_page_slots(const int32_t* held, const int32_t* new_tokens, int32_t* table, const int32_t* pool,
+                     const int32_t* taken, int32_t* slots, int32_t* positions, int32_t* cu, int32_t* held_after,
+                     int32_t* taken_after, uint32_t requests, uint32_t width, uint32_t page, uint32_t pool_size,
+                     uint32_t tokens, uint32_t flags, void* stream);
+/* Heads of the QKV projection: qkv [tokens][(heads + 2 kv_heads) * dim], fp32 with MIORI_ROPE_F32, else bf16, rows
+ * qkv_row elements apart, q heads first, then k, then v; dim 64 or 128.  q and k heads are normed, x * rsqrt(mean(x^2) +
+ * eps) * gamma, where gamma_q / gamma_k (bf16 [dim], each may be NULL) is given; then the pairs of their first `rotary`
+ * elements (a multiple of 16) are turned: pair j by positions[axes[j]][t] * turns[j] in units of 2^-64 turns, any
+ * int32 position exactly.  positions [num_axes][tokens], num_axes 1..4 (text: 1; image and video: time, height, width);
+ * axes [rotary / 2], NULL: all 0.  q out: bf16 [tokens][heads][dim].  k and v go to slots[t] of the caches as bf16;
+ * a slot outside the cache is not written.  cache_strides: page, head, slot of k_cache, then of v_cache, in
+ * elements, multiples of 8.  fp32 throughout, rounded once.  turns, axes and gammas are weights (MIORI_LAUNCH_PDL). */
+int miori_rope_kv(const void* qkv, int64_t qkv_row, const uint64_t* turns, const int32_t* axes, const int32_t* positions,
+                  const int32_t* slots, const void* gamma_q, const void* gamma_k, float eps, void* q, void* k_cache,
+                  void* v_cache, const int64_t* cache_strides, uint32_t tokens, uint32_t heads, uint32_t kv_heads,
+                  uint32_t dim, uint32_t rotary, uint32_t num_axes, uint32_t pages, uint32_t page, uint32_t flags,
+                  void* stream);
+/* Bytes of the workspace of the two below: zeroed once by its owner, left so by every launch; launches that may
+ * run concurrently need workspaces of their own.  It lets the keys of one request be shared by several SMs; without
+ * one (NULL) a call is right, but as slow as its longest request. */
+size_t miori_attention_workspace_bytes(void);
+/* out[t][h] = sum_p softmax_p(scale * q[t][h] . k[p]) v[p] over the positions that token t sees: token i of the n of a request
+ * of lens[r] positions (the new ones included, already in the cache) sees the first lens - n + i + 1, with
+ * MIORI_ATTENTION_FULL all.  A token that sees none gets zeros.  What is in slots beyond the length, or belongs
+ * to positions that a token does not see, has no influence, whatever its bits are.  q and out [tokens][heads][dim] bf16,
+ * dim 64 or 128, heads a multiple (up to 64 times) of kv_heads; head h reads key head h / (heads / kv_heads).  page is a
+ * power of two from 8 to 65536.  table [requests][width].  strides in elements, positive multiples of 8: token and head of
+ * q, token and head of out, page, head and slot of k_cache, the same of v_cache.  max_new: the most tokens that a request
+ * has in this call; it decides only which kernel runs.  Sums and softmax in fp32, probabilities rounded to bf16
+ * for their product with v. */
+int miori_attention_paged(const void* q, const void* k_cache, const void* v_cache, void* out, const int64_t* strides,
+                          const int32_t* table, const int32_t* lens, const int32_t* cu, uint32_t requests,
+                          uint32_t tokens, uint32_t width, uint32_t pages, uint32_t page, uint32_t heads,
+                          uint32_t kv_heads, uint32_t dim, uint32_t max_new, float scale, uint32_t flags,
+                          void* workspace, size_t workspace_bytes, void* stream);
+/* The same over packed keys: request r has the tokens cu[r] .. cu[r + 1] - 1 of q and the keys cu_k[r] ..
+ * cu_k[r + 1] - 1 of k and v [keys][kv_heads][dim] (cu_k NULL: cu, the prompt itself).  strides: token and head of q,
+ * of out, of k, of v. */
+int miori_attention_prompt(const void* q, const void* k, const void* v, void* out, const int64_t* strides,
+                           const int32_t* cu, const int32_t* cu_k, uint32_t requests, uint32_t tokens, uint32_t keys,
+                           uint32_t heads, uint32_t kv_heads, uint32_t dim, float scale, uint32_t flags, void* workspace,
+                           size_t workspace_bytes, void* stream);
 
 /* Non-zero if a kernel of this library recorded an internal error on the current
  * device since the last call (bounded wait expired); clears the record. */

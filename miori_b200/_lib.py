@@ -15,8 +15,10 @@ LIB_PATH = os.environ.get("MIORI_B200_LIB") or os.path.join(HERE, "libmiori_b200
 HEADER = os.path.join(HERE, "..", "include", "miori_b200.h")
 
 OUT_F32, OUT_BF16, LAUNCH_PDL, GEMV_EXACT = 0, 1, 2, 4
+ROPE_ADJACENT, ROPE_F32, ATTENTION_FULL = 8, 16, 32
 
 _p, _u32, _sz, _i = C.c_void_p, C.c_uint32, C.c_size_t, C.c_int
+_strides = C.POINTER(C.c_int64)
 
 _SIGS = {
     "miori_last_error": (C.c_char_p, []),
@@ -81,6 +83,11 @@ _SIGS = {
     "miori_gemv4_rmsnorm_silu": (_i, [_p, _p, _p, _p, _p, C.c_float, _p, _u32, _u32, _u32, _u32, _u32, _p]),
     "miori_gemv4_rmsnorm": (_i, [_p, _p, _p, _p, _p, C.c_float, _p, _u32, _u32, _u32, _u32, _u32, _p]),
     "miori_gemv8_rmsnorm": (_i, [_p, _p, _p, _p, _p, C.c_float, _p, _u32, _u32, _u32, _u32, _u32, _p]),
+    "miori_page_slots": (_i, [_p] * 10 + [_u32] * 6 + [_p]),
+    "miori_rope_kv": (_i, [_p, C.c_int64] + [_p] * 6 + [C.c_float] + [_p] * 3 + [_strides] + [_u32] * 9 + [_p]),
+    "miori_attention_workspace_bytes": (_sz, []),
+    "miori_attention_paged": (_i, [_p] * 4 + [_strides] + [_p] * 3 + [_u32] * 9 + [C.c_float, _u32, _p, _sz, _p]),
+    "miori_attention_prompt": (_i, [_p] * 4 + [_strides] + [_p] * 2 + [_u32] * 6 + [C.c_float, _u32, _p, _sz, _p]),
     "miori_device_error_poll": (_i, []),
 }
 

@@ -1,0 +1,91 @@
+// What the attention kernels share: their arguments, how a launch's work is dealt out, and how parts of it meet again.
+//
+//   o[i] = sum_j softmax_j(scale * q_i . k_j) * v_j     over the positions j <= length - n + i that token i of n sees
+//
+// Both kernels (attention_decode.cuh, attention_prompt.cuh) go over the keys once with the running maximum m and sum l of a
+// softmax, fp32: with t = scale * log2(e) * q . k, m' = max(m, t), l' = l * 2^(m - m') + sum 2^(t - m'), and o likewise.  A
+// row's keys may be split over CTAs: parts (m, l, o) of a row join as o = sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p.
+//
+// An item is a block of a request's tokens with one key head: all the query heads that share the head are rows of the item
+// (row = token * group + head), so keys and values are read once for all of them.  An item's work is its number of key
+// tiles, known on the device alone (lengths live there: a recorded graph serves every step).  So every launch is a fixed number
+// of CTAs; each finds its share [k * total / G, (k + 1) * total / G) of the tiles of all items, in order, by the same
+// arithmetic.  Shares differ by one tile whatever the lengths are, and need no list and no counter.
+#pragma once
+#include "common.cuh"
+
+namespace miori_b200 {
+namespace attention {
+
+struct Args {
+    const uint16_t *q, *k, *v;
+    uint16_t* out;
+    const int32_t *cu, *lens, *table;  // lens: positions of each request (paged) or first position of each (cu_k, packed)
+    int64_t q_token, q_head, o_token, o_head;
+    int64_t k_page, k_head, k_slot, v_page, v_head, v_slot;  // packed: slot is the token's stride, page unused
+    uint32_t requests, heads, kv_heads, group, tokens, keys;   // tokens, keys: rows of q and of packed k
+    uint32_t width, page_shift, pages;                           // of the table; page size as a power of two
+    uint32_t causal;
+    float scale_log2;  // scale * log2(e)
+    uint32_t* counters;
+    float* parts;      // null: items are not split
+};
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ float exp2_fast(float x) {  // 2^x, 2 ulp, 0 for x = -inf
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// Bits of a pair of bf16 with those halves zero that are not finite.
+__device__ __forceinline__ uint32_t finite_or_zero(uint32_t pair) {
+    if ((pair & 0x7F80u) == 0x7F80u) pair &= 0xFFFF0000u;
+    if ((pair & 0x7F800000u) == 0x7F800000u) pair &= 0x0000FFFFu;
+    return pair;
+}
+
+// A request as the kernels see it.  Lengths that contradict one another are cut off to what is there: no row of q or k beyond
+// the tensors, no column beyond the table is ever read.
+struct Request {
+    uint32_t q0, n;   // first token in q, number of tokens
+    uint32_t k0, len;  // first row of packed k (0 where paged), number of positions
+};
+template <bool PAGED>
+__device__ __forceinline__ Request request(const Args& a, uint32_t r) {
+    Request x;
+    const int32_t q0 = ld_fresh(a.cu + r), q1 = ld_fresh(a.cu + r + 1);
+    x.q0 = min((uint32_t)max(q0, 0), a.tokens);
+    x.n = min((uint32_t)max(q1, 0), a.tokens);
+    x.n = x.n > x.q0 ? x.n - x.q0 : 0u;
+    if constexpr (PAGED) {
+        x.k0 = 0u;
+        const uint64_t room = (uint64_t)a.width << a.page_shift;
+        x.len = (uint32_t)max(ld_fresh(a.lens + r), 0);
+        if ((uint64_t)x.len > room) x.len = (uint32_t)room;
+    } else {
+        const int32_t k0 = ld_fresh(a.lens + r), k1 = ld_fresh(a.lens + r + 1);
+        x.k0 = min((uint32_t)max(k0, 0), a.keys);
+        x.len = min((uint32_t)max(k1, 0), a.keys);
+        x.len = x.len > x.k0 ? x.len - x.k0 : 0u;
+    }
+    return x;
+}
+// Positions that token i of the request sees.
+__device__ __forceinline__ uint32_t seen(const Args& a, const Request& x, uint32_t i) {
+    if (!a.causal) return x.len;
+    const int64_t s = (int64_t)x.len - (int64_t)x.n + (int64_t)i + 1;
+    return s <= 0 ? 0u : min((uint32_t)s, x.len);
+}
+
+// Number of shares, first unit of share k of G, and the share that holds unit u.  No share is empty: whoever adds parts up
+// counts on every CTA between the first and the last of an item.
+__device__ __forceinline__ uint32_t shares_of(uint64_t total, uint32_t ctas) { return (uint32_t)min((uint64_t)ctas, total); }
+__device__ __forceinline__ uint64_t share_begin(uint64_t total, uint32_t k, uint32_t G) { return total * k / G; }
+__device__ __forceinline__ uint32_t share_of(uint64_t total, uint64_t u, uint32_t G) { return (uint32_t)(((u + 1u) * G - 1u) / total); }
+
+}  // namespace attention
+}  // namespace miori_b200

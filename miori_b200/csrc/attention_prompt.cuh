@@ -1,0 +1,705 @@
+// Attention of prompts and of chunks of them on the 5th-generation tensor cores: packed keys or the paged cache, causal or not.
+//
+// Tensor-bound: 4 * D operations a (row, key) pair, and one exponential.
+//
+// * An item has up to 256 rows: two tiles of 128 rows (tokens x the heads that share the key head).  Per tile of 128 keys a row
+//   tile takes S = Q K^T (128 x 128 x D) into TMEM, its softmax, and O += P V (128 x D x 128) with P read from TMEM,
+//   where it lies over the S it came from.  TMEM: S0, S1 (128 columns each), O0, O1 (D each).
+// * Warps 0-3 and 4-7 are the softmax of the two row tiles, a thread a row: no shuffle anywhere.  The two take turns on the
+//   tensor cores: while one exponentiates, the other's products run.  Warp 8 issues the copies (TMA, 128-byte swizzle, a
+//   ring of 32-KB halves: keys, values, keys, ...), one thread of warp 9 the MMAs, warps 10-11 look through the values of edge tiles.
+// * The running maximum moves only when a row's exceeds it by 2^8: until then p grows up to 256, which costs no precision in
+//   fp32 sums and bf16 rounding, and O stays where it is.  O is rescaled by the softmax warps themselves, in TMEM.
+// * P is rounded to bf16 for the second product, as the values are; l sums the unrounded p.
+// * Edge tiles (keys that some rows do not see, or past the end).  Their scores are masked one by one.  Their values are looked
+//   through before the product: rows past the end are zeroed (a page's unwritten tail, the next prompt's rows) and so are
+//   numbers that are not finite, since 0 * inf would reach rows that do not see them; rows that do see them get them added
+//   at the end.
+// * Shares of the items' key tiles are cut anywhere (attention.cuh); parts of an item meet in attention_join_kernel.
+#pragma once
+#include "attention.cuh"
+#include "tma_host.cuh"
+
+namespace miori_b200 {
+namespace attention {
+
+constexpr int PROMPT_THREADS = 384, KEYS = 128, ROW_TILE = 128;
+constexpr uint32_t ITEM_COST = 1;  // an item's set-up and end, in key tiles
+
+template <int D>
+struct PromptCfg {
+    static constexpr int HALVES = D / 64;                  // 128-byte columns of a row
+    static constexpr int BLOCK = KEYS * 128;               // one of them, 128 rows
+    static constexpr int TILE_BYTES = HALVES * BLOCK;
+    static constexpr int STAGES = D == 128 ? 5 : 10;
+    static constexpr int SMEM = 1024 + (2 + STAGES) * TILE_BYTES;
+    static constexpr int PART_FLOATS = 2 * ROW_TILE * (D + 2);  // [D / 4][256] pieces of O, then m and l
+};
+constexpr int SETMAXNREG_SOFTMAX = 224, SETMAXNREG_OTHERS = 56;  // (256 * 224 + 128 * 56) = 384 * 168, what a launch has
+static_assert(256 * SETMAXNREG_SOFTMAX + 128 * SETMAXNREG_OTHERS <= PROMPT_THREADS * 168, "a split above the launch's registers waits forever");
+
+// ---- how the work is dealt ---------------------------------------------------------------
+
+// Sum over i < n of floor((a i + b) / m).
+__device__ __forceinline__ uint64_t floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
+    uint64_t sum = 0;
+    while (n) {
+        sum += (uint64_t)n * (n - 1u) / 2u * (a / m) + (uint64_t)n * (b / m);
+        a %= m, b %= m;
+        const uint32_t y = a * n + b;  // a, b < m <= 256, n < 2^23
+        n = y / m, b = y % m;
+        const uint32_t swap = m;
+        m = a, a = swap;
+        if (!m) break;
+    }
+    return sum;
+}
+__device__ __forceinline__ uint32_t item_tokens(const Args& a) { return 2u * (ROW_TILE / a.group); }
+__device__ __forceinline__ uint32_t key_tiles(uint32_t positions) { return max((positions + KEYS - 1u) / KEYS, 1u); }
+// Key tiles of item t of a request.
+__device__ __forceinline__ uint32_t tiles_of(const Args& a, const Request& x, uint32_t t) {
+    return key_tiles(seen(a, x, min((t + 1u) * item_tokens(a), x.n) - 1u));
+}
+// Cost of items 0 .. t-1 of one head.
+__device__ __forceinline__ uint64_t cost_before(const Args& a, const Request& x, uint32_t t, uint32_t items) {
+    if (t == 0) return 0;
+    if (!a.causal) return (uint64_t)t * (ITEM_COST + key_tiles(x.len));
+    uint64_t cost = (uint64_t)t * ITEM_COST;
+    uint32_t full = t;
+    if (t == items) cost += key_tiles(x.len), --full;  // the last one's tokens may end early
+    const uint32_t step = item_tokens(a);
+    // the first `flat` items see at most one tile of keys, the others ceil((len - n + (i + 1) step) / 128)
+    const int64_t before = (int64_t)x.len - (int64_t)x.n;
+    const int64_t room = (int64_t)KEYS - before;
+    const uint32_t flat = room < (int64_t)step ? 0u : min((uint32_t)(room / step), full);
+    cost += flat;
+    const uint32_t more = full - flat;
+    if (more) {
+        const uint64_t b = (uint64_t)(before + (int64_t)(flat + 1u) * step) + KEYS - 1u;
+        cost += (uint64_t)more * (b / KEYS) + floor_sum(more, KEYS, step, (uint32_t)(b % KEYS));
+    }
+    return cost;
+}
+
+struct Item {
+    Request x;
+    uint32_t r, head, t, items, tiles;
+    uint64_t start;  // its first unit
+    __device__ __forceinline__ void enter(const Args& a, uint32_t id, uint32_t per_item, bool paged) {
+        r = id;
+        x = paged ? request<true>(a, r) : request<false>(a, r);
+        items = (x.n + per_item - 1u) / per_item;
+    }
+    __device__ __forceinline__ void next(const Args& a, uint32_t per_item, bool paged, uint64_t end) {
+        start += ITEM_COST + tiles;
+        if (start >= end) return;  // there may be no further request
+        if (++t == items) {
+            t = 0u;
+            if (++head == a.kv_heads) {
+                head = 0u;
+                do enter(a, r + 1u, per_item, paged);
+                while (items == 0u && r + 1u < a.requests);
+            }
+        }
+        tiles = tiles_of(a, x, t);
+    }
+};
+
+template <bool PAGED>
+__device__ __forceinline__ uint64_t request_cost(const Args& a, uint32_t r) {
+    const Request x = request<PAGED>(a, r);
+    const uint32_t per_item = item_tokens(a), items = (x.n + per_item - 1u) / per_item;
+    return cost_before(a, x, items, items) * a.kv_heads;
+}
+template <bool PAGED>
+__device__ uint64_t total_cost(const Args& a) {  // by a whole warp
+    uint64_t total = 0;
+    for (uint32_t r0 = 0; r0 < a.requests; r0 += 32u) {
+        uint64_t w = r0 + (threadIdx.x & 31u) < a.requests ? request_cost<PAGED>(a, r0 + (threadIdx.x & 31u)) : 0u;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xFFFFFFFFu, w, o);
+        total += w;
+    }
+    return total;
+}
+// The item that holds `unit` < total; by a whole warp.
+template <bool PAGED>
+__device__ Item item_at(const Args& a, uint64_t unit) {
+    const uint32_t lane = threadIdx.x & 31u, per_item = item_tokens(a);
+    uint64_t before = 0;
+    uint32_t found = 0;
+    for (uint32_t r0 = 0; r0 < a.requests; r0 += 32u) {
+        const uint64_t w = r0 + lane < a.requests ? request_cost<PAGED>(a, r0 + lane) : 0u;
+        uint64_t sum = w;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint64_t y = __shfl_up_sync(0xFFFFFFFFu, sum, o);
+            if (lane >= (uint32_t)o) sum += y;
+        }
+        const uint32_t past = __ballot_sync(0xFFFFFFFFu, before + sum > unit);
+        if (past) {
+            const uint32_t l = __ffs(past) - 1u;
+            before += __shfl_sync(0xFFFFFFFFu, sum - w, l);
+            found = r0 + l;
+            break;
+        }
+        before += __shfl_sync(0xFFFFFFFFu, sum, 31);
+    }
+    Item it;
+    it.enter(a, found, per_item, PAGED);
+    const uint64_t per_head = cost_before(a, it.x, it.items, it.items);
+    it.head = (uint32_t)((unit - before) / per_head);
+    it.start = before + it.head * per_head;
+    const uint64_t in = unit - it.start;
+    uint32_t lo = 0, width = it.items;  // the item is in [lo, lo + width)
+    while (width > 1u) {
+        const uint32_t step = (width + 31u) / 32u, t = lo + lane * step;
+        const uint32_t below = __ballot_sync(0xFFFFFFFFu, lane * step < width && cost_before(a, it.x, t, it.items) <= in);
+        const uint32_t l = 31u - __clz(below);  // lane 0 always is
+        lo += l * step;
+        width = min(step, width - l * step);
+    }
+    it.t = lo;
+    it.start += cost_before(a, it.x, lo, it.items);
+    it.tiles = tiles_of(a, it.x, lo);
+    return it;
+}
+// What of an item's key tiles falls into the share [begin, end).  Without a workspace items stay whole.
+struct Span {
+    uint32_t k0, k1;
+    bool whole;
+};
+__device__ __forceinline__ Span span_of(const Item& it, uint64_t begin, uint64_t end, bool split) {
+    const uint64_t first = it.start + ITEM_COST;
+    Span s;
+    s.k0 = begin > first ? (uint32_t)min(begin - first, (uint64_t)it.tiles) : 0u;
+    s.k1 = end > first ? (uint32_t)min(end - first, (uint64_t)it.tiles) : 0u;
+    if (!split && s.k1 > s.k0) {
+        if (s.k0 > 0u) s.k1 = s.k0;
+        else s.k1 = it.tiles;
+    }
+    s.whole = s.k0 == 0u && s.k1 == it.tiles;
+    return s;
+}
+
+// ---- tensor-core and TMEM instructions -------------------------------------------------------
+
+// Shared-memory matrix descriptor, 128-byte swizzle, version of sm_100.  K-major: rows of 64 elements, 8-row atoms 1024 bytes
+// apart.  MN-major (values: 64 dimensions contiguous, keys down the rows): lead = bytes from one 64 dimensions to the next.
+__device__ __forceinline__ uint64_t smem_desc(uint32_t at, uint32_t lead) {
+    return (uint64_t)((at & 0x3FFFFu) >> 4) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// Instruction descriptor: D fp32, A and B bf16, 128 x n; B MN-major where `transposed`.
+__device__ __forceinline__ constexpr uint32_t mma_desc(uint32_t n, bool transposed) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | ((transposed ? 1u : 0u) << 16) | ((n >> 3) << 17) | ((uint32_t)(ROW_TILE >> 4) << 24);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_load32(uint32_t at, float* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]), "=f"(r[9]), "=f"(r[10]),
+          "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]), "=f"(r[16]), "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]),
+          "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]),
+          "=f"(r[31])
+        : "r"(at)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(at),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+        "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
+        "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map),
+        "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map),
+        "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
+        : "memory");
+}
+
+// ---- the kernel ------------------------------------------------------------------------------
+
+template <int D, bool PAGED>
+__global__ void __launch_bounds__(PROMPT_THREADS, 1)
+attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Args a) {
+    using C = PromptCfg<D>;
+    constexpr uint32_t ST = C::STAGES, BARS = 4 * ST + 10;
+    extern __shared__ uint8_t smem[];
+    __shared__ __align__(8) uint64_t bars[BARS];
+    __shared__ uint32_t tmem_slot, dirty_item[8];
+    __shared__ volatile uint32_t abort_flag;
+    const uint32_t base = (smem_addr(smem) + 1023u) & ~1023u;
+    const uint32_t q_at = base, ring = base + 2u * C::TILE_BYTES;
+    auto bar = [&](uint32_t i) { return smem_addr(&bars[i]); };
+    auto full = [&](uint32_t s) { return bar(s); };
+    auto empty = [&](uint32_t s) { return bar(ST + s); };
+    // The values of an edge tile arrive at `raw`, and the products wait for `checked`, where they have been looked through; everything
+    // else arrives at `full`.  A place of the ring is filled again only after its products, so nobody is ever a turn ahead
+    // at any of a place's barriers; which turn each is at, one bit a place says (`turns`).
+    auto raw = [&](uint32_t s) { return bar(2 * ST + s); };
+    auto checked = [&](uint32_t s) { return bar(3 * ST + s); };
+    const uint32_t q_full = bar(4 * ST), q_empty = bar(4 * ST + 1);
+    auto s_full = [&](uint32_t t) { return bar(4 * ST + 2 + t); };
+    auto p_full = [&](uint32_t t) { return bar(4 * ST + 4 + t); };
+    auto o_full = [&](uint32_t t) { return bar(4 * ST + 6 + t); };  // one more product has been added to O
+    auto o_free = [&](uint32_t t) { return bar(4 * ST + 8 + t); };  // the item's O has been read
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+
+    pdl_launch_dependents();
+    if (threadIdx.x == 0) {
+        abort_flag = 0u;
+        for (uint32_t i = 0; i < ST; ++i) mbar_init(full(i), 1), mbar_init(empty(i), 1), mbar_init(raw(i), 1), mbar_init(checked(i), 2);
+        mbar_init(q_full, 1), mbar_init(q_empty, 1);
+        for (uint32_t t = 0; t < 2; ++t) mbar_init(s_full(t), 1), mbar_init(p_full(t), 4), mbar_init(o_full(t), 1), mbar_init(o_free(t), 4);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_q) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
+    }
+    if (threadIdx.x < 8) dirty_item[threadIdx.x] = 0u;
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&tmem_slot)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = tmem_slot;
+    pdl_wait_prior();
+
+    const uint32_t group = a.group, per_tile = ROW_TILE / group, per_item = 2u * per_tile;
+    const uint64_t total = total_cost<PAGED>(a);
+    const uint32_t shares = shares_of(total, gridDim.x);
+    const bool split = a.parts != nullptr;
+    uint64_t begin = 0, end = 0;
+    Item it;
+    it.start = 0;
+    if (blockIdx.x < shares) {
+        begin = share_begin(total, blockIdx.x, shares), end = share_begin(total, blockIdx.x + 1u, shares);
+        it = item_at<PAGED>(a, begin);
+    }
+    auto has_second = [&]() { return it.x.n > it.t * per_item + per_tile; };
+    // first key tile of the item that some row does not see to its end
+    auto first_edge = [&](uint32_t row_tile) { return seen(a, it.x, it.t * per_item + row_tile * per_tile) / KEYS; };
+
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(SETMAXNREG_OTHERS));
+        if (warp == 8) {
+            // ---- copies
+            uint32_t n_tile = 0, n_item = 0;
+            bool ok = true;
+            while (ok && it.start < end) {
+                const Span span = span_of(it, begin, end, split);
+                if (span.k1 > span.k0) {
+                    if (lane == 0) ok = mbar_wait(q_empty, (n_item & 1u) ^ 1u, &abort_flag, 1);
+                    ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
+                    if (!ok) break;
+                    ++n_item;
+                    if (lane == 0) {
+                        const uint32_t tiles = has_second() ? 2u : 1u;
+                        mbar_expect_tx(q_full, tiles * C::HALVES * per_tile * group * 128u);
+                        for (uint32_t t = 0; t < tiles; ++t)
+                            for (uint32_t h = 0; h < (uint32_t)C::HALVES; ++h)
+                                tma_load_3d(q_at + t * C::TILE_BYTES + h * C::BLOCK, &map_q, (int)(64u * h), (int)(it.head * group),
+                                            (int)(it.x.q0 + it.t * per_item + t * per_tile), q_full);
+                    }
+                    const uint32_t edge = first_edge(0);
+                    for (uint32_t k = span.k0; ok && k < span.k1; ++k) {
+                        int page = 0, row = (int)(it.x.k0 + k * KEYS);
+                        uint32_t boxes = C::HALVES, box_rows = KEYS, mine = lane / C::HALVES;
+                        const uint32_t half = lane % C::HALVES;
+                        bool issue = lane < (uint32_t)C::HALVES;
+                        if (PAGED) {
+                            const uint32_t key0 = k * KEYS, left = it.x.len > key0 ? min(it.x.len - key0, (uint32_t)KEYS) : 0u;
+                            const uint32_t in_box = min(1u << a.page_shift, (uint32_t)KEYS);
+                            issue = mine * in_box < left;
+                            if (issue) {
+                                const uint32_t key = key0 + mine * in_box;
+                                page = ld_fresh(a.table + (size_t)it.r * a.width + (key >> a.page_shift));
+                                row = (int)(key & ((1u << a.page_shift) - 1u));
+                                issue = (uint32_t)page < a.pages;
+                            }
+                            box_rows = in_box;
+                            boxes = __popc(__ballot_sync(0xFFFFFFFFu, issue));
+                        }
+#pragma unroll 1
+                        for (uint32_t which = 0; which < 2u; ++which, ++n_tile) {
+                            const uint32_t s = n_tile % ST, turn = n_tile / ST;
+                            if (lane == 0) ok = mbar_wait(empty(s), (turn & 1u) ^ 1u, &abort_flag, 2);
+                            ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
+                            if (!ok) break;
+                            const uint32_t arrive = which && k >= edge ? raw(s) : full(s);
+                            if (lane == 0) mbar_expect_tx(arrive, boxes * box_rows * 128u);
+                            __syncwarp();
+                            const uint32_t dst = ring + s * C::TILE_BYTES + half * C::BLOCK + mine * box_rows * 128u;
+                            const CUtensorMap* map = which ? &map_v : &map_k;
+                            if (issue) {
+                                if (PAGED) tma_load_4d(dst, map, (int)(64u * half), row, (int)it.head, page, arrive);
+                                else tma_load_3d(dst, map, (int)(64u * half), (int)it.head, row, arrive);
+                            }
+                        }
+                    }
+                }
+                it.next(a, per_item, PAGED, end);
+            }
+        } else if (warp == 9) {
+            // ---- products
+            if (lane == 0) {
+                constexpr uint32_t idesc_s = mma_desc(KEYS, false), idesc_o = mma_desc(D, true);
+                uint32_t n_tile = 0, n_item = 0, full_turns = 0, check_turns = 0, n_p[2] = {0, 0}, n_o[2] = {0, 0};
+                bool ok = true;
+                auto wait_full = [&](uint32_t s, uint32_t where) {
+                    const bool there = mbar_wait(full(s), full_turns >> s & 1u, &abort_flag, where);
+                    full_turns ^= 1u << s;
+                    return there;
+                };
+                while (ok && it.start < end) {
+                    const Span span = span_of(it, begin, end, split);
+                    if (span.k1 > span.k0) {
+                        const uint32_t tiles = has_second() ? 2u : 1u, edge = first_edge(0);
+                        if (!(ok = mbar_wait(q_full, n_item & 1u, &abort_flag, 3))) break;
+                        ++n_item;
+                        auto scores = [&](uint32_t t, uint32_t s) {
+#pragma unroll
+                            for (uint32_t k = 0; k < D / 16u; ++k)
+                                mma_ss(tmem + t * KEYS, smem_desc(q_at + t * C::TILE_BYTES + (k / 4u) * C::BLOCK + (k % 4u) * 32u, 16u),
+                                       smem_desc(ring + s * C::TILE_BYTES + (k / 4u) * C::BLOCK + (k % 4u) * 32u, 16u), idesc_s, k > 0u);
+                            mma_commit(s_full(t));
+                        };
+                        {
+                            const uint32_t s = n_tile % ST;
+                            if (!(ok = wait_full(s, 4))) break;
+                            fence_after();
+                            for (uint32_t t = 0; t < tiles; ++t) scores(t, s);
+                            mma_commit(empty(s));
+                            if (span.k0 + 1u == span.k1) mma_commit(q_empty);
+                        }
+                        for (uint32_t k = span.k0; ok && k < span.k1; ++k, n_tile += 2u) {
+                            const uint32_t vs = (n_tile + 1u) % ST, ks = (n_tile + 2u) % ST;
+                            if (k >= edge) {
+                                ok = mbar_wait(checked(vs), check_turns >> vs & 1u, &abort_flag, 6);
+                                check_turns ^= 1u << vs;
+                            } else {
+                                ok = wait_full(vs, 5);
+                            }
+                            if (!ok) break;
+                            const bool more = k + 1u < span.k1;
+                            for (uint32_t t = 0; t < tiles; ++t) {
+                                if (k == span.k0) {  // the last item's O has been read
+                                    if (!(ok = mbar_wait(o_free(t), (n_o[t] & 1u) ^ 1u, &abort_flag, 7))) break;
+                                    ++n_o[t];
+                                }
+                                if (!(ok = mbar_wait(p_full(t), n_p[t] & 1u, &abort_flag, 8))) break;
+                                ++n_p[t];
+                                fence_after();
+#pragma unroll
+                                for (uint32_t i = 0; i < KEYS / 16u; ++i)
+                                    mma_ts(tmem + 2u * KEYS + t * D, tmem + t * KEYS + 8u * i, smem_desc(ring + vs * C::TILE_BYTES + i * 2048u, C::BLOCK), idesc_o,
+                                           k > span.k0 || i > 0u);
+                                mma_commit(o_full(t));
+                                if (more) {
+                                    if (t == 0u) {
+                                        if (!(ok = wait_full(ks, 4))) break;
+                                        fence_after();
+                                    }
+                                    scores(t, ks);
+                                }
+                            }
+                            if (!ok) break;
+                            mma_commit(empty(vs));
+                            if (more) {
+                                mma_commit(empty(ks));
+                                if (k + 2u == span.k1) mma_commit(q_empty);
+                            }
+                        }
+                    }
+                    it.next(a, per_item, PAGED, end);
+                }
+            }
+        } else {
+            // ---- values of edge tiles: half the rows for each of two warps
+            uint32_t n_tile = 0, n_item = 0, turns = 0;
+            bool ok = true;
+            while (ok && it.start < end) {
+                const Span span = span_of(it, begin, end, split);
+                if (span.k1 > span.k0) {
+                    const uint32_t edge = first_edge(0);
+                    for (uint32_t k = span.k0; ok && k < span.k1; ++k, n_tile += 2u) {
+                        if (k < edge) continue;
+                        const uint32_t s = (n_tile + 1u) % ST;
+                        ok = mbar_wait(raw(s), turns >> s & 1u, &abort_flag, 9);
+                        turns ^= 1u << s;
+                        ok = __all_sync(0xFFFFFFFFu, ok);
+                        if (!ok) break;
+                        const uint32_t there = it.x.len > k * KEYS ? min(it.x.len - k * KEYS, (uint32_t)KEYS) : 0u;
+                        bool changed = false, bad = false;
+                        // 16-byte pieces; rows of 128 bytes, so the swizzle does not matter
+#pragma unroll 4
+                        for (uint32_t e = lane; e < 64u * 8u * C::HALVES; e += 32u) {
+                            const uint32_t row = 64u * (warp - 10u) + (e / 8u) % 64u;
+                            const uint32_t at = ring + s * C::TILE_BYTES + (e / 512u) * C::BLOCK + row * 128u + (e % 8u) * 16u;
+                            uint32_t w[4], z[4];
+                            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+                            bool differs = false;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                z[i] = row < there ? finite_or_zero(w[i]) : 0u;
+                                differs |= z[i] != w[i];
+                            }
+                            bad |= differs && row < there;
+                            if (differs) {
+                                changed = true;
+                                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(z[0]), "r"(z[1]), "r"(z[2]), "r"(z[3]) : "memory");
+                            }
+                        }
+                        if (bad) dirty_item[n_item & 7u] = n_item + 1u;
+                        if (__any_sync(0xFFFFFFFFu, changed)) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(checked(s));
+                    }
+                    ++n_item;
+                }
+                it.next(a, per_item, PAGED, end);
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SETMAXNREG_SOFTMAX));
+        // ---- softmax of a row tile, a thread a row
+        const uint32_t t = warp >> 2, row = threadIdx.x & 127u;
+        const uint32_t lanes = ((warp & 3u) * 32u) << 16;
+        const uint32_t s_at = tmem + lanes + t * KEYS, o_at = tmem + lanes + 2u * KEYS + t * D;
+        const bool wide = (reinterpret_cast<uintptr_t>(a.out) & 31u) == 0u && a.o_token % 16 == 0 && a.o_head % 16 == 0;
+        uint32_t n_s = 0, n_item = 0;
+        bool ok = true;
+        while (ok && it.start < end) {
+            const Span span = span_of(it, begin, end, split);
+            if (span.k1 > span.k0) {
+                const uint32_t item_id = n_item++;
+                if (t == 0u || has_second()) {
+                    const uint32_t i = it.t * per_item + t * per_tile + row / group;
+                    const bool there = row < per_tile * group && i < it.x.n;
+                    const uint32_t sees = there ? seen(a, it.x, i) : 0u;
+                    const uint32_t edge = first_edge(t);
+                    float m = -INFINITY, l = 0.0f;
+                    for (uint32_t k = span.k0; k < span.k1; ++k, ++n_s) {
+                        ok = mbar_wait(s_full(t), n_s & 1u, &abort_flag, 10);
+                        ok = __all_sync(0xFFFFFFFFu, ok);
+                        if (!ok) break;
+                        fence_after();
+                        float s[KEYS];
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) tmem_load32(s_at + 32u * c, s + 32 * c);
+                        tmem_wait_load();
+                        if (k >= edge) {
+                            const uint32_t key0 = k * KEYS;
+                            const uint32_t count = sees > key0 ? sees - key0 : 0u;
+#pragma unroll
+                            for (uint32_t j = 0; j < KEYS; ++j) s[j] = j < count ? s[j] : -INFINITY;
+                        }
+                        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                        for (int j = 0; j < KEYS; ++j) top[j & 3] = fmaxf(top[j & 3], s[j]);
+                        float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
+                        if (k == span.k0) {
+                            m = now;
+                        } else if (__any_sync(0xFFFFFFFFu, now > m + 8.0f)) {
+                            now = fmaxf(now, m);
+                            const float from = now == -INFINITY ? 0.0f : now;
+                            const float keep = exp2_fast(m - from);
+                            m = now;
+                            l *= keep;
+                            ok = mbar_wait(o_full(t), (n_s - 1u) & 1u, &abort_flag, 11);
+                            ok = __all_sync(0xFFFFFFFFu, ok);
+                            if (!ok) break;
+                            fence_after();
+#pragma unroll 1
+                            for (uint32_t c = 0; c < D; c += 32u) {
+                                float o[32];
+                                tmem_load32(o_at + c, o);
+                                tmem_wait_load();
+#pragma unroll
+                                for (int j = 0; j < 32; ++j) o[j] *= keep;
+                                tmem_store32(o_at + c, reinterpret_cast<const uint32_t*>(o));
+                            }
+                            tmem_wait_store();
+                        }
+                        const float from = m == -INFINITY ? 0.0f : m;
+                        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            uint32_t p[32];
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) {
+                                const float x = exp2_fast(fmaf(s[64 * c + 2 * j], a.scale_log2, -from)), y = exp2_fast(fmaf(s[64 * c + 2 * j + 1], a.scale_log2, -from));
+                                sum[j & 3] += x + y;
+                                p[j] = pack_bf16(x, y);
+                            }
+                            tmem_store32(s_at + 32u * c, p);
+                        }
+                        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                        tmem_wait_store();
+                        fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(p_full(t));
+                    }
+                    if (!ok) break;
+                    ok = mbar_wait(o_full(t), (n_s - 1u) & 1u, &abort_flag, 12);
+                    ok = __all_sync(0xFFFFFFFFu, ok);
+                    if (!ok) break;
+                    fence_after();
+                    const bool dirty = *(volatile uint32_t*)&dirty_item[item_id & 7u] == item_id + 1u;
+                    const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;  // no key: zeros; NaN stays
+                    const float factor = span.whole ? inv : 1.0f;
+                    uint16_t* const to = a.out + (int64_t)(it.x.q0 + (there ? i : 0u)) * a.o_token + (int64_t)(it.head * group + row % group) * a.o_head;
+                    float* part = nullptr;
+                    if (!span.whole) {
+                        const uint32_t first = share_of(total, it.start + ITEM_COST, shares);
+                        part = a.parts + (size_t)(2u * blockIdx.x + (first == blockIdx.x ? 1u : 0u)) * C::PART_FLOATS;
+                        part[2u * ROW_TILE * D + t * ROW_TILE + row] = m;
+                        part[2u * ROW_TILE * (D + 1) + t * ROW_TILE + row] = l;
+                    }
+#pragma unroll 1
+                    for (uint32_t c = 0; c < D; c += 32u) {
+                        float o[32];
+                        tmem_load32(o_at + c, o);
+                        tmem_wait_load();
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) o[j] *= factor;
+                        if (dirty) {  // values that are not finite, left out of the product, reach the rows that see them
+#pragma unroll 1
+                            for (uint32_t key = max(first_edge(0), span.k0) * KEYS; key < min(sees, span.k1 * KEYS); ++key) {
+                                int64_t at = (int64_t)it.head * a.v_head + c;
+                                if (PAGED) {
+                                    const uint32_t pg = (uint32_t)ld_fresh(a.table + (size_t)it.r * a.width + (key >> a.page_shift));
+                                    if (pg >= a.pages) continue;
+                                    at += (int64_t)pg * a.v_page + (int64_t)(key & ((1u << a.page_shift) - 1u)) * a.v_slot;
+                                } else {
+                                    at += (int64_t)(it.x.k0 + key) * a.v_slot;
+                                }
+#pragma unroll
+                                for (int j = 0; j < 32; ++j) {
+                                    const float v = bf16_bits_to_float(ld_fresh(a.v + at + j));
+                                    if (!(fabsf(v) < INFINITY)) o[j] += v;
+                                }
+                            }
+                        }
+                        if (!span.whole) {
+#pragma unroll
+                            for (int j = 0; j < 8; ++j)
+                                *reinterpret_cast<float4*>(part + ((size_t)(c / 4u + j) * 2u * ROW_TILE + t * ROW_TILE + row) * 4u) =
+                                    make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+                        } else if (there) {
+                            uint32_t w[16];
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) w[j] = pack_bf16(o[2 * j], o[2 * j + 1]);
+                            if (wide) {  // whole sectors: a lane's row is its own
+#pragma unroll
+                                for (int j = 0; j < 2; ++j)
+                                    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to + c + 16 * j), "r"(w[8 * j]), "r"(w[8 * j + 1]),
+                                                 "r"(w[8 * j + 2]), "r"(w[8 * j + 3]), "r"(w[8 * j + 4]), "r"(w[8 * j + 5]), "r"(w[8 * j + 6]), "r"(w[8 * j + 7])
+                                                 : "memory");
+                            } else {
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(to + c + 8 * j) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+                            }
+                        }
+                    }
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(o_free(t));
+                }
+            }
+            it.next(a, per_item, PAGED, end);
+        }
+    }
+
+    // on abort give copies and MMAs in flight time to land before TMEM is freed
+    __syncwarp();
+    if (abort_flag) {
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000LL) __nanosleep(1000);
+    }
+    fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+}
+
+// Parts of items that more than one CTA worked on, added up in the order of their keys.  CTA (k, y): rows [64 y, 64 y + 64) of the
+// item that CTA k of the kernel above began and did not end, if there is one.
+constexpr int JOIN_THREADS = 512, JOIN_ROWS = 64;
+template <int D, bool PAGED>
+__global__ void __launch_bounds__(JOIN_THREADS) attention_join_kernel(const Args a, uint32_t ctas) {
+    using C = PromptCfg<D>;
+    pdl_launch_dependents();
+    pdl_wait_prior();
+    const uint64_t total = total_cost<PAGED>(a);
+    const uint32_t k = blockIdx.x, shares = shares_of(total, ctas);
+    if (k >= shares) return;
+    const uint64_t end = share_begin(total, k + 1u, shares);
+    const Item it = item_at<PAGED>(a, end - 1u);
+    const uint64_t stop = it.start + ITEM_COST + it.tiles;
+    const uint32_t first = share_of(total, it.start + ITEM_COST, shares), last = share_of(total, stop - 1u, shares);
+    if (first != k || last == k) return;
+    const uint32_t group = a.group, per_tile = ROW_TILE / group, per_item = 2u * per_tile;
+    auto part = [&](uint32_t c) { return a.parts + (size_t)(2u * c + (c == first ? 1u : 0u)) * C::PART_FLOATS; };
+    for (uint32_t e = threadIdx.x; e < JOIN_ROWS * (D / 8u); e += JOIN_THREADS) {
+        const uint32_t row = JOIN_ROWS * blockIdx.y + e % JOIN_ROWS, c8 = e / JOIN_ROWS;
+        const uint32_t in_tile = row % ROW_TILE, i = it.t * per_item + (row / ROW_TILE) * per_tile + in_tile / group;
+        if (in_tile >= per_tile * group || i >= it.x.n) continue;
+        float m = -INFINITY;
+        for (uint32_t c = first; c <= last; ++c) m = fmaxf(m, ld_fresh(part(c) + 2u * ROW_TILE * D + row));
+        const float from = m == -INFINITY ? 0.0f : m;
+        float l = 0.0f, o[8] = {};
+#pragma unroll 4
+        for (uint32_t c = first; c <= last; ++c) {
+            const float f = exp2_fast(ld_fresh(part(c) + 2u * ROW_TILE * D + row) - from);
+            l = fmaf(ld_fresh(part(c) + 2u * ROW_TILE * (D + 1) + row), f, l);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float4 x = ld_fresh(reinterpret_cast<const float4*>(part(c)) + (size_t)(2u * c8 + h) * 2u * ROW_TILE + row);
+                o[4 * h] = fmaf(x.x, f, o[4 * h]), o[4 * h + 1] = fmaf(x.y, f, o[4 * h + 1]);
+                o[4 * h + 2] = fmaf(x.z, f, o[4 * h + 2]), o[4 * h + 3] = fmaf(x.w, f, o[4 * h + 3]);
+            }
+        }
+        const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
+        uint16_t* to = a.out + (int64_t)(it.x.q0 + i) * a.o_token + (int64_t)(it.head * group + in_tile % group) * a.o_head + 8u * c8;
+        *reinterpret_cast<uint4*>(to) = make_uint4(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv), pack_bf16(o[4] * inv, o[5] * inv),
+                                                   pack_bf16(o[6] * inv, o[7] * inv));
+    }
+}
+
+}  // namespace attention
+}  // namespace miori_b200

@@ -17,6 +17,7 @@
 
 #include <dlfcn.h>
 
+#include <cmath>
 #include <cstdint>
 #include <cstring>
 #include <exception>
@@ -32,7 +33,8 @@ PyObject* g_error = nullptr;  // _lib.MioriError
     X(last_error) X(gemv4) X(gemv8) X(dequant4_rowmajor) X(dequant8_rowmajor) X(dequant4_cache)  \
     X(cache_bytes) X(gemm_bf16_cache_ws) X(gemm_bf16_strided) X(gemv_bf16_cache) X(linear4)      \
     X(rmsnorm) X(post_norm_add) X(silu_mul) X(embed8) X(argmax) X(gemv4_rmsnorm)                 \
-    X(gemv8_rmsnorm) X(gemv4_silu) X(gemv4_post_norm_add) X(gemv4_rmsnorm_silu)
+    X(gemv8_rmsnorm) X(gemv4_silu) X(gemv4_post_norm_add) X(gemv4_rmsnorm_silu) X(page_slots)    \
+    X(rope_kv) X(attention_paged) X(attention_prompt)
 
 struct Abi {
 #define X(name) decltype(&miori_##name) name;
@@ -416,6 +418,140 @@ OP(gemv4_rmsnorm_silu, 6, "q", "s", "b", "x", "gamma", "eps", "group", "flags", 
     return y.result();
 }
 
+// Whole numbers of a step's plan: int32, on the GPU, contiguous.
+const int32_t* ints(const at::Tensor& t, const char* what, int64_t numel) {
+    if (!t.is_cuda()) raise(PyExc_ValueError, "miori_b200 ops need CUDA tensors (there is no CPU path)");
+    if (t.scalar_type() != at::kInt) raise(PyExc_TypeError, "%s: an int32 tensor is expected", what);
+    if (!t.is_contiguous()) raise(PyExc_ValueError, "miori_b200 ops need contiguous tensors");
+    if (numel >= 0 && t.numel() != numel) raise(PyExc_ValueError, "%s: %lld numbers expected, got %lld", what, (long long)numel, (long long)t.numel());
+    return static_cast<const int32_t*>(t.data_ptr());
+}
+// A bf16 tensor of `dims` dimensions whose last one is contiguous; the others lie as they like.
+void need_heads(const at::Tensor& t, const char* what, int64_t dims) {
+    if (!t.is_cuda()) raise(PyExc_ValueError, "miori_b200 ops need CUDA tensors (there is no CPU path)");
+    if (t.scalar_type() != at::kBFloat16) raise(PyExc_TypeError, "%s: a bf16 tensor is expected", what);
+    if (t.dim() != dims) raise(PyExc_ValueError, "%s: %lld dimensions expected, got %lld", what, (long long)dims, (long long)t.dim());
+    if (t.size(dims - 1) != 1 && t.stride(dims - 1) != 1) raise(PyExc_ValueError, "%s: the last dimension must be contiguous", what);
+}
+// A stride, or where there is only one step to take any that passes the library's checks.
+int64_t step(const at::Tensor& t, int64_t d) { return t.size(d) == 1 ? t.size(t.dim() - 1) : t.stride(d); }
+
+PyObject* tuple_of(std::initializer_list<at::Tensor*> ts) {
+    PyObject* all = PyTuple_New((Py_ssize_t)ts.size());
+    if (!all) throw Failed();
+    Py_ssize_t i = 0;
+    for (at::Tensor* t : ts) PyTuple_SET_ITEM(all, i++, THPVariable_Wrap(std::move(*t)));
+    return all;
+}
+
+OP(page_slots, 7, "held", "new", "table", "pool", "taken", "page", "tokens", "flags") {
+    const at::Tensor &held = a.tensor(0), &fresh = a.tensor(1), &table = a.tensor(2), &pool = a.tensor(3), &taken = a.tensor(4);
+    const int64_t R = held.numel();
+    const int32_t *hp = ints(held, "held", -1), *fp = ints(fresh, "new", R), *tp = ints(table, "table", -1), *pp = ints(pool, "pool", -1),
+                  *kp = ints(taken, "taken", 1);
+    if (table.dim() != 2 || table.size(0) != R) raise(PyExc_ValueError, "table: [%lld][width] expected", (long long)R);
+    const uint32_t page = a.u32(5, 0), T = a.u32(6, 0), flags = a.u32(7, 0);
+    at::Tensor slots = empty({T}, at::kInt, held), positions = empty({T}, at::kInt, held), cu = empty({R + 1}, at::kInt, held),
+               after = empty({R}, at::kInt, held), taken_after = empty({1}, at::kInt, held);
+    auto out = [](at::Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); };
+    call(abi.page_slots, hp, fp, const_cast<int32_t*>(tp), pp, kp, out(slots), out(positions), out(cu), out(after), out(taken_after), R,
+         table.size(1), page, pool.numel(), T, flags, stream());
+    return tuple_of({&slots, &positions, &cu, &after, &taken_after});
+}
+
+OP(rope_kv, 7, "qkv", "turns", "positions", "slots", "k_cache", "v_cache", "heads", "axes", "gamma_q", "gamma_k", "eps", "flags", "out") {
+    const at::Tensor &qkv = a.tensor(0), &turns = a.tensor(1), &positions = a.tensor(2), &slots = a.tensor(3), &k = a.tensor(4), &v = a.tensor(5);
+    if (!qkv.is_cuda() || !turns.is_cuda()) raise(PyExc_ValueError, "miori_b200 ops need CUDA tensors (there is no CPU path)");
+    const bool fp32 = qkv.scalar_type() == at::kFloat;
+    if (!fp32 && qkv.scalar_type() != at::kBFloat16) raise(PyExc_TypeError, "qkv: an fp32 or bf16 tensor is expected");
+    if (turns.scalar_type() != at::kLong || !turns.is_contiguous()) raise(PyExc_TypeError, "turns: a contiguous int64 tensor is expected");
+    need_heads(k, "k_cache", 4);
+    need_heads(v, "v_cache", 4);
+    if (k.sizes() != v.sizes()) raise(PyExc_ValueError, "k_cache and v_cache differ in shape");
+    if (qkv.dim() != 2 || (qkv.size(1) != 1 && qkv.stride(1) != 1)) raise(PyExc_ValueError, "qkv: [tokens][columns] with contiguous rows expected");
+    const int64_t T = qkv.size(0), G = k.size(1), D = k.size(3), H = a.u32(6, 0), half = turns.numel();
+    if (qkv.size(1) != (H + 2 * G) * D)
+        raise(PyExc_ValueError, "qkv: %lld columns expected for %lld + 2 * %lld heads of %lld, got %lld", (long long)((H + 2 * G) * D), (long long)H, (long long)G,
+              (long long)D, (long long)qkv.size(1));
+    if (positions.dim() > 2 || positions.dim() < 1 || positions.size(positions.dim() - 1) != T) raise(PyExc_ValueError, "positions: [tokens] or [axes][tokens] expected");
+    const int64_t A = positions.dim() == 2 ? positions.size(0) : 1;
+    const int32_t *pp = ints(positions, "positions", -1), *sp = ints(slots, "slots", T), *ap = a.given(7) ? ints(a.tensor(7), "axes", half) : nullptr;
+    auto gamma = [&](int i, const char* what) -> const void* {
+        if (!a.given(i)) return nullptr;
+        need_heads(a.tensor(i), what, 1);
+        if (a.tensor(i).numel() != D) raise(PyExc_ValueError, "%s: %lld weights expected", what, (long long)D);
+        return a.tensor(i).data_ptr();
+    };
+    const void *gq = gamma(8, "gamma_q"), *gk = gamma(9, "gamma_k");
+    const float eps = a.given(10) ? a.f32(10) : 0.0f;
+    const uint32_t flags = (a.u32(11, 0) & ~MIORI_ROPE_F32) | (fp32 ? MIORI_ROPE_F32 : 0u);
+    const int64_t strides[6] = {step(k, 0), step(k, 1), step(k, 2), step(v, 0), step(v, 1), step(v, 2)};
+    Out o = output(a, 12, {T, H, D}, at::kBFloat16, qkv);
+    call(abi.rope_kv, qkv.data_ptr(), T == 1 ? qkv.size(1) : qkv.stride(0), static_cast<const uint64_t*>(turns.data_ptr()), ap, pp, sp, gq, gk, eps, o.ptr(),
+         k.data_ptr(), v.data_ptr(), strides, T, H, G, D, 2 * half, A, k.size(0), k.size(2), flags, stream());
+    return o.result();
+}
+
+// scale given, or 1 / sqrt(dim)
+float scale_of(const Args& a, int i, int64_t D) { return a.given(i) ? a.f32(i) : 1.0f / std::sqrt((float)D); }
+// The output of q's shape: strided views of the caller's are fine.
+Out heads_out(const Args& a, int i, const at::Tensor& q) {
+    Out o;
+    if (!a.given(i)) {
+        o.made = empty(q.sizes(), at::kBFloat16, q);
+        return o;
+    }
+    need_heads(a.tensor(i), "out", 3);
+    if (a.tensor(i).sizes() != q.sizes()) raise(PyExc_ValueError, "out: the shape of q is expected");
+    o.given = a.v[i];
+    return o;
+}
+
+OP(attention_paged, 7, "q", "k_cache", "v_cache", "table", "lens", "cu", "max_new", "scale", "flags", "out", "workspace") {
+    const at::Tensor &q = a.tensor(0), &k = a.tensor(1), &v = a.tensor(2), &table = a.tensor(3), &lens = a.tensor(4), &cu = a.tensor(5);
+    need_heads(q, "q", 3);
+    need_heads(k, "k_cache", 4);
+    need_heads(v, "v_cache", 4);
+    if (k.sizes() != v.sizes()) raise(PyExc_ValueError, "k_cache and v_cache differ in shape");
+    const int64_t T = q.size(0), H = q.size(1), D = q.size(2), G = k.size(1), R = lens.numel();
+    if (k.size(3) != D) raise(PyExc_ValueError, "heads of q and of the cache differ in size");
+    const int32_t *tp = ints(table, "table", -1), *lp = ints(lens, "lens", -1), *cp = ints(cu, "cu", R + 1);
+    if (table.dim() != 2 || table.size(0) != R) raise(PyExc_ValueError, "table: [%lld][width] expected", (long long)R);
+    const uint32_t max_new = a.u32(6, 0), flags = a.u32(8, 0);
+    const float scale = scale_of(a, 7, D);
+    Out o = heads_out(a, 9, q);
+    const at::Tensor& out = o.given ? THPVariable_Unpack(o.given) : o.made;
+    void* wp;
+    size_t wb;
+    workspace(a, 10, wp, wb);
+    const int64_t strides[10] = {step(q, 0), step(q, 1), step(out, 0), step(out, 1), step(k, 0), step(k, 1), step(k, 2), step(v, 0), step(v, 1), step(v, 2)};
+    call(abi.attention_paged, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), strides, tp, lp, cp, R, T, table.size(1), k.size(0), k.size(2), H, G, D,
+         max_new, scale, flags, wp, wb, stream());
+    return o.result();
+}
+
+OP(attention_prompt, 4, "q", "k", "v", "cu", "cu_k", "scale", "flags", "out", "workspace") {
+    const at::Tensor &q = a.tensor(0), &k = a.tensor(1), &v = a.tensor(2), &cu = a.tensor(3);
+    need_heads(q, "q", 3);
+    need_heads(k, "k", 3);
+    need_heads(v, "v", 3);
+    if (k.sizes() != v.sizes()) raise(PyExc_ValueError, "k and v differ in shape");
+    const int64_t T = q.size(0), H = q.size(1), D = q.size(2), G = k.size(1), R = cu.numel() - 1;
+    if (k.size(2) != D) raise(PyExc_ValueError, "heads of q and of k differ in size");
+    if (!a.given(4) && k.size(0) != T) raise(PyExc_ValueError, "k: %lld rows expected, as q has (or give cu_k)", (long long)T);
+    const int32_t *cp = ints(cu, "cu", -1), *kp = a.given(4) ? ints(a.tensor(4), "cu_k", R + 1) : nullptr;
+    const float scale = scale_of(a, 5, D);
+    const uint32_t flags = a.u32(6, 0);
+    Out o = heads_out(a, 7, q);
+    const at::Tensor& out = o.given ? THPVariable_Unpack(o.given) : o.made;
+    void* wp;
+    size_t wb;
+    workspace(a, 8, wp, wb);
+    const int64_t strides[8] = {step(q, 0), step(q, 1), step(out, 0), step(out, 1), step(k, 0), step(k, 1), step(v, 0), step(v, 1)};
+    call(abi.attention_prompt, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), strides, cp, kp, R, T, k.size(0), H, G, D, scale, flags, wp, wb, stream());
+    return o.result();
+}
+
 // bind(handle, error): take the library's functions from the handle that ctypes opened.
 PyObject* py_bind(PyObject*, PyObject* args) {
     unsigned long long h = 0;
@@ -476,6 +612,21 @@ PyMethodDef methods[] = {
     FAST(gemv4_rmsnorm_silu, "q, s, b, x, gamma, eps, group=32, flags=0, out=None",
          "bf16(silu(gate) * up) [M][N/2] of the fused gate + up weights applied to bf16(rmsnorm(x) * gamma),\n"
          "x fp32 [M][K], M <= 4: one launch for the norm, both projections and the activation."),
+    FAST(page_slots, "held, new, table, pool, taken, page, tokens, flags=0",
+         "(slots, positions, cu, held_after, taken_after) of a step in which request r adds new[r] tokens to its held[r]:\n"
+         "new pages come from pool[taken:] and are written into table [requests][width]; all int32.  slots and positions\n"
+         "have `tokens` rows; rows without a token, or without a page for it, get slot -1."),
+    FAST(rope_kv, "qkv, turns, positions, slots, k_cache, v_cache, heads, axes=None, gamma_q=None, gamma_k=None, eps=0.0, flags=0, out=None",
+         "q [T][heads][dim] bf16 of qkv [T][(heads + 2 kv_heads) * dim] (fp32 or bf16): q and k heads normed (gamma) and turned\n"
+         "by their positions [T] or [axes][T]; k and v written into slots[t] of the caches [pages][kv_heads][page][dim].\n"
+         "turns, axes: see rope_turns.  flags: ROPE_ADJACENT, LAUNCH_PDL."),
+    FAST(attention_paged, "q, k_cache, v_cache, table, lens, cu, max_new, scale=None, flags=0, out=None, workspace=None",
+         "Causal attention of the packed tokens q [T][heads][dim] (request r: rows cu[r] to cu[r + 1] - 1, its newest) over the\n"
+         "pages of each request, lens[r] positions; bf16.  max_new: the most tokens of a request.  workspace:\n"
+         "attention_workspace(), lets SMs share a request.  flags: ATTENTION_FULL, LAUNCH_PDL."),
+    FAST(attention_prompt, "q, k, v, cu, cu_k=None, scale=None, flags=0, out=None, workspace=None",
+         "Causal attention of packed prompts: q [T][heads][dim], k and v [T][kv_heads][dim] bf16, prompt r being rows cu[r] to\n"
+         "cu[r + 1] - 1 (keys: cu_k, where they are others').  workspace, flags: as attention_paged."),
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", "Native call path of the operators, " MIORI_TORCH_TAG, -1, methods,

@@ -5,4 +5,6 @@
 #include "ops_api.cu"
 #include "gemm_tcgen05.cu"
 #include "neighbors.cu"
+#include "pages.cu"
+#include "attention.cu"
 #include "peers.cu"
