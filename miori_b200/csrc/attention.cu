@@ -12,7 +12,7 @@
 namespace miori_b200 {
 namespace attention {
 
-constexpr size_t COUNTER_BYTES = 4096;
+constexpr size_t COUNTER_BYTES = 4096, JOIN_BYTES = 12288;  // for up to 768 SMs
 static size_t part_bytes() { return 2u * (size_t)sm_count() * PromptCfg<128>::PART_FLOATS * 4u; }
 
 static int make_map(CUtensorMap* map, const void* base, int rank, const uint64_t* dims, const int64_t* strides, const uint32_t* box) {
@@ -48,6 +48,13 @@ static int check_common(const char* fn, const void* q, const void* k, const void
     return MIORI_OK;
 }
 
+static void use_workspace(Args& a, void* workspace) {
+    if (!workspace) return;
+    a.counters = (uint32_t*)workspace;
+    a.joins = (uint4*)((char*)workspace + COUNTER_BYTES);
+    a.parts = (float*)((char*)workspace + COUNTER_BYTES + JOIN_BYTES);
+}
+
 template <int D, bool PAGED>
 static int launch_prompt(const Args& a, bool may_split, uint32_t flags, cudaStream_t stream) {
     CUtensorMap mq, mk, mv;
@@ -80,7 +87,7 @@ static int launch_prompt(const Args& a, bool may_split, uint32_t flags, cudaStre
     cudaError_t e = launch(attention_prompt_kernel<D, PAGED>, dim3(G), dim3(PROMPT_THREADS), PromptCfg<D>::SMEM, stream, (flags & MIORI_LAUNCH_PDL) != 0, mq, mk, mv, a);
     if (e != cudaSuccess) return cuda_fail(e, "attention_prompt launch");
     if (a.parts && may_split) {
-        e = launch(attention_join_kernel<D, PAGED>, dim3(G, 2 * ROW_TILE / JOIN_ROWS), dim3(JOIN_THREADS), 0, stream, true, a, G);
+        e = launch(attention_join_kernel<D>, dim3(G, 2 * ROW_TILE / JOIN_ROWS), dim3(JOIN_THREADS), 0, stream, true, a);
         if (e != cudaSuccess) return cuda_fail(e, "attention_join launch");
     }
     return MIORI_OK;
@@ -100,7 +107,7 @@ static int launch_decode(const Args& a, uint32_t rows, uint32_t flags, cudaStrea
 
 using namespace miori_b200;
 
-MIORI_API size_t miori_attention_workspace_bytes(void) { return attention::COUNTER_BYTES + attention::part_bytes(); }
+MIORI_API size_t miori_attention_workspace_bytes(void) { return attention::COUNTER_BYTES + attention::JOIN_BYTES + attention::part_bytes(); }
 
 MIORI_API int miori_attention_paged(const void* q, const void* k_cache, const void* v_cache, void* out, const int64_t* strides,
                                     const int32_t* table, const int32_t* lens, const int32_t* cu, uint32_t requests, uint32_t tokens,
@@ -123,7 +130,7 @@ MIORI_API int miori_attention_paged(const void* q, const void* k_cache, const vo
     while ((1u << a.page_shift) < page) ++a.page_shift;
     a.causal = (flags & MIORI_ATTENTION_FULL) == 0;
     a.scale_log2 = scale * 1.4426950408889634f;
-    if (workspace) a.counters = (uint32_t*)workspace, a.parts = (float*)((char*)workspace + COUNTER_BYTES);
+    use_workspace(a, workspace);
     const uint64_t rows = (uint64_t)(max_new ? max_new : 1u) * a.group;
     const cudaStream_t s = (cudaStream_t)stream;
     if (rows <= 16) return dim == 128 ? launch_decode<128>(a, (uint32_t)rows, flags, s) : launch_decode<64>(a, (uint32_t)rows, flags, s);
@@ -146,7 +153,7 @@ MIORI_API int miori_attention_prompt(const void* q, const void* k, const void* v
     a.requests = requests, a.heads = heads, a.kv_heads = kv_heads, a.group = heads / kv_heads, a.tokens = tokens, a.keys = keys;
     a.causal = (flags & MIORI_ATTENTION_FULL) == 0;
     a.scale_log2 = scale * 1.4426950408889634f;
-    if (workspace) a.counters = (uint32_t*)workspace, a.parts = (float*)((char*)workspace + COUNTER_BYTES);
+    use_workspace(a, workspace);
     const bool may_split = keys > (uint32_t)KEYS;
     return dim == 128 ? launch_prompt<128, false>(a, may_split, flags, (cudaStream_t)stream) : launch_prompt<64, false>(a, may_split, flags, (cudaStream_t)stream);
 }

@@ -27,8 +27,10 @@ struct Args {
     uint32_t width, page_shift, pages;                           // of the table; page size as a power of two
     uint32_t causal;
     float scale_log2;  // scale * log2(e)
-    uint32_t* counters;
-    float* parts;      // null: items are not split
+    // workspace, all null without one: then items are not split
+    uint32_t* counters;  // of CTAs that are done with an item (decode)
+    uint4* joins;        // what is to be added up behind the prompt kernel
+    float* parts;
 };
 
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {

@@ -24,7 +24,8 @@ namespace miori_b200 {
 namespace attention {
 
 constexpr int PROMPT_THREADS = 384, KEYS = 128, ROW_TILE = 128;
-constexpr uint32_t ITEM_COST = 1;  // an item's set-up and end, in key tiles
+constexpr uint32_t ITEM_COST = 256;     // an item's set-up and end, in positions
+constexpr uint32_t LEAST_SHARE = 256;   // positions; a tile of keys at least
 
 template <int D>
 struct PromptCfg {
@@ -35,145 +36,157 @@ struct PromptCfg {
     static constexpr int SMEM = 1024 + (2 + STAGES) * TILE_BYTES;
     static constexpr int PART_FLOATS = 2 * ROW_TILE * (D + 2);  // [D / 4][256] pieces of O, then m and l
 };
-constexpr int SETMAXNREG_SOFTMAX = 224, SETMAXNREG_OTHERS = 56;  // (256 * 224 + 128 * 56) = 384 * 168, what a launch has
+// Of every PAIRS_OF pairs of exponentials so many are computed by exp2_pair, the others by the special-function unit.
+constexpr int PAIRS_COMPUTED = 1, PAIRS_OF = 4;
+constexpr int SETMAXNREG_SOFTMAX = 208, SETMAXNREG_OTHERS = 88;  // (256 * 224 + 128 * 56) = 384 * 168, what a launch has
 static_assert(256 * SETMAXNREG_SOFTMAX + 128 * SETMAXNREG_OTHERS <= PROMPT_THREADS * 168, "a split above the launch's registers waits forever");
 
 // ---- how the work is dealt ---------------------------------------------------------------
+//
+// An item costs ITEM_COST + the positions that its last token sees, so that the sum over the items of a head has a closed form
+// (a product and a square) and a CTA finds its share in about a microsecond, however long the prompts are.  Tile k of an item belongs to
+// the share that holds unit start + ITEM_COST - 1 + 128 k.  A share is never shorter than a tile of keys: of the shares between the
+// first and the last of an item each holds at least one of its tiles.
 
-// Sum over i < n of floor((a i + b) / m).
-__device__ __forceinline__ uint64_t floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
-    uint64_t sum = 0;
-    while (n) {
-        sum += (uint64_t)n * (n - 1u) / 2u * (a / m) + (uint64_t)n * (b / m);
-        a %= m, b %= m;
-        const uint32_t y = a * n + b;  // a, b < m <= 256, n < 2^23
-        n = y / m, b = y % m;
-        const uint32_t swap = m;
-        m = a, a = swap;
-        if (!m) break;
-    }
-    return sum;
-}
 __device__ __forceinline__ uint32_t item_tokens(const Args& a) { return 2u * (ROW_TILE / a.group); }
-__device__ __forceinline__ uint32_t key_tiles(uint32_t positions) { return max((positions + KEYS - 1u) / KEYS, 1u); }
-// Key tiles of item t of a request.
-__device__ __forceinline__ uint32_t tiles_of(const Args& a, const Request& x, uint32_t t) {
-    return key_tiles(seen(a, x, min((t + 1u) * item_tokens(a), x.n) - 1u));
-}
+// Positions that the last token of item t sees.
+__device__ __forceinline__ uint32_t item_seen(const Args& a, const Request& x, uint32_t t, uint32_t step) { return seen(a, x, min((t + 1u) * step, x.n) - 1u); }
 // Cost of items 0 .. t-1 of one head.
-__device__ __forceinline__ uint64_t cost_before(const Args& a, const Request& x, uint32_t t, uint32_t items) {
-    if (t == 0) return 0;
-    if (!a.causal) return (uint64_t)t * (ITEM_COST + key_tiles(x.len));
+__device__ __forceinline__ uint64_t cost_before(const Args& a, const Request& x, uint32_t t, uint32_t items, uint32_t step) {
     uint64_t cost = (uint64_t)t * ITEM_COST;
+    if (!a.causal) return cost + (uint64_t)t * x.len;
     uint32_t full = t;
-    if (t == items) cost += key_tiles(x.len), --full;  // the last one's tokens may end early
-    const uint32_t step = item_tokens(a);
-    // the first `flat` items see at most one tile of keys, the others ceil((len - n + (i + 1) step) / 128)
+    if (t == items && t) cost += x.len, --full;  // the last one may hold fewer tokens
     const int64_t before = (int64_t)x.len - (int64_t)x.n;
-    const int64_t room = (int64_t)KEYS - before;
-    const uint32_t flat = room < (int64_t)step ? 0u : min((uint32_t)(room / step), full);
-    cost += flat;
-    const uint32_t more = full - flat;
-    if (more) {
-        const uint64_t b = (uint64_t)(before + (int64_t)(flat + 1u) * step) + KEYS - 1u;
-        cost += (uint64_t)more * (b / KEYS) + floor_sum(more, KEYS, step, (uint32_t)(b % KEYS));
-    }
-    return cost;
+    const uint32_t none = before < 0 ? min((uint32_t)-before / step, full) : 0u;  // items none of whose tokens sees anything
+    // item i sees before + (i + 1) step
+    return cost + (uint64_t)((int64_t)(full - none) * before) + (((uint64_t)full * (full + 1u) - (uint64_t)none * (none + 1u)) / 2u) * step;
 }
 
+struct Shares {
+    uint64_t total;
+    uint32_t count;
+    __device__ __forceinline__ uint64_t begin(uint32_t k) const {  // the same number wherever it is computed
+        return k == count ? total : (uint64_t)((double)total * (double)k / (double)count);
+    }
+    __device__ __forceinline__ uint32_t of(uint64_t unit) const {
+        uint32_t k = min((uint32_t)((double)unit * (double)count / (double)total), count - 1u);
+        while (begin(k) > unit) --k;
+        while (begin(k + 1u) <= unit) ++k;
+        return k;
+    }
+};
 struct Item {
     Request x;
-    uint32_t r, head, t, items, tiles;
+    uint32_t r, head, t, items, sees, tiles;
     uint64_t start;  // its first unit
-    __device__ __forceinline__ void enter(const Args& a, uint32_t id, uint32_t per_item, bool paged) {
-        r = id;
-        x = paged ? request<true>(a, r) : request<false>(a, r);
-        items = (x.n + per_item - 1u) / per_item;
+    __device__ __forceinline__ void measure(const Args& a, uint32_t step) {
+        sees = item_seen(a, x, t, step);
+        tiles = max((sees + KEYS - 1u) / KEYS, 1u);
     }
-    __device__ __forceinline__ void next(const Args& a, uint32_t per_item, bool paged, uint64_t end) {
-        start += ITEM_COST + tiles;
+    __device__ __forceinline__ uint64_t mark() const { return start + ITEM_COST - 1u; }  // of its first tile
+    __device__ __forceinline__ uint64_t last_mark() const { return mark() + (uint64_t)(tiles - 1u) * KEYS; }
+    template <bool PAGED>
+    __device__ __forceinline__ void next(const Args& a, uint32_t step, uint64_t end) {
+        start += ITEM_COST + sees;
         if (start >= end) return;  // there may be no further request
         if (++t == items) {
             t = 0u;
             if (++head == a.kv_heads) {
                 head = 0u;
-                do enter(a, r + 1u, per_item, paged);
-                while (items == 0u && r + 1u < a.requests);
+                do {
+                    x = request<PAGED>(a, ++r);
+                    items = (x.n + step - 1u) / step;
+                } while (items == 0u && r + 1u < a.requests);
             }
         }
-        tiles = tiles_of(a, x, t);
+        measure(a, step);
     }
 };
-
+// This CTA's share and the item that it begins in (begin == end: nothing to do).  By a whole warp.
+struct Start {
+    Shares shares;
+    uint64_t begin, end;
+    Item it;
+};
 template <bool PAGED>
-__device__ __forceinline__ uint64_t request_cost(const Args& a, uint32_t r) {
-    const Request x = request<PAGED>(a, r);
-    const uint32_t per_item = item_tokens(a), items = (x.n + per_item - 1u) / per_item;
-    return cost_before(a, x, items, items) * a.kv_heads;
-}
-template <bool PAGED>
-__device__ uint64_t total_cost(const Args& a) {  // by a whole warp
-    uint64_t total = 0;
+__device__ __forceinline__ Start find_share(const Args& a) {
+    const uint32_t lane = threadIdx.x & 31u, step = item_tokens(a);
+    Start st;
+    st.shares.total = 0;
+    Request mine = {};
+    uint64_t cost = 0;
+    auto load = [&](uint32_t r0) {
+        cost = 0;
+        if (r0 + lane < a.requests) {
+            mine = request<PAGED>(a, r0 + lane);
+            const uint32_t items = (mine.n + step - 1u) / step;
+            cost = cost_before(a, mine, items, items, step) * a.kv_heads;
+        }
+    };
     for (uint32_t r0 = 0; r0 < a.requests; r0 += 32u) {
-        uint64_t w = r0 + (threadIdx.x & 31u) < a.requests ? request_cost<PAGED>(a, r0 + (threadIdx.x & 31u)) : 0u;
+        load(r0);
+        uint64_t sum = cost;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xFFFFFFFFu, w, o);
-        total += w;
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+        st.shares.total += sum;
     }
-    return total;
-}
-// The item that holds `unit` < total; by a whole warp.
-template <bool PAGED>
-__device__ Item item_at(const Args& a, uint64_t unit) {
-    const uint32_t lane = threadIdx.x & 31u, per_item = item_tokens(a);
+    st.shares.count = (uint32_t)min((uint64_t)gridDim.x, max(st.shares.total / LEAST_SHARE, (uint64_t)1));
+    st.begin = st.end = 0;
+    st.it = Item{};
+    if (blockIdx.x >= st.shares.count || st.shares.total == 0) return st;
+    st.begin = st.shares.begin(blockIdx.x), st.end = st.shares.begin(blockIdx.x + 1u);
     uint64_t before = 0;
-    uint32_t found = 0;
     for (uint32_t r0 = 0; r0 < a.requests; r0 += 32u) {
-        const uint64_t w = r0 + lane < a.requests ? request_cost<PAGED>(a, r0 + lane) : 0u;
-        uint64_t sum = w;
+        if (a.requests > 32u) load(r0);
+        uint64_t sum = cost;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const uint64_t y = __shfl_up_sync(0xFFFFFFFFu, sum, o);
             if (lane >= (uint32_t)o) sum += y;
         }
-        const uint32_t past = __ballot_sync(0xFFFFFFFFu, before + sum > unit);
+        const uint32_t past = __ballot_sync(0xFFFFFFFFu, before + sum > st.begin);
         if (past) {
             const uint32_t l = __ffs(past) - 1u;
-            before += __shfl_sync(0xFFFFFFFFu, sum - w, l);
-            found = r0 + l;
+            before += __shfl_sync(0xFFFFFFFFu, sum - cost, l);
+            st.it.r = r0 + l;
+            st.it.x.q0 = __shfl_sync(0xFFFFFFFFu, mine.q0, l), st.it.x.n = __shfl_sync(0xFFFFFFFFu, mine.n, l);
+            st.it.x.k0 = __shfl_sync(0xFFFFFFFFu, mine.k0, l), st.it.x.len = __shfl_sync(0xFFFFFFFFu, mine.len, l);
             break;
         }
         before += __shfl_sync(0xFFFFFFFFu, sum, 31);
     }
-    Item it;
-    it.enter(a, found, per_item, PAGED);
-    const uint64_t per_head = cost_before(a, it.x, it.items, it.items);
-    it.head = (uint32_t)((unit - before) / per_head);
+    Item& it = st.it;
+    it.items = (it.x.n + step - 1u) / step;
+    const uint64_t per_head = cost_before(a, it.x, it.items, it.items, step);
+    it.head = (uint32_t)((st.begin - before) / per_head);
     it.start = before + it.head * per_head;
-    const uint64_t in = unit - it.start;
+    const uint64_t in = st.begin - it.start;
     uint32_t lo = 0, width = it.items;  // the item is in [lo, lo + width)
     while (width > 1u) {
-        const uint32_t step = (width + 31u) / 32u, t = lo + lane * step;
-        const uint32_t below = __ballot_sync(0xFFFFFFFFu, lane * step < width && cost_before(a, it.x, t, it.items) <= in);
+        const uint32_t stride = (width + 31u) / 32u;
+        const uint32_t below = __ballot_sync(0xFFFFFFFFu, lane * stride < width && cost_before(a, it.x, lo + lane * stride, it.items, step) <= in);
         const uint32_t l = 31u - __clz(below);  // lane 0 always is
-        lo += l * step;
-        width = min(step, width - l * step);
+        lo += l * stride;
+        width = min(stride, width - l * stride);
     }
     it.t = lo;
-    it.start += cost_before(a, it.x, lo, it.items);
-    it.tiles = tiles_of(a, it.x, lo);
-    return it;
+    it.start += cost_before(a, it.x, lo, it.items, step);
+    it.measure(a, step);
+    return st;
 }
 // What of an item's key tiles falls into the share [begin, end).  Without a workspace items stay whole.
 struct Span {
     uint32_t k0, k1;
     bool whole;
 };
+__device__ __forceinline__ uint32_t tiles_below(const Item& it, uint64_t unit) {
+    return unit <= it.mark() ? 0u : (uint32_t)min((unit - it.mark() + KEYS - 1u) / KEYS, (uint64_t)it.tiles);
+}
 __device__ __forceinline__ Span span_of(const Item& it, uint64_t begin, uint64_t end, bool split) {
-    const uint64_t first = it.start + ITEM_COST;
     Span s;
-    s.k0 = begin > first ? (uint32_t)min(begin - first, (uint64_t)it.tiles) : 0u;
-    s.k1 = end > first ? (uint32_t)min(end - first, (uint64_t)it.tiles) : 0u;
+    s.k0 = tiles_below(it, begin);
+    s.k1 = tiles_below(it, end);
     if (!split && s.k1 > s.k0) {
         if (s.k0 > 0u) s.k1 = s.k0;
         else s.k1 = it.tiles;
@@ -222,14 +235,20 @@ __device__ __forceinline__ void tmem_load32(uint32_t at, float* r) {
         : "r"(at)
         : "memory");
 }
-__device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t* r) {
+__device__ __forceinline__ void tmem_load16(uint32_t at, float* r) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(at),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
-        "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
-        "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]), "=f"(r[9]), "=f"(r[10]),
+          "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
+        : "r"(at)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(at), "r"(r[0]),
+        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
+        "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
 __device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -245,6 +264,49 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
         "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map),
         "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
         : "memory");
+}
+
+// ---- two fp32 numbers at a time, and 2^x without the special-function unit -------------------
+
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {  // NaN if any of them is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// 2^x for x <= 8: n = x rounded to a whole number (adding 1.5 * 2^23 leaves it in the low bits), 2^(x - n) by a polynomial on
+// [-0.5, 0.5], n added to the exponent.  The coefficients minimise the largest relative error (2^-18.4; a linear program
+// over 4001 points) with the constant term held at 1, so that x <= -127 gives exactly 0: 1.0's bits less 127 exponents.
+__device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
+    float lo, hi;
+    unpair(x, lo, hi);
+    x = pair(fmaxf(lo, -127.0f), fmaxf(hi, -127.0f));
+    const uint64_t t = add2(x, pair(12582912.0f, 12582912.0f));
+    const uint64_t n = add2(t, pair(-12582912.0f, -12582912.0f));
+    const uint64_t f = fma2(n, pair(-1.0f, -1.0f), x);
+    uint64_t p = fma2(f, pair(0x1.3a1804p-7f, 0x1.3a1804p-7f), pair(0x1.c9fcb2p-5f, 0x1.c9fcb2p-5f));
+    p = fma2(p, f, pair(0x1.ec0326p-3f, 0x1.ec0326p-3f));
+    p = fma2(p, f, pair(0x1.62e12cp-1f, 0x1.62e12cp-1f));
+    p = fma2(p, f, pair(1.0f, 1.0f));
+    float tl, th;
+    unpair(t, tl, th);
+    unpair(p, lo, hi);
+    return pair(__uint_as_float(__float_as_uint(lo) + (__float_as_uint(tl) << 23)), __uint_as_float(__float_as_uint(hi) + (__float_as_uint(th) << 23)));
 }
 
 // ---- the kernel ------------------------------------------------------------------------------
@@ -298,16 +360,10 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     pdl_wait_prior();
 
     const uint32_t group = a.group, per_tile = ROW_TILE / group, per_item = 2u * per_tile;
-    const uint64_t total = total_cost<PAGED>(a);
-    const uint32_t shares = shares_of(total, gridDim.x);
     const bool split = a.parts != nullptr;
-    uint64_t begin = 0, end = 0;
-    Item it;
-    it.start = 0;
-    if (blockIdx.x < shares) {
-        begin = share_begin(total, blockIdx.x, shares), end = share_begin(total, blockIdx.x + 1u, shares);
-        it = item_at<PAGED>(a, begin);
-    }
+    Start start = find_share<PAGED>(a);
+    Item& it = start.it;
+    const uint64_t begin = start.begin, end = start.end;
     auto has_second = [&]() { return it.x.n > it.t * per_item + per_tile; };
     // first key tile of the item that some row does not see to its end
     auto first_edge = [&](uint32_t row_tile) { return seen(a, it.x, it.t * per_item + row_tile * per_tile) / KEYS; };
@@ -370,7 +426,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                         }
                     }
                 }
-                it.next(a, per_item, PAGED, end);
+                it.next<PAGED>(a, per_item, end);
             }
         } else if (warp == 9) {
             // ---- products
@@ -443,7 +499,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                             }
                         }
                     }
-                    it.next(a, per_item, PAGED, end);
+                    it.next<PAGED>(a, per_item, end);
                 }
             }
         } else {
@@ -462,34 +518,41 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                         ok = __all_sync(0xFFFFFFFFu, ok);
                         if (!ok) break;
                         const uint32_t there = it.x.len > k * KEYS ? min(it.x.len - k * KEYS, (uint32_t)KEYS) : 0u;
-                        bool changed = false, bad = false;
-                        // 16-byte pieces; rows of 128 bytes, so the swizzle does not matter
-#pragma unroll 4
-                        for (uint32_t e = lane; e < 64u * 8u * C::HALVES; e += 32u) {
-                            const uint32_t row = 64u * (warp - 10u) + (e / 8u) % 64u;
-                            const uint32_t at = ring + s * C::TILE_BYTES + (e / 512u) * C::BLOCK + row * 128u + (e % 8u) * 16u;
-                            uint32_t w[4], z[4];
-                            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
-                            bool differs = false;
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                z[i] = row < there ? finite_or_zero(w[i]) : 0u;
-                                differs |= z[i] != w[i];
-                            }
-                            bad |= differs && row < there;
-                            if (differs) {
-                                changed = true;
-                                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(z[0]), "r"(z[1]), "r"(z[2]), "r"(z[3]) : "memory");
-                            }
+                        // 16-byte pieces; rows are 128 bytes, so the swizzle does not matter.  A number is not finite where its
+                        // exponent bits are all set: first the largest exponents, and a second look only where one is
+                        const uint32_t row0 = 64u * (warp - 10u), rows = there > row0 ? min(there - row0, 64u) : 0u;
+                        auto piece = [&](uint32_t e) { return ring + s * C::TILE_BYTES + (e / 512u) * C::BLOCK + (row0 + e / 8u % 64u) * 128u + e % 8u * 16u; };
+                        uint32_t most = 0u;
+#pragma unroll 8
+                        for (uint32_t e = lane; e < 512u * C::HALVES; e += 32u) {
+                            uint32_t w[4];
+                            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(piece(e)) : "memory");
+                            const uint32_t top = __vmaxu2(__vmaxu2(w[0] & 0x7F807F80u, w[1] & 0x7F807F80u), __vmaxu2(w[2] & 0x7F807F80u, w[3] & 0x7F807F80u));
+                            if (e / 8u % 64u < rows) most = __vmaxu2(most, top);
                         }
-                        if (bad) dirty_item[n_item & 7u] = n_item + 1u;
-                        if (__any_sync(0xFFFFFFFFu, changed)) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        const bool bad = __any_sync(0xFFFFFFFFu, (most & 0xFFFFu) == 0x7F80u || most >> 16 == 0x7F80u);
+                        const bool changed = bad || rows < 64u;
+                        if (changed) {
+#pragma unroll 1
+                            for (uint32_t e = lane + (bad ? 0u : rows * 8u); e < 512u * C::HALVES; e += 32u) {
+                                uint32_t w[4] = {};
+                                if (e / 8u % 64u < rows) {
+                                    if (!bad) continue;
+                                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(piece(e)) : "memory");
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i) w[i] = finite_or_zero(w[i]);
+                                }
+                                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(piece(e)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+                            }
+                            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        }
+                        if (bad && lane == 0) dirty_item[n_item & 7u] = n_item + 1u;
                         __syncwarp();
                         if (lane == 0) mbar_arrive(checked(s));
                     }
                     ++n_item;
                 }
-                it.next(a, per_item, PAGED, end);
+                it.next<PAGED>(a, per_item, end);
             }
         }
     } else {
@@ -500,6 +563,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         const uint32_t s_at = tmem + lanes + t * KEYS, o_at = tmem + lanes + 2u * KEYS + t * D;
         const bool wide = (reinterpret_cast<uintptr_t>(a.out) & 31u) == 0u && a.o_token % 16 == 0 && a.o_head % 16 == 0;
         uint32_t n_s = 0, n_item = 0;
+        uint4 to_join = make_uint4(0u, 0u, 0u, 0u);
         bool ok = true;
         while (ok && it.start < end) {
             const Span span = span_of(it, begin, end, split);
@@ -526,16 +590,19 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
 #pragma unroll
                             for (uint32_t j = 0; j < KEYS; ++j) s[j] = j < count ? s[j] : -INFINITY;
                         }
-                        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                        float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                        for (int j = 0; j < KEYS; ++j) top[j & 3] = fmaxf(top[j & 3], s[j]);
-                        float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
+                        for (int j = 4; j + 8 <= KEYS; j += 8) {
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) top[c] = max3_nan(top[c], s[j + c], s[j + 4 + c]);
+                        }
+                        float now = max3_nan(max3_nan(top[0], top[1], top[2]), max3_nan(top[3], s[KEYS - 4], s[KEYS - 3]), max3_nan(s[KEYS - 2], s[KEYS - 1], top[0])) * a.scale_log2;
+                        if (now == INFINITY) now = NAN;  // inf - inf, for the whole row
                         if (k == span.k0) {
                             m = now;
-                        } else if (__any_sync(0xFFFFFFFFu, now > m + 8.0f)) {
-                            now = fmaxf(now, m);
-                            const float from = now == -INFINITY ? 0.0f : now;
-                            const float keep = exp2_fast(m - from);
+                        } else if (__any_sync(0xFFFFFFFFu, !(now <= m + 8.0f))) {
+                            now = max3_nan(now, m, m);
+                            const float keep = now == -INFINITY ? 1.0f : exp2_fast(m - now);
                             m = now;
                             l *= keep;
                             ok = mbar_wait(o_full(t), (n_s - 1u) & 1u, &abort_flag, 11);
@@ -543,34 +610,47 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                             if (!ok) break;
                             fence_after();
 #pragma unroll 1
-                            for (uint32_t c = 0; c < D; c += 32u) {
-                                float o[32];
-                                tmem_load32(o_at + c, o);
+                            for (uint32_t c = 0; c < D; c += 16u) {
+                                float o[16];
+                                tmem_load16(o_at + c, o);
                                 tmem_wait_load();
 #pragma unroll
-                                for (int j = 0; j < 32; ++j) o[j] *= keep;
-                                tmem_store32(o_at + c, reinterpret_cast<const uint32_t*>(o));
+                                for (int j = 0; j < 16; ++j) o[j] *= keep;
+                                tmem_store16(o_at + c, reinterpret_cast<const uint32_t*>(o));
                             }
                             tmem_wait_store();
                         }
-                        const float from = m == -INFINITY ? 0.0f : m;
-                        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        const float from = m == -INFINITY ? 0.0f : -m;
+                        const uint64_t scale2 = pair(a.scale_log2, a.scale_log2), from2 = pair(from, from);
 #pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            uint32_t p[32];
+                        for (int c = 0; c < KEYS; c += 32) {
+                            uint32_t p[16];
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) {
-                                const float x = exp2_fast(fmaf(s[64 * c + 2 * j], a.scale_log2, -from)), y = exp2_fast(fmaf(s[64 * c + 2 * j + 1], a.scale_log2, -from));
-                                sum[j & 3] += x + y;
+                            for (int j = 0; j < 16; ++j) {
+                                float &x = s[c + 2 * j], &y = s[c + 2 * j + 1];
+                                uint64_t e = fma2(pair(x, y), scale2, from2);
+                                if (j % PAIRS_OF < PAIRS_COMPUTED) {
+                                    unpair(exp2_pair(e), x, y);
+                                } else {
+                                    unpair(e, x, y);
+                                    x = exp2_fast(x), y = exp2_fast(y);
+                                }
                                 p[j] = pack_bf16(x, y);
                             }
-                            tmem_store32(s_at + 32u * c, p);
+                            tmem_store16(s_at + c / 2, p);
                         }
-                        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                         tmem_wait_store();
                         fence_before();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(p_full(t));
+                        uint64_t sum[4];  // while the product runs
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) sum[j] = pair(s[2 * j], s[2 * j + 1]);
+#pragma unroll
+                        for (int j = 4; j < KEYS / 2; ++j) sum[j & 3] = add2(sum[j & 3], pair(s[2 * j], s[2 * j + 1]));
+                        float sl, sh;
+                        unpair(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), sl, sh);
+                        l += sl + sh;
                     }
                     if (!ok) break;
                     ok = mbar_wait(o_full(t), (n_s - 1u) & 1u, &abort_flag, 12);
@@ -583,7 +663,8 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                     uint16_t* const to = a.out + (int64_t)(it.x.q0 + (there ? i : 0u)) * a.o_token + (int64_t)(it.head * group + row % group) * a.o_head;
                     float* part = nullptr;
                     if (!span.whole) {
-                        const uint32_t first = share_of(total, it.start + ITEM_COST, shares);
+                        const uint32_t first = start.shares.of(it.mark());
+                        if (first == blockIdx.x) to_join = make_uint4(start.shares.of(it.last_mark()) - first + 1u, it.x.q0 + it.t * per_item, it.x.n - it.t * per_item, it.head);
                         part = a.parts + (size_t)(2u * blockIdx.x + (first == blockIdx.x ? 1u : 0u)) * C::PART_FLOATS;
                         part[2u * ROW_TILE * D + t * ROW_TILE + row] = m;
                         part[2u * ROW_TILE * (D + 1) + t * ROW_TILE + row] = l;
@@ -639,8 +720,9 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                     if (lane == 0) mbar_arrive(o_free(t));
                 }
             }
-            it.next(a, per_item, PAGED, end);
+            it.next<PAGED>(a, per_item, end);
         }
+        if (split && threadIdx.x == 0) a.joins[blockIdx.x] = to_join;
     }
 
     // on abort give copies and MMAs in flight time to land before TMEM is freed
@@ -658,27 +740,22 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
 }
 
 // Parts of items that more than one CTA worked on, added up in the order of their keys.  CTA (k, y): rows [64 y, 64 y + 64) of the
-// item that CTA k of the kernel above began and did not end, if there is one.
+// item that CTA k of the kernel above began and did not end, if there is one (joins[k]: CTAs, first token, tokens left, key head).
 constexpr int JOIN_THREADS = 512, JOIN_ROWS = 64;
-template <int D, bool PAGED>
-__global__ void __launch_bounds__(JOIN_THREADS) attention_join_kernel(const Args a, uint32_t ctas) {
+template <int D>
+__global__ void __launch_bounds__(JOIN_THREADS) attention_join_kernel(const Args a) {
     using C = PromptCfg<D>;
     pdl_launch_dependents();
     pdl_wait_prior();
-    const uint64_t total = total_cost<PAGED>(a);
-    const uint32_t k = blockIdx.x, shares = shares_of(total, ctas);
-    if (k >= shares) return;
-    const uint64_t end = share_begin(total, k + 1u, shares);
-    const Item it = item_at<PAGED>(a, end - 1u);
-    const uint64_t stop = it.start + ITEM_COST + it.tiles;
-    const uint32_t first = share_of(total, it.start + ITEM_COST, shares), last = share_of(total, stop - 1u, shares);
-    if (first != k || last == k) return;
-    const uint32_t group = a.group, per_tile = ROW_TILE / group, per_item = 2u * per_tile;
+    const uint4 join = ld_fresh(a.joins + blockIdx.x);
+    if (join.x == 0u) return;
+    const uint32_t first = blockIdx.x, last = first + join.x - 1u;
+    const uint32_t group = a.group, per_tile = ROW_TILE / group;
     auto part = [&](uint32_t c) { return a.parts + (size_t)(2u * c + (c == first ? 1u : 0u)) * C::PART_FLOATS; };
     for (uint32_t e = threadIdx.x; e < JOIN_ROWS * (D / 8u); e += JOIN_THREADS) {
         const uint32_t row = JOIN_ROWS * blockIdx.y + e % JOIN_ROWS, c8 = e / JOIN_ROWS;
-        const uint32_t in_tile = row % ROW_TILE, i = it.t * per_item + (row / ROW_TILE) * per_tile + in_tile / group;
-        if (in_tile >= per_tile * group || i >= it.x.n) continue;
+        const uint32_t in_tile = row % ROW_TILE, i = (row / ROW_TILE) * per_tile + in_tile / group;
+        if (in_tile >= per_tile * group || i >= join.z) continue;
         float m = -INFINITY;
         for (uint32_t c = first; c <= last; ++c) m = fmaxf(m, ld_fresh(part(c) + 2u * ROW_TILE * D + row));
         const float from = m == -INFINITY ? 0.0f : m;
@@ -695,7 +772,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) attention_join_kernel(const Args
             }
         }
         const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
-        uint16_t* to = a.out + (int64_t)(it.x.q0 + i) * a.o_token + (int64_t)(it.head * group + in_tile % group) * a.o_head + 8u * c8;
+        uint16_t* to = a.out + (int64_t)(join.y + i) * a.o_token + (int64_t)(join.w * group + in_tile % group) * a.o_head + 8u * c8;
         *reinterpret_cast<uint4*>(to) = make_uint4(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv), pack_bf16(o[4] * inv, o[5] * inv),
                                                    pack_bf16(o[6] * inv, o[7] * inv));
     }
