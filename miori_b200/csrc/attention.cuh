@@ -83,11 +83,38 @@ __device__ __forceinline__ uint32_t seen(const Args& a, const Request& x, uint32
     return s <= 0 ? 0u : min((uint32_t)s, x.len);
 }
 
-// Number of shares, first unit of share k of G, and the share that holds unit u.  No share is empty: whoever adds parts up
-// counts on every CTA between the first and the last of an item.
-__device__ __forceinline__ uint32_t shares_of(uint64_t total, uint32_t ctas) { return (uint32_t)min((uint64_t)ctas, total); }
-__device__ __forceinline__ uint64_t share_begin(uint64_t total, uint32_t k, uint32_t G) { return total * k / G; }
-__device__ __forceinline__ uint32_t share_of(uint64_t total, uint64_t u, uint32_t G) { return (uint32_t)(((u + 1u) * G - 1u) / total); }
+// `total` units cut into shares of the same length, at least `least` and no more of them than CTAs; the last one may be shorter.
+// None before it is empty: whoever adds parts up counts on every CTA between the first and the last of an item.
+struct Shares {
+    uint64_t total, size;
+    __device__ __forceinline__ Shares(uint64_t total_, uint32_t ctas, uint32_t least) : total(total_) {
+        // both branches, since a division of 64 bits costs a few hundred cycles
+        if (total >> 32) size = (total + ctas - 1u) / ctas;
+        else size = ((uint32_t)total + (uint64_t)ctas - 1u) >> 32 ? (total + ctas - 1u) / ctas : ((uint32_t)total + ctas - 1u) / ctas;
+        size = max(size, (uint64_t)least);
+    }
+    __device__ __forceinline__ uint64_t begin(uint32_t k) const { return min(k * size, total); }
+    __device__ __forceinline__ uint32_t of(uint64_t unit) const { return (uint32_t)(unit / size); }
+};
+// a / b where the result is small: no division of 64 bits.
+__device__ __forceinline__ uint32_t small_quotient(uint64_t a, uint64_t b) {
+    uint32_t q = (uint32_t)__fdividef((float)a, (float)b);  // off by one at most below 2^20
+    while (q > 0u && q * b > a) --q;
+    while ((q + 1u) * b <= a) ++q;
+    return q;
+}
+// Sum over a warp of numbers below 2^51.
+__device__ __forceinline__ uint64_t warp_sum(uint64_t x) {
+    return __reduce_add_sync(0xFFFFFFFFu, (uint32_t)x & 0xFFFFFFu) + ((uint64_t)__reduce_add_sync(0xFFFFFFFFu, (uint32_t)(x >> 24)) << 24);
+}
+__device__ __forceinline__ uint64_t warp_prefix_sum(uint64_t x) {  // inclusive
+#pragma unroll
+    for (uint32_t o = 1; o < 32u; o <<= 1) {
+        const uint64_t y = __shfl_up_sync(0xFFFFFFFFu, x, o);
+        if ((threadIdx.x & 31u) >= o) x += y;
+    }
+    return x;
+}
 
 }  // namespace attention
 }  // namespace miori_b200

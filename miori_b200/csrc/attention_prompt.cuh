@@ -63,19 +63,6 @@ __device__ __forceinline__ uint64_t cost_before(const Args& a, const Request& x,
     return cost + (uint64_t)((int64_t)(full - none) * before) + (((uint64_t)full * (full + 1u) - (uint64_t)none * (none + 1u)) / 2u) * step;
 }
 
-struct Shares {
-    uint64_t total;
-    uint32_t count;
-    __device__ __forceinline__ uint64_t begin(uint32_t k) const {  // the same number wherever it is computed
-        return k == count ? total : (uint64_t)((double)total * (double)k / (double)count);
-    }
-    __device__ __forceinline__ uint32_t of(uint64_t unit) const {
-        uint32_t k = min((uint32_t)((double)unit * (double)count / (double)total), count - 1u);
-        while (begin(k) > unit) --k;
-        while (begin(k + 1u) <= unit) ++k;
-        return k;
-    }
-};
 struct Item {
     Request x;
     uint32_t r, head, t, items, sees, tiles;
@@ -112,39 +99,28 @@ struct Start {
 template <bool PAGED>
 __device__ __forceinline__ Start find_share(const Args& a) {
     const uint32_t lane = threadIdx.x & 31u, step = item_tokens(a);
-    Start st;
-    st.shares.total = 0;
     Request mine = {};
-    uint64_t cost = 0;
-    auto load = [&](uint32_t r0) {
-        cost = 0;
-        if (r0 + lane < a.requests) {
-            mine = request<PAGED>(a, r0 + lane);
-            const uint32_t items = (mine.n + step - 1u) / step;
-            cost = cost_before(a, mine, items, items, step) * a.kv_heads;
-        }
+    auto cost_of = [&](uint32_t r0) -> uint64_t {
+        if (r0 + lane >= a.requests) return 0;
+        mine = request<PAGED>(a, r0 + lane);
+        const uint32_t items = (mine.n + step - 1u) / step;
+        return cost_before(a, mine, items, items, step) * a.kv_heads;
     };
+    uint64_t total = 0, cost = 0;
     for (uint32_t r0 = 0; r0 < a.requests; r0 += 32u) {
-        load(r0);
-        uint64_t sum = cost;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-        st.shares.total += sum;
+        cost = cost_of(r0);
+        total += warp_sum(cost);
     }
-    st.shares.count = (uint32_t)min((uint64_t)gridDim.x, max(st.shares.total / LEAST_SHARE, (uint64_t)1));
-    st.begin = st.end = 0;
-    st.it = Item{};
-    if (blockIdx.x >= st.shares.count || st.shares.total == 0) return st;
+    Start st = {Shares(total, gridDim.x, LEAST_SHARE), 0, 0, {}};
     st.begin = st.shares.begin(blockIdx.x), st.end = st.shares.begin(blockIdx.x + 1u);
+    if (st.begin == st.end) {
+        st.it.start = st.end;  // no item before the end
+        return st;
+    }
     uint64_t before = 0;
     for (uint32_t r0 = 0; r0 < a.requests; r0 += 32u) {
-        if (a.requests > 32u) load(r0);
-        uint64_t sum = cost;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint64_t y = __shfl_up_sync(0xFFFFFFFFu, sum, o);
-            if (lane >= (uint32_t)o) sum += y;
-        }
+        if (a.requests > 32u) cost = cost_of(r0);
+        const uint64_t sum = warp_prefix_sum(cost);
         const uint32_t past = __ballot_sync(0xFFFFFFFFu, before + sum > st.begin);
         if (past) {
             const uint32_t l = __ffs(past) - 1u;
@@ -159,7 +135,7 @@ __device__ __forceinline__ Start find_share(const Args& a) {
     Item& it = st.it;
     it.items = (it.x.n + step - 1u) / step;
     const uint64_t per_head = cost_before(a, it.x, it.items, it.items, step);
-    it.head = (uint32_t)((st.begin - before) / per_head);
+    it.head = small_quotient(st.begin - before, per_head);
     it.start = before + it.head * per_head;
     const uint64_t in = st.begin - it.start;
     uint32_t lo = 0, width = it.items;  // the item is in [lo, lo + width)
@@ -446,10 +422,12 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                         if (!(ok = mbar_wait(q_full, n_item & 1u, &abort_flag, 3))) break;
                         ++n_item;
                         auto scores = [&](uint32_t t, uint32_t s) {
+                            const uint64_t rows = smem_desc(q_at + t * C::TILE_BYTES, 16u), keys = smem_desc(ring + s * C::TILE_BYTES, 16u);
 #pragma unroll
-                            for (uint32_t k = 0; k < D / 16u; ++k)
-                                mma_ss(tmem + t * KEYS, smem_desc(q_at + t * C::TILE_BYTES + (k / 4u) * C::BLOCK + (k % 4u) * 32u, 16u),
-                                       smem_desc(ring + s * C::TILE_BYTES + (k / 4u) * C::BLOCK + (k % 4u) * 32u, 16u), idesc_s, k > 0u);
+                            for (uint32_t k = 0; k < D / 16u; ++k) {  // 16 dimensions, 32 bytes further in the 128-byte rows
+                                const uint32_t at = (k / 4u) * (C::BLOCK / 16u) + (k % 4u) * 2u;
+                                mma_ss(tmem + t * KEYS, rows + at, keys + at, idesc_s, k > 0u);
+                            }
                             mma_commit(s_full(t));
                         };
                         {
@@ -470,6 +448,8 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                             }
                             if (!ok) break;
                             const bool more = k + 1u < span.k1;
+                            // groups of 16 keys that some row sees: one at least, which then begins O
+                            const uint32_t steps = it.sees > k * KEYS ? (min(it.sees - k * KEYS, (uint32_t)KEYS) + 15u) / 16u : 1u;
                             for (uint32_t t = 0; t < tiles; ++t) {
                                 if (k == span.k0) {  // the last item's O has been read
                                     if (!(ok = mbar_wait(o_free(t), (n_o[t] & 1u) ^ 1u, &abort_flag, 7))) break;
@@ -478,10 +458,17 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                                 if (!(ok = mbar_wait(p_full(t), n_p[t] & 1u, &abort_flag, 8))) break;
                                 ++n_p[t];
                                 fence_after();
+                                const uint64_t values = smem_desc(ring + vs * C::TILE_BYTES, C::BLOCK);
+                                auto add = [&](uint32_t i) {  // 16 keys, 2048 bytes further
+                                    mma_ts(tmem + 2u * KEYS + t * D, tmem + t * KEYS + 8u * i, values + 128u * i, idesc_o, k > span.k0 || i > 0u);
+                                };
+                                if (steps == KEYS / 16u) {
 #pragma unroll
-                                for (uint32_t i = 0; i < KEYS / 16u; ++i)
-                                    mma_ts(tmem + 2u * KEYS + t * D, tmem + t * KEYS + 8u * i, smem_desc(ring + vs * C::TILE_BYTES + i * 2048u, C::BLOCK), idesc_o,
-                                           k > span.k0 || i > 0u);
+                                    for (uint32_t i = 0; i < KEYS / 16u; ++i) add(i);
+                                } else {
+#pragma unroll 1
+                                    for (uint32_t i = 0; i < steps; ++i) add(i);
+                                }
                                 mma_commit(o_full(t));
                                 if (more) {
                                     if (t == 0u) {
@@ -531,21 +518,27 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                             if (e / 8u % 64u < rows) most = __vmaxu2(most, top);
                         }
                         const bool bad = __any_sync(0xFFFFFFFFu, (most & 0xFFFFu) == 0x7F80u || most >> 16 == 0x7F80u);
-                        const bool changed = bad || rows < 64u;
-                        if (changed) {
+                        // past the end: up to the next multiple of 16 keys, where the product stops
+                        const uint32_t stop = there == 0u && warp == 10u ? 16u : min((rows + 15u) & ~15u, 64u);
+                        if (rows < stop) {
+                            for (uint32_t e = rows * 8u + lane; e < stop * 8u; e += 32u)
+#pragma unroll
+                                for (uint32_t h = 0; h < (uint32_t)C::HALVES; ++h)
+                                    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(piece(e + 512u * h)), "r"(0u) : "memory");
+                        }
+                        if (bad) {
 #pragma unroll 1
-                            for (uint32_t e = lane + (bad ? 0u : rows * 8u); e < 512u * C::HALVES; e += 32u) {
+                            for (uint32_t e = lane; e < 512u * C::HALVES; e += 32u) {
                                 uint32_t w[4] = {};
                                 if (e / 8u % 64u < rows) {
-                                    if (!bad) continue;
                                     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(piece(e)) : "memory");
 #pragma unroll
                                     for (int i = 0; i < 4; ++i) w[i] = finite_or_zero(w[i]);
                                 }
                                 asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(piece(e)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
                             }
-                            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                         }
+                        if (bad || rows < stop) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                         if (bad && lane == 0) dirty_item[n_item & 7u] = n_item + 1u;
                         __syncwarp();
                         if (lane == 0) mbar_arrive(checked(s));

@@ -436,6 +436,13 @@ void need_heads(const at::Tensor& t, const char* what, int64_t dims) {
 // A stride, or where there is only one step to take any that passes the library's checks.
 int64_t step(const at::Tensor& t, int64_t d) { return t.size(d) == 1 ? t.size(t.dim() - 1) : t.stride(d); }
 
+// A contiguous piece of `whole` as a tensor of its own (several small outputs of one allocation: each of its own costs a microsecond).
+at::Tensor piece(const at::Tensor& whole, int64_t offset, int64_t numel) {
+    at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(), whole.dtype());
+    t.unsafeGetTensorImpl()->set_storage_offset(offset);
+    t.unsafeGetTensorImpl()->set_sizes_contiguous({numel});
+    return t;
+}
 PyObject* tuple_of(std::initializer_list<at::Tensor*> ts) {
     PyObject* all = PyTuple_New((Py_ssize_t)ts.size());
     if (!all) throw Failed();
@@ -451,8 +458,11 @@ OP(page_slots, 7, "held", "new", "table", "pool", "taken", "page", "tokens", "fl
                   *kp = ints(taken, "taken", 1);
     if (table.dim() != 2 || table.size(0) != R) raise(PyExc_ValueError, "table: [%lld][width] expected", (long long)R);
     const uint32_t page = a.u32(5, 0), T = a.u32(6, 0), flags = a.u32(7, 0);
-    at::Tensor slots = empty({T}, at::kInt, held), positions = empty({T}, at::kInt, held), cu = empty({R + 1}, at::kInt, held),
-               after = empty({R}, at::kInt, held), taken_after = empty({1}, at::kInt, held);
+    auto room = [](int64_t n) { return (n + 3) / 4 * 4; };  // pieces begin on 16-byte boundaries
+    const int64_t at_positions = room(T), at_cu = at_positions + room(T), at_after = at_cu + room(R + 1), at_taken = at_after + room(R);
+    const at::Tensor whole = empty({at_taken + 1}, at::kInt, held);
+    at::Tensor slots = piece(whole, 0, T), positions = piece(whole, at_positions, T), cu = piece(whole, at_cu, R + 1), after = piece(whole, at_after, R),
+               taken_after = piece(whole, at_taken, 1);
     auto out = [](at::Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); };
     call(abi.page_slots, hp, fp, const_cast<int32_t*>(tp), pp, kp, out(slots), out(positions), out(cu), out(after), out(taken_after), R,
          table.size(1), page, pool.numel(), T, flags, stream());
