@@ -285,6 +285,19 @@ __device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
     return pair(__uint_as_float(__float_as_uint(lo) + (__float_as_uint(tl) << 23)), __uint_as_float(__float_as_uint(hi) + (__float_as_uint(th) << 23)));
 }
 
+// A value that all lanes hold, for the compiler to know that they do.
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xFFFFFFFFu, x, 0); }
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0u;
+}
+// mbar_wait by a whole warp, with one answer for it.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile uint32_t* abort, uint32_t where) {
+    if (__all_sync(0xFFFFFFFFu, mbar_try(bar, parity))) return true;
+    return __all_sync(0xFFFFFFFFu, mbar_wait<false>(bar, parity, abort, where));
+}
+
 // ---- the kernel ------------------------------------------------------------------------------
 
 template <int D, bool PAGED>
@@ -405,89 +418,92 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                 it.next<PAGED>(a, per_item, end);
             }
         } else if (warp == 9) {
-            // ---- products
-            if (lane == 0) {
-                constexpr uint32_t idesc_s = mma_desc(KEYS, false), idesc_o = mma_desc(D, true);
-                uint32_t n_tile = 0, n_item = 0, full_turns = 0, check_turns = 0, n_p[2] = {0, 0}, n_o[2] = {0, 0};
-                bool ok = true;
-                auto wait_full = [&](uint32_t s, uint32_t where) {
-                    const bool there = mbar_wait(full(s), full_turns >> s & 1u, &abort_flag, where);
-                    full_turns ^= 1u << s;
-                    return there;
-                };
-                while (ok && it.start < end) {
-                    const Span span = span_of(it, begin, end, split);
-                    if (span.k1 > span.k0) {
-                        const uint32_t tiles = has_second() ? 2u : 1u, edge = first_edge(0);
-                        if (!(ok = mbar_wait(q_full, n_item & 1u, &abort_flag, 3))) break;
-                        ++n_item;
-                        auto scores = [&](uint32_t t, uint32_t s) {
-                            const uint64_t rows = smem_desc(q_at + t * C::TILE_BYTES, 16u), keys = smem_desc(ring + s * C::TILE_BYTES, 16u);
+            // ---- products.  The whole warp walks the loop and one elected thread issues: descriptors and addresses then stay in uniform
+            // registers.  Issued from a branch of one lane an MMA took 88 cycles beside busy softmax warps, so 75 (and 64 without them).
+            constexpr uint32_t idesc_s = mma_desc(KEYS, false), idesc_o = mma_desc(D, true);
+            const uint32_t tm = uniform(tmem);
+            const uint64_t rows = smem_desc(q_at, 16u), keys = smem_desc(ring, 16u), values = smem_desc(ring, C::BLOCK);
+            uint32_t place = 0, full_turns = 0, check_turns = 0, n_item = 0, n_p = 0, n_p1 = 0, n_o = 0, n_o1 = 0;
+            auto wait_full = [&](uint32_t s, uint32_t where) {
+                const bool there = warp_wait(full(s), full_turns >> s & 1u, &abort_flag, where);
+                full_turns ^= 1u << s;
+                return there;
+            };
+            auto scores = [&](uint32_t t, uint32_t s, bool last) {
+                const uint64_t q = rows + t * (C::TILE_BYTES / 16u), at = keys + s * (C::TILE_BYTES / 16u);
+                if (elect_one()) {
 #pragma unroll
-                            for (uint32_t k = 0; k < D / 16u; ++k) {  // 16 dimensions, 32 bytes further in the 128-byte rows
-                                const uint32_t at = (k / 4u) * (C::BLOCK / 16u) + (k % 4u) * 2u;
-                                mma_ss(tmem + t * KEYS, rows + at, keys + at, idesc_s, k > 0u);
-                            }
-                            mma_commit(s_full(t));
-                        };
-                        {
-                            const uint32_t s = n_tile % ST;
-                            if (!(ok = wait_full(s, 4))) break;
-                            fence_after();
-                            for (uint32_t t = 0; t < tiles; ++t) scores(t, s);
-                            mma_commit(empty(s));
-                            if (span.k0 + 1u == span.k1) mma_commit(q_empty);
+                    for (uint32_t k = 0; k < D / 16u; ++k) {  // 16 dimensions, 32 bytes further in the 128-byte rows
+                        const uint32_t step = (k / 4u) * (C::BLOCK / 16u) + (k % 4u) * 2u;
+                        mma_ss(tm + t * KEYS, q + step, at + step, idesc_s, k > 0u);
+                    }
+                    mma_commit(s_full(t));
+                    if (last) mma_commit(empty(s));  // the keys have been read
+                }
+            };
+            while (__all_sync(0xFFFFFFFFu, it.start < end)) {
+                const Span span = span_of(it, begin, end, split);
+                const uint32_t k0 = uniform(span.k0), k1 = uniform(span.k1), sees = uniform(it.sees), edge = uniform(first_edge(0));
+                const bool second = uniform(has_second() ? 1u : 0u) != 0u;
+                if (k1 > k0) {
+                    if (!warp_wait(q_full, n_item & 1u, &abort_flag, 3)) break;
+                    ++n_item;
+                    if (!wait_full(place, 4)) break;
+                    fence_after();
+                    scores(0u, place, !second);
+                    if (second) scores(1u, place, true);
+                    bool ok = true;
+                    for (uint32_t k = k0; k < k1; ++k) {
+                        const uint32_t vs = place + 1u == ST ? 0u : place + 1u, ks = vs + 1u == ST ? 0u : vs + 1u;
+                        const bool more = k + 1u < k1;
+                        if (!more && elect_one()) mma_commit(q_empty);  // the last scores are under way
+                        if (k >= edge) {
+                            ok = warp_wait(checked(vs), check_turns >> vs & 1u, &abort_flag, 6);
+                            check_turns ^= 1u << vs;
+                        } else {
+                            ok = wait_full(vs, 5);
                         }
-                        for (uint32_t k = span.k0; ok && k < span.k1; ++k, n_tile += 2u) {
-                            const uint32_t vs = (n_tile + 1u) % ST, ks = (n_tile + 2u) % ST;
-                            if (k >= edge) {
-                                ok = mbar_wait(checked(vs), check_turns >> vs & 1u, &abort_flag, 6);
-                                check_turns ^= 1u << vs;
-                            } else {
-                                ok = wait_full(vs, 5);
+                        if (!ok) break;
+                        // groups of 16 keys that some row sees: one at least, which then begins O
+                        const uint32_t steps = sees > k * KEYS ? (min(sees - k * KEYS, (uint32_t)KEYS) + 15u) / 16u : 1u;
+                        const uint64_t at = values + vs * (C::TILE_BYTES / 16u);
+                        auto add = [&](uint32_t t, uint32_t& o_turn, uint32_t& p_turn, bool last) {
+                            if (k == k0) {  // the last item's O has been read
+                                if (!warp_wait(o_free(t), (o_turn & 1u) ^ 1u, &abort_flag, 7)) return false;
+                                ++o_turn;
                             }
-                            if (!ok) break;
-                            const bool more = k + 1u < span.k1;
-                            // groups of 16 keys that some row sees: one at least, which then begins O
-                            const uint32_t steps = it.sees > k * KEYS ? (min(it.sees - k * KEYS, (uint32_t)KEYS) + 15u) / 16u : 1u;
-                            for (uint32_t t = 0; t < tiles; ++t) {
-                                if (k == span.k0) {  // the last item's O has been read
-                                    if (!(ok = mbar_wait(o_free(t), (n_o[t] & 1u) ^ 1u, &abort_flag, 7))) break;
-                                    ++n_o[t];
-                                }
-                                if (!(ok = mbar_wait(p_full(t), n_p[t] & 1u, &abort_flag, 8))) break;
-                                ++n_p[t];
-                                fence_after();
-                                const uint64_t values = smem_desc(ring + vs * C::TILE_BYTES, C::BLOCK);
-                                auto add = [&](uint32_t i) {  // 16 keys, 2048 bytes further
-                                    mma_ts(tmem + 2u * KEYS + t * D, tmem + t * KEYS + 8u * i, values + 128u * i, idesc_o, k > span.k0 || i > 0u);
-                                };
+                            if (!warp_wait(p_full(t), p_turn & 1u, &abort_flag, 8)) return false;
+                            ++p_turn;
+                            fence_after();
+                            if (elect_one()) {
+                                const uint32_t o = tm + 2u * KEYS + t * D, p = tm + t * KEYS;
                                 if (steps == KEYS / 16u) {
 #pragma unroll
-                                    for (uint32_t i = 0; i < KEYS / 16u; ++i) add(i);
+                                    for (uint32_t i = 0; i < KEYS / 16u; ++i) mma_ts(o, p + 8u * i, at + 128u * i, idesc_o, k > k0 || i > 0u);  // 16 keys, 2048 bytes further
                                 } else {
 #pragma unroll 1
-                                    for (uint32_t i = 0; i < steps; ++i) add(i);
+                                    for (uint32_t i = 0; i < steps; ++i) mma_ts(o, p + 8u * i, at + 128u * i, idesc_o, k > k0 || i > 0u);
                                 }
                                 mma_commit(o_full(t));
-                                if (more) {
-                                    if (t == 0u) {
-                                        if (!(ok = wait_full(ks, 4))) break;
-                                        fence_after();
-                                    }
-                                    scores(t, ks);
-                                }
+                                if (last) mma_commit(empty(vs));
                             }
-                            if (!ok) break;
-                            mma_commit(empty(vs));
-                            if (more) {
-                                mma_commit(empty(ks));
-                                if (k + 2u == span.k1) mma_commit(q_empty);
-                            }
+                            return true;
+                        };
+                        if (!(ok = add(0u, n_o, n_p, !second))) break;
+                        if (more) {
+                            if (!(ok = wait_full(ks, 4))) break;
+                            fence_after();
+                            scores(0u, ks, !second);
                         }
+                        if (second) {
+                            if (!(ok = add(1u, n_o1, n_p1, true))) break;
+                            if (more) scores(1u, ks, true);
+                        }
+                        place = ks;
                     }
-                    it.next<PAGED>(a, per_item, end);
+                    if (!ok) break;
                 }
+                it.next<PAGED>(a, per_item, end);
             }
         } else {
             // ---- values of edge tiles: half the rows for each of two warps
