@@ -12,6 +12,7 @@
 namespace miori_b200 {
 namespace attention {
 
+constexpr uint32_t DECODE_ROWS = 32;
 constexpr size_t COUNTER_BYTES = 4096, JOIN_BYTES = 12288;  // for up to 768 SMs
 static size_t part_bytes() { return 2u * (size_t)sm_count() * PromptCfg<128>::PART_FLOATS * 4u; }
 
@@ -97,8 +98,9 @@ template <int D>
 static int launch_decode(const Args& a, uint32_t rows, uint32_t flags, cudaStream_t stream) {
     const dim3 grid((uint32_t)sm_count()), block(DECODE_THREADS);
     const bool pdl = (flags & MIORI_LAUNCH_PDL) != 0;
-    const cudaError_t e = rows <= 8u ? launch(attention_decode_kernel<D, 1>, grid, block, DecodeCfg<D, 1>::SMEM, stream, pdl, a)
-                                     : launch(attention_decode_kernel<D, 2>, grid, block, DecodeCfg<D, 2>::SMEM, stream, pdl, a);
+    const cudaError_t e = rows <= 8u    ? launch(attention_decode_kernel<D, 1>, grid, block, DecodeCfg<D, 1>::SMEM, stream, pdl, a)
+                          : rows <= 16u ? launch(attention_decode_kernel<D, 2>, grid, block, DecodeCfg<D, 2>::SMEM, stream, pdl, a)
+                                        : launch(attention_decode_kernel<D, 4>, grid, block, DecodeCfg<D, 4>::SMEM, stream, pdl, a);
     return e == cudaSuccess ? MIORI_OK : cuda_fail(e, "attention_decode launch");
 }
 
@@ -133,7 +135,7 @@ MIORI_API int miori_attention_paged(const void* q, const void* k_cache, const vo
     use_workspace(a, workspace);
     const uint64_t rows = (uint64_t)(max_new ? max_new : 1u) * a.group;
     const cudaStream_t s = (cudaStream_t)stream;
-    if (rows <= 16) return dim == 128 ? launch_decode<128>(a, (uint32_t)rows, flags, s) : launch_decode<64>(a, (uint32_t)rows, flags, s);
+    if (rows <= DECODE_ROWS) return dim == 128 ? launch_decode<128>(a, (uint32_t)rows, flags, s) : launch_decode<64>(a, (uint32_t)rows, flags, s);
     const bool may_split = (uint64_t)width * page > KEYS;
     return dim == 128 ? launch_prompt<128, true>(a, may_split, flags, s) : launch_prompt<64, true>(a, may_split, flags, s);
 }

@@ -3,7 +3,7 @@
 // HBM-bound: every cached key and value is read once, 4 * D bytes a position and key head, for 4 * D * rows operations.  What
 // counts is bytes in flight and an even share for every SM.
 //
-// * An item has up to 8 or 16 rows (NT = 1, 2 columns of eight).  Keys are the MMA's 16 rows and the item's rows its 8 columns:
+// * An item has up to 8, 16 or 32 rows (NT = 1, 2, 4 columns of eight).  Keys are the MMA's 16 rows and the item's rows its 8 columns:
 //   S^T = K Q^T, then O^T = V^T P^T, so that with up to eight rows no half of an MMA is padding.  K is the A operand as it lies
 //   in shared memory (ldmatrix), V through ldmatrix.trans; P^T takes one movmatrix per eight keys and columns.
 // * A warp owns 16 of a unit's 128 keys, with a ring of its own (STAGES tiles of 16 keys and values), its own running maximum, sum
@@ -28,7 +28,7 @@ struct DecodeCfg {
     static constexpr int STAGES = D == 128 ? 3 : 6;
     static constexpr int TILE_BYTES = TILE * D * 2;                       // of keys, or of values
     static constexpr int RING = DECODE_WARPS * STAGES * 2 * TILE_BYTES;
-    static constexpr int MEET = DECODE_WARPS * 8 * (D + 4) * 4;           // eight rows of every warp's O
+    static constexpr int MEET = DECODE_WARPS * 8 * D * 4;                 // eight rows of every warp's O
     static constexpr int SMEM = RING + MEET;
     static constexpr int PART_FLOATS = ROWS * (D + 2);                    // O, then m and l of each row
 };
@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(DECODE_THREADS, 1) attention_decode_kernel(con
     constexpr int KS = D / 16;        // k steps of the first product, 16-row tiles of the second
     constexpr uint32_t CH = D / 8;    // 16-byte pieces of a row
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ float2 meet_ml[DECODE_WARPS][16];
+    __shared__ float2 meet_ml[DECODE_WARPS][C::ROWS];
     __shared__ uint32_t dirty, last_one;
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
     pdl_launch_dependents();
@@ -316,7 +316,8 @@ __global__ void __launch_bounds__(DECODE_THREADS, 1) attention_decode_kernel(con
         const uint32_t first = whole ? blockIdx.x : shares.of(at.mark()), last = whole ? blockIdx.x : shares.of(at.last_mark());
         // two parts a CTA: of the item that its share begins in and of the one that it ends in
         float* const part = a.parts + (size_t)(2u * blockIdx.x + (first == blockIdx.x ? 1u : 0u)) * C::PART_FLOATS;
-        float* const sum_o = reinterpret_cast<float*>(smem + C::RING);  // [warp][8][D + 4]: no two lanes of a store share a bank
+        float* const sum_o = reinterpret_cast<float*>(smem + C::RING);  // [warp][8][D], swizzled so that no two lanes of a store share a bank
+        auto in_row = [](uint32_t row, uint32_t d) { return row * D + (d ^ ((row >> 1 & 3u) << 3)); };
         auto store = [&](uint32_t row, uint32_t d, float4 v, float l_all) {
             const float inv = l_all > 0.0f ? 1.0f / l_all : l_all == 0.0f ? 0.0f : l_all;  // no key: zeros; NaN stays
             const uint32_t i = at.block * per_block + row / group;
@@ -338,14 +339,14 @@ __global__ void __launch_bounds__(DECODE_THREADS, 1) attention_decode_kernel(con
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             if (n > 0) {
-                if (rows <= 8u) break;
+                if (rows <= 8u * n) break;
                 __syncthreads();
             }
 #pragma unroll
             for (int k = 0; k < KS; ++k)
 #pragma unroll
                 for (int j = 0; j < 4; ++j)  // accumulator: row of the MMA = dimension, column = row of the item
-                    sum_o[(warp * 8u + 2u * (lane & 3u) + (j & 1u)) * (D + 4) + 16u * k + lane / 4u + (j >= 2 ? 8u : 0u)] = o[n][k][j];
+                    sum_o[in_row(warp * 8u + 2u * (lane & 3u) + (j & 1u), 16u * k + lane / 4u + (j >= 2 ? 8u : 0u))] = o[n][k][j];
             __syncthreads();
 #pragma unroll 1
             for (uint32_t e = threadIdx.x; e < 8u * D / 4u; e += DECODE_THREADS) {
@@ -360,7 +361,7 @@ __global__ void __launch_bounds__(DECODE_THREADS, 1) attention_decode_kernel(con
                 for (int w = 0; w < DECODE_WARPS; ++w) {
                     const float2 ml = meet_ml[w][row];
                     const float f = exp2_fast(ml.x - from);
-                    const float4 x = *reinterpret_cast<const float4*>(sum_o + (w * 8u + r8) * (D + 4) + d);
+                    const float4 x = *reinterpret_cast<const float4*>(sum_o + in_row(w * 8u + r8, d));
                     sum = fmaf(ml.y, f, sum);
                     v.x = fmaf(x.x, f, v.x), v.y = fmaf(x.y, f, v.y), v.z = fmaf(x.z, f, v.z), v.w = fmaf(x.w, f, v.w);
                 }

@@ -11,6 +11,10 @@
 // * The running maximum moves only when a row's exceeds it by 2^8: until then p grows up to 256, which costs no precision in
 //   fp32 sums and bf16 rounding, and O stays where it is.  O is rescaled by the softmax warps themselves, in TMEM.
 // * P is rounded to bf16 for the second product, as the values are; l sums the unrounded p.
+// * Tried and dropped (432 GFLOP of prompts up to 8192, us): an MMA warp for each row tile (454), the MMAs issued by the softmax warps
+//   (473), scores of 64 keys double-buffered (684 as issued then: twice the steps), the product begun at half of the probabilities
+//   (403 - 430), a quarter or half of the exponentials by a polynomial on the FMA pipe (404, 466).  404 as it is; the MMA
+//   warp's bookkeeping between products is what keeps the tensor cores at about two thirds.
 // * Edge tiles (keys that some rows do not see, or past the end).  Their scores are masked one by one.  Their values are looked
 //   through before the product: rows past the end are zeroed (a page's unwritten tail, the next prompt's rows) and so are
 //   numbers that are not finite, since 0 * inf would reach rows that do not see them; rows that do see them get them added
@@ -36,8 +40,6 @@ struct PromptCfg {
     static constexpr int SMEM = 1024 + (2 + STAGES) * TILE_BYTES;
     static constexpr int PART_FLOATS = 2 * ROW_TILE * (D + 2);  // [D / 4][256] pieces of O, then m and l
 };
-// Of every PAIRS_OF pairs of exponentials so many are computed by exp2_pair, the others by the special-function unit.
-constexpr int PAIRS_COMPUTED = 1, PAIRS_OF = 4;
 constexpr int SETMAXNREG_SOFTMAX = 208, SETMAXNREG_OTHERS = 88;  // (256 * 224 + 128 * 56) = 384 * 168, what a launch has
 static_assert(256 * SETMAXNREG_SOFTMAX + 128 * SETMAXNREG_OTHERS <= PROMPT_THREADS * 168, "a split above the launch's registers waits forever");
 
@@ -242,7 +244,7 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
         : "memory");
 }
 
-// ---- two fp32 numbers at a time, and 2^x without the special-function unit -------------------
+// ---- two fp32 numbers at a time -----------------------------------------------------------
 
 __device__ __forceinline__ uint64_t pair(float lo, float hi) {
     uint64_t r;
@@ -265,26 +267,6 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {  // NaN i
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-// 2^x for x <= 8: n = x rounded to a whole number (adding 1.5 * 2^23 leaves it in the low bits), 2^(x - n) by a polynomial on
-// [-0.5, 0.5], n added to the exponent.  The coefficients minimise the largest relative error (2^-18.4; a linear program
-// over 4001 points) with the constant term held at 1, so that x <= -127 gives exactly 0: 1.0's bits less 127 exponents.
-__device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
-    float lo, hi;
-    unpair(x, lo, hi);
-    x = pair(fmaxf(lo, -127.0f), fmaxf(hi, -127.0f));
-    const uint64_t t = add2(x, pair(12582912.0f, 12582912.0f));
-    const uint64_t n = add2(t, pair(-12582912.0f, -12582912.0f));
-    const uint64_t f = fma2(n, pair(-1.0f, -1.0f), x);
-    uint64_t p = fma2(f, pair(0x1.3a1804p-7f, 0x1.3a1804p-7f), pair(0x1.c9fcb2p-5f, 0x1.c9fcb2p-5f));
-    p = fma2(p, f, pair(0x1.ec0326p-3f, 0x1.ec0326p-3f));
-    p = fma2(p, f, pair(0x1.62e12cp-1f, 0x1.62e12cp-1f));
-    p = fma2(p, f, pair(1.0f, 1.0f));
-    float tl, th;
-    unpair(t, tl, th);
-    unpair(p, lo, hi);
-    return pair(__uint_as_float(__float_as_uint(lo) + (__float_as_uint(tl) << 23)), __uint_as_float(__float_as_uint(hi) + (__float_as_uint(th) << 23)));
-}
-
 // A value that all lanes hold, for the compiler to know that they do.
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xFFFFFFFFu, x, 0); }
 __device__ __forceinline__ bool elect_one() {
@@ -322,7 +304,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     const uint32_t q_full = bar(4 * ST), q_empty = bar(4 * ST + 1);
     auto s_full = [&](uint32_t t) { return bar(4 * ST + 2 + t); };
     auto p_full = [&](uint32_t t) { return bar(4 * ST + 4 + t); };
-    auto o_full = [&](uint32_t t) { return bar(4 * ST + 6 + t); };  // one more product has been added to O
+    auto o_full = [&](uint32_t t) { return bar(4 * ST + 6 + t); };  // the item's O is complete
     auto o_free = [&](uint32_t t) { return bar(4 * ST + 8 + t); };  // the item's O has been read
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
 
@@ -419,7 +401,8 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
             }
         } else if (warp == 9) {
             // ---- products.  The whole warp walks the loop and one elected thread issues: descriptors and addresses then stay in uniform
-            // registers.  Issued from a branch of one lane an MMA took 88 cycles beside busy softmax warps, so 75 (and 64 without them).
+            // registers.  Issued from a branch of one lane an MMA took 88 cycles beside busy softmax warps, so 75 (and 64 without them); without
+            // the __syncwarp behind each issue, lanes that run ahead into the next wait cost 15 % of the whole.
             constexpr uint32_t idesc_s = mma_desc(KEYS, false), idesc_o = mma_desc(D, true);
             const uint32_t tm = uniform(tmem);
             const uint64_t rows = smem_desc(q_at, 16u), keys = smem_desc(ring, 16u), values = smem_desc(ring, C::BLOCK);
@@ -440,6 +423,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                     mma_commit(s_full(t));
                     if (last) mma_commit(empty(s));  // the keys have been read
                 }
+                __syncwarp();
             };
             while (__all_sync(0xFFFFFFFFu, it.start < end)) {
                 const Span span = span_of(it, begin, end, split);
@@ -484,9 +468,10 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
 #pragma unroll 1
                                     for (uint32_t i = 0; i < steps; ++i) mma_ts(o, p + 8u * i, at + 128u * i, idesc_o, k > k0 || i > 0u);
                                 }
-                                mma_commit(o_full(t));
+                                if (k + 1u == k1) mma_commit(o_full(t));
                                 if (last) mma_commit(empty(vs));
                             }
+                            __syncwarp();
                             return true;
                         };
                         if (!(ok = add(0u, n_o, n_p, !second))) break;
@@ -571,7 +556,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         const uint32_t lanes = ((warp & 3u) * 32u) << 16;
         const uint32_t s_at = tmem + lanes + t * KEYS, o_at = tmem + lanes + 2u * KEYS + t * D;
         const bool wide = (reinterpret_cast<uintptr_t>(a.out) & 31u) == 0u && a.o_token % 16 == 0 && a.o_head % 16 == 0;
-        uint32_t n_s = 0, n_item = 0;
+        uint32_t n_s = 0, n_o = 0, n_item = 0;
         uint4 to_join = make_uint4(0u, 0u, 0u, 0u);
         bool ok = true;
         while (ok && it.start < end) {
@@ -585,8 +570,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                     const uint32_t edge = first_edge(t);
                     float m = -INFINITY, l = 0.0f;
                     for (uint32_t k = span.k0; k < span.k1; ++k, ++n_s) {
-                        ok = mbar_wait(s_full(t), n_s & 1u, &abort_flag, 10);
-                        ok = __all_sync(0xFFFFFFFFu, ok);
+                        ok = warp_wait(s_full(t), n_s & 1u, &abort_flag, 10);
                         if (!ok) break;
                         fence_after();
                         float s[KEYS];
@@ -614,10 +598,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                             const float keep = now == -INFINITY ? 1.0f : exp2_fast(m - now);
                             m = now;
                             l *= keep;
-                            ok = mbar_wait(o_full(t), (n_s - 1u) & 1u, &abort_flag, 11);
-                            ok = __all_sync(0xFFFFFFFFu, ok);
-                            if (!ok) break;
-                            fence_after();
+                            // O stands still: the product before was issued in front of these scores, and they are complete
 #pragma unroll 1
                             for (uint32_t c = 0; c < D; c += 16u) {
                                 float o[16];
@@ -638,12 +619,8 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                             for (int j = 0; j < 16; ++j) {
                                 float &x = s[c + 2 * j], &y = s[c + 2 * j + 1];
                                 uint64_t e = fma2(pair(x, y), scale2, from2);
-                                if (j % PAIRS_OF < PAIRS_COMPUTED) {
-                                    unpair(exp2_pair(e), x, y);
-                                } else {
-                                    unpair(e, x, y);
-                                    x = exp2_fast(x), y = exp2_fast(y);
-                                }
+                                unpair(e, x, y);
+                                x = exp2_fast(x), y = exp2_fast(y);
                                 p[j] = pack_bf16(x, y);
                             }
                             tmem_store16(s_at + c / 2, p);
@@ -662,8 +639,8 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                         l += sl + sh;
                     }
                     if (!ok) break;
-                    ok = mbar_wait(o_full(t), (n_s - 1u) & 1u, &abort_flag, 12);
-                    ok = __all_sync(0xFFFFFFFFu, ok);
+                    ok = warp_wait(o_full(t), n_o & 1u, &abort_flag, 12);
+                    ++n_o;
                     if (!ok) break;
                     fence_after();
                     const bool dirty = *(volatile uint32_t*)&dirty_item[item_id & 7u] == item_id + 1u;

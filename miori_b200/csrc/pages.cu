@@ -163,15 +163,23 @@ __device__ __forceinline__ void unpack8(const uint4& w, float (&x)[8]) {
     x[0] = bf16lo(w.x), x[1] = bf16hi(w.x), x[2] = bf16lo(w.y), x[3] = bf16hi(w.y);
     x[4] = bf16lo(w.z), x[5] = bf16hi(w.z), x[6] = bf16lo(w.w), x[7] = bf16hi(w.w);
 }
+// Eight elements as they lie in memory.
 template <bool FP32>
-__device__ __forceinline__ void load8(const void* p, int64_t at, float (&x)[8]) {
-    if constexpr (FP32) {
-        const float4 lo = ld_fresh<float4, true>(static_cast<const float4*>(p) + at / 4), hi = ld_fresh<float4, true>(static_cast<const float4*>(p) + at / 4 + 1);
-        x[0] = lo.x, x[1] = lo.y, x[2] = lo.z, x[3] = lo.w, x[4] = hi.x, x[5] = hi.y, x[6] = hi.z, x[7] = hi.w;
-    } else {
-        unpack8(ld_fresh<uint4, true>(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + at)), x);
+struct Raw8 {
+    uint4 w[FP32 ? 2 : 1];
+    __device__ __forceinline__ void load(const void* p, int64_t at) {
+        const uint4* from = reinterpret_cast<const uint4*>(static_cast<const char*>(p) + at * (FP32 ? 4 : 2));
+#pragma unroll
+        for (int i = 0; i < (FP32 ? 2 : 1); ++i) w[i] = ld_fresh<uint4, true>(from + i);
     }
-}
+    __device__ __forceinline__ void get(float (&x)[8]) const {
+        if constexpr (FP32) {
+            memcpy(x, w, sizeof(x));
+        } else {
+            unpack8(w[0], x);
+        }
+    }
+};
 
 template <int D, bool FP32, bool ADJACENT>
 __global__ void __launch_bounds__(ROPE_THREADS) rope_kv_kernel(const RopeArgs a) {
@@ -197,6 +205,16 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_kv_kernel(const RopeArgs a)
         }
     }
     pdl_wait_prior();
+    const uint32_t all = a.heads + 2u * a.kv_heads, first = part * HPW + lane / TPH;
+    const int64_t row = (int64_t)t * a.row;
+    // this head's elements, read ahead of what is done with the one before (and of the sines)
+    Raw8<FP32> rx, ry;
+    auto read = [&](uint32_t h) {
+        const int64_t from = row + (int64_t)min(h, all - 1u) * D;
+        rx.load(a.qkv, from + e0), ry.load(a.qkv, from + e1);
+    };
+    read(first);
+    const int32_t slot = ld_fresh(a.slots + t);
     float c[8], s[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -206,17 +224,15 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_kv_kernel(const RopeArgs a)
         const uint64_t phase = (uint64_t)(int64_t)pos * turn[j];
         sincospif((float)(int32_t)(uint32_t)(phase >> 32) * 0x1p-31f, &s[j], &c[j]);
     }
-    const int32_t slot = ld_fresh(a.slots + t);
     const bool kept = slot >= 0 && (uint32_t)slot < a.pages * a.page;
     const uint32_t in_page = kept ? (uint32_t)slot / a.page : 0u, at = kept ? (uint32_t)slot % a.page : 0u;
-    const uint32_t all = a.heads + 2u * a.kv_heads;
-    for (uint32_t h = part * HPW + lane / TPH; h - lane / TPH < all; h += a.parts * HPW) {
+#pragma unroll 1
+    for (uint32_t h = first; h - lane / TPH < all; h += a.parts * HPW) {
         const bool there = h < all;
         const uint32_t hh = there ? h : all - 1u;
-        const int64_t from = (int64_t)t * a.row + (int64_t)hh * D;
         float x[8], y[8];
-        load8<FP32>(a.qkv, from + e0, x);
-        load8<FP32>(a.qkv, from + e1, y);
+        rx.get(x), ry.get(y);
+        if (h - lane / TPH + a.parts * HPW < all) read(h + a.parts * HPW);
         const bool is_q = hh < a.heads, is_v = hh >= a.heads + a.kv_heads;
         const uint16_t* gamma = is_v ? nullptr : is_q ? a.gamma_q : a.gamma_k;
         if (a.gamma_q || a.gamma_k) {  // the same for the whole warp: the shuffles are
