@@ -6,13 +6,24 @@
 #include "attention.cuh"
 #include "attention_decode.cuh"
 #include "attention_prompt.cuh"
+#include "attention_short.cuh"
 
 #include <cmath>
 
 namespace miori_b200 {
 namespace attention {
 
-constexpr uint32_t DECODE_ROWS = 32;
+// Rows of an item (new tokens x heads that share a key head) up to which the decode kernel takes a call, by the size of a head.  us, decode
+// against prompt kernel: 20 rows of 128, 8 requests of 1000 positions 21.0, 20.1; 32 rows of 128, 32 requests of 4000 115, 69; 20 rows of 64,
+// 9 requests of 3000 24.5, 29.5; 32 rows of 64, 32 requests of 4000 78.6, 93.9.
+constexpr uint32_t DECODE_ROWS_128 = 16, DECODE_ROWS_64 = 32;
+// Packed calls that the short kernel takes: up to 512 tokens (and keys), or up to 2048 of prompts of 64 on average.  us, short against prompt
+// kernel, 16 heads of 128 over 4: one prompt of 77 6.6, 11.1, of 256 10.3, 17.8, of 512 16.7, 20.6, of 1024 39.1, 24.5; 32 of 32
+// 7.8, 12.4; 32 of 64 13.6, 14.1; 2 of 512 22.8, 21.4.  32 heads of 64 over 8: one of 512 16.2, 17.0; 32 of 64 14.9, 17.2.
+static bool takes_short(uint32_t tokens, uint32_t keys, uint32_t requests) {
+    const uint32_t most = tokens > keys ? tokens : keys;
+    return most <= 512u || (most <= 2048u && most <= 64u * requests);
+}
 constexpr size_t COUNTER_BYTES = 4096, JOIN_BYTES = 12288;  // for up to 768 SMs
 static size_t part_bytes() { return 2u * (size_t)sm_count() * PromptCfg<128>::PART_FLOATS * 4u; }
 
@@ -98,10 +109,19 @@ template <int D>
 static int launch_decode(const Args& a, uint32_t rows, uint32_t flags, cudaStream_t stream) {
     const dim3 grid((uint32_t)sm_count()), block(DECODE_THREADS);
     const bool pdl = (flags & MIORI_LAUNCH_PDL) != 0;
-    const cudaError_t e = rows <= 8u    ? launch(attention_decode_kernel<D, 1>, grid, block, DecodeCfg<D, 1>::SMEM, stream, pdl, a)
-                          : rows <= 16u ? launch(attention_decode_kernel<D, 2>, grid, block, DecodeCfg<D, 2>::SMEM, stream, pdl, a)
-                                        : launch(attention_decode_kernel<D, 4>, grid, block, DecodeCfg<D, 4>::SMEM, stream, pdl, a);
+    cudaError_t e = cudaSuccess;
+    if (rows <= 8u) e = launch(attention_decode_kernel<D, 1>, grid, block, DecodeCfg<D, 1>::SMEM, stream, pdl, a);
+    else if (rows <= 16u) e = launch(attention_decode_kernel<D, 2>, grid, block, DecodeCfg<D, 2>::SMEM, stream, pdl, a);
+    else if constexpr (D == 64) e = launch(attention_decode_kernel<D, 4>, grid, block, DecodeCfg<D, 4>::SMEM, stream, pdl, a);
     return e == cudaSuccess ? MIORI_OK : cuda_fail(e, "attention_decode launch");
+}
+
+template <int D>
+static int launch_short(const Args& a, uint32_t flags, cudaStream_t stream) {
+    const uint32_t per_block = SHORT_ROWS / a.group;
+    const dim3 grid((a.tokens + per_block - 1u) / per_block + a.requests, a.kv_heads);
+    const cudaError_t e = launch(attention_short_kernel<D>, grid, dim3(SHORT_THREADS), ShortCfg<D>::SMEM, stream, (flags & MIORI_LAUNCH_PDL) != 0, a);
+    return e == cudaSuccess ? MIORI_OK : cuda_fail(e, "attention_short launch");
 }
 
 }  // namespace attention
@@ -135,7 +155,7 @@ MIORI_API int miori_attention_paged(const void* q, const void* k_cache, const vo
     use_workspace(a, workspace);
     const uint64_t rows = (uint64_t)(max_new ? max_new : 1u) * a.group;
     const cudaStream_t s = (cudaStream_t)stream;
-    if (rows <= DECODE_ROWS) return dim == 128 ? launch_decode<128>(a, (uint32_t)rows, flags, s) : launch_decode<64>(a, (uint32_t)rows, flags, s);
+    if (rows <= (dim == 128 ? DECODE_ROWS_128 : DECODE_ROWS_64)) return dim == 128 ? launch_decode<128>(a, (uint32_t)rows, flags, s) : launch_decode<64>(a, (uint32_t)rows, flags, s);
     const bool may_split = (uint64_t)width * page > KEYS;
     return dim == 128 ? launch_prompt<128, true>(a, may_split, flags, s) : launch_prompt<64, true>(a, may_split, flags, s);
 }
@@ -156,6 +176,8 @@ MIORI_API int miori_attention_prompt(const void* q, const void* k, const void* v
     a.causal = (flags & MIORI_ATTENTION_FULL) == 0;
     a.scale_log2 = scale * 1.4426950408889634f;
     use_workspace(a, workspace);
+    if (takes_short(tokens, keys, requests) && kv_heads <= 65535u)
+        return dim == 128 ? launch_short<128>(a, flags, (cudaStream_t)stream) : launch_short<64>(a, flags, (cudaStream_t)stream);
     const bool may_split = keys > (uint32_t)KEYS;
     return dim == 128 ? launch_prompt<128, false>(a, may_split, flags, (cudaStream_t)stream) : launch_prompt<64, false>(a, may_split, flags, (cudaStream_t)stream);
 }

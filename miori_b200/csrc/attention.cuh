@@ -97,20 +97,22 @@ struct Shares {
     __device__ __forceinline__ uint32_t of(uint64_t unit) const { return (uint32_t)(unit / size); }
 };
 // a / b where the result is small: no division of 64 bits.
-__device__ __forceinline__ uint32_t small_quotient(uint64_t a, uint64_t b) {
+template <class U>
+__device__ __forceinline__ uint32_t small_quotient(U a, U b) {
     uint32_t q = (uint32_t)__fdividef((float)a, (float)b);  // off by one at most below 2^20
-    while (q > 0u && q * b > a) --q;
-    while ((q + 1u) * b <= a) ++q;
+    while ((uint64_t)q * b > a) --q;
+    while (a - q * b >= b) ++q;
     return q;
 }
 // Sum over a warp of numbers below 2^51.
 __device__ __forceinline__ uint64_t warp_sum(uint64_t x) {
     return __reduce_add_sync(0xFFFFFFFFu, (uint32_t)x & 0xFFFFFFu) + ((uint64_t)__reduce_add_sync(0xFFFFFFFFu, (uint32_t)(x >> 24)) << 24);
 }
-__device__ __forceinline__ uint64_t warp_prefix_sum(uint64_t x) {  // inclusive
+template <class U>
+__device__ __forceinline__ U warp_prefix_sum(U x) {  // inclusive
 #pragma unroll
     for (uint32_t o = 1; o < 32u; o <<= 1) {
-        const uint64_t y = __shfl_up_sync(0xFFFFFFFFu, x, o);
+        const U y = __shfl_up_sync(0xFFFFFFFFu, x, o);
         if ((threadIdx.x & 31u) >= o) x += y;
     }
     return x;

@@ -131,30 +131,29 @@ __global__ void __launch_bounds__(DECODE_THREADS, 1) attention_decode_kernel(con
     const bool split = a.parts != nullptr;
 
     // this CTA's share and where it begins
-    Request mine = {};
-    auto cost_of = [&](uint32_t r0) -> uint64_t {  // of request r0 + lane
-        if (r0 + lane >= a.requests) return 0;
-        mine = request<true>(a, r0 + lane);
-        return (uint64_t)((mine.n + per_block - 1u) / per_block) * (DECODE_ITEM_COST + mine.len) * a.kv_heads;
+    Request mine = {}, other;
+    auto cost_of = [&](uint32_t r, Request& x) -> uint64_t {
+        if (r >= a.requests) return 0;
+        x = request<true>(a, r);
+        return (uint64_t)((x.n + per_block - 1u) / per_block) * (DECODE_ITEM_COST + x.len) * a.kv_heads;
     };
-    uint64_t total = 0, cost = 0;
-    for (uint32_t r0 = 0; r0 < a.requests; r0 += 32u) {
-        cost = cost_of(r0);
-        total += warp_sum(cost);
-    }
+    const uint64_t cost = cost_of(lane, mine);
+    uint64_t total = warp_sum(cost);
+    for (uint32_t r0 = 32u; r0 < a.requests; r0 += 32u) total += warp_sum(cost_of(r0 + lane, other));
     const Shares shares(total, gridDim.x, UNIT);
     const uint64_t begin = shares.begin(blockIdx.x), end = shares.begin(blockIdx.x + 1u);
     if (begin == end) return;
     Place at;
-    {
-        uint64_t before = 0;
-        for (uint32_t r0 = 0; r0 < a.requests; r0 += 32u) {
-            if (a.requests > 32u) cost = cost_of(r0);
-            const uint64_t sum = warp_prefix_sum(cost);
-            const uint32_t past = __ballot_sync(0xFFFFFFFFu, before + sum > begin);
-            if (past) {
-                const uint32_t l = __ffs(past) - 1u;
-                before += __shfl_sync(0xFFFFFFFFu, sum - cost, l);
+    auto find = [&](auto cost_here, auto at_unit) {  // in 32 bits where the whole launch costs less than 2^32
+        using U = decltype(at_unit);
+        U before = 0;
+        for (uint32_t r0 = 0;; r0 += 32u) {
+            if (r0) cost_here = (U)cost_of(r0 + lane, mine);
+            const U sum = a.requests == 1u ? cost_here : warp_prefix_sum(cost_here);
+            const uint32_t past = __ballot_sync(0xFFFFFFFFu, r0 + lane < a.requests && before + sum > at_unit);
+            if (past || r0 + 32u >= a.requests) {
+                const uint32_t l = past ? __ffs(past) - 1u : 0u;  // there always is one
+                before += __shfl_sync(0xFFFFFFFFu, sum - cost_here, l);
                 at.r = r0 + l;
                 at.x.q0 = __shfl_sync(0xFFFFFFFFu, mine.q0, l), at.x.n = __shfl_sync(0xFFFFFFFFu, mine.n, l);
                 at.x.k0 = 0u, at.x.len = __shfl_sync(0xFFFFFFFFu, mine.len, l);
@@ -162,15 +161,18 @@ __global__ void __launch_bounds__(DECODE_THREADS, 1) attention_decode_kernel(con
             }
             before += __shfl_sync(0xFFFFFFFFu, sum, 31);
         }
-        at.measure(per_block);
-        const uint32_t per_head = DECODE_ITEM_COST + at.x.len, item = small_quotient(begin - before, per_head);
-        at.start = before + (uint64_t)item * per_head;
+        const U per_head = DECODE_ITEM_COST + at.x.len;
+        const uint32_t item = small_quotient((U)(at_unit - before), per_head);
+        at.start = before + item * per_head;
         at.block = item / a.kv_heads, at.head = item % a.kv_heads;
-        at.more = true;
-        at.cut(begin, end, split);
-        if (at.unit >= at.stop) at.next(a, per_block, begin, end);
-        if (!at.more) return;
-    }
+    };
+    if (total >> 32) find(cost, begin);
+    else find((uint32_t)cost, (uint32_t)begin);
+    at.measure(per_block);
+    at.more = true;
+    at.cut(begin, end, split);
+    if (at.unit >= at.stop) at.next(a, per_block, begin, end);
+    if (!at.more) return;
 
     // ---- the ring: this warp's 16 keys of a unit, rows of D swizzled by 16-byte pieces
     const uint32_t ring = smem_addr(smem) + warp * (C::STAGES * 2 * C::TILE_BYTES);
@@ -203,26 +205,12 @@ __global__ void __launch_bounds__(DECODE_THREADS, 1) attention_decode_kernel(con
             }
         }
     };
-    Place ahead = at;
-    auto fill_next = [&](uint32_t stage) {
-        if (ahead.more) {
-            fill(ahead, stage);
-            if (++ahead.unit == ahead.stop) ahead.next(a, per_block, begin, end);
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-#pragma unroll 1
-    for (uint32_t s = 0; s < C::STAGES - 1u; ++s) fill_next(s);
-
     uint32_t qf[NT][KS][2];
     float o[NT][KS][4], m[NT][2], l[NT][2];
     uint32_t sees[NT][2];  // positions that the lane's columns see
-    uint32_t stage = 0;
-    if (threadIdx.x == 0) dirty = 0u;
-    __syncthreads();
-#pragma unroll 1
-    do {
-        const uint32_t rows = min(per_block, at.x.n - at.block * per_block) * group;
+    uint32_t rows;
+    auto begin_item = [&] {
+        rows = min(per_block, at.x.n - at.block * per_block) * group;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             const uint32_t row = 8u * n + lane / 4u, i = at.block * per_block + row / group;
@@ -241,6 +229,24 @@ __global__ void __launch_bounds__(DECODE_THREADS, 1) attention_decode_kernel(con
                 m[n][j] = -INFINITY, l[n][j] = 0.0f;
             }
         }
+    };
+    begin_item();  // its loads travel with the first keys'
+    Place ahead = at;
+    auto fill_next = [&](uint32_t stage) {
+        if (ahead.more) {
+            fill(ahead, stage);
+            if (++ahead.unit == ahead.stop) ahead.next(a, per_block, begin, end);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll 1
+    for (uint32_t s = 0; s < C::STAGES - 1u; ++s) fill_next(s);
+
+    uint32_t stage = 0;
+    if (threadIdx.x == 0) dirty = 0u;
+    __syncthreads();
+#pragma unroll 1
+    do {
         // keys that some rows see and others do not: 0 * inf must not reach those that do not
         const uint32_t edge = a.causal && at.x.n > 1u ? first_edge_key(at.x) : 0xFFFFFFFFu;
         const bool whole = at.unit == 0u && at.stop == at.units;
@@ -421,6 +427,7 @@ __global__ void __launch_bounds__(DECODE_THREADS, 1) attention_decode_kernel(con
             }
         }
         at.next(a, per_block, begin, end);
+        if (at.more) begin_item();
         __syncthreads();  // the meeting's memory is free again
         if (threadIdx.x == 0) dirty = 0u;
         __syncthreads();

@@ -324,15 +324,20 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&tmem_slot)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    pdl_wait_prior();
+    const uint32_t group = a.group, per_tile = ROW_TILE / group, per_item = 2u * per_tile;
+    const bool split = a.parts != nullptr;
+    __shared__ __align__(8) uint32_t plan[sizeof(Start) / 4];
+    if (warp == 8) {  // for all: the code is cold, and one warp fetches it sooner than twelve
+        const Start found = find_share<PAGED>(a);
+        if (lane == 0) memcpy(plan, &found, sizeof(Start));
+    }
     fence_before();
     __syncthreads();
     fence_after();
     const uint32_t tmem = tmem_slot;
-    pdl_wait_prior();
-
-    const uint32_t group = a.group, per_tile = ROW_TILE / group, per_item = 2u * per_tile;
-    const bool split = a.parts != nullptr;
-    Start start = find_share<PAGED>(a);
+    Start start = {Shares(0, 1, 1), 0, 0, {}};
+    memcpy(&start, plan, sizeof(Start));
     Item& it = start.it;
     const uint64_t begin = start.begin, end = start.end;
     auto has_second = [&]() { return it.x.n > it.t * per_item + per_tile; };

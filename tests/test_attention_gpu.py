@@ -106,6 +106,43 @@ def test_longer_prompts(D, lengths, causal, workspace):
     prompt_case(2, lengths, 8, 2, D, workspace, causal=causal)
 
 
+@pytest.mark.parametrize("H,G,D", [(16, 4, 128), (8, 8, 128), (4, 1, 64), (15, 5, 128), (14, 2, 64), (12, 4, 128), (64, 1, 64), (7, 1, 128)])
+@pytest.mark.parametrize("lengths", [[1, 600], [77, 512], [700, 128], [129, 1, 300, 211], [0, 5, 0, 64, 777, 63, 65, 0]])
+@pytest.mark.parametrize("shared", [True, False])
+def test_prompts_beside_long_ones(H, G, D, lengths, shared, workspace):
+    """Odd lengths among so many tokens that the tensor-memory kernel takes them."""
+    prompt_case(31, lengths, H, G, D, workspace if shared else None)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_many_short_prompts(D, workspace):
+    prompt_case(32, [(i * 5) % 67 for i in range(60)], 8, 2, D, workspace)
+    prompt_case(33, [60] * 34, 8, 2, D, workspace, causal=False)
+
+
+@pytest.mark.parametrize("tokens,keys", [([700, 3], [9, 600]), ([40, 800], [1, 1]), ([600, 10], [0, 400]), ([3, 650], [2000, 650])])
+@pytest.mark.parametrize("causal", [True, False])
+def test_many_keys_of_their_own(tokens, keys, causal, workspace):
+    prompt_case(34, tokens, 4, 2, 64, workspace, keys=keys, causal=causal)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("at", [599, 640, 700, 701])
+def test_what_a_token_of_a_long_prompt_does_not_see(bad, at, workspace):
+    """As below, in the tensor-memory kernel: a value that is not finite reaches exactly the tokens that see it, in its dimensions."""
+    g = torch.Generator(device=DEV).manual_seed(35)
+    lengths, H, G, D = [701, 150], 4, 2, 128
+    q, k, v = rand(g, 851, H, D), rand(g, 851, G, D), rand(g, 851, G, D)
+    clean = mb.attention_prompt(q, k, v, cu_of(lengths), workspace=workspace)
+    v[at, 1, 3::5] = bad
+    got = mb.attention_prompt(q, k, v, cu_of(lengths), workspace=workspace)
+    check_errors()
+    hit = torch.zeros(851, H, D, dtype=torch.bool, device=DEV)
+    hit[at:(701 if at < 701 else 851), H // 2:, 3::5] = True
+    assert torch.equal(got[~hit], clean[~hit])
+    assert (torch.isnan(got[hit].float()) if bad != bad else got[hit].float() == bad).all()
+
+
 def test_more_requests_than_a_warp(workspace):
     prompt_case(3, [(i * 7) % 23 for i in range(300)], 4, 2, 64, workspace)
 
