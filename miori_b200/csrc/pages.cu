@@ -136,9 +136,9 @@ __global__ void __launch_bounds__(SLOT_THREADS) page_slots_kernel(const SlotArgs
 // radians at position 65536).  Its upper 32 bits are the sine's argument, off by 2^-32 turns.
 //
 // A thread holds eight pairs, which is two 8-element pieces of a head: D / 16 threads share a head, and for one token the same
-// threads take further heads with the same sines.  HBM-bound for many tokens (one warp walks all heads of a token), latency-bound
+// threads take further heads with the same sines.  A warp's threads compute each sine once and hand it to those that need it.  HBM-bound for many tokens (one warp walks all heads of a token), latency-bound
 // for few (a warp for every 32 / (D / 16) heads): `parts` warps share a token.
-constexpr uint32_t ROPE_THREADS = 256;
+constexpr uint32_t ROPE_THREADS = 128;  // 16384 tokens: 41.0 us, with 256 44.5 (fewer warps fit an SM)
 
 struct RopeArgs {
     const void* qkv;
@@ -194,14 +194,16 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_kv_kernel(const RopeArgs a)
     const bool turns_here = u < turning;
     const uint32_t e0 = turns_here && !ADJACENT ? 8u * u : 16u * u;
     const uint32_t e1 = turns_here && !ADJACENT ? e0 + a.rotary / 2u : e0 + 8u;
-    // weights, so read ahead of the wait
-    uint64_t turn[8] = {};
-    uint32_t axis[8] = {};
+    // the threads of a warp that hold the same pairs, of HPW heads, compute PER of them each; weights are read ahead of the wait
+    constexpr uint32_t PER = 8u / HPW;
+    uint64_t turn[PER] = {};
+    uint32_t axis[PER] = {};
     if (turns_here) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            turn[j] = __ldg(a.turns + 8u * u + j);
-            axis[j] = a.axes ? min((uint32_t)__ldg(a.axes + 8u * u + j), a.num_axes - 1u) : 0u;
+        for (uint32_t i = 0; i < PER; ++i) {
+            const uint32_t j = 8u * u + lane / TPH * PER + i;
+            turn[i] = __ldg(a.turns + j);
+            axis[i] = a.axes ? min((uint32_t)__ldg(a.axes + j), a.num_axes - 1u) : 0u;
         }
     }
     pdl_wait_prior();
@@ -215,14 +217,19 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_kv_kernel(const RopeArgs a)
     };
     read(first);
     const int32_t slot = ld_fresh(a.slots + t);
-    float c[8], s[8];
+    float mine_c[PER], mine_s[PER], c[8], s[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        c[j] = 1.0f, s[j] = 0.0f;
+    for (uint32_t i = 0; i < PER; ++i) {
+        mine_c[i] = 1.0f, mine_s[i] = 0.0f;
         if (!turns_here) continue;
-        const int32_t pos = ld_fresh(a.positions + (size_t)axis[j] * a.tokens + t);
-        const uint64_t phase = (uint64_t)(int64_t)pos * turn[j];
-        sincospif((float)(int32_t)(uint32_t)(phase >> 32) * 0x1p-31f, &s[j], &c[j]);
+        const int32_t pos = ld_fresh(a.positions + (size_t)axis[i] * a.tokens + t);
+        const uint64_t phase = (uint64_t)(int64_t)pos * turn[i];
+        sincospif((float)(int32_t)(uint32_t)(phase >> 32) * 0x1p-31f, &mine_s[i], &mine_c[i]);
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j) {
+        c[j] = __shfl_sync(0xFFFFFFFFu, mine_c[j % PER], j / PER * TPH + u);
+        s[j] = __shfl_sync(0xFFFFFFFFu, mine_s[j % PER], j / PER * TPH + u);
     }
     const bool kept = slot >= 0 && (uint32_t)slot < a.pages * a.page;
     const uint32_t in_page = kept ? (uint32_t)slot / a.page : 0u, at = kept ? (uint32_t)slot % a.page : 0u;
