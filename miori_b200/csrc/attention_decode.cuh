@@ -19,7 +19,7 @@
 namespace miori_b200 {
 namespace attention {
 
-constexpr uint32_t DECODE_ITEM_COST = 256;  // an item's begin and end, in positions
+constexpr uint32_t DECODE_ITEM_COST = 384;  // an item's begin and end, in positions
 constexpr int DECODE_WARPS = 8, DECODE_THREADS = DECODE_WARPS * 32, TILE = 16, UNIT = DECODE_WARPS * TILE;
 
 template <int D, int NT>
@@ -284,29 +284,41 @@ __global__ void __launch_bounds__(DECODE_THREADS, 1) attention_decode_kernel(con
 #pragma unroll
                 for (int n = 0; n < NT; ++n) mma16816(s[n], f, qf[n][k][0], qf[n][k][1]);
             }
+            // The running maximum moves only when a score exceeds it by 2^8 (p grows up to 256 then, which costs no precision): most tiles
+            // need neither the maximum over the lanes nor a rescaled O.
             uint32_t pf[NT][2];
             const uint32_t key = key0 + lane / 4u;
+            bool higher = false;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    s[n][j] = key + (j >= 2 ? 8u : 0u) < sees[n][j & 1] ? s[n][j] * a.scale_log2 : -INFINITY;
+                    higher |= s[n][j] > m[n][j & 1] + 8.0f;
+                }
+            if (__any_sync(0xFFFFFFFFu, higher)) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        float top = fmaxf(m[n][j], fmaxf(s[n][j], s[n][j + 2]));
+                        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 4));
+                        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
+                        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
+                        const float keep = top == -INFINITY ? 1.0f : exp2_fast(m[n][j] - top);
+                        m[n][j] = top;
+                        l[n][j] *= keep;
+#pragma unroll
+                        for (int k = 0; k < KS; ++k) o[n][k][j] *= keep, o[n][k][j + 2] *= keep;
+                    }
+            }
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                float p[4];
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const float t0 = key < sees[n][j] ? s[n][j] * a.scale_log2 : -INFINITY;
-                    const float t1 = key + 8u < sees[n][j] ? s[n][j + 2] * a.scale_log2 : -INFINITY;
-                    float top = fmaxf(t0, t1);
-                    top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 4));
-                    top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 8));
-                    top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 16));
-                    const float now = fmaxf(m[n][j], top), from = now == -INFINITY ? 0.0f : now;
-                    const float keep = exp2_fast(m[n][j] - from);
-                    m[n][j] = now;
-                    p[j] = exp2_fast(t0 - from), p[j + 2] = exp2_fast(t1 - from);
-                    l[n][j] = l[n][j] * keep + p[j] + p[j + 2];
-#pragma unroll
-                    for (int k = 0; k < KS; ++k) o[n][k][j] *= keep, o[n][k][j + 2] *= keep;
-                }
-                pf[n][0] = movmatrix(pack_bf16(p[0], p[1]));
-                pf[n][1] = movmatrix(pack_bf16(p[2], p[3]));
+                for (int j = 0; j < 4; ++j) s[n][j] = exp2_fast(s[n][j] - (m[n][j & 1] == -INFINITY ? 0.0f : m[n][j & 1]));
+                l[n][0] += s[n][0] + s[n][2], l[n][1] += s[n][1] + s[n][3];
+                pf[n][0] = movmatrix(pack_bf16(s[n][0], s[n][1]));
+                pf[n][1] = movmatrix(pack_bf16(s[n][2], s[n][3]));
             }
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
