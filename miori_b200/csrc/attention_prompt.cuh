@@ -7,14 +7,17 @@
 //   where it lies over the S it came from.  TMEM: S0, S1 (128 columns each), O0, O1 (D each).
 // * Warps 0-3 and 4-7 are the softmax of the two row tiles, a thread a row: no shuffle anywhere.  The two take turns on the
 //   tensor cores: while one exponentiates, the other's products run.  Warp 8 issues the copies (TMA, 128-byte swizzle, a
-//   ring of 32-KB halves: keys, values, keys, ...), one thread of warp 9 the MMAs, warps 10-11 look through the values of edge tiles.
+//   ring of tiles: keys, values, keys, ...), an elected thread of warp 9 the MMAs, warps 10-11 look through the values of edge tiles.
 // * The running maximum moves only when a row's exceeds it by 2^8: until then p grows up to 256, which costs no precision in
 //   fp32 sums and bf16 rounding, and O stays where it is.  O is rescaled by the softmax warps themselves, in TMEM.
 // * P is rounded to bf16 for the second product, as the values are; l sums the unrounded p.
 // * Tried and dropped (432 GFLOP of prompts up to 8192, us): an MMA warp for each row tile (454), the MMAs issued by the softmax warps
 //   (473), scores of 64 keys double-buffered (684 as issued then: twice the steps), the product begun at half of the probabilities
-//   (403 - 430), a quarter or half of the exponentials by a polynomial on the FMA pipe (404, 466).  404 as it is; the MMA
-//   warp's bookkeeping between products is what keeps the tensor cores at about two thirds.
+//   (403 - 430), a quarter or half of the exponentials by a polynomial on the FMA pipe (404, 466), exponentials with the maximum
+//   of the tile before, taken again where that is too low (401); 404 then, 376 (1.15 PFLOP/s) with the registers and the item's cost
+//   as they are now.  The tensor pipe is active 62 % of the cycles and the special-function unit 58 % (one prompt of 8192): a row
+//   tile's chain of scores, softmax and product is hidden by one other chain only, and the MMA warp's bookkeeping between
+//   products comes on top.
 // * Edge tiles (keys that some rows do not see, or past the end).  Their scores are masked one by one.  Their values are looked
 //   through before the product: rows past the end are zeroed (a page's unwritten tail, the next prompt's rows) and so are
 //   numbers that are not finite, since 0 * inf would reach rows that do not see them; rows that do see them get them added
@@ -28,7 +31,7 @@ namespace miori_b200 {
 namespace attention {
 
 constexpr int PROMPT_THREADS = 384, KEYS = 128, ROW_TILE = 128;
-constexpr uint32_t ITEM_COST = 256;     // an item's set-up and end, in positions
+constexpr uint32_t ITEM_COST = 384;     // an item's set-up and end, in positions (prompts of up to 8192: 256 386 us, 384 376, 640 384)
 constexpr uint32_t LEAST_SHARE = 256;   // positions; a tile of keys at least
 
 template <int D>
@@ -40,7 +43,7 @@ struct PromptCfg {
     static constexpr int SMEM = 1024 + (2 + STAGES) * TILE_BYTES;
     static constexpr int PART_FLOATS = 2 * ROW_TILE * (D + 2);  // [D / 4][256] pieces of O, then m and l
 };
-constexpr int SETMAXNREG_SOFTMAX = 208, SETMAXNREG_OTHERS = 88;  // (256 * 224 + 128 * 56) = 384 * 168, what a launch has
+constexpr int SETMAXNREG_SOFTMAX = 192, SETMAXNREG_OTHERS = 120;  // 256 * 192 + 128 * 120 = 384 * 168, what a launch has; 208 and 88 1.5 % slower
 static_assert(256 * SETMAXNREG_SOFTMAX + 128 * SETMAXNREG_OTHERS <= PROMPT_THREADS * 168, "a split above the launch's registers waits forever");
 
 // ---- how the work is dealt ---------------------------------------------------------------
