@@ -149,6 +149,7 @@ struct RopeArgs {
     int64_t row, k_page, k_head, k_slot, v_page, v_head, v_slot;  // strides in elements
     uint32_t tokens, heads, kv_heads, rotary, num_axes, page, pages, parts;
     float eps;
+    uint32_t early;  // weights may be read ahead of the wait
 };
 
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
@@ -194,8 +195,9 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_kv_kernel(const RopeArgs a)
     const bool turns_here = u < turning;
     const uint32_t e0 = turns_here && !ADJACENT ? 8u * u : 16u * u;
     const uint32_t e1 = turns_here && !ADJACENT ? e0 + a.rotary / 2u : e0 + 8u;
-    // the threads of a warp that hold the same pairs, of HPW heads, compute PER of them each; weights are read ahead of the wait
+    // the threads of a warp that hold the same pairs, of HPW heads, compute PER of them each
     constexpr uint32_t PER = 8u / HPW;
+    if (!a.early) pdl_wait_prior();
     uint64_t turn[PER] = {};
     uint32_t axis[PER] = {};
     if (turns_here) {
@@ -298,8 +300,8 @@ MIORI_API int miori_page_slots(const int32_t* held, const int32_t* fresh, int32_
     const SlotArgs a = {held, fresh, table, pool, taken, slots, positions, cu, held_after, taken_after, requests, width, page, pool_size, tokens,
                         aligned16(slots) && aligned16(positions)};
     const uint32_t grid = tokens ? (tokens + TOKENS_PER_CTA - 1u) / TOKENS_PER_CTA : 1u;
-    const cudaError_t e = launch(page_slots_kernel, dim3(grid), dim3(SLOT_THREADS), 8u * (requests + 1u), (cudaStream_t)stream,
-                                 (flags & MIORI_LAUNCH_PDL) != 0, a);
+    (void)flags;  // it reads nothing ahead of its wait: every launch may begin beside the one before (slots of a decode step 6.2 us a call without)
+    const cudaError_t e = launch(page_slots_kernel, dim3(grid), dim3(SLOT_THREADS), 8u * (requests + 1u), (cudaStream_t)stream, true, a);
     return e == cudaSuccess ? MIORI_OK : cuda_fail(e, "page_slots launch");
 }
 
@@ -323,7 +325,7 @@ MIORI_API int miori_rope_kv(const void* qkv, int64_t qkv_row, const uint64_t* tu
         if (cache_strides[i] % 8) return fail(MIORI_E_INVALID, "rope_kv: strides of the caches must be multiples of 8 elements");
     RopeArgs a = {qkv, turns, axes, positions, slots, (const uint16_t*)gamma_q, (const uint16_t*)gamma_k, (uint16_t*)q, (uint16_t*)k_cache, (uint16_t*)v_cache,
                   qkv_row, cache_strides[0], cache_strides[1], cache_strides[2], cache_strides[3], cache_strides[4], cache_strides[5],
-                  tokens, heads, kv_heads, rotary, num_axes, page, pages, 1u, eps};
+                  tokens, heads, kv_heads, rotary, num_axes, page, pages, 1u, eps, flags & MIORI_LAUNCH_PDL};
     // as many warps a token as keep 16 warps an SM busy
     const uint32_t heads_a_warp = 512u / dim, most = (heads + 2u * kv_heads + heads_a_warp - 1u) / heads_a_warp;
     const uint32_t wanted = (16u * (uint32_t)sm_count() + tokens - 1u) / tokens;
@@ -337,6 +339,6 @@ MIORI_API int miori_rope_kv(const void* qkv, int64_t qkv_row, const uint64_t* tu
                                   : (adjacent ? rope_kv_kernel<128, false, true> : rope_kv_kernel<128, false, false>);
     else kernel = fp32 ? (adjacent ? rope_kv_kernel<64, true, true> : rope_kv_kernel<64, true, false>)
                        : (adjacent ? rope_kv_kernel<64, false, true> : rope_kv_kernel<64, false, false>);
-    const cudaError_t e = launch(kernel, grid, dim3(ROPE_THREADS), 0, (cudaStream_t)stream, (flags & MIORI_LAUNCH_PDL) != 0, a);
+    const cudaError_t e = launch(kernel, grid, dim3(ROPE_THREADS), 0, (cudaStream_t)stream, true, a);
     return e == cudaSuccess ? MIORI_OK : cuda_fail(e, "rope_kv launch");
 }
