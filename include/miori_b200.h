@@ -376,7 +376,9 @@ int miori_gemv8_rmsnorm(const void* q, const void* s, const void* b, const void*
  * position p is in page table[request][p / page], at p % page; its slot is that page's number * page + p % page.
  * Tokens of a step are packed: those of request r are rows cu[r] .. cu[r + 1] - 1 of q.  Lengths, tables and
  * cu live on the device and are read there, so a recorded graph serves every step; lengths that contradict
- * one another are cut off at the end of the tensors given, nothing beyond is read or written. */
+ * one another are cut off at the end of the tensors given, nothing beyond is read or written.  These launches may begin
+ * while the one before on the stream drains, with MIORI_LAUNCH_PDL or without: they wait for it before they read or
+ * write anything (with the flag miori_rope_kv reads turns and axes ahead). */
 
 /* Positions, slots and new pages of a step's tokens.  Request r (1..16384 of them) holds held[r] positions and gets
  * new_tokens[r] more: it then owns ceil((held + new) / page) pages, at most `width`.  New ones are
@@ -396,7 +398,7 @@ int miori_page_slots(const int32_t* held, const int32_t* new_tokens, int32_t* ta
  * int32 position exactly.  positions [num_axes][tokens], num_axes 1..4 (text: 1; image and video: time, height, width);
  * axes [rotary / 2], NULL: all 0.  q out: bf16 [tokens][heads][dim].  k and v go to slots[t] of the caches as bf16;
  * a slot outside the cache is not written.  cache_strides: page, head, slot of k_cache, then of v_cache, in
- * elements, multiples of 8.  fp32 throughout, rounded once.  turns, axes and gammas are weights (MIORI_LAUNCH_PDL). */
+ * elements, multiples of 8.  fp32 throughout, rounded once.  turns and axes are weights (MIORI_LAUNCH_PDL). */
 int miori_rope_kv(const void* qkv, int64_t qkv_row, const uint64_t* turns, const int32_t* axes, const int32_t* positions,
                   const int32_t* slots, const void* gamma_q, const void* gamma_k, float eps, void* q, void* k_cache,
                   void* v_cache, const int64_t* cache_strides, uint32_t tokens, uint32_t heads, uint32_t kv_heads,

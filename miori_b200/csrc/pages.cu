@@ -16,6 +16,7 @@ namespace pages {
 // Latency-bound: 8 bytes a request read and 8 a token written.  Every CTA does the prefix sums by itself (8 bytes a request
 // from L2), so that none waits for another; they then share the tokens and the new table entries.  A token's page is taken from
 // the pool and not from the table entry that another CTA writes beside it, so nothing here depends on the order of the CTAs.
+// 32 requests of one token 4.7 us, 64 prompts of 41 thousand tokens 4.5.
 constexpr uint32_t SLOT_THREADS = 512, TOKENS_PER_CTA = 4 * SLOT_THREADS, MAX_REQUESTS = 16384;
 
 struct SlotArgs {
@@ -137,7 +138,8 @@ __global__ void __launch_bounds__(SLOT_THREADS) page_slots_kernel(const SlotArgs
 //
 // A thread holds eight pairs, which is two 8-element pieces of a head: D / 16 threads share a head, and for one token the same
 // threads take further heads with the same sines.  A warp's threads compute each sine once and hand it to those that need it.  HBM-bound for many tokens (one warp walks all heads of a token), latency-bound
-// for few (a warp for every 32 / (D / 16) heads): `parts` warps share a token.
+// for few (a warp for every 32 / (D / 16) heads): `parts` warps share a token.  16384 tokens of 24 heads of 128 in bf16 37.3 us, 5.4 TB/s of
+// reads and writes; 32 tokens of fp32 2.4 us.
 constexpr uint32_t ROPE_THREADS = 128;  // 16384 tokens: 41.0 us, with 256 44.5 (fewer warps fit an SM)
 
 struct RopeArgs {
