@@ -413,10 +413,10 @@ size_t miori_attention_workspace_bytes(void);
  * MIORI_ATTENTION_FULL all.  A token that sees none gets zeros.  What is in slots beyond the length, or belongs
  * to positions that a token does not see, has no influence, whatever its bits are.  q and out [tokens][heads][dim] bf16,
  * dim 64 or 128, heads a multiple (up to 64 times) of kv_heads; head h reads key head h / (heads / kv_heads).  page is a
- * power of two from 8 to 65536.  table [requests][width].  strides in elements, positive multiples of 8: token and head of
- * q, token and head of out, page, head and slot of k_cache, the same of v_cache.  max_new: the most tokens that a request
- * has in this call; it decides only which kernel runs.  Sums and softmax in fp32, probabilities rounded to bf16
- * for their product with v. */
+ * power of two from 8 to 65536.  table [requests][width]: positions whose entry is no page of the cache are seen by no token.
+ * strides in elements, positive multiples of 8: token and head of q, token and head of out, page, head and slot of
+ * k_cache, the same of v_cache.  max_new: the most tokens that a request has in this call; it decides only which kernel
+ * runs.  Sums and softmax in fp32, probabilities rounded to bf16 for their product with v. */
 int miori_attention_paged(const void* q, const void* k_cache, const void* v_cache, void* out, const int64_t* strides,
                           const int32_t* table, const int32_t* lens, const int32_t* cu, uint32_t requests,
                           uint32_t tokens, uint32_t width, uint32_t pages, uint32_t page, uint32_t heads,

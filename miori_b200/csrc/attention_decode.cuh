@@ -8,7 +8,8 @@
 //   in shared memory (ldmatrix), V through ldmatrix.trans; P^T takes one movmatrix per eight keys and columns.
 // * A warp owns 16 of a unit's 128 keys, with a ring of its own (STAGES tiles of 16 keys and values), its own running maximum, sum
 //   and O: no barrier in the main loop.  cp.async fills the ring, so a page may be as short as 8 positions and strides are
-//   free; what lies beyond the length arrives as zeros, never as what the page held before.
+//   free; what lies beyond the length, or in a page that the cache does not have, arrives as zeros, never as what the page or the
+//   ring held before.
 // * A CTA's share may begin and end inside an item.  The warps' parts meet in shared memory at the end of an item; an item
 //   shared by several CTAs meets in the workspace: the CTA that arrives last adds the parts up in the order of the keys, so a
 //   result does not depend on which one that is.
@@ -181,6 +182,7 @@ __global__ void __launch_bounds__(DECODE_THREADS, 1) attention_decode_kernel(con
     // ---- the ring: this warp's 16 keys of a unit, rows of D swizzled by 16-byte pieces
     const uint32_t ring = smem_addr(smem) + warp * (C::STAGES * 2 * C::TILE_BYTES);
     auto piece = [](uint32_t row, uint32_t c) { return row * (D * 2u) + ((c ^ (row & 7u)) << 4); };
+    uint32_t absent = 0;  // of a stage's keys, a bit for each eight: no page
     auto fill = [&](const Place& p, uint32_t stage) {
         const uint32_t key0 = p.unit * UNIT + warp * TILE;
         const uint32_t kdst = ring + stage * 2u * C::TILE_BYTES, vdst = kdst + C::TILE_BYTES;
@@ -195,6 +197,8 @@ __global__ void __launch_bounds__(DECODE_THREADS, 1) attention_decode_kernel(con
         for (uint32_t half = 0; half < 2; ++half) {
             const uint32_t first = key0 + 8u * half, in = first & mask;
             const bool known = pg[half] < a.pages;
+            const uint32_t bit = 1u << (2u * stage + half);
+            absent = known ? absent & ~bit : absent | bit;
             const uint32_t count = known ? p.x.len - first : 0u, number = known ? pg[half] : 0u;
             const uint32_t row0 = lane / CH, c = lane % CH;
             const uint16_t* kp = a.k + (int64_t)number * a.k_page + (int64_t)p.head * a.k_head + (int64_t)in * a.k_slot + 8u * c;
@@ -259,7 +263,7 @@ __global__ void __launch_bounds__(DECODE_THREADS, 1) attention_decode_kernel(con
             asm volatile("cp.async.wait_group %0;" ::"n"(C::STAGES - 2) : "memory");
             __syncwarp();
             fill_next(stage == 0u ? C::STAGES - 1u : stage - 1u);  // the place read last is free
-            const uint32_t kb = ring + stage * 2u * C::TILE_BYTES, vb = kb + C::TILE_BYTES;
+            const uint32_t kb = ring + stage * 2u * C::TILE_BYTES, vb = kb + C::TILE_BYTES, gone = absent >> (2u * stage) & 3u;
             stage = stage + 1u == C::STAGES ? 0u : stage + 1u;
             const uint32_t key0 = at.unit * UNIT + warp * TILE;
             if (key0 >= at.x.len) continue;
@@ -287,6 +291,12 @@ __global__ void __launch_bounds__(DECODE_THREADS, 1) attention_decode_kernel(con
                 ldmatrix4(f, kb + piece(lane & 15u, 2u * k + (lane >> 4)));
 #pragma unroll
                 for (int n = 0; n < NT; ++n) mma16816(s[n], f, qf[n][k][0], qf[n][k][1]);
+            }
+            if (gone) {  // no page: nobody sees these keys
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) s[n][j] = gone >> (j / 2) & 1u ? -INFINITY : s[n][j];
             }
             // The running maximum moves only when a score exceeds it by 2^8 (p grows up to 256 then, which costs no precision): most tiles
             // need neither the maximum over the lanes nor a rescaled O.

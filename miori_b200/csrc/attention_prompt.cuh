@@ -22,6 +22,8 @@
 //   through before the product: rows past the end are zeroed (a page's unwritten tail, the next prompt's rows) and so are
 //   numbers that are not finite, since 0 * inf would reach rows that do not see them; rows that do see them get them added
 //   at the end.
+// * Positions whose table entry is no page of the cache are seen by nobody: the copying warp clears their rows of the tile, which hold what
+//   was there before, and leaves word of them in `absent` for the softmax, which gives them no weight.
 // * Shares of the items' key tiles are cut anywhere (attention.cuh); parts of an item meet in attention_join_kernel.
 #pragma once
 #include "attention.cuh"
@@ -293,6 +295,9 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     extern __shared__ uint8_t smem[];
     __shared__ __align__(8) uint64_t bars[BARS];
     __shared__ uint32_t tmem_slot, dirty_item[8];
+    // Of the last eight key tiles, a bit for each eight keys: no page.  Tile n + 8 is copied after the values of tile n + 5 at least have
+    // been multiplied, and so after every softmax has read the word of tile n.
+    __shared__ volatile uint32_t absent[8];
     __shared__ volatile uint32_t abort_flag;
     const uint32_t base = (smem_addr(smem) + 1023u) & ~1023u;
     const uint32_t q_at = base, ring = base + 2u * C::TILE_BYTES;
@@ -374,6 +379,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                         uint32_t boxes = C::HALVES, box_rows = KEYS, mine = lane / C::HALVES;
                         const uint32_t half = lane % C::HALVES;
                         bool issue = lane < (uint32_t)C::HALVES;
+                        uint32_t gone = 0;
                         if (PAGED) {
                             const uint32_t key0 = k * KEYS, left = it.x.len > key0 ? min(it.x.len - key0, (uint32_t)KEYS) : 0u;
                             const uint32_t in_box = min(1u << a.page_shift, (uint32_t)KEYS);
@@ -384,6 +390,8 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                                 row = (int)(key & ((1u << a.page_shift) - 1u));
                                 issue = (uint32_t)page < a.pages;
                             }
+                            const uint32_t lost = __ballot_sync(0xFFFFFFFFu, mine * in_box < left && !issue);
+                            if (lost) gone = __ballot_sync(0xFFFFFFFFu, lane < KEYS / 8u && lost >> (8u * lane / in_box * C::HALVES) & 1u);
                             box_rows = in_box;
                             boxes = __popc(__ballot_sync(0xFFFFFFFFu, issue));
                         }
@@ -394,6 +402,15 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                             ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
                             if (!ok) break;
                             const uint32_t arrive = which && k >= edge ? raw(s) : full(s);
+                            if (PAGED && gone) {
+                                __syncwarp();
+                                for (uint32_t e = lane; e < (uint32_t)C::TILE_BYTES / 16u; e += 32u)
+                                    if (gone >> (e / 64u % 16u) & 1u)
+                                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(ring + s * C::TILE_BYTES + 16u * e), "r"(0u) : "memory");
+                                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                                __syncwarp();
+                            }
+                            if (PAGED && lane == 0 && which == 0u) absent[n_tile / 2u % 8u] = gone;
                             if (lane == 0) mbar_expect_tx(arrive, boxes * box_rows * 128u);
                             __syncwarp();
                             const uint32_t dst = ring + s * C::TILE_BYTES + half * C::BLOCK + mine * box_rows * 128u;
@@ -564,7 +581,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         const uint32_t lanes = ((warp & 3u) * 32u) << 16;
         const uint32_t s_at = tmem + lanes + t * KEYS, o_at = tmem + lanes + 2u * KEYS + t * D;
         const bool wide = (reinterpret_cast<uintptr_t>(a.out) & 31u) == 0u && a.o_token % 16 == 0 && a.o_head % 16 == 0;
-        uint32_t n_s = 0, n_o = 0, n_item = 0;
+        uint32_t n_s = 0, n_o = 0, n_item = 0, tile0 = 0;  // tile0: key tiles of the items before
         uint4 to_join = make_uint4(0u, 0u, 0u, 0u);
         bool ok = true;
         while (ok && it.start < end) {
@@ -590,6 +607,13 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                             const uint32_t count = sees > key0 ? sees - key0 : 0u;
 #pragma unroll
                             for (uint32_t j = 0; j < KEYS; ++j) s[j] = j < count ? s[j] : -INFINITY;
+                        }
+                        if (PAGED) {
+                            const uint32_t gone = absent[(tile0 + k - span.k0) % 8u];
+                            if (gone) {
+#pragma unroll
+                                for (uint32_t j = 0; j < KEYS; ++j) s[j] = gone >> (j / 8u) & 1u ? -INFINITY : s[j];
+                            }
                         }
                         float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
@@ -713,6 +737,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                     __syncwarp();
                     if (lane == 0) mbar_arrive(o_free(t));
                 }
+                tile0 += span.k1 - span.k0;
             }
             it.next<PAGED>(a, per_item, end);
         }
