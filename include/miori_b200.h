@@ -376,7 +376,8 @@ int miori_gemv8_rmsnorm(const void* q, const void* s, const void* b, const void*
  * position p is in page table[request][p / page], at p % page; its slot is that page's number * page + p % page.
  * Tokens of a step are packed: those of request r are rows cu[r] .. cu[r + 1] - 1 of q.  Lengths, tables and
  * cu live on the device and are read there, so a recorded graph serves every step; lengths that contradict
- * one another are cut off at the end of the tensors given, nothing beyond is read or written.  These launches may begin
+ * one another are cut off at the end of the tensors given, nothing beyond is read or written, and what is there is as it
+ * would be if the rest were there too.  These launches may begin
  * while the one before on the stream drains, with MIORI_LAUNCH_PDL or without: they wait for it before they read or
  * write anything (with the flag miori_rope_kv reads turns and axes ahead). */
 

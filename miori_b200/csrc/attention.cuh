@@ -51,10 +51,12 @@ __device__ __forceinline__ uint32_t finite_or_zero(uint32_t pair) {
 }
 
 // A request as the kernels see it.  Lengths that contradict one another are cut off to what is there: no row of q or k beyond
-// the tensors, no column beyond the table is ever read.
+// the tensors, no column beyond the table is ever read.  Where its tokens stand is another matter: that follows from the
+// lengths as they were given, or the tokens that are there would see positions that are not theirs.
 struct Request {
     uint32_t q0, n;   // first token in q, number of tokens
     uint32_t k0, len;  // first row of packed k (0 where paged), number of positions
+    int32_t before;     // positions in front of the first token (n > 0)
 };
 template <bool PAGED>
 __device__ __forceinline__ Request request(const Args& a, uint32_t r) {
@@ -67,11 +69,13 @@ __device__ __forceinline__ Request request(const Args& a, uint32_t r) {
         x.k0 = 0u;
         const uint64_t room = (uint64_t)a.width << a.page_shift;
         x.len = (uint32_t)max(ld_fresh(a.lens + r), 0);
+        x.before = (int32_t)(x.len - (uint32_t)max(q1, 0) + x.q0);  // 2^32 drops off: where n > 0 it is within -2^31 .. 2^31
         if ((uint64_t)x.len > room) x.len = (uint32_t)room;
     } else {
-        const int32_t k0 = ld_fresh(a.lens + r), k1 = ld_fresh(a.lens + r + 1);
-        x.k0 = min((uint32_t)max(k0, 0), a.keys);
-        x.len = min((uint32_t)max(k1, 0), a.keys);
+        const uint32_t k0 = (uint32_t)max(ld_fresh(a.lens + r), 0), k1 = (uint32_t)max(ld_fresh(a.lens + r + 1), 0);
+        x.before = (int32_t)((k1 > k0 ? k1 - k0 : 0u) - (uint32_t)max(q1, 0) + x.q0);
+        x.k0 = min(k0, a.keys);
+        x.len = min(k1, a.keys);
         x.len = x.len > x.k0 ? x.len - x.k0 : 0u;
     }
     return x;
@@ -79,7 +83,7 @@ __device__ __forceinline__ Request request(const Args& a, uint32_t r) {
 // Positions that token i of the request sees.
 __device__ __forceinline__ uint32_t seen(const Args& a, const Request& x, uint32_t i) {
     if (!a.causal) return x.len;
-    const int64_t s = (int64_t)x.len - (int64_t)x.n + (int64_t)i + 1;
+    const int64_t s = (int64_t)x.before + (int64_t)i + 1;
     return s <= 0 ? 0u : min((uint32_t)s, x.len);
 }
 

@@ -60,7 +60,10 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
 }
 
 // First key of the edge tiles of a request: those with keys that its first token does not see.
-__device__ __forceinline__ uint32_t first_edge_key(const Request& x) { return x.len > x.n ? (x.len - x.n + 1u) / TILE * TILE : 0u; }
+__device__ __forceinline__ uint32_t first_edge_key(const Args& a, const Request& x) {
+    const uint32_t all_see = seen(a, x, 0u);
+    return all_see < x.len ? all_see / TILE * TILE : 0xFFFFFFFFu;
+}
 
 // Where a share stands: an item (request, block of its tokens, key head), a unit of its keys, and where the share leaves the item.
 // An item costs ITEM_COST + its positions; unit k belongs to the share that holds start + ITEM_COST - 1 + UNIT k (the dealing
@@ -109,7 +112,7 @@ struct Place {
 __device__ __noinline__ float4 add_left_out(float4 v, const Args& a, const Place& at, uint32_t token, uint32_t d) {
     float e[4] = {v.x, v.y, v.z, v.w};
     const uint32_t stop = seen(a, at.x, token);
-    for (uint32_t j = first_edge_key(at.x); j < stop; ++j) {
+    for (uint32_t j = first_edge_key(a, at.x); j < stop; ++j) {
         const uint32_t pg = (uint32_t)ld_fresh(a.table + (size_t)at.r * a.width + (j >> a.page_shift));
         if (pg >= a.pages) continue;
         const uint16_t* vp = a.v + (int64_t)pg * a.v_page + (int64_t)at.head * a.v_head + (int64_t)(j & ((1u << a.page_shift) - 1u)) * a.v_slot + d;
@@ -161,7 +164,7 @@ __global__ void __launch_bounds__(DECODE_THREADS, 1) attention_decode_kernel(con
                 before += __shfl_sync(0xFFFFFFFFu, sum - cost_here, l);
                 at.r = r0 + l;
                 at.x.q0 = __shfl_sync(0xFFFFFFFFu, mine.q0, l), at.x.n = __shfl_sync(0xFFFFFFFFu, mine.n, l);
-                at.x.k0 = 0u, at.x.len = __shfl_sync(0xFFFFFFFFu, mine.len, l);
+                at.x.k0 = 0u, at.x.len = __shfl_sync(0xFFFFFFFFu, mine.len, l), at.x.before = __shfl_sync(0xFFFFFFFFu, mine.before, l);
                 break;
             }
             before += __shfl_sync(0xFFFFFFFFu, sum, 31);
@@ -256,7 +259,7 @@ __global__ void __launch_bounds__(DECODE_THREADS, 1) attention_decode_kernel(con
 #pragma unroll 1
     do {
         // keys that some rows see and others do not: 0 * inf must not reach those that do not
-        const uint32_t edge = a.causal && at.x.n > 1u ? first_edge_key(at.x) : 0xFFFFFFFFu;
+        const uint32_t edge = first_edge_key(a, at.x);
         const bool whole = at.unit == 0u && at.stop == at.units;
 #pragma unroll 1
         for (; at.unit < at.stop; ++at.unit) {

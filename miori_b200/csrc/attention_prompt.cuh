@@ -63,9 +63,13 @@ __device__ __forceinline__ uint64_t cost_before(const Args& a, const Request& x,
     uint64_t cost = (uint64_t)t * ITEM_COST;
     if (!a.causal) return cost + (uint64_t)t * x.len;
     uint32_t full = t;
-    if (t == items && t) cost += x.len, --full;  // the last one may hold fewer tokens
-    const int64_t before = (int64_t)x.len - (int64_t)x.n;
+    if (t == items && t) cost += item_seen(a, x, t - 1u, step), --full;  // the last one may hold fewer tokens
+    const int64_t before = x.before, after = (int64_t)x.len - before;
     const uint32_t none = before < 0 ? min((uint32_t)-before / step, full) : 0u;  // items none of whose tokens sees anything
+    if (after < (int64_t)x.n) {  // and those whose last token stands at the end of what is there, or behind it
+        const uint32_t in_front = after > 0 ? max(min(((uint32_t)after + step - 1u) / step - 1u, full), none) : none;
+        cost += (uint64_t)(full - in_front) * x.len, full = in_front;
+    }
     // item i sees before + (i + 1) step
     return cost + (uint64_t)((int64_t)(full - none) * before) + (((uint64_t)full * (full + 1u) - (uint64_t)none * (none + 1u)) / 2u) * step;
 }
@@ -135,6 +139,7 @@ __device__ __forceinline__ Start find_share(const Args& a) {
             st.it.r = r0 + l;
             st.it.x.q0 = __shfl_sync(0xFFFFFFFFu, mine.q0, l), st.it.x.n = __shfl_sync(0xFFFFFFFFu, mine.n, l);
             st.it.x.k0 = __shfl_sync(0xFFFFFFFFu, mine.k0, l), st.it.x.len = __shfl_sync(0xFFFFFFFFu, mine.len, l);
+            st.it.x.before = __shfl_sync(0xFFFFFFFFu, mine.before, l);
             break;
         }
         before += __shfl_sync(0xFFFFFFFFu, sum, 31);

@@ -49,6 +49,7 @@ __global__ void __launch_bounds__(SHORT_THREADS) attention_short_kernel(const __
             block -= __shfl_sync(0xFFFFFFFFu, sum - blocks, l);
             x.q0 = __shfl_sync(0xFFFFFFFFu, mine.q0, l), x.n = __shfl_sync(0xFFFFFFFFu, mine.n, l);
             x.k0 = __shfl_sync(0xFFFFFFFFu, mine.k0, l), x.len = __shfl_sync(0xFFFFFFFFu, mine.len, l);
+            x.before = __shfl_sync(0xFFFFFFFFu, mine.before, l);
             found = true;
         } else {
             block -= __shfl_sync(0xFFFFFFFFu, sum, 31);
