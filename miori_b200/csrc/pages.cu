@@ -151,7 +151,7 @@ struct RopeArgs {
     int64_t row, k_page, k_head, k_slot, v_page, v_head, v_slot;  // strides in elements
     uint32_t tokens, heads, kv_heads, rotary, num_axes, page, pages, parts;
     float eps;
-    uint32_t early;  // weights may be read ahead of the wait
+    uint32_t early;  // turns and axes may be read ahead of the wait
 };
 
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
@@ -206,8 +206,8 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_kv_kernel(const RopeArgs a)
 #pragma unroll
         for (uint32_t i = 0; i < PER; ++i) {
             const uint32_t j = 8u * u + lane / TPH * PER + i;
-            turn[i] = __ldg(a.turns + j);
-            axis[i] = a.axes ? min((uint32_t)__ldg(a.axes + j), a.num_axes - 1u) : 0u;
+            turn[i] = ld_fresh(a.turns + j);
+            axis[i] = a.axes ? min((uint32_t)ld_fresh(a.axes + j), a.num_axes - 1u) : 0u;
         }
     }
     pdl_wait_prior();
@@ -255,8 +255,8 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_kv_kernel(const RopeArgs a)
             if (gamma) {
                 const float inv = rsqrtf(sum * (1.0f / D) + a.eps);
                 float gx[8], gy[8];
-                unpack8(__ldg(reinterpret_cast<const uint4*>(gamma + e0)), gx);
-                unpack8(__ldg(reinterpret_cast<const uint4*>(gamma + e1)), gy);
+                unpack8(ld_fresh(reinterpret_cast<const uint4*>(gamma + e0)), gx);
+                unpack8(ld_fresh(reinterpret_cast<const uint4*>(gamma + e1)), gy);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) x[j] *= inv * gx[j], y[j] *= inv * gy[j];
             }
