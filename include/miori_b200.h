@@ -386,8 +386,9 @@ int miori_gemv8_rmsnorm(const void* q, const void* s, const void* b, const void*
  * pool[*taken], pool[*taken + 1], ..., in the order of the requests, and are written into table[r][..].  Out:
  * cu[requests + 1], the first token of each request; held_after[r]; *taken_after; and for each of `tokens`
  * tokens positions[t] and slots[t].  Where the table or the pool is too short slots are -1 (and new table entries -1 too):
- * *taken_after > pool_size tells.  tokens behind cu[requests] get slot -1 and position 0.  No output but
- * the table may be an input too. */
+ * *taken_after > pool_size tells.  So they are where a request would hold more than 2^31 - 1 positions (held_after stops
+ * there), or a slot's number would be 2^31 or more.  page up to 2^30; fewer than 2^31 table entries, and new tokens in
+ * all.  tokens behind cu[requests] get slot -1 and position 0.  No output but the table may be an input too. */
 int miori_page_slots(const int32_t* held, const int32_t* new_tokens, int32_t* table, const int32_t* pool,
                      const int32_t* taken, int32_t* slots, int32_t* positions, int32_t* cu, int32_t* held_after,
                      int32_t* taken_after, uint32_t requests, uint32_t width, uint32_t page, uint32_t pool_size,

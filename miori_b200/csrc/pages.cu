@@ -16,8 +16,9 @@ namespace pages {
 // Latency-bound: 8 bytes a request read and 8 a token written.  Every CTA does the prefix sums by itself (8 bytes a request
 // from L2), so that none waits for another; they then share the tokens and the new table entries.  A token's page is taken from
 // the pool and not from the table entry that another CTA writes beside it, so nothing here depends on the order of the CTAs.
+// A request holds 2^31 - 1 positions at most: its further tokens have no slot.
 // 32 requests of one token 4.7 us, 64 prompts of 41 thousand tokens 4.5.
-constexpr uint32_t SLOT_THREADS = 512, TOKENS_PER_CTA = 4 * SLOT_THREADS, MAX_REQUESTS = 16384;
+constexpr uint32_t SLOT_THREADS = 512, TOKENS_PER_CTA = 4 * SLOT_THREADS, MAX_REQUESTS = 16384, MAX_POSITIONS = 0x7FFFFFFFu;
 
 struct SlotArgs {
     const int32_t *held, *fresh;
@@ -46,7 +47,7 @@ __global__ void __launch_bounds__(SLOT_THREADS) page_slots_kernel(const SlotArgs
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
     pdl_launch_dependents();
     pdl_wait_prior();
-    const int32_t cap = (int32_t)a.width, page = (int32_t)a.page;
+    const int32_t cap = (int32_t)a.width;
     const int32_t taken = ld_fresh(a.taken);
     auto owned = [&](int32_t n) { return min((int32_t)(((uint32_t)n + a.page - 1u) / a.page), cap); };
     int2 base = make_int2(0, 0);
@@ -56,8 +57,9 @@ __global__ void __launch_bounds__(SLOT_THREADS) page_slots_kernel(const SlotArgs
         if (r < a.requests) {
             const int32_t held = max(ld_fresh(a.held + r), 0);
             mine.x = max(ld_fresh(a.fresh + r), 0);
-            mine.y = owned(held + mine.x) - owned(held);
-            if (blockIdx.x == 0) a.held_after[r] = held + mine.x;
+            const int32_t after = (int32_t)min((uint32_t)held + (uint32_t)mine.x, MAX_POSITIONS);
+            mine.y = owned(after) - owned(held);
+            if (blockIdx.x == 0) a.held_after[r] = after;
         }
         int2 sum = mine;
 #pragma unroll
@@ -94,10 +96,10 @@ __global__ void __launch_bounds__(SLOT_THREADS) page_slots_kernel(const SlotArgs
         const int64_t at = (int64_t)taken + j;
         return at >= 0 && at < (int64_t)a.pool_size ? ld_fresh(a.pool + at) : -1;
     };
-    for (int32_t j = (int32_t)(blockIdx.x * SLOT_THREADS + threadIdx.x); j < new_pages; j += (int32_t)(gridDim.x * SLOT_THREADS)) {
-        const uint32_t r = row_of(first_page, a.requests + 1u, j);
+    for (uint32_t j = blockIdx.x * SLOT_THREADS + threadIdx.x; j < (uint32_t)new_pages; j += gridDim.x * SLOT_THREADS) {
+        const uint32_t r = row_of(first_page, a.requests + 1u, (int32_t)j);
         const int32_t held = max(ld_fresh(a.held + r), 0);
-        a.table[(size_t)r * a.width + (uint32_t)(owned(held) + j - first_page[r])] = from_pool(j);
+        a.table[(size_t)r * a.width + (uint32_t)(owned(held) + (int32_t)j - first_page[r])] = from_pool((int32_t)j);
     }
     // four tokens a thread, stored as one piece each way where the outputs are 16-byte aligned
     const uint32_t t0 = blockIdx.x * TOKENS_PER_CTA + threadIdx.x * 4u;
@@ -113,11 +115,13 @@ __global__ void __launch_bounds__(SLOT_THREADS) page_slots_kernel(const SlotArgs
         if (t >= total || t0 + i >= a.tokens) continue;
         while (t >= first_token[r + 1u]) ++r, known = false;
         if (!known) held = max(ld_fresh(a.held + r), 0), own = owned(held), known = true;
-        pos[i] = held + t - first_token[r];
-        const int32_t col = pos[i] / page;
-        if (col >= cap) continue;
+        const uint32_t at = (uint32_t)held + ((uint32_t)t - (uint32_t)first_token[r]);
+        pos[i] = (int32_t)min(at, MAX_POSITIONS);
+        const int32_t col = (int32_t)((uint32_t)pos[i] / a.page);
+        if (at >= MAX_POSITIONS || col >= cap) continue;
         const int32_t p = col < own ? ld_fresh(a.table + (size_t)r * a.width + (uint32_t)col) : from_pool(first_page[r] + col - own);
-        if (p >= 0) slot[i] = p * page + pos[i] % page;
+        const int64_t to = (int64_t)p * a.page + (uint32_t)pos[i] % a.page;
+        if (to >= 0 && to <= 0x7FFFFFFF) slot[i] = (int32_t)to;  // slots are int32
     }
     if (t0 + 4u <= a.tokens && a.aligned) {
         *reinterpret_cast<int4*>(a.slots + t0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
@@ -296,6 +300,8 @@ MIORI_API int miori_page_slots(const int32_t* held, const int32_t* fresh, int32_
         return fail(MIORI_E_INVALID, "page_slots: null pointer");
     if (requests == 0 || requests > MAX_REQUESTS) return fail(MIORI_E_INVALID, "page_slots: 1..%u requests, got %u", MAX_REQUESTS, requests);
     if (width == 0 || page == 0) return fail(MIORI_E_INVALID, "page_slots: empty table or page (width=%u page=%u)", width, page);
+    if (page > (1u << 30)) return fail(MIORI_E_INVALID, "page_slots: pages of up to 2^30 positions, got %u", page);
+    if ((uint64_t)requests * width > 0x7FFFFFFFull) return fail(MIORI_E_INVALID, "page_slots: a table of 2^31 entries or more");
     if (tokens > 0x7FFFFFFFu - TOKENS_PER_CTA) return fail(MIORI_E_INVALID, "page_slots: too many tokens (%u)", tokens);
     if (held_after == held || held_after == fresh || taken_after == taken || cu == held || cu == fresh)
         return fail(MIORI_E_INVALID, "page_slots: every CTA reads the inputs, none may be an output too");
