@@ -3,8 +3,15 @@
 // Tensor-bound: 4 * D operations a (row, key) pair, and one exponential.
 //
 // * An item has up to 256 rows: two tiles of 128 rows (tokens x the heads that share the key head).  Per tile of 128 keys a row
-//   tile takes S = Q K^T (128 x 128 x D) into TMEM, its softmax, and O += P V (128 x D x 128) with P read from TMEM,
-//   where it lies over the S it came from.  TMEM: S0, S1 (128 columns each), O0, O1 (D each).
+//   tile takes S = Q K^T (128 x 128 x D) into TMEM, its softmax, and O += P V (128 x D x 128) with P read from TMEM.
+//   TMEM: O0, O1 (D columns each), P0, P1 (64 each), and S in what is left: with D = 64 128 columns for each row tile, with D = 128
+//   128 that both use in turn, which they can since a softmax loads its S whole and at once.
+// * MMAs with different accumulators complete in no order that is promised, so what one reads and another writes is handed over by
+//   barriers and commits alone.  D = 64: the next scores are issued behind a tile's product, so that the commit that hands them to
+//   the softmax says that the product is complete too, O stands still and P may be written.  D = 128: the next scores are issued in front
+//   of it, once the softmax of the other row tile has loaded its own (s_free), and the softmax waits for the product
+//   by itself (o_full).  Scores over the P that a product may still be reading would save those two waits
+//   (prompts of up to 8192 tokens of 128 dimensions 376 us, so 387), in an order that nothing guarantees.
 // * Warps 0-3 and 4-7 are the softmax of the two row tiles, a thread a row: no shuffle anywhere.  The two take turns on the
 //   tensor cores: while one exponentiates, the other's products run.  Warp 8 issues the copies (TMA, 128-byte swizzle, a
 //   ring of tiles: keys, values, keys, ...), an elected thread of warp 9 the MMAs, warps 10-11 look through the values of edge tiles.
@@ -44,8 +51,12 @@ struct PromptCfg {
     static constexpr int STAGES = D == 128 ? 5 : 10;
     static constexpr int SMEM = 1024 + (2 + STAGES) * TILE_BYTES;
     static constexpr int PART_FLOATS = 2 * ROW_TILE * (D + 2);  // [D / 4][256] pieces of O, then m and l
+    // columns of TMEM, 512 in all
+    static constexpr int SCORES = D == 64 ? 2 : 1;         // places for S
+    static constexpr int P_COLUMN = SCORES * KEYS, O_COLUMN = P_COLUMN + KEYS;
+    static_assert(O_COLUMN + 2 * D == 512, "TMEM");
 };
-constexpr int SETMAXNREG_SOFTMAX = 192, SETMAXNREG_OTHERS = 120;  // 256 * 192 + 128 * 120 = 384 * 168, what a launch has; 208 and 88 1.5 % slower
+constexpr int SETMAXNREG_SOFTMAX = 184, SETMAXNREG_OTHERS = 136;  // 256 * 184 + 128 * 136 = 384 * 168, what a launch has; 192 and 120 1 % slower
 static_assert(256 * SETMAXNREG_SOFTMAX + 128 * SETMAXNREG_OTHERS <= PROMPT_THREADS * 168, "a split above the launch's registers waits forever");
 
 // ---- how the work is dealt ---------------------------------------------------------------
@@ -296,7 +307,7 @@ template <int D, bool PAGED>
 __global__ void __launch_bounds__(PROMPT_THREADS, 1)
 attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Args a) {
     using C = PromptCfg<D>;
-    constexpr uint32_t ST = C::STAGES, BARS = 4 * ST + 10;
+    constexpr uint32_t ST = C::STAGES, BARS = 4 * ST + 11;
     extern __shared__ uint8_t smem[];
     __shared__ __align__(8) uint64_t bars[BARS];
     __shared__ uint32_t tmem_slot, dirty_item[8];
@@ -317,8 +328,9 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     const uint32_t q_full = bar(4 * ST), q_empty = bar(4 * ST + 1);
     auto s_full = [&](uint32_t t) { return bar(4 * ST + 2 + t); };
     auto p_full = [&](uint32_t t) { return bar(4 * ST + 4 + t); };
-    auto o_full = [&](uint32_t t) { return bar(4 * ST + 6 + t); };  // the item's O is complete
+    auto o_full = [&](uint32_t t) { return bar(4 * ST + 6 + t); };  // the item's O is complete; D = 128: the tile's product is
     auto o_free = [&](uint32_t t) { return bar(4 * ST + 8 + t); };  // the item's O has been read
+    const uint32_t s_free = bar(4 * ST + 10);                          // D = 128: S has been loaded
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
 
     pdl_launch_dependents();
@@ -327,6 +339,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         for (uint32_t i = 0; i < ST; ++i) mbar_init(full(i), 1), mbar_init(empty(i), 1), mbar_init(raw(i), 1), mbar_init(checked(i), 2);
         mbar_init(q_full, 1), mbar_init(q_empty, 1);
         for (uint32_t t = 0; t < 2; ++t) mbar_init(s_full(t), 1), mbar_init(p_full(t), 4), mbar_init(o_full(t), 1), mbar_init(o_free(t), 4);
+        mbar_init(s_free, 4);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_q) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
@@ -436,24 +449,27 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
             constexpr uint32_t idesc_s = mma_desc(KEYS, false), idesc_o = mma_desc(D, true);
             const uint32_t tm = uniform(tmem);
             const uint64_t rows = smem_desc(q_at, 16u), keys = smem_desc(ring, 16u), values = smem_desc(ring, C::BLOCK);
-            uint32_t place = 0, full_turns = 0, check_turns = 0, n_item = 0, n_p = 0, n_p1 = 0, n_o = 0, n_o1 = 0;
+            uint32_t place = 0, full_turns = 0, check_turns = 0, n_item = 0, n_p = 0, n_p1 = 0, n_o = 0, n_o1 = 0, n_s = 0;
             auto wait_full = [&](uint32_t s, uint32_t where) {
                 const bool there = warp_wait(full(s), full_turns >> s & 1u, &abort_flag, where);
                 full_turns ^= 1u << s;
                 return there;
             };
             auto scores = [&](uint32_t t, uint32_t s, bool last) {
+                if (C::SCORES == 1 && !warp_wait(s_free, (n_s++ & 1u) ^ 1u, &abort_flag, 13)) return false;
+                fence_after();
                 const uint64_t q = rows + t * (C::TILE_BYTES / 16u), at = keys + s * (C::TILE_BYTES / 16u);
                 if (elect_one()) {
 #pragma unroll
                     for (uint32_t k = 0; k < D / 16u; ++k) {  // 16 dimensions, 32 bytes further in the 128-byte rows
                         const uint32_t step = (k / 4u) * (C::BLOCK / 16u) + (k % 4u) * 2u;
-                        mma_ss(tm + t * KEYS, q + step, at + step, idesc_s, k > 0u);
+                        mma_ss(tm + t % C::SCORES * KEYS, q + step, at + step, idesc_s, k > 0u);
                     }
                     mma_commit(s_full(t));
                     if (last) mma_commit(empty(s));  // the keys have been read
                 }
                 __syncwarp();
+                return true;
             };
             while (__all_sync(0xFFFFFFFFu, it.start < end)) {
                 const Span span = span_of(it, begin, end, split);
@@ -463,14 +479,11 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                     if (!warp_wait(q_full, n_item & 1u, &abort_flag, 3)) break;
                     ++n_item;
                     if (!wait_full(place, 4)) break;
-                    fence_after();
-                    scores(0u, place, !second);
-                    if (second) scores(1u, place, true);
-                    bool ok = true;
+                    bool ok = scores(0u, place, !second) && (!second || scores(1u, place, true));
+                    if (!ok) break;
                     for (uint32_t k = k0; k < k1; ++k) {
                         const uint32_t vs = place + 1u == ST ? 0u : place + 1u, ks = vs + 1u == ST ? 0u : vs + 1u;
                         const bool more = k + 1u < k1;
-                        if (!more && elect_one()) mma_commit(q_empty);  // the last scores are under way
                         if (k >= edge) {
                             ok = warp_wait(checked(vs), check_turns >> vs & 1u, &abort_flag, 6);
                             check_turns ^= 1u << vs;
@@ -478,6 +491,8 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                             ok = wait_full(vs, 5);
                         }
                         if (!ok) break;
+                        if (!more && elect_one()) mma_commit(q_empty);  // the last scores are under way
+                        if (more && !(ok = wait_full(ks, 4))) break;
                         // groups of 16 keys that some row sees: one at least, which then begins O
                         const uint32_t steps = sees > k * KEYS ? (min(sees - k * KEYS, (uint32_t)KEYS) + 15u) / 16u : 1u;
                         const uint64_t at = values + vs * (C::TILE_BYTES / 16u);
@@ -490,7 +505,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                             ++p_turn;
                             fence_after();
                             if (elect_one()) {
-                                const uint32_t o = tm + 2u * KEYS + t * D, p = tm + t * KEYS;
+                                const uint32_t o = tm + C::O_COLUMN + t * D, p = tm + C::P_COLUMN + t * (KEYS / 2);
                                 if (steps == KEYS / 16u) {
 #pragma unroll
                                     for (uint32_t i = 0; i < KEYS / 16u; ++i) mma_ts(o, p + 8u * i, at + 128u * i, idesc_o, k > k0 || i > 0u);  // 16 keys, 2048 bytes further
@@ -498,22 +513,17 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
 #pragma unroll 1
                                     for (uint32_t i = 0; i < steps; ++i) mma_ts(o, p + 8u * i, at + 128u * i, idesc_o, k > k0 || i > 0u);
                                 }
-                                if (k + 1u == k1) mma_commit(o_full(t));
+                                if (C::SCORES == 1 || !more) mma_commit(o_full(t));
                                 if (last) mma_commit(empty(vs));
                             }
                             __syncwarp();
                             return true;
                         };
-                        if (!(ok = add(0u, n_o, n_p, !second))) break;
-                        if (more) {
-                            if (!(ok = wait_full(ks, 4))) break;
-                            fence_after();
-                            scores(0u, ks, !second);
-                        }
-                        if (second) {
-                            if (!(ok = add(1u, n_o1, n_p1, true))) break;
-                            if (more) scores(1u, ks, true);
-                        }
+                        auto go_on = [&](uint32_t t, uint32_t& o_turn, uint32_t& p_turn, bool last) {
+                            if (C::SCORES == 2) return add(t, o_turn, p_turn, last) && (!more || scores(t, ks, last));
+                            return (!more || scores(t, ks, last)) && add(t, o_turn, p_turn, last);
+                        };
+                        if (!(ok = go_on(0u, n_o, n_p, !second) && (!second || go_on(1u, n_o1, n_p1, true)))) break;
                         place = ks;
                     }
                     if (!ok) break;
@@ -584,7 +594,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         // ---- softmax of a row tile, a thread a row
         const uint32_t t = warp >> 2, row = threadIdx.x & 127u;
         const uint32_t lanes = ((warp & 3u) * 32u) << 16;
-        const uint32_t s_at = tmem + lanes + t * KEYS, o_at = tmem + lanes + 2u * KEYS + t * D;
+        const uint32_t s_at = tmem + lanes + t % C::SCORES * KEYS, p_at = tmem + lanes + C::P_COLUMN + t * (KEYS / 2), o_at = tmem + lanes + C::O_COLUMN + t * D;
         const bool wide = (reinterpret_cast<uintptr_t>(a.out) & 31u) == 0u && a.o_token % 16 == 0 && a.o_head % 16 == 0;
         uint32_t n_s = 0, n_o = 0, n_item = 0, tile0 = 0;  // tile0: key tiles of the items before
         uint4 to_join = make_uint4(0u, 0u, 0u, 0u);
@@ -607,6 +617,11 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
 #pragma unroll
                         for (int c = 0; c < 4; ++c) tmem_load32(s_at + 32u * c, s + 32 * c);
                         tmem_wait_load();
+                        if (C::SCORES == 1) {
+                            fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(s_free);
+                        }
                         if (k >= edge) {
                             const uint32_t key0 = k * KEYS;
                             const uint32_t count = sees > key0 ? sees - key0 : 0u;
@@ -628,6 +643,11 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                         }
                         float now = max3_nan(max3_nan(top[0], top[1], top[2]), max3_nan(top[3], s[KEYS - 4], s[KEYS - 3]), max3_nan(s[KEYS - 2], s[KEYS - 1], top[0])) * a.scale_log2;
                         if (now == INFINITY) now = NAN;  // inf - inf, for the whole row
+                        if (C::SCORES == 1 && k > span.k0) {  // the product before is complete: P may be written, O stands still
+                            ok = warp_wait(o_full(t), n_o++ & 1u, &abort_flag, 11);
+                            if (!ok) break;
+                            fence_after();
+                        }
                         if (k == span.k0) {
                             m = now;
                         } else if (__any_sync(0xFFFFFFFFu, !(now <= m + 8.0f))) {
@@ -635,7 +655,6 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                             const float keep = now == -INFINITY ? 1.0f : exp2_fast(m - now);
                             m = now;
                             l *= keep;
-                            // O stands still: the product before was issued in front of these scores, and they are complete
 #pragma unroll 1
                             for (uint32_t c = 0; c < D; c += 16u) {
                                 float o[16];
@@ -660,7 +679,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                                 x = exp2_fast(x), y = exp2_fast(y);
                                 p[j] = pack_bf16(x, y);
                             }
-                            tmem_store16(s_at + c / 2, p);
+                            tmem_store16(p_at + c / 2, p);
                         }
                         tmem_wait_store();
                         fence_before();
