@@ -310,7 +310,9 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     constexpr uint32_t ST = C::STAGES, BARS = 4 * ST + 11;
     extern __shared__ uint8_t smem[];
     __shared__ __align__(8) uint64_t bars[BARS];
-    __shared__ uint32_t tmem_slot, dirty_item[8];
+    // Items of either row tile from whose values something was left out.  The ring holds five tiles, and a row tile's next item but one is
+    // multiplied only after it has read the word of this one: eight words are enough.
+    __shared__ uint32_t tmem_slot, dirty_item[2][8];
     // Of the last eight key tiles, a bit for each eight keys: no page.  Tile n + 8 is copied after the values of tile n + 5 at least have
     // been multiplied, and so after every softmax has read the word of tile n.
     __shared__ volatile uint32_t absent[8];
@@ -345,7 +347,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
     }
-    if (threadIdx.x < 8) dirty_item[threadIdx.x] = 0u;
+    if (threadIdx.x < 16) dirty_item[threadIdx.x / 8u][threadIdx.x % 8u] = 0u;
     if (warp == 9) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&tmem_slot)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -532,7 +534,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
             }
         } else {
             // ---- values of edge tiles: half the rows for each of two warps
-            uint32_t n_tile = 0, n_item = 0, turns = 0;
+            uint32_t n_tile = 0, n_item[2] = {}, turns = 0;
             bool ok = true;
             while (ok && it.start < end) {
                 const Span span = span_of(it, begin, end, split);
@@ -580,11 +582,14 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                             }
                         }
                         if (bad || rows < stop) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                        if (bad && lane == 0) dirty_item[n_item & 7u] = n_item + 1u;
+                        if (bad && lane == 0) {
+                            dirty_item[0][n_item[0] & 7u] = n_item[0] + 1u;
+                            if (has_second()) dirty_item[1][n_item[1] & 7u] = n_item[1] + 1u;
+                        }
                         __syncwarp();
                         if (lane == 0) mbar_arrive(checked(s));
                     }
-                    ++n_item;
+                    ++n_item[0], n_item[1] += has_second();
                 }
                 it.next<PAGED>(a, per_item, end);
             }
@@ -602,8 +607,8 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         while (ok && it.start < end) {
             const Span span = span_of(it, begin, end, split);
             if (span.k1 > span.k0) {
-                const uint32_t item_id = n_item++;
                 if (t == 0u || has_second()) {
+                    const uint32_t item_id = n_item++;
                     const uint32_t i = it.t * per_item + t * per_tile + row / group;
                     const bool there = row < per_tile * group && i < it.x.n;
                     const uint32_t sees = there ? seen(a, it.x, i) : 0u;
@@ -699,7 +704,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                     ++n_o;
                     if (!ok) break;
                     fence_after();
-                    const bool dirty = *(volatile uint32_t*)&dirty_item[item_id & 7u] == item_id + 1u;
+                    const bool dirty = *(volatile uint32_t*)&dirty_item[t][item_id & 7u] == item_id + 1u;
                     const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;  // no key: zeros; NaN stays
                     const float factor = span.whole ? inv : 1.0f;
                     uint16_t* const to = a.out + (int64_t)(it.x.q0 + (there ? i : 0u)) * a.o_token + (int64_t)(it.head * group + row % group) * a.o_head;
