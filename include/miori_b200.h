@@ -418,7 +418,7 @@ size_t miori_attention_workspace_bytes(void);
  * power of two from 8 to 65536.  table [requests][width]: positions whose entry is no page of the cache are seen by no token.
  * strides in elements, positive multiples of 8: token and head of q, token and head of out, page, head and slot of
  * k_cache, the same of v_cache.  max_new: the most tokens that a request has in this call; it decides only which kernel
- * runs.  Sums and softmax in fp32, probabilities rounded to bf16 for their product with v. */
+ * runs.  Sums and softmax in fp32, probabilities rounded to bf16 for their product with v and for their sum. */
 int miori_attention_paged(const void* q, const void* k_cache, const void* v_cache, void* out, const int64_t* strides,
                           const int32_t* table, const int32_t* lens, const int32_t* cu, uint32_t requests,
                           uint32_t tokens, uint32_t width, uint32_t pages, uint32_t page, uint32_t heads,

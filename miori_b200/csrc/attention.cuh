@@ -43,6 +43,14 @@ __device__ __forceinline__ float exp2_fast(float x) {  // 2^x, 2 ulp, 0 for x = 
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// A pair of bf16 added up in fp32 without being unpacked: the lower to x and the upper to y, or both to one sum.
+__device__ __forceinline__ void add_bf16(float& x, float& y, uint32_t pair) {
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tadd.rn.f32.bf16 %0, lo, %0;\n\tadd.rn.f32.bf16 %1, hi, %1;\n\t}" : "+f"(x), "+f"(y) : "r"(pair));
+}
+__device__ __forceinline__ float add_bf16(float sum, uint32_t pair) {
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tadd.rn.f32.bf16 %0, lo, %0;\n\tadd.rn.f32.bf16 %0, hi, %0;\n\t}" : "+f"(sum) : "r"(pair));
+    return sum;
+}
 // Bits of a pair of bf16 with those halves zero that are not finite.
 __device__ __forceinline__ uint32_t finite_or_zero(uint32_t pair) {
     if ((pair & 0x7F80u) == 0x7F80u) pair &= 0xFFFF0000u;

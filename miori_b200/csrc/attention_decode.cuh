@@ -13,7 +13,9 @@
 // * A CTA's share may begin and end inside an item.  The warps' parts meet in shared memory at the end of an item; an item
 //   shared by several CTAs meets in the workspace: the CTA that arrives last adds the parts up in the order of the keys, so a
 //   result does not depend on which one that is.
-// * P is rounded to bf16 for the second product, as the values are; l sums the unrounded p.
+// * P is rounded to bf16 for the second product, as the values are, since an MMA has one type for both; l sums the rounded p, so that
+//   O / l is a mean of values whatever their weights are off by: a key that outweighs all others is weighed by one, although its p
+//   is not one with a maximum that stands still.
 //
 // 32 requests of up to 32768 positions (719 MB), 16 heads of 128 over 4: 120 us, 5.9 TB/s (a copy reaches 6.56; DRAM reads are 1.001 of the
 // bytes).  One request of 1000: 8.1 us, latency.  9 requests of 5 drafts and up to 5000 positions, 32 heads of 64 over 8: 19.6 us, bound by
@@ -301,8 +303,8 @@ __global__ void __launch_bounds__(DECODE_THREADS, 1) attention_decode_kernel(con
 #pragma unroll
                     for (int j = 0; j < 4; ++j) s[n][j] = gone >> (j / 2) & 1u ? -INFINITY : s[n][j];
             }
-            // The running maximum moves only when a score exceeds it by 2^8 (p grows up to 256 then, which costs no precision): most tiles
-            // need neither the maximum over the lanes nor a rescaled O.
+            // The running maximum moves only when a score exceeds it by 2^8 (p grows up to 256 then): most tiles need neither the
+            // maximum over the lanes nor a rescaled O.
             uint32_t pf[NT][2];
             const uint32_t key = key0 + lane / 4u;
             bool higher = false;
@@ -333,9 +335,9 @@ __global__ void __launch_bounds__(DECODE_THREADS, 1) attention_decode_kernel(con
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) s[n][j] = exp2_fast(s[n][j] - (m[n][j & 1] == -INFINITY ? 0.0f : m[n][j & 1]));
-                l[n][0] += s[n][0] + s[n][2], l[n][1] += s[n][1] + s[n][3];
-                pf[n][0] = movmatrix(pack_bf16(s[n][0], s[n][1]));
-                pf[n][1] = movmatrix(pack_bf16(s[n][2], s[n][3]));
+                const uint32_t low = pack_bf16(s[n][0], s[n][1]), high = pack_bf16(s[n][2], s[n][3]);
+                add_bf16(l[n][0], l[n][1], low), add_bf16(l[n][0], l[n][1], high);
+                pf[n][0] = movmatrix(low), pf[n][1] = movmatrix(high);
             }
 #pragma unroll
             for (int k = 0; k < KS; ++k) {

@@ -15,9 +15,12 @@
 // * Warps 0-3 and 4-7 are the softmax of the two row tiles, a thread a row: no shuffle anywhere.  The two take turns on the
 //   tensor cores: while one exponentiates, the other's products run.  Warp 8 issues the copies (TMA, 128-byte swizzle, a
 //   ring of tiles: keys, values, keys, ...), an elected thread of warp 9 the MMAs, warps 10-11 look through the values of edge tiles.
-// * The running maximum moves only when a row's exceeds it by 2^8: until then p grows up to 256, which costs no precision in
-//   fp32 sums and bf16 rounding, and O stays where it is.  O is rescaled by the softmax warps themselves, in TMEM.
-// * P is rounded to bf16 for the second product, as the values are; l sums the unrounded p.
+// * The running maximum moves only when a row's exceeds it by 2^8: until then p grows up to 256 and O stays where it is.  O is rescaled
+//   by the softmax warps themselves, in TMEM.
+// * P is rounded to bf16 for the second product, as the values are, since an MMA has one type for both; l sums the rounded p, so that
+//   O / l is a mean of values whatever their weights are off by: a key that outweighs all others is weighed by one, although its p
+//   is not one with a maximum that stands still.  (Sums of the unrounded p: prompts of up to 8192 tokens 387 us, so 395, but off by up
+//   to 2^-8 where one key dominates.  The rounded p unpacked and added as fp32 pairs 404, added on mma.sync 401.)
 // * Tried and dropped (432 GFLOP of prompts up to 8192, us): an MMA warp for each row tile (454), the MMAs issued by the softmax warps
 //   (473), scores of 64 keys double-buffered (684 as issued then: twice the steps), the product begun at half of the probabilities
 //   (403 - 430), a quarter or half of the exponentials by a polynomial on the FMA pipe (404, 466), exponentials with the maximum
@@ -276,11 +279,6 @@ __device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) { asm("
 __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
     uint64_t r;
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {  // NaN if any of them is
@@ -672,6 +670,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                             tmem_wait_store();
                         }
                         const float from = m == -INFINITY ? 0.0f : -m;
+                        float sum[4] = {};
                         const uint64_t scale2 = pair(a.scale_log2, a.scale_log2), from2 = pair(from, from);
 #pragma unroll
                         for (int c = 0; c < KEYS; c += 32) {
@@ -683,6 +682,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                                 unpair(e, x, y);
                                 x = exp2_fast(x), y = exp2_fast(y);
                                 p[j] = pack_bf16(x, y);
+                                sum[j & 3] = add_bf16(sum[j & 3], p[j]);
                             }
                             tmem_store16(p_at + c / 2, p);
                         }
@@ -690,14 +690,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                         fence_before();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(p_full(t));
-                        uint64_t sum[4];  // while the product runs
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) sum[j] = pair(s[2 * j], s[2 * j + 1]);
-#pragma unroll
-                        for (int j = 4; j < KEYS / 2; ++j) sum[j & 3] = add2(sum[j & 3], pair(s[2 * j], s[2 * j + 1]));
-                        float sl, sh;
-                        unpair(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), sl, sh);
-                        l += sl + sh;
+                        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                     }
                     if (!ok) break;
                     ok = warp_wait(o_full(t), n_o & 1u, &abort_flag, 12);

@@ -8,7 +8,8 @@
 //   (ldmatrix, ldmatrix.trans), and the scores' accumulators are the probabilities' A operand as they lie.
 // * Blocks are dealt by the grid: (block, key head), the host's bound on the blocks being tokens / tokens-a-block + requests.
 // * What a row must not see: rows past the end arrive as zeros, values that are not finite are zeroed in every tile that some row
-//   does not see as a whole and added at the end for the rows that see them.  P is rounded to bf16, l sums the unrounded p.
+//   does not see as a whole and added at the end for the rows that see them.  P is rounded to bf16, l sums
+//   the rounded p: see attention_decode.cuh.
 //
 // Latency-bound: one prompt of 77 tokens 6.5 us (the prompt kernel 11.1), 32 of 32 7.3 (12.4), 16 heads of 128 over 4.
 #pragma once
@@ -79,7 +80,7 @@ __global__ void __launch_bounds__(SHORT_THREADS) attention_short_kernel(const __
 
     // rows lane / 4 and lane / 4 + 8 of the warp's sixteen
     uint32_t qf[KS][4], sees[2];
-    float o[2 * KS][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {};
+    float o[2 * KS][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {}, l_odd[2] = {};
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const uint32_t row = 16u * warp + lane / 4u + 8u * h, i = row / group;
@@ -117,6 +118,7 @@ __global__ void __launch_bounds__(SHORT_THREADS) attention_short_kernel(const __
         }
         if (__syncthreads_or(bad) && dirty_from == 0xFFFFFFFFu) dirty_from = tile;
         float s[NK][4];
+        uint32_t p[NK][2];
 #pragma unroll
         for (int n = 0; n < NK; ++n)
 #pragma unroll
@@ -145,28 +147,24 @@ __global__ void __launch_bounds__(SHORT_THREADS) attention_short_kernel(const __
             top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
             const float now = fmaxf(m[h], top), from = now == -INFINITY ? 0.0f : now, keep = exp2_fast(m[h] - from);
             m[h] = now;
-            l[h] *= keep;
+            l[h] *= keep, l_odd[h] *= keep;
 #pragma unroll
-            for (int n = 0; n < NK; ++n)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    float& t = s[n][2 * h + j];
-                    t = exp2_fast(t - from);
-                    l[h] += t;
-                }
+            for (int n = 0; n < NK; ++n) {
+                p[n][h] = pack_bf16(exp2_fast(s[n][2 * h] - from), exp2_fast(s[n][2 * h + 1] - from));
+                add_bf16(l[h], l_odd[h], p[n][h]);
+            }
 #pragma unroll
             for (int d = 0; d < 2 * KS; ++d) o[d][2 * h] *= keep, o[d][2 * h + 1] *= keep;
         }
 #pragma unroll
         for (int k = 0; k < NK / 2; ++k) {
-            const uint32_t p[4] = {pack_bf16(s[2 * k][0], s[2 * k][1]), pack_bf16(s[2 * k][2], s[2 * k][3]), pack_bf16(s[2 * k + 1][0], s[2 * k + 1][1]),
-                                   pack_bf16(s[2 * k + 1][2], s[2 * k + 1][3])};
+            const uint32_t pa[4] = {p[2 * k][0], p[2 * k][1], p[2 * k + 1][0], p[2 * k + 1][1]};
 #pragma unroll
             for (int d = 0; d < 2 * KS; d += 2) {
                 uint32_t f[4];  // dimensions 8d .. 8d + 15 of sixteen keys
                 ldmatrix4_trans(f, vb + piece(16u * k + (lane & 15u), d + (lane >> 4)));
-                mma16816(o[d], p, f[0], f[1]);
-                mma16816(o[d + 1], p, f[2], f[3]);
+                mma16816(o[d], pa, f[0], f[1]);
+                mma16816(o[d + 1], pa, f[2], f[3]);
             }
         }
         __syncthreads();  // the tile is free
@@ -174,7 +172,7 @@ __global__ void __launch_bounds__(SHORT_THREADS) attention_short_kernel(const __
 
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        float sum = l[h];
+        float sum = l[h] + l_odd[h];
         sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
         sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
         const float inv = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum;  // no key: zeros; NaN stays
