@@ -616,6 +616,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                         ok = warp_wait(s_full(t), n_s & 1u, &abort_flag, 10);
                         if (!ok) break;
                         fence_after();
+                        const uint32_t gone = PAGED ? absent[(tile0 + k - span.k0) % 8u] : 0u;
                         float s[KEYS];
 #pragma unroll
                         for (int c = 0; c < 4; ++c) tmem_load32(s_at + 32u * c, s + 32 * c);
@@ -625,18 +626,11 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                             __syncwarp();
                             if (lane == 0) mbar_arrive(s_free);
                         }
-                        if (k >= edge) {
+                        if (k >= edge || gone) {
                             const uint32_t key0 = k * KEYS;
                             const uint32_t count = sees > key0 ? sees - key0 : 0u;
 #pragma unroll
-                            for (uint32_t j = 0; j < KEYS; ++j) s[j] = j < count ? s[j] : -INFINITY;
-                        }
-                        if (PAGED) {
-                            const uint32_t gone = absent[(tile0 + k - span.k0) % 8u];
-                            if (gone) {
-#pragma unroll
-                                for (uint32_t j = 0; j < KEYS; ++j) s[j] = gone >> (j / 8u) & 1u ? -INFINITY : s[j];
-                            }
+                            for (uint32_t j = 0; j < KEYS; ++j) s[j] = j < count && !(gone >> (j / 8u) & 1u) ? s[j] : -INFINITY;
                         }
                         float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
