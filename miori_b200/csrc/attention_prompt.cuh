@@ -45,6 +45,9 @@ namespace attention {
 constexpr int PROMPT_THREADS = 384, KEYS = 128, ROW_TILE = 128;
 constexpr uint32_t ITEM_COST = 384;     // an item's set-up and end, in positions (prompts of up to 8192: 256 386 us, 384 376, 640 384)
 constexpr uint32_t LEAST_SHARE = 256;   // positions; a tile of keys at least
+// From here on scores are scaled first and then held against the maximum, which was rounded as they are.  The one fma that does both rounds
+// at the end only, so that p is off by 2^(half an ulp of the maximum), the same for the whole row: by two here, and beyond fp32 at 2^31.
+constexpr float HUGE_SCORE = 0x1p25f;
 
 template <int D>
 struct PromptCfg {
@@ -645,15 +648,19 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                             if (!ok) break;
                             fence_after();
                         }
-                        if (k == span.k0) {
-                            m = now;
-                        } else if (__any_sync(0xFFFFFFFFu, !(now <= m + 8.0f))) {
+                        if (k == span.k0) m = now;
+                        if (__any_sync(0xFFFFFFFFu, !(now <= m + 8.0f) || fabsf(m) >= HUGE_SCORE)) {
                             now = max3_nan(now, m, m);
                             const float keep = now == -INFINITY ? 1.0f : exp2_fast(m - now);
                             m = now;
                             l *= keep;
+                            if (fabsf(m) >= HUGE_SCORE && m != -INFINITY) {  // what the fma below makes the difference of
+                                const float back = 1.0f / a.scale_log2;
+#pragma unroll
+                                for (int j = 0; j < KEYS; ++j) s[j] = __fadd_rn(__fmul_rn(s[j], a.scale_log2), -m) * back;
+                            }
 #pragma unroll 1
-                            for (uint32_t c = 0; c < D; c += 16u) {
+                            for (uint32_t c = 0; c < (k > span.k0 ? D : 0u); c += 16u) {
                                 float o[16];
                                 tmem_load16(o_at + c, o);
                                 tmem_wait_load();
@@ -663,7 +670,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                             }
                             tmem_wait_store();
                         }
-                        const float from = m == -INFINITY ? 0.0f : -m;
+                        const float from = fabsf(m) >= HUGE_SCORE ? 0.0f : -m;
                         float sum[4] = {};
                         const uint64_t scale2 = pair(a.scale_log2, a.scale_log2), from2 = pair(from, from);
 #pragma unroll
