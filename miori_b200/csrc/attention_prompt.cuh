@@ -62,7 +62,7 @@ struct PromptCfg {
     static constexpr int P_COLUMN = SCORES * KEYS, O_COLUMN = P_COLUMN + KEYS;
     static_assert(O_COLUMN + 2 * D == 512, "TMEM");
 };
-constexpr int SETMAXNREG_SOFTMAX = 184, SETMAXNREG_OTHERS = 136;  // 256 * 184 + 128 * 136 = 384 * 168, what a launch has; 192 and 120 1 % slower
+constexpr int SETMAXNREG_SOFTMAX = 200, SETMAXNREG_OTHERS = 104;  // 256 * 200 + 128 * 104 = 384 * 168, what a launch has; 192 and 120, 184 and 136 0.5 % slower, 208 and 88 5 %
 static_assert(256 * SETMAXNREG_SOFTMAX + 128 * SETMAXNREG_OTHERS <= PROMPT_THREADS * 168, "a split above the launch's registers waits forever");
 
 // ---- how the work is dealt ---------------------------------------------------------------
@@ -357,6 +357,8 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     const uint32_t group = a.group, per_tile = ROW_TILE / group, per_item = 2u * per_tile;
     const bool split = a.parts != nullptr;
     __shared__ __align__(8) uint32_t plan[sizeof(Start) / 4];
+    // where a softmax warp stands: its registers are for the scores (beside them they spilled: prompts of up to 8192 395 us, so 384)
+    __shared__ __align__(8) uint32_t places[8][sizeof(Start) / 4];
     if (warp == 8) {  // for all: the code is cold, and one warp fetches it sooner than twelve
         const Start found = find_share<PAGED>(a);
         if (lane == 0) memcpy(plan, &found, sizeof(Start));
@@ -603,8 +605,15 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         const uint32_t s_at = tmem + lanes + t % C::SCORES * KEYS, p_at = tmem + lanes + C::P_COLUMN + t * (KEYS / 2), o_at = tmem + lanes + C::O_COLUMN + t * D;
         const bool wide = (reinterpret_cast<uintptr_t>(a.out) & 31u) == 0u && a.o_token % 16 == 0 && a.o_head % 16 == 0;
         uint32_t n_s = 0, n_o = 0, n_item = 0, tile0 = 0;  // tile0: key tiles of the items before
-        uint4 to_join = make_uint4(0u, 0u, 0u, 0u);
+        memcpy(places[warp], plan, sizeof(Start));
+        __syncwarp();
+        Start& start = *reinterpret_cast<Start*>(places[warp]);
+        Item& it = start.it;
+        const uint64_t begin = start.begin, end = start.end;
+        if (split && threadIdx.x == 0) a.joins[blockIdx.x] = make_uint4(0u, 0u, 0u, 0u);
         bool ok = true;
+        auto has_second = [&]() { return it.x.n > it.t * per_item + per_tile; };
+        auto first_edge = [&](uint32_t row_tile) { return seen(a, it.x, it.t * per_item + row_tile * per_tile) / KEYS; };
         while (ok && it.start < end) {
             const Span span = span_of(it, begin, end, split);
             if (span.k1 > span.k0) {
@@ -629,27 +638,36 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                             __syncwarp();
                             if (lane == 0) mbar_arrive(s_free);
                         }
-                        if (k >= edge || gone) {
+                        if (k >= edge) {
                             const uint32_t key0 = k * KEYS;
                             const uint32_t count = sees > key0 ? sees - key0 : 0u;
 #pragma unroll
-                            for (uint32_t j = 0; j < KEYS; ++j) s[j] = j < count && !(gone >> (j / 8u) & 1u) ? s[j] : -INFINITY;
+                            for (uint32_t j = 0; j < KEYS; ++j) s[j] = j < count ? s[j] : -INFINITY;
                         }
-                        float top[4] = {s[0], s[1], s[2], s[3]};
+                        auto largest = [&] {
+                            float top[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                        for (int j = 4; j + 8 <= KEYS; j += 8) {
+                            for (int j = 4; j + 8 <= KEYS; j += 8) {
 #pragma unroll
-                            for (int c = 0; c < 4; ++c) top[c] = max3_nan(top[c], s[j + c], s[j + 4 + c]);
-                        }
-                        float now = max3_nan(max3_nan(top[0], top[1], top[2]), max3_nan(top[3], s[KEYS - 4], s[KEYS - 3]), max3_nan(s[KEYS - 2], s[KEYS - 1], top[0])) * a.scale_log2;
-                        if (now == INFINITY) now = NAN;  // inf - inf, for the whole row
+                                for (int c = 0; c < 4; ++c) top[c] = max3_nan(top[c], s[j + c], s[j + 4 + c]);
+                            }
+                            const float all = max3_nan(max3_nan(top[0], top[1], top[2]), max3_nan(top[3], s[KEYS - 4], s[KEYS - 3]), max3_nan(s[KEYS - 2], s[KEYS - 1], top[0])) * a.scale_log2;
+                            return all == INFINITY ? NAN : all;  // inf - inf, for the whole row
+                        };
+                        float now = largest();
                         if (C::SCORES == 1 && k > span.k0) {  // the product before is complete: P may be written, O stands still
                             ok = warp_wait(o_full(t), n_o++ & 1u, &abort_flag, 11);
                             if (!ok) break;
                             fence_after();
                         }
                         if (k == span.k0) m = now;
-                        if (__any_sync(0xFFFFFFFFu, !(now <= m + 8.0f) || fabsf(m) >= HUGE_SCORE)) {
+                        if (__any_sync(0xFFFFFFFFu, !(now <= m + 8.0f) || fabsf(m) >= HUGE_SCORE || gone)) {
+                            if (gone) {  // scores of no page are zeros so far; here, since a test of its own costs 5 % of a chunk's time
+#pragma unroll
+                                for (uint32_t j = 0; j < KEYS; ++j) s[j] = gone >> (j / 8u) & 1u ? -INFINITY : s[j];
+                                now = largest();
+                                if (k == span.k0) m = now;
+                            }
                             now = max3_nan(now, m, m);
                             const float keep = now == -INFINITY ? 1.0f : exp2_fast(m - now);
                             m = now;
@@ -705,7 +723,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                     float* part = nullptr;
                     if (!span.whole) {
                         const uint32_t first = start.shares.of(it.mark());
-                        if (first == blockIdx.x) to_join = make_uint4(start.shares.of(it.last_mark()) - first + 1u, it.x.q0 + it.t * per_item, it.x.n - it.t * per_item, it.head);
+                        if (first == blockIdx.x && threadIdx.x == 0) a.joins[blockIdx.x] = make_uint4(start.shares.of(it.last_mark()) - first + 1u, it.x.q0 + it.t * per_item, it.x.n - it.t * per_item, it.head);
                         part = a.parts + (size_t)(2u * blockIdx.x + (first == blockIdx.x ? 1u : 0u)) * C::PART_FLOATS;
                         part[2u * ROW_TILE * D + t * ROW_TILE + row] = m;
                         part[2u * ROW_TILE * (D + 1) + t * ROW_TILE + row] = l;
@@ -762,9 +780,10 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                 }
                 tile0 += span.k1 - span.k0;
             }
-            it.next<PAGED>(a, per_item, end);
+            __syncwarp();
+            if (lane == 0) it.next<PAGED>(a, per_item, end);
+            __syncwarp();
         }
-        if (split && threadIdx.x == 0) a.joins[blockIdx.x] = to_join;
     }
 
     // on abort give copies and MMAs in flight time to land before TMEM is freed
