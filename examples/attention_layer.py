@@ -97,6 +97,8 @@ def main(device="cuda:0"):
         graph.replay()
     end.record()
     torch.cuda.synchronize()
+    # a recorded step cannot stop where the pool runs out: positions without a page are then seen by no token, and `taken` says so
+    assert int(cache.taken) <= cache.pool.numel(), "not enough pages"
     assert mb.lib.miori_device_error_poll() == 0 and torch.isfinite(y).all()
     print(f"{len(layers)} attention layers, positions {cache.held.tolist()}: {begin.elapsed_time(end) / steps * 1e3:.1f} us a decode step, "
           f"{int(cache.taken)} pages of {cache.page} taken")

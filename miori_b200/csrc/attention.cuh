@@ -33,11 +33,6 @@ struct Args {
     float* parts;
 };
 
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
 __device__ __forceinline__ float exp2_fast(float x) {  // 2^x, 2 ulp, 0 for x = -inf
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

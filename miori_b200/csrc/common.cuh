@@ -230,6 +230,12 @@ __device__ __forceinline__ float bf16lo(uint32_t pair) { return __uint_as_float(
 __device__ __forceinline__ float bf16hi(uint32_t pair) {
     return __uint_as_float(pair & 0xFFFF0000u);
 }
+// Two fp32 as a pair of bf16, rounded to nearest, NaN kept.
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
 // RNE fp32 -> bf16 bits for finite inputs, the reference's rule (src/cpu_ref.h:16-23).
 __device__ __forceinline__ uint32_t float_to_bf16_bits(float f) {
     uint32_t u = __float_as_uint(f);
