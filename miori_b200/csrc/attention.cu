@@ -13,13 +13,15 @@
 namespace miori_b200 {
 namespace attention {
 
-// Rows of an item (new tokens x heads that share a key head) up to which the decode kernel takes a call, by the size of a head.  us, decode
-// against prompt kernel: 20 rows of 128, 8 requests of 1000 positions 21.0, 20.1; 32 rows of 128, 32 requests of 4000 115, 69; 20 rows of 64,
-// 9 requests of 3000 24.5, 29.5; 32 rows of 64, 32 requests of 4000 78.6, 93.9.
+// Rows of an item (new tokens x heads that share a key head) up to which the decode kernel takes a call, by the size of a head.  us in a
+// graph, decode against prompt kernel.  16 rows of 128: a request of 1000 positions 11.8, 14.4; 8 of 1000 13.1, 18.5; 32 of 4000 52.3, 62.2, with
+// heads that share nothing 93.2, 105.  32 rows of 64: 8 of 1000 17.0, 18.7; 9 of 3000 25.4, 29.6; 32 of 4000 76.7, 94.1.  With 32 rows
+// of 128 the decode kernel has no registers left (32 of 4000: 115 when it was tried, 69).
 constexpr uint32_t DECODE_ROWS_128 = 16, DECODE_ROWS_64 = 32;
-// Packed calls that the short kernel takes: up to 512 tokens (and keys), or up to 2048 of prompts of 64 on average.  us, short against prompt
-// kernel, 16 heads of 128 over 4: one prompt of 77 6.6, 11.1, of 256 10.3, 17.8, of 512 16.7, 20.6, of 1024 39.1, 24.5; 32 of 32
-// 7.8, 12.4; 32 of 64 13.6, 14.1; 2 of 512 22.8, 21.4.  32 heads of 64 over 8: one of 512 16.2, 17.0; 32 of 64 14.9, 17.2.
+// Packed calls that the short kernel takes: up to 512 tokens (and keys), or up to 2048 of prompts of 64 on average.  us in a graph, short
+// against prompt kernel, 16 heads of 128 over 4: one prompt of 77 6.5, 10.0, of 256 10.7, 17.2, of 448 17.6, 19.2, of 512 21, 19 (where 2 of 256
+// are 12.5, 18.2: the host knows the sum only), of 1024 39, 24.5; 32 of 32 7.4, 12.0; 32 of 64 13.2, 13.4; 2 of 512 22.3, 21.5.  32 heads of
+// 64 over 8: one of 512 18.3, 17.1; 32 of 64 14.4, 16.8.  16 heads of 64 that share nothing: one of 512 14.8, 15.7; 32 of 64 9.9, 23.4.
 static bool takes_short(uint32_t tokens, uint32_t keys, uint32_t requests) {
     const uint32_t most = tokens > keys ? tokens : keys;
     return most <= 512u || (most <= 2048u && most <= 64u * requests);

@@ -2,15 +2,17 @@
 //
 //   o[i] = sum_j softmax_j(scale * q_i . k_j) * v_j     over the positions j <= length - n + i that token i of n sees
 //
-// Both kernels (attention_decode.cuh, attention_prompt.cuh) go over the keys once with the running maximum m and sum l of a
+// The kernels (attention_decode.cuh, attention_prompt.cuh, attention_short.cuh) go over the keys once with the running maximum m and sum l of a
 // softmax, fp32: with t = scale * log2(e) * q . k, m' = max(m, t), l' = l * 2^(m - m') + sum 2^(t - m'), and o likewise.  A
 // row's keys may be split over CTAs: parts (m, l, o) of a row join as o = sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p.
 //
 // An item is a block of a request's tokens with one key head: all the query heads that share the head are rows of the item
-// (row = token * group + head), so keys and values are read once for all of them.  An item's work is its number of key
-// tiles, known on the device alone (lengths live there: a recorded graph serves every step).  So every launch is a fixed number
-// of CTAs; each finds its share [k * total / G, (k + 1) * total / G) of the tiles of all items, in order, by the same
-// arithmetic.  Shares differ by one tile whatever the lengths are, and need no list and no counter.
+// (row = token * group + head), so keys and values are read once for all of them.  An item's work is known on the device alone
+// (lengths live there: a recorded graph serves every step), so the decode and the prompt kernel are a fixed number of CTAs, and each
+// finds its share by the same arithmetic: an item costs the positions that it goes over and a constant more for its beginning and
+// end, and share k of G is units [k * size, (k + 1) * size) of all items' costs, in order, with size = ceil(total / G) and a tile of keys
+// at least.  The last shares may be shorter or empty.  That needs no list and no counter.  Without a workspace an item stays whole and belongs
+// to the share that holds its first tile.  The short kernel is dealt by its grid.
 #pragma once
 #include "common.cuh"
 

@@ -17,16 +17,17 @@
 //   O / l is a mean of values whatever their weights are off by: a key that outweighs all others is weighed by one, although its p
 //   is not one with a maximum that stands still.
 //
-// 32 requests of up to 32768 positions (719 MB), 16 heads of 128 over 4: 120 us, 5.9 TB/s (a copy reaches 6.56; DRAM reads are 1.001 of the
-// bytes).  One request of 1000: 8.1 us, latency.  9 requests of 5 drafts and up to 5000 positions, 32 heads of 64 over 8: 19.6 us, bound by
-// instructions: 32 columns of which 20 are rows.
+// 32 requests of up to 32768 positions (719 MB), 16 heads of 128 over 4: 124 us on changing inputs, 5.8 TB/s (a copy reaches 6.56; DRAM reads
+// are 1.001 of the bytes), 120 in a graph.  One request of 1000: 8.2 and 8.0 us, latency.  9 requests of 5 drafts and up to 5000 positions, 32
+// heads of 64 over 8: 22.1 and 20.6 us, bound by instructions: 32 columns of which 20 are rows.  32 requests of 8000, one token, in a graph:
+// 32 heads of 64 over 8 105.6 us (5.0 TB/s); of 4000, 16 heads that share nothing, of 64 106.8 (4.9), of 128 172 (6.1).
 #pragma once
 #include "attention.cuh"
 
 namespace miori_b200 {
 namespace attention {
 
-constexpr uint32_t DECODE_ITEM_COST = 384;  // an item's begin and end, in positions
+constexpr uint32_t DECODE_ITEM_COST = 384;  // an item's begin and end, in positions: 32 requests and drafts 119.6, 20.7 us (256 118.8, 21.7; 640 121.5, 20.4)
 constexpr int DECODE_WARPS = 8, DECODE_THREADS = DECODE_WARPS * 32, TILE = 16, UNIT = DECODE_WARPS * TILE;
 
 template <int D, int NT>

@@ -21,13 +21,15 @@
 //   O / l is a mean of values whatever their weights are off by: a key that outweighs all others is weighed by one, although its p
 //   is not one with a maximum that stands still.  (Sums of the unrounded p: prompts of up to 8192 tokens 387 us, so 395, but off by up
 //   to 2^-8 where one key dominates.  The rounded p unpacked and added as fp32 pairs 404, added on mma.sync 401.)
-// * Tried and dropped (432 GFLOP of prompts up to 8192, us): an MMA warp for each row tile (454), the MMAs issued by the softmax warps
-//   (473), scores of 64 keys double-buffered (684 as issued then: twice the steps), the product begun at half of the probabilities
-//   (403 - 430), a quarter or half of the exponentials by a polynomial on the FMA pipe (404, 466), exponentials with the maximum
-//   of the tile before, taken again where that is too low (401); 404 then, 376 (1.15 PFLOP/s) with the registers and the item's cost
-//   as they are now.  The tensor pipe is active 62 % of the cycles and the special-function unit 58 % (one prompt of 8192): a row
-//   tile's chain of scores, softmax and product is hidden by one other chain only, and the MMA warp's bookkeeping between
-//   products comes on top.
+// * 432 GFLOP of prompts of up to 8192 tokens, 16 heads of 128 over 4: 456 us (0.95 PFLOP/s) call after call, when the power limit holds the
+//   SMs at 1.66 GHz, and 387 (1.12) in a short graph.  Chunks of up to 512 tokens over 16 thousand: 177 and 148 us (0.85 and 1.02).
+//   Narrow heads: 103 and 102.  The tensor pipe is active 60 % of the cycles and the special-function unit 56 % (one prompt of 8192).  A softmax
+//   warp is busy nearly all the time (heads of 128; 3.3 thousand cycles a tile of keys, of which its exponentials alone would take one), two to an
+//   SM's quarter: what it does one after the other bounds the kernel, and each branch in its loop costs percents.
+// * Tried and dropped, all before the issue order, registers and sums as they are now, and so no proof against them (us, 404 then): an MMA warp
+//   for each row tile (454), the MMAs issued by the softmax warps (473), scores of 64 keys double-buffered (684), the product begun at
+//   half of the probabilities (403 - 430), a quarter or half of the exponentials by a polynomial on the FMA pipe (404, 466),
+//   exponentials with the maximum of the tile before, taken again where that is too low (401).
 // * Edge tiles (keys that some rows do not see, or past the end).  Their scores are masked one by one.  Their values are looked
 //   through before the product: rows past the end are zeroed (a page's unwritten tail, the next prompt's rows) and so are
 //   numbers that are not finite, since 0 * inf would reach rows that do not see them; rows that do see them get them added
@@ -43,7 +45,7 @@ namespace miori_b200 {
 namespace attention {
 
 constexpr int PROMPT_THREADS = 384, KEYS = 128, ROW_TILE = 128;
-constexpr uint32_t ITEM_COST = 384;     // an item's set-up and end, in positions (prompts of up to 8192: 256 386 us, 384 376, 640 384)
+constexpr uint32_t ITEM_COST = 384;     // an item's set-up and end, in positions: long prompts, narrow heads, chunks 387, 102, 148 us (256 389, 99, 150; 640 397, 109, 150)
 constexpr uint32_t LEAST_SHARE = 256;   // positions; a tile of keys at least
 // From here on scores are scaled first and then held against the maximum, which was rounded as they are.  The one fma that does both rounds
 // at the end only, so that p is off by 2^(half an ulp of the maximum), the same for the whole row: by two here, and beyond fp32 at 2^31.

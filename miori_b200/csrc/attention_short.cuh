@@ -8,10 +8,10 @@
 //   (ldmatrix, ldmatrix.trans), and the scores' accumulators are the probabilities' A operand as they lie.
 // * Blocks are dealt by the grid: (block, key head), the host's bound on the blocks being tokens / tokens-a-block + requests.
 // * What a row must not see: rows past the end arrive as zeros, values that are not finite are zeroed in every tile that some row
-//   does not see as a whole and added at the end for the rows that see them.  P is rounded to bf16, l sums
-//   the rounded p: see attention_decode.cuh.
+//   does not see as a whole and added at the end for the rows that see them.  P is rounded to bf16,
+//   l sums the rounded p: see attention_decode.cuh.
 //
-// Latency-bound: one prompt of 77 tokens 6.5 us (the prompt kernel 11.1), 32 of 32 7.3 (12.4), 16 heads of 128 over 4.
+// Latency-bound: one prompt of 77 tokens 6.5 us (the prompt kernel 10.0), 32 of 32 7.4 (12.0), 16 heads of 128 over 4, in a graph.
 #pragma once
 #include "attention.cuh"
 #include "attention_decode.cuh"

@@ -138,13 +138,13 @@ __global__ void __launch_bounds__(SLOT_THREADS) page_slots_kernel(const SlotArgs
 //
 // The angle of pair j is position[axes[j]] * turns[j] in units of 2^-64 turns: a 64-bit product that wraps around drops whole
 // turns exactly, so that the angle is as good at position 2^31 as at 1 (an fp32 product is off by 2^-24 of the whole angle: 0.004
-// radians at position 65536).  Its upper 32 bits are the sine's argument, off by 2^-32 turns.
+// radians at position 65536).  Its upper 32 bits, rounded to the 24 of an fp32, are the sine's argument: off by 2^-26 turns at most.
 //
 // A thread holds eight pairs, which is two 8-element pieces of a head: D / 16 threads share a head, and for one token the same
-// threads take further heads with the same sines.  A warp's threads compute each sine once and hand it to those that need it.  HBM-bound for many tokens (one warp walks all heads of a token), latency-bound
-// for few (a warp for every 32 / (D / 16) heads): `parts` warps share a token.  16384 tokens of 24 heads of 128 in bf16 37.3 us, 5.4 TB/s of
-// reads and writes; 32 tokens of fp32 2.4 us.
-constexpr uint32_t ROPE_THREADS = 128;  // 16384 tokens: 41.0 us, with 256 44.5 (fewer warps fit an SM)
+// threads take further heads with the same sines.  A warp's threads compute each sine once and hand it to those that need it.
+// HBM-bound for many tokens (one warp walks all heads of a token), latency-bound for few (a warp for every 32 / (D / 16) heads):
+// `parts` warps share a token.  16384 tokens of 24 heads of 128 in bf16 37.4 us, 5.4 TB/s of reads and writes; 32 tokens of fp32 2.4 us.
+constexpr uint32_t ROPE_THREADS = 128;  // 16384 tokens: 37.4 us, with 256 40.3 (fewer warps fit an SM)
 
 struct RopeArgs {
     const void* qkv;
