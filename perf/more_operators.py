@@ -100,8 +100,9 @@ def _quantized(x, tile):
     """(values, scales) of the blocks of x, tile x 128 elements each; rows of the values begin on 16-byte boundaries."""
     blocks = _whole_blocks(x.float(), tile)
     top = blocks.abs().amax((1, 3)).clamp(min=LEAST)
-    q = (blocks * (TOP / top)[:, None, :, None]).to(FP8).flatten(2).flatten(0, 1)
-    return q[:x.shape[0], :x.shape[1]], top / TOP
+    most = torch.full_like(top, TOP)  # a plain number would be divided by as a product with its reciprocal
+    q = (blocks * (most / top)[:, None, :, None]).to(FP8).flatten(2).flatten(0, 1)
+    return q[:x.shape[0], :x.shape[1]], top / most
 
 
 def _activations(g, rows, K):
