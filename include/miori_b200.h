@@ -48,6 +48,9 @@ extern "C" {
 #define MIORI_ROPE_ADJACENT 8u     /* rope_kv: elements 2j and 2j + 1 are a pair (else j and j + rotary / 2) */
 #define MIORI_ROPE_F32 16u         /* rope_kv: qkv is fp32, as projections write it (else bf16) */
 #define MIORI_ATTENTION_FULL 32u   /* attention: every token sees all of its request's positions (else causal) */
+#define MIORI_QUANT_F32 64u        /* quant_fp8: x is fp32 (else bf16) */
+#define MIORI_MOE_SIGMOID 128u     /* moe: an expert's score is the sigmoid of its logit (else the softmax over all) */
+#define MIORI_MOE_NORM 1024u       /* moe: the weights of a token's experts are divided by their sum */
 const char* miori_last_error(void);
 /* Library version string, e.g. "miori_b200 0.1 sm_100a". */
 const char* miori_version(void);
@@ -431,6 +434,53 @@ int miori_attention_prompt(const void* q, const void* k, const void* v, void* ou
                            const int32_t* cu, const int32_t* cu_k, uint32_t requests, uint32_t tokens, uint32_t keys,
                            uint32_t heads, uint32_t kv_heads, uint32_t dim, float scale, uint32_t flags, void* workspace,
                            size_t workspace_bytes, void* stream);
+
+/* ---- 8-bit floating point with a scale for each block of 128 ------------------------------------
+ *
+ * Values are e4m3 (largest 448), rows `pitch` elements apart that begin on 16-byte boundaries.  A block is 128 elements along K of
+ * one row (activations) or of 128 rows (weights, whose blocks begin at rows 0, 128, ...); the last ones may be shorter.
+ * Scales are fp32, one a block, at scales[row block * scale_row + column block * scale_col].  All of it is launched so that
+ * it may begin while the launch before drains; it waits for that one before it reads or writes anything. */
+
+/* q = e4m3(x * (448 / a)), scale = a / 448, a = max(largest |x| of the block, 2^-100), each operation in fp32 and rounded
+ * once.  tile: 1 or 128 rows a block.  x bf16 (fp32 with MIORI_QUANT_F32), rows x_row elements apart (whole 16 bytes, and x
+ * 16-byte aligned, is the fast case).  A NaN stays one and does not count for the largest; a block with an infinity gets an infinite
+ * scale.  What lies behind K in a row of q is left as it was. */
+int miori_quant_fp8(const void* x, int64_t x_row, void* q, int64_t q_row, float* scales, int64_t scale_row,
+                    int64_t scale_col, uint32_t rows, uint32_t K, uint32_t tile, uint32_t flags, void* stream);
+/* C[m][n] (fp32, or bf16 with MIORI_OUT_BF16; rows ldc elements apart) = sum_b sa[m][b] sw[n / 128][b] sum_{k in block b} a[m][k]
+ * w[n][k]: activations in blocks of one row times weights in blocks of 128, any M, N, K >= 1, fp32 sums.  What lies behind N in
+ * a row of C is left as it was. */
+int miori_gemm_fp8(const void* a, int64_t lda, const float* sa, int64_t sa_row, int64_t sa_col, const void* w,
+                   int64_t ldw, const float* sw, int64_t sw_row, int64_t sw_col, void* C, int64_t ldc, uint32_t M,
+                   uint32_t N, uint32_t K, uint32_t flags, void* stream);
+
+/* ---- a layer of experts for the tokens of a decode step ------------------------------------------
+ *
+ * l = x router^T; p = softmax(l), or sigmoid(l) with MIORI_MOE_SIGMOID; a token's experts are the `top` of largest p + bias
+ * (of largest l without a bias; ties: lowest index), their weights w = p, divided by their sum with MIORI_MOE_NORM, times factor;
+ *   out[t] = sum_e w_e W_down,e (silu(g) * u),  g = W_up,e[0 .. ff) x[t],  u = W_up,e[ff .. 2 ff) x[t].
+ * An expert whose bias is -inf is never chosen; a token left with fewer than `top` has fewer, with none its row is zeros.  An expert whose
+ * score is not a number comes last.  x [tokens][hidden] and router [experts][hidden] bf16, bias fp32 [experts] or NULL, out
+ * [tokens][hidden] fp32 (bf16 with MIORI_OUT_BF16), which may not be x.  1..32 tokens, 1..256 experts, top 1..16.  The choice is made from
+ * fp32 sums; the chosen experts' weights are read once.  A token's result depends on the other tokens in the order of its sums only.
+ * workspace: miori_moe_workspace_bytes, zeroed once by its owner, left so that the next launch may use it; launches that may run
+ * concurrently need workspaces of their own.  One cooperative launch, whose CTAs wait for one another once; should the wait run
+ * out (a second), miori_device_error_poll tells and the workspace has to be zeroed again. */
+size_t miori_moe_workspace_bytes(uint32_t tokens, uint32_t top, uint32_t ff);
+/* Packed 4-bit weights as of miori_gemv4, the experts one behind the other: up [experts][2 ff][hidden], gate rows first; down
+ * [experts][hidden][ff].  hidden and ff multiples of 128. */
+int miori_moe4(const void* x, const void* router, const float* bias, const void* q_up, const void* s_up,
+               const void* b_up, const void* q_down, const void* s_down, const void* b_down, void* out,
+               uint32_t tokens, uint32_t experts, uint32_t top, uint32_t hidden, uint32_t ff, uint32_t group,
+               float factor, uint32_t flags, void* workspace, size_t workspace_bytes, void* stream);
+/* Weights in e4m3 with a scale for each 128 x 128 of an expert's matrix, contiguous: w_up [experts][2 ff][hidden], s_up
+ * [experts][ceil(2 ff / 128)][ceil(hidden / 128)], and so down.  The activations are not quantized.  hidden and ff multiples
+ * of 16. */
+int miori_moe_fp8(const void* x, const void* router, const float* bias, const void* w_up, const float* s_up,
+                  const void* w_down, const float* s_down, void* out, uint32_t tokens, uint32_t experts,
+                  uint32_t top, uint32_t hidden, uint32_t ff, float factor, uint32_t flags, void* workspace,
+                  size_t workspace_bytes, void* stream);
 
 /* Non-zero if a kernel of this library recorded an internal error on the current
  * device since the last call (bounded wait expired); clears the record. */

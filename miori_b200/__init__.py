@@ -14,8 +14,10 @@ _OPS = ("gemv4", "gemv8", "dequant4_rowmajor", "dequant8_rowmajor", "dequant4_ca
         "cache_to_rowmajor", "gemm_bf16_cache", "gemv_bf16_cache", "gemm_workspace", "gemm_bf16_strided", "linear4",
         "rmsnorm", "post_norm_add", "silu_mul", "embed8", "argmax", "gemv4_rmsnorm", "gemv8_rmsnorm",
         "gemv4_silu", "gemv4_post_norm_add", "gemv4_rmsnorm_silu", "page_slots", "rope_kv", "rope_turns",
-        "attention_paged", "attention_prompt", "attention_workspace")
-_LIB = ("lib", "check", "MioriError", "OUT_F32", "OUT_BF16", "LAUNCH_PDL", "GEMV_EXACT", "ROPE_ADJACENT", "ATTENTION_FULL")
+        "attention_paged", "attention_prompt", "attention_workspace", "quant_fp8", "gemm_fp8", "moe4", "moe_fp8",
+        "moe_workspace")
+_LIB = ("lib", "check", "MioriError", "OUT_F32", "OUT_BF16", "LAUNCH_PDL", "GEMV_EXACT", "ROPE_ADJACENT", "ATTENTION_FULL",
+        "MOE_SIGMOID", "MOE_NORM")
 
 __all__ = list(_OPS + _LIB)
 

@@ -16,8 +16,9 @@ HEADER = os.path.join(HERE, "..", "include", "miori_b200.h")
 
 OUT_F32, OUT_BF16, LAUNCH_PDL, GEMV_EXACT = 0, 1, 2, 4
 ROPE_ADJACENT, ROPE_F32, ATTENTION_FULL = 8, 16, 32
+QUANT_F32, MOE_SIGMOID, MOE_NORM = 64, 128, 1024
 
-_p, _u32, _sz, _i = C.c_void_p, C.c_uint32, C.c_size_t, C.c_int
+_p, _u32, _sz, _i, _i64 = C.c_void_p, C.c_uint32, C.c_size_t, C.c_int, C.c_int64
 _strides = C.POINTER(C.c_int64)
 
 _SIGS = {
@@ -88,6 +89,11 @@ _SIGS = {
     "miori_attention_workspace_bytes": (_sz, []),
     "miori_attention_paged": (_i, [_p] * 4 + [_strides] + [_p] * 3 + [_u32] * 9 + [C.c_float, _u32, _p, _sz, _p]),
     "miori_attention_prompt": (_i, [_p] * 4 + [_strides] + [_p] * 2 + [_u32] * 6 + [C.c_float, _u32, _p, _sz, _p]),
+    "miori_quant_fp8": (_i, [_p, _i64, _p, _i64, _p, _i64, _i64, _u32, _u32, _u32, _u32, _p]),
+    "miori_gemm_fp8": (_i, [_p, _i64, _p, _i64, _i64, _p, _i64, _p, _i64, _i64, _p, _i64, _u32, _u32, _u32, _u32, _p]),
+    "miori_moe_workspace_bytes": (_sz, [_u32, _u32, _u32]),
+    "miori_moe4": (_i, [_p] * 10 + [_u32] * 6 + [C.c_float, _u32, _p, _sz, _p]),
+    "miori_moe_fp8": (_i, [_p] * 8 + [_u32] * 5 + [C.c_float, _u32, _p, _sz, _p]),
     "miori_device_error_poll": (_i, []),
 }
 

@@ -26,7 +26,7 @@
 
 namespace {
 
-constexpr int MAX_ARGS = 13;
+constexpr int MAX_ARGS = 15;
 PyObject* g_error = nullptr;  // _lib.MioriError
 
 #define MIORI_ENTRIES(X)                                                                         \
@@ -34,7 +34,7 @@ PyObject* g_error = nullptr;  // _lib.MioriError
     X(cache_bytes) X(gemm_bf16_cache_ws) X(gemm_bf16_strided) X(gemv_bf16_cache) X(linear4)      \
     X(rmsnorm) X(post_norm_add) X(silu_mul) X(embed8) X(argmax) X(gemv4_rmsnorm)                 \
     X(gemv8_rmsnorm) X(gemv4_silu) X(gemv4_post_norm_add) X(gemv4_rmsnorm_silu) X(page_slots)    \
-    X(rope_kv) X(attention_paged) X(attention_prompt)
+    X(rope_kv) X(attention_paged) X(attention_prompt) X(quant_fp8) X(gemm_fp8) X(moe4) X(moe_fp8)
 
 struct Abi {
 #define X(name) decltype(&miori_##name) name;
@@ -562,6 +562,152 @@ OP(attention_prompt, 4, "q", "k", "v", "cu", "cu_k", "scale", "flags", "out", "w
     return o.result();
 }
 
+// A matrix of 8-bit floating point: rows may lie apart, on 16-byte boundaries (the library checks those).
+void need_fp8(const at::Tensor& t, const char* what, int64_t dims) {
+    if (!t.is_cuda()) raise(PyExc_ValueError, "miori_b200 ops need CUDA tensors (there is no CPU path)");
+    if (t.scalar_type() != at::kFloat8_e4m3fn) raise(PyExc_TypeError, "%s: a float8_e4m3fn tensor is expected", what);
+    if (t.dim() != dims) raise(PyExc_ValueError, "%s: %lld dimensions expected, got %lld", what, (long long)dims, (long long)t.dim());
+    if (t.size(dims - 1) != 1 && t.stride(dims - 1) != 1) raise(PyExc_ValueError, "%s: the last dimension must be contiguous", what);
+}
+// Scales [rows][cols] fp32 of any strides.
+void need_scales(const at::Tensor& t, const char* what, int64_t rows, int64_t cols) {
+    if (!t.is_cuda()) raise(PyExc_ValueError, "miori_b200 ops need CUDA tensors (there is no CPU path)");
+    if (t.scalar_type() != at::kFloat) raise(PyExc_TypeError, "%s: an fp32 tensor is expected", what);
+    if (t.dim() != 2 || t.size(0) != rows || t.size(1) != cols) raise(PyExc_ValueError, "%s: [%lld][%lld] expected", what, (long long)rows, (long long)cols);
+}
+// The pitch of a matrix's rows; that of a single one is of no account.
+int64_t pitch(const at::Tensor& t, int64_t unit) { return t.size(0) == 1 ? (t.size(1) + unit - 1) / unit * unit : t.stride(0); }
+int64_t blocks(int64_t n) { return (n + 127) / 128; }
+// Sizes that the library counts in 32 bits.
+void need_u32(const char* fn, std::initializer_list<int64_t> sizes) {
+    for (const int64_t n : sizes)
+        if (n > 0x7FFFFFFF) raise(PyExc_ValueError, "%s: a size of %lld", fn, (long long)n);
+}
+
+OP(quant_fp8, 1, "x", "tile", "flags", "out", "scales") {
+    const at::Tensor& x = a.tensor(0);
+    if (!x.is_cuda()) raise(PyExc_ValueError, "miori_b200 ops need CUDA tensors (there is no CPU path)");
+    const bool fp32 = x.scalar_type() == at::kFloat;
+    if (!fp32 && x.scalar_type() != at::kBFloat16) raise(PyExc_TypeError, "x: an fp32 or bf16 tensor is expected");
+    if (x.dim() != 2 || (x.size(1) != 1 && x.stride(1) != 1)) raise(PyExc_ValueError, "x: [rows][K] with contiguous rows expected");
+    const int64_t R = x.size(0), K = x.size(1), tile = a.u32(1, 1);
+    if (tile != 1 && tile != 128) raise(PyExc_ValueError, "tile: 1 or 128 rows expected, got %lld", (long long)tile);
+    need_u32("quant_fp8", {R, K});
+    const int64_t row_blocks = (R + tile - 1) / tile;
+    const uint32_t flags = (a.u32(2, 0) & ~MIORI_QUANT_F32) | (fp32 ? MIORI_QUANT_F32 : 0u);
+    at::Tensor q, s;
+    if (a.given(3)) {
+        q = a.tensor(3);
+        need_fp8(q, "out", 2);
+        if (q.size(0) != R || q.size(1) != K) raise(PyExc_ValueError, "out: the shape of x is expected");
+    } else {  // rows begin on 16-byte boundaries
+        const int64_t whole = (K + 15) / 16 * 16;
+        q = empty({R, whole}, at::kFloat8_e4m3fn, x);
+        if (whole != K) q.unsafeGetTensorImpl()->set_sizes_and_strides(std::vector<int64_t>{R, K}, std::vector<int64_t>{whole, 1});
+    }
+    if (a.given(4)) {
+        s = a.tensor(4);
+        need_scales(s, "scales", row_blocks, blocks(K));
+    } else {
+        s = empty({row_blocks, blocks(K)}, at::kFloat, x);
+    }
+    call(abi.quant_fp8, x.data_ptr(), R == 1 ? K : x.stride(0), q.data_ptr(), pitch(q, 16), static_cast<float*>(s.data_ptr()), s.stride(0), s.stride(1), R, K, tile,
+         flags, stream());
+    return tuple_of({&q, &s});
+}
+
+OP(gemm_fp8, 4, "a", "sa", "w", "sw", "flags", "out") {
+    const at::Tensor &x = a.tensor(0), &sa = a.tensor(1), &w = a.tensor(2), &sw = a.tensor(3);
+    need_fp8(x, "a", 2);
+    need_fp8(w, "w", 2);
+    const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
+    if (w.size(1) != K) raise(PyExc_ValueError, "w: rows of %lld expected, as a has, got %lld", (long long)K, (long long)w.size(1));
+    need_u32("gemm_fp8", {M, N, K});
+    need_scales(sa, "sa", M, blocks(K));
+    need_scales(sw, "sw", blocks(N), blocks(K));
+    const uint32_t flags = a.u32(4, 0);
+    const at::ScalarType dt = out_type(flags);
+    Out o;  // rows of a caller's output may lie apart
+    if (a.given(5)) a.tensor(5), o.given = a.v[5];
+    else o.made = empty({M, N}, dt, x);
+    const at::Tensor& c = o.given ? THPVariable_Unpack(o.given) : o.made;
+    if (!c.is_cuda()) raise(PyExc_ValueError, "out: a CUDA tensor is expected");
+    if (c.scalar_type() != dt || c.dim() != 2 || c.size(0) != M || c.size(1) != N || (N != 1 && c.stride(1) != 1))
+        raise(PyExc_ValueError, "out: [%lld][%lld] of the output's type with contiguous rows expected", (long long)M, (long long)N);
+    call(abi.gemm_fp8, x.data_ptr(), pitch(x, 16), static_cast<const float*>(sa.data_ptr()), sa.stride(0), sa.stride(1), w.data_ptr(), pitch(w, 16),
+         static_cast<const float*>(sw.data_ptr()), sw.stride(0), sw.stride(1), c.data_ptr(), M == 1 ? N : c.stride(0), M, N, K, flags, stream());
+    return o.result();
+}
+
+// What both layers of experts are called with beside their weights.
+struct Layer {
+    int64_t T, H, E;
+    const float* bias = nullptr;
+    void* workspace;
+    size_t bytes;
+};
+Layer layer(const Args& a, int x_at, int workspace_at, int bias_at) {
+    const at::Tensor &x = a.tensor(x_at), &router = a.tensor(x_at + 1);
+    need_cuda({&x, &router});
+    if (x.scalar_type() != at::kBFloat16 || router.scalar_type() != at::kBFloat16) raise(PyExc_TypeError, "x and router: bf16 tensors are expected");
+    Layer l;
+    rows_of(x, l.T, l.H);
+    if (router.dim() != 2 || router.size(1) != l.H) raise(PyExc_ValueError, "router: [experts][%lld] expected", (long long)l.H);
+    l.E = router.size(0);
+    need_u32("moe", {l.T, l.H, l.E});
+    if (a.given(bias_at)) {
+        const at::Tensor& b = a.tensor(bias_at);
+        need_cuda({&b});
+        if (b.scalar_type() != at::kFloat || b.numel() != l.E) raise(PyExc_ValueError, "bias: fp32, one an expert, expected");
+        l.bias = static_cast<const float*>(b.data_ptr());
+    }
+    if (!a.given(workspace_at)) raise(PyExc_TypeError, "workspace: a tensor is expected (moe_workspace)");
+    workspace(a, workspace_at, l.workspace, l.bytes);
+    return l;
+}
+// A tensor of the experts' weights: contiguous, of this type and shape.
+const void* weights(const at::Tensor& t, const char* what, at::ScalarType dt, int64_t E, int64_t rows, int64_t cols) {
+    need_cuda({&t});
+    if (t.scalar_type() != dt) raise(PyExc_TypeError, "%s: a tensor of another type is expected", what);
+    if (t.dim() != 3 || t.size(0) != E || t.size(1) != rows || t.size(2) != cols)
+        raise(PyExc_ValueError, "%s: [%lld][%lld][%lld] expected", what, (long long)E, (long long)rows, (long long)cols);
+    return t.data_ptr();
+}
+int64_t ff_of(const at::Tensor& up, const char* what) {
+    if (up.dim() != 3 || up.size(1) % 2) raise(PyExc_ValueError, "%s: [experts][2 ff][..] expected", what);
+    need_u32("moe", {up.size(1)});
+    return up.size(1) / 2;
+}
+
+OP(moe4, 10, "x", "router", "q_up", "s_up", "b_up", "q_down", "s_down", "b_down", "top", "workspace", "bias", "group", "factor", "flags", "out") {
+    const Layer l = layer(a, 0, 9, 10);
+    const int64_t F = ff_of(a.tensor(2), "q_up"), group = a.u32(11, 32);
+    if (group != 32 && group != 64) raise(PyExc_ValueError, "group must be 32 or 64, got %lld", (long long)group);
+    if (l.H % 128 || F % 128) raise(PyExc_ValueError, "hidden and ff are multiples of 128, got %lld and %lld", (long long)l.H, (long long)F);
+    const void *qu = weights(a.tensor(2), "q_up", at::kInt, l.E, 2 * F, l.H / 8), *su = weights(a.tensor(3), "s_up", at::kBFloat16, l.E, 2 * F, l.H / group),
+               *bu = weights(a.tensor(4), "b_up", at::kBFloat16, l.E, 2 * F, l.H / group), *qd = weights(a.tensor(5), "q_down", at::kInt, l.E, l.H, F / 8),
+               *sd = weights(a.tensor(6), "s_down", at::kBFloat16, l.E, l.H, F / group), *bd = weights(a.tensor(7), "b_down", at::kBFloat16, l.E, l.H, F / group);
+    const uint32_t top = a.u32(8, 0), flags = a.u32(13, 0);
+    const float factor = a.given(12) ? a.f32(12) : 1.0f;
+    Out o = output(a, 14, {l.T, l.H}, out_type(flags), a.tensor(0));
+    call(abi.moe4, a.tensor(0).data_ptr(), a.tensor(1).data_ptr(), l.bias, qu, su, bu, qd, sd, bd, o.ptr(), l.T, l.E, top, l.H, F, group, factor, flags, l.workspace,
+         l.bytes, stream());
+    return o.result();
+}
+
+OP(moe_fp8, 8, "x", "router", "w_up", "s_up", "w_down", "s_down", "top", "workspace", "bias", "factor", "flags", "out") {
+    const Layer l = layer(a, 0, 7, 8);
+    const int64_t F = ff_of(a.tensor(2), "w_up");
+    const void *wu = weights(a.tensor(2), "w_up", at::kFloat8_e4m3fn, l.E, 2 * F, l.H), *su = weights(a.tensor(3), "s_up", at::kFloat, l.E, blocks(2 * F), blocks(l.H)),
+               *wd = weights(a.tensor(4), "w_down", at::kFloat8_e4m3fn, l.E, l.H, F), *sd = weights(a.tensor(5), "s_down", at::kFloat, l.E, blocks(l.H), blocks(F));
+    const uint32_t top = a.u32(6, 0), flags = a.u32(10, 0);
+    const float factor = a.given(9) ? a.f32(9) : 1.0f;
+    Out o = output(a, 11, {l.T, l.H}, out_type(flags), a.tensor(0));
+    call(abi.moe_fp8, a.tensor(0).data_ptr(), a.tensor(1).data_ptr(), l.bias, wu, static_cast<const float*>(su), wd, static_cast<const float*>(sd), o.ptr(), l.T, l.E,
+         top, l.H, F, factor, flags, l.workspace, l.bytes, stream());
+    return o.result();
+}
+
 // bind(handle, error): take the library's functions from the handle that ctypes opened.
 PyObject* py_bind(PyObject*, PyObject* args) {
     unsigned long long h = 0;
@@ -637,6 +783,18 @@ PyMethodDef methods[] = {
     FAST(attention_prompt, "q, k, v, cu, cu_k=None, scale=None, flags=0, out=None, workspace=None",
          "Causal attention of packed prompts: q [T][heads][dim], k and v [T][kv_heads][dim] bf16, prompt r being rows cu[r] to\n"
          "cu[r + 1] - 1 (keys: cu_k, where they are others').  workspace, flags: as attention_paged."),
+    FAST(quant_fp8, "x, tile=1, flags=0, out=None, scales=None",
+         "(q, scales) of x [rows][K] fp32 or bf16: q float8_e4m3fn, scales fp32 [rows / tile][K / 128] (both rounded up), a scale for\n"
+         "each block of 128 along K of one row (tile=1: activations) or of 128 rows (tile=128: weights)."),
+    FAST(gemm_fp8, "a, sa, w, sw, flags=0, out=None",
+         "C[M][N] (fp32, OUT_BF16: bf16) of a [M][K] and w [N][K] float8_e4m3fn, with the scales of quant_fp8(tile=1) and\n"
+         "quant_fp8(tile=128); rows may lie apart, on 16-byte boundaries."),
+    FAST(moe4, "x, router, q_up, s_up, b_up, q_down, s_down, b_down, top, workspace, bias=None, group=32, factor=1.0, flags=0, out=None",
+         "A layer of experts for up to 32 tokens, x [T][H] bf16 -> [T][H] fp32 (OUT_BF16: bf16): router [E][H] bf16, packed 4-bit\n"
+         "weights [E][2 F][H] (gate rows first) and [E][H][F].  Each token's `top` experts by softmax (MOE_SIGMOID: sigmoid) + bias;\n"
+         "MOE_NORM: their weights sum to one.  workspace: moe_workspace()."),
+    FAST(moe_fp8, "x, router, w_up, s_up, w_down, s_down, top, workspace, bias=None, factor=1.0, flags=0, out=None",
+         "moe4 with float8_e4m3fn weights [E][2 F][H] and [E][H][F] and their scales for each 128 x 128."),
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", "Native call path of the operators, " MIORI_TORCH_TAG, -1, methods,

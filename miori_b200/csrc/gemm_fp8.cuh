@@ -1,0 +1,580 @@
+// Products in 8-bit floating point: C[m][n] = sum_b sa[m][b] sw[n / 128][b] sum_{k in block b} a[m][k] w[n][k], a and w e4m3 with
+// K contiguous, blocks of 128 along K (a: one row, w: 128 rows), sums in fp32.
+//
+// The tensor core adds up one block (four tcgen05.mma of kind::f8f6f4, 32 elements each); the scales differ from block to block,
+// so what it has summed leaves tensor memory once a block and is added, times the block's scale, to fp32
+// accumulators in registers.  That is one tcgen05.ld and half a packed FMA (fma.rn.f32x2) an element and block: of the 512 cycles that the
+// matrix unit takes for a 128 x 256 x 128 block, 256 of the tensor memory's reading and 128 to 256 of issue, beside it.  Two
+// or four blocks' sums fit tensor memory, so that the unit never waits for the readers.
+// (Scales that are powers of two could ride along inside the MMA; a checkpoint's are any fp32.)
+//
+// Two kernels:
+//   pair   more than a hundred rows or so: 256 x 256 or 256 x 128 tiles on SM pairs (cta_group::2), persistent; each CTA pulls 32 KB a
+//          block through L2 for 512 cycles of its matrix unit.
+//   swap   few rows, or few tiles: 128 rows of w are the MMA's M, up to 128 rows of a its N; K is split over the CTAs of a
+//          cluster and the partial sums meet in distributed shared memory, in rank order.
+// Ends of M, N and K are zeros by TMA; what lies behind N in a row of C is left as it was.  Every wait is bounded.
+#pragma once
+#include "common.cuh"
+#include "tma_host.cuh"
+
+namespace miori_b200 {
+namespace fp8 {
+
+constexpr int KB_BYTES = 128;               // a k-block of a row: one row of the 128-byte swizzle
+constexpr int UMMA_KB = 32;                 // bytes of K an MMA takes
+constexpr uint32_t PEER_MASK = 0xFEFFFFFFu;  // clears the CTA-rank bit of a shared::cluster address
+
+struct GemmArgs {
+    void* c;
+    const float *sa, *sw;
+    int64_t ldc, sa_row, sa_col, sw_row, sw_col;  // elements
+    uint32_t M, N, K;
+    uint32_t bf16;
+    uint32_t by_tma;  // C's rows begin on 16-byte boundaries: stored by TMA
+};
+
+// K-major, 128-byte swizzle: rows of 128 bytes, eight of them an atom of 1024 bytes.
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr) {
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// D fp32, A and B e4m3, both K-major, shape m x n.
+__host__ __device__ constexpr uint32_t idesc_e4m3(uint32_t m, uint32_t n) { return (1u << 4) | ((n >> 3) << 17) | ((m >> 4) << 24); }
+
+template <int CTAS>
+__device__ __forceinline__ void umma_e4m3(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    if constexpr (CTAS == 2)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+                     ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+                     ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void commit_one(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+// the same barrier offset in both CTAs of the pair
+__device__ __forceinline__ void commit_both(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+}
+__device__ __forceinline__ void arrive_leader(uint32_t bar) {
+    asm volatile("{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %0, 0;\n\tmbarrier.arrive.release.cluster.shared::cluster.b64 _, [ra];\n\t}" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void load_pair(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(taddr));
+}
+// The registers pass through the wait, so that nothing that reads them can be moved in front of it.
+__device__ __forceinline__ void tmem_wait16(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
+                   "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]) :: "memory");
+}
+__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
+    return v;
+}
+// (acc.x + v.x s, acc.y + v.y s)
+__device__ __forceinline__ void fma2(uint64_t& acc, uint64_t v, uint64_t s) { asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(v), "l"(s)); }
+
+// ---- 256-row tiles on SM pairs ----------------------------------------------------------------------------
+
+template <int BN>
+struct PairCfg {
+    static constexpr int A_BYTES = 128 * KB_BYTES, B_BYTES = BN / 2 * KB_BYTES, STAGE_BYTES = A_BYTES + B_BYTES;
+    static constexpr int STAGES = BN == 256 ? 5 : 6;
+    static constexpr int BUFS = 512 / BN;        // sums of k-blocks in tensor memory
+    static constexpr int COLS = BN / 2;          // columns of an epilogue warp
+    static constexpr int OUT_BYTES = 8 * 2 * 32 * 128;  // two buffers of 32 rows x 128 bytes an epilogue warp
+    static constexpr int SMEM = STAGES * STAGE_BYTES + OUT_BYTES + 1024 + 256;
+};
+constexpr int PAIR_THREADS = 320;
+constexpr uint32_t GROUP_TILES = 8;  // row tiles that share what L2 holds of w
+
+struct Tile {
+    uint32_t m, n;
+};
+__device__ __forceinline__ Tile tile_at(uint32_t t, uint32_t m_tiles, uint32_t n_tiles) {
+    const uint32_t per_group = GROUP_TILES * n_tiles, group = t / per_group, first = group * GROUP_TILES;
+    const uint32_t gm = min(GROUP_TILES, m_tiles - first), r = t - group * per_group;
+    return {first + r % gm, r / gm};
+}
+
+template <int BN>
+__global__ void __launch_bounds__(PAIR_THREADS, 1)
+gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_c,
+                     const GemmArgs g) {
+    using C = PairCfg<BN>;
+    constexpr int STAGES = C::STAGES, STAGE_BYTES = C::STAGE_BYTES, BUFS = C::BUFS, COLS = C::COLS;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile uint32_t abort_flag;
+    const uint32_t ring = (smem_addr(smem_raw) + 1023u) & ~1023u, out_stage = ring + STAGES * STAGE_BYTES, bars = out_stage + C::OUT_BYTES;
+    auto full = [&](uint32_t s) { return bars + 8u * s; };
+    auto empty = [&](uint32_t s) { return bars + 8u * (STAGES + s); };
+    auto summed = [&](uint32_t b) { return bars + 8u * (2 * STAGES + b); };
+    auto taken = [&](uint32_t b) { return bars + 8u * (2 * STAGES + BUFS + b); };
+
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    uint32_t rank;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    const uint32_t pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const uint32_t m_tiles = (g.M + 255u) / 256u, n_tiles = (g.N + BN - 1u) / BN, tiles = m_tiles * n_tiles;
+    const uint32_t k_blocks = (g.K + KB_BYTES - 1u) / KB_BYTES;
+
+    pdl_launch_dependents();
+    if (threadIdx.x == 0) {
+        abort_flag = 0u;
+        for (int s = 0; s < STAGES; ++s) mbar_init(full(s), 1), mbar_init(empty(s), 1);
+        for (int b = 0; b < BUFS; ++b) mbar_init(summed(b), 1), mbar_init(taken(b), 16);  // the leader's: eight epilogue warps of each CTA
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_c) : "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    cluster_barrier();  // both CTAs' barriers exist before anything arrives from the other
+    fence_after();
+    const uint32_t tmem = tmem_slot;
+    pdl_wait_prior();
+
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t s = 0, parity = 1u;
+            bool ok = true;
+            for (uint32_t t = pair; t < tiles && ok; t += pairs) {
+                const Tile tc = tile_at(t, m_tiles, n_tiles);
+                const int m = (int)(tc.m * 256u + rank * 128u), n = (int)(tc.n * BN + rank * (BN / 2));
+                for (uint32_t kb = 0; kb < k_blocks; ++kb) {
+                    if (!(ok = mbar_wait(empty(s), parity, &abort_flag, 0x71))) break;
+                    const uint32_t at = ring + s * STAGE_BYTES, bar = full(s) & PEER_MASK;
+                    if (rank == 0) mbar_expect_tx(full(s), 2u * STAGE_BYTES);
+                    load_pair(at, &map_a, (int)(kb * KB_BYTES), m, bar);
+                    load_pair(at + C::A_BYTES, &map_w, (int)(kb * KB_BYTES), n, bar);
+                    if (++s == STAGES) s = 0u, parity ^= 1u;
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            constexpr uint32_t idesc = idesc_e4m3(256, BN);
+            uint32_t s = 0, parity = 0u, b = 0, b_parity = 1u;
+            bool ok = true;
+            for (uint32_t t = pair; t < tiles && ok; t += pairs) {
+                for (uint32_t kb = 0; kb < k_blocks; ++kb) {
+                    if (!(ok = mbar_wait(taken(b), b_parity, &abort_flag, 0x72))) break;
+                    if (!(ok = mbar_wait(full(s), parity, &abort_flag, 0x73))) break;
+                    fence_after();
+                    const uint64_t ad = desc_sw128(ring + s * STAGE_BYTES), wd = desc_sw128(ring + s * STAGE_BYTES + C::A_BYTES);
+#pragma unroll
+                    for (uint32_t k = 0; k < KB_BYTES / UMMA_KB; ++k) umma_e4m3<2>(tmem + b * BN, ad + 2u * k, wd + 2u * k, idesc, k != 0u);
+                    commit_both(empty(s));
+                    commit_both(summed(b));
+                    if (++s == STAGES) s = 0u, parity ^= 1u;
+                    if (++b == BUFS) b = 0u, b_parity ^= 1u;
+                }
+            }
+        }
+    } else {
+        const uint32_t quad = warp & 3u, half = (warp - 2u) >> 2;  // TMEM lanes and columns of this warp
+        const uint32_t bufs = out_stage + (warp - 2u) * 2u * 4096u, sw_lane = lane & 7u;
+        uint32_t b = 0, b_parity = 0u;
+        bool ok = true;
+        for (uint32_t t = pair; t < tiles && ok; t += pairs) {
+            const Tile tc = tile_at(t, m_tiles, n_tiles);
+            const uint32_t row0 = tc.m * 256u + rank * 128u + quad * 32u, col0 = tc.n * BN + half * COLS;
+            const float* sa = g.sa + (int64_t)min(row0 + lane, g.M - 1u) * g.sa_row;
+            const float* sw = g.sw + (int64_t)(min(col0, g.N - 1u) / 128u) * g.sw_row;
+            uint64_t acc[COLS / 2];
+            float scale = __fmul_rn(ld_fresh(sa), ld_fresh(sw));
+            for (uint32_t kb = 0; kb < k_blocks; ++kb) {
+                float next_a = 0.0f, next_w = 0.0f;
+                if (kb + 1u < k_blocks) next_a = ld_fresh(sa + (int64_t)(kb + 1u) * g.sa_col), next_w = ld_fresh(sw + (int64_t)(kb + 1u) * g.sw_col);
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait(summed(b), b_parity, &abort_flag, 0x74));
+                if (!ok) break;
+                fence_after();
+                const uint32_t from = tmem + ((quad * 32u) << 16) + b * BN + half * COLS;
+                const uint64_t s2 = pack2(__float_as_uint(scale), __float_as_uint(scale));
+                uint32_t r[2][16];
+                tmem_ld16(from, r[0]);
+                tmem_wait16(r[0]);
+                if (kb == 0) {
+#pragma unroll
+                    for (int i = 0; i < COLS / 2; ++i) acc[i] = 0ull;
+                }
+#pragma unroll
+                for (int c = 0; c < COLS / 16; ++c) {
+                    if (c + 1 < COLS / 16) tmem_ld16(from + (c + 1) * 16, r[(c + 1) & 1]);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) fma2(acc[c * 8 + j], pack2(r[c & 1][2 * j], r[c & 1][2 * j + 1]), s2);
+                    if (c + 1 < COLS / 16) tmem_wait16(r[(c + 1) & 1]);
+                }
+                fence_before();
+                __syncwarp();
+                if (lane == 0) arrive_leader(taken(b));
+                if (++b == BUFS) b = 0u, b_parity ^= 1u;
+                scale = __fmul_rn(next_a, next_w);
+            }
+            if (!ok) break;
+            // 32 rows x 128 bytes at a time through shared memory, in the 128-byte swizzle
+            if (row0 >= g.M) continue;
+            const uint32_t per = g.bf16 ? 64u : 32u;  // columns of a buffer
+            auto word = [&](int i) { return (uint32_t)(i & 1 ? acc[i >> 1] >> 32 : acc[i >> 1]); };
+#pragma unroll
+            for (int f = 0; f < COLS / 32; ++f) {
+                if (g.bf16 && f >= COLS / 64) break;
+                if (col0 + f * per >= g.N) break;
+                const uint32_t buf = bufs + (f & 1) * 4096u, rowp = buf + lane * 128u;
+                if (lane == 0) tma_store_wait_read<1>();  // the store issued two buffers ago has read this one
+                __syncwarp();
+                if (g.bf16) {
+                    if (f < COLS / 64) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            uint32_t v[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const int at = (f * 64 + j * 8 + e * 2) % COLS;
+                                v[e] = pack_bf16(__uint_as_float(word(at)), __uint_as_float(word(at + 1)));
+                            }
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                                         ::"r"(rowp + (((uint32_t)j ^ sw_lane) << 4)), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                                     ::"r"(rowp + (((uint32_t)j ^ sw_lane) << 4)), "r"(word(f * 32 + j * 4)), "r"(word(f * 32 + j * 4 + 1)),
+                                       "r"(word(f * 32 + j * 4 + 2)), "r"(word(f * 32 + j * 4 + 3)) : "memory");
+                }
+                if (g.by_tma) {
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) {
+                        tma_store_3d(&map_c, (int)(col0 + f * per), (int)row0, 0, buf);
+                        tma_store_commit();
+                    }
+                } else {
+                    __syncwarp();
+                    const uint32_t rows = min(32u, g.M - row0), col = col0 + f * per + lane * (g.bf16 ? 2u : 1u);
+                    for (uint32_t r = 0; r < rows; ++r) {
+                        uint32_t w;
+                        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(buf + r * 128u + (((lane >> 2) ^ (r & 7u)) << 4) + (lane & 3u) * 4u) : "memory");
+                        const int64_t at = (int64_t)(row0 + r) * g.ldc + col;
+                        if (g.bf16) {
+                            if (col < g.N) static_cast<uint16_t*>(g.c)[at] = (uint16_t)w;
+                            if (col + 1u < g.N) static_cast<uint16_t*>(g.c)[at + 1] = (uint16_t)(w >> 16);
+                        } else if (col < g.N) {
+                            static_cast<uint32_t*>(g.c)[at] = w;
+                        }
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+        if (lane == 0) tma_store_wait_read<0>();  // shared memory is read; the writes are the grid's to complete
+    }
+
+    // teardown: on abort give in-flight copies and MMAs time to land before freeing TMEM
+    __syncwarp();
+    if (abort_flag) {
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000LL) __nanosleep(1000);
+    }
+    fence_before();
+    __syncthreads();
+    cluster_barrier();  // the other CTA may still signal this one's barriers or read its shared memory
+    if (warp == 1) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+// ---- few rows: w's rows as the MMA's M, K over a cluster ------------------------------------------------------
+
+constexpr int SWAP_THREADS = 192;
+constexpr int SWAP_MAX_STAGES = 8;
+__host__ __device__ constexpr int SWAP_BUFS(int mp) { return mp >= 128 ? 2 : 4; }  // at most 256 columns: two CTAs an SM fit
+
+struct SwapGeo {
+    uint32_t cs, stages, m_tiles;
+};
+
+// MP: columns of the MMA, rows of a padded to 16, 32, 64 or 128
+template <int MP>
+__global__ void __launch_bounds__(SWAP_THREADS)
+gemm_fp8_swap_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, const GemmArgs g, const SwapGeo geo) {
+    constexpr int W_BYTES = 128 * KB_BYTES, A_BYTES = MP * KB_BYTES, STAGE_BYTES = W_BYTES + A_BYTES, BUFS = SWAP_BUFS(MP);
+    constexpr uint32_t TMEM_COLS = BUFS * MP < 32 ? 32 : BUFS * MP;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t bars_mem[2 * SWAP_MAX_STAGES + 2 * BUFS];
+    __shared__ uint32_t tmem_slot;
+    __shared__ volatile uint32_t abort_flag;
+    const uint32_t ring = (smem_addr(smem_raw) + 1023u) & ~1023u, bars = smem_addr(bars_mem);
+    auto full = [&](uint32_t s) { return bars + 8u * s; };
+    auto empty = [&](uint32_t s) { return bars + 8u * (SWAP_MAX_STAGES + s); };
+    auto summed = [&](uint32_t b) { return bars + 8u * (2 * SWAP_MAX_STAGES + b); };
+    auto taken = [&](uint32_t b) { return bars + 8u * (2 * SWAP_MAX_STAGES + BUFS + b); };
+    const uint32_t scales = ring + geo.stages * STAGE_BYTES;  // [k-block of the slice][MP]
+
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    const uint32_t rank = blockIdx.x % geo.cs, tile = blockIdx.x / geo.cs, m_tile = tile % geo.m_tiles, n_tile = tile / geo.m_tiles;
+    const uint32_t m0 = m_tile * MP;
+    const uint32_t k_blocks = (g.K + KB_BYTES - 1u) / KB_BYTES;
+    const uint32_t kb0 = rank * k_blocks / geo.cs, nkb = (rank + 1u) * k_blocks / geo.cs - kb0;
+
+    pdl_launch_dependents();
+    if (threadIdx.x == 0) {
+        abort_flag = 0u;
+        for (uint32_t s = 0; s < geo.stages; ++s) mbar_init(full(s), 1), mbar_init(empty(s), 1);
+        for (uint32_t b = 0; b < (uint32_t)BUFS; ++b) mbar_init(summed(b), 1), mbar_init(taken(b), 4);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)), "r"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = tmem_slot;
+    pdl_wait_prior();
+
+    bool ok = true;
+    float acc[MP];
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t s = 0, parity = 1u;
+            for (uint32_t i = 0; i < nkb; ++i) {
+                if (!(ok = mbar_wait(empty(s), parity, &abort_flag, 0x75))) break;
+                mbar_expect_tx(full(s), STAGE_BYTES);
+                const uint32_t at = ring + s * STAGE_BYTES;
+                tma_load_2d(at, &map_w, (int)((kb0 + i) * KB_BYTES), (int)(n_tile * 128u), full(s));
+                tma_load_2d(at + W_BYTES, &map_a, (int)((kb0 + i) * KB_BYTES), (int)m0, full(s));
+                if (++s == geo.stages) s = 0u, parity ^= 1u;
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = idesc_e4m3(128, MP);
+            uint32_t s = 0, parity = 0u, b = 0, b_parity = 1u;
+            for (uint32_t i = 0; i < nkb; ++i) {
+                if (!(ok = mbar_wait(taken(b), b_parity, &abort_flag, 0x76))) break;
+                if (!(ok = mbar_wait(full(s), parity, &abort_flag, 0x77))) break;
+                fence_after();
+                const uint64_t wd = desc_sw128(ring + s * STAGE_BYTES), ad = desc_sw128(ring + s * STAGE_BYTES + W_BYTES);
+#pragma unroll
+                for (uint32_t k = 0; k < KB_BYTES / UMMA_KB; ++k) umma_e4m3<1>(tmem + b * MP, wd + 2u * k, ad + 2u * k, idesc, k != 0u);
+                commit_one(empty(s));
+                commit_one(summed(b));
+                if (++s == geo.stages) s = 0u, parity ^= 1u;
+                if (++b == (uint32_t)BUFS) b = 0u, b_parity ^= 1u;
+            }
+        }
+    } else {
+        // the slice's scales, multiplied out: no row's weight is read twice
+        const float* sw = g.sw + (int64_t)n_tile * g.sw_row + (int64_t)kb0 * g.sw_col;
+        for (uint32_t i = threadIdx.x - 64u; i < nkb * MP; i += 128u) {
+            const uint32_t kb = i / MP, m = m0 + i % MP;
+            float v = 0.0f;
+            if (m < g.M) v = __fmul_rn(ld_fresh(g.sa + (int64_t)m * g.sa_row + (int64_t)(kb0 + kb) * g.sa_col), ld_fresh(sw + (int64_t)kb * g.sw_col));
+            asm volatile("st.shared.f32 [%0], %1;" ::"r"(scales + i * 4u), "f"(v) : "memory");
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+#pragma unroll
+        for (int j = 0; j < MP; ++j) acc[j] = 0.0f;
+        uint32_t b = 0, b_parity = 0u;
+        for (uint32_t i = 0; i < nkb; ++i) {
+            ok = __all_sync(0xFFFFFFFFu, mbar_wait(summed(b), b_parity, &abort_flag, 0x78));
+            if (!ok) break;
+            fence_after();
+#pragma unroll
+            for (int c = 0; c < MP; c += 16) {
+                uint32_t r[16];
+                tmem_ld16(tmem + (((warp & 3u) * 32u) << 16) + b * MP + c, r);
+                tmem_wait16(r);
+#pragma unroll
+                for (int j = 0; j < 16; j += 4) {
+                    float4 s;
+                    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(s.x), "=f"(s.y), "=f"(s.z), "=f"(s.w) : "r"(scales + (i * MP + c + j) * 4u) : "memory");
+                    acc[c + j] = __fmaf_rn(__uint_as_float(r[j]), s.x, acc[c + j]);
+                    acc[c + j + 1] = __fmaf_rn(__uint_as_float(r[j + 1]), s.y, acc[c + j + 1]);
+                    acc[c + j + 2] = __fmaf_rn(__uint_as_float(r[j + 2]), s.z, acc[c + j + 2]);
+                    acc[c + j + 3] = __fmaf_rn(__uint_as_float(r[j + 3]), s.w, acc[c + j + 3]);
+                }
+            }
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(taken(b));
+            if (++b == (uint32_t)BUFS) b = 0u, b_parity ^= 1u;
+        }
+    }
+    __syncwarp();
+
+    const uint32_t row = (warp & 3u) * 32u + lane, n = n_tile * 128u + row, rows = min((uint32_t)MP, g.M - m0);
+    auto store = [&](uint32_t m, float v) {  // 32 lanes: neighbouring elements of a row of C
+        const int64_t at = (int64_t)(m0 + m) * g.ldc + n;
+        if (n >= g.N) return;
+        if (g.bf16) static_cast<uint16_t*>(g.c)[at] = (uint16_t)pack_bf16(v, 0.0f);
+        else static_cast<float*>(g.c)[at] = v;
+    };
+    if (geo.cs == 1u) {
+        if (warp >= 2u && ok) {
+#pragma unroll
+            for (int j = 0; j < MP; ++j)
+                if ((uint32_t)j < rows) store((uint32_t)j, acc[j]);
+        }
+    } else {
+        // CTA r of the cluster adds up rows r, r + cs, ... of a, in rank order.  All MMAs are done (their sums have been read): the rings
+        // take the partial sums, [source][row / cs][row of w].
+        cluster_barrier();
+        const uint32_t share = (rows + geo.cs - 1u) / geo.cs;
+        if (warp >= 2u) {
+            uint32_t to_rank = 0, at = 0;
+#pragma unroll
+            for (int j = 0; j < MP; ++j) {
+                if ((uint32_t)j < rows) {
+                    uint32_t to;
+                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(ring + ((rank * share + at) * 128u + row) * 4u), "r"(to_rank));
+                    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(acc[j]) : "memory");
+                    if (++to_rank == geo.cs) to_rank = 0u, ++at;
+                }
+            }
+        }
+        cluster_barrier();
+        if (warp >= 2u && ok) {
+            for (uint32_t at = 0, m = rank; m < rows; ++at, m += geo.cs) {
+                float v = 0.0f;
+#pragma unroll 4
+                for (uint32_t p = 0; p < geo.cs; ++p) {
+                    float w;
+                    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(w) : "r"(ring + ((p * share + at) * 128u + row) * 4u) : "memory");
+                    v = p == 0u ? w : v + w;
+                }
+                store(m, v);
+            }
+        }
+    }
+
+    if (abort_flag) {
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000LL) __nanosleep(1000);
+    }
+    fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+    }
+}
+
+// ---- launches -------------------------------------------------------------------------------------------------
+
+struct GemmOperands {
+    const void *a, *w;
+    int64_t lda, ldw;
+};
+inline int bytes_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t K, uint32_t box_rows, int64_t pitch) {
+    return make_tmap_2d(map, base, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K, rows, KB_BYTES, box_rows, CU_TENSOR_MAP_SWIZZLE_128B, (uint64_t)pitch);
+}
+
+template <class K, class... Args>
+inline cudaError_t launch_cluster(K kernel, uint32_t grid, uint32_t threads, size_t smem, uint32_t cluster, cudaStream_t stream, const Args&... args) {
+    cudaError_t e = set_up_kernel(reinterpret_cast<const void*>(kernel), Split::DRIVERS);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1u ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+template <int BN>
+inline int launch_pair(const GemmOperands& o, GemmArgs g, cudaStream_t stream) {
+    CUtensorMap ma, mw, mc;
+    if (const int rc = bytes_map(&ma, o.a, g.M, g.K, 128, o.lda)) return rc;
+    if (const int rc = bytes_map(&mw, o.w, g.N, g.K, BN / 2, o.ldw)) return rc;
+    mc = ma;  // unused where C is stored otherwise
+    if (g.by_tma) {
+        const int rc = g.bf16 ? make_tmap_3d(&mc, g.c, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, g.N, g.M, 1, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B, (uint64_t)g.ldc)
+                              : make_tmap_3d(&mc, g.c, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, g.N, g.M, 1, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B, (uint64_t)g.ldc);
+        if (rc) return rc;
+    }
+    const uint64_t tiles = (uint64_t)((g.M + 255u) / 256u) * ((g.N + BN - 1u) / BN);
+    const uint32_t pairs = (uint32_t)(tiles < (uint64_t)(sm_count() / 2) ? tiles : (uint64_t)(sm_count() / 2));
+    const cudaError_t e = launch_cluster(gemm_fp8_pair_kernel<BN>, 2u * pairs, PAIR_THREADS, PairCfg<BN>::SMEM, 2, stream, ma, mw, mc, g);
+    return e == cudaSuccess ? MIORI_OK : cuda_fail(e, "gemm_fp8 (pair) launch");
+}
+
+template <int MP>
+inline int launch_swap(const GemmOperands& o, const GemmArgs& g, uint32_t cs, cudaStream_t stream) {
+    constexpr uint32_t STAGE_BYTES = (128 + MP) * KB_BYTES;
+    CUtensorMap ma, mw;
+    if (const int rc = bytes_map(&mw, o.w, g.N, g.K, 128, o.ldw)) return rc;
+    if (const int rc = bytes_map(&ma, o.a, g.M, g.K, MP, o.lda)) return rc;
+    SwapGeo geo;
+    geo.cs = cs;
+    geo.m_tiles = (g.M + MP - 1u) / MP;
+    const uint32_t k_blocks = (g.K + KB_BYTES - 1u) / KB_BYTES, slice = (k_blocks + cs - 1u) / cs;
+    const uint32_t scale_bytes = slice * MP * 4u;
+    // clusters of eight find a place on half SMs only
+    const uint32_t budget = (cs == 8u ? 108u : 200u) * 1024u - scale_bytes;
+    geo.stages = budget / STAGE_BYTES;
+    if (geo.stages > (uint32_t)SWAP_MAX_STAGES) geo.stages = SWAP_MAX_STAGES;
+    if (geo.stages > slice) geo.stages = slice;
+    size_t smem = (size_t)geo.stages * STAGE_BYTES + scale_bytes;
+    const uint32_t rows = g.M < (uint32_t)MP ? g.M : (uint32_t)MP;
+    const size_t recv = cs > 1u ? (size_t)(rows + cs) * 512u : 0;
+    if (smem < recv) smem = recv;
+    const cudaError_t e = launch_cluster(gemm_fp8_swap_kernel<MP>, (g.N + 127u) / 128u * geo.m_tiles * cs, SWAP_THREADS, smem + 1024, cs, stream, mw, ma, g, geo);
+    return e == cudaSuccess ? MIORI_OK : cuda_fail(e, "gemm_fp8 (few rows) launch");
+}
+
+// Which kernel takes a product, and how.
+struct GemmPlan {
+    uint32_t pair_n;  // columns of a pair's tile, 0: the kernel of few rows
+    uint32_t mp, cs;
+};
+inline GemmPlan plan_gemm_fp8(uint32_t M, uint32_t N, uint32_t K) {
+    const uint32_t sms = (uint32_t)sm_count(), k_blocks = (K + KB_BYTES - 1u) / KB_BYTES;
+    GemmPlan p = {0, 16, 1};
+    while (p.mp < M && p.mp < 128u) p.mp *= 2u;
+    const uint64_t tiles = (uint64_t)((N + 127u) / 128u) * ((M + p.mp - 1u) / p.mp);
+    if ((M > 128u && tiles > sms) || k_blocks > 128u) {  // the kernel of few rows keeps its scales in shared memory
+        p.pair_n = N > 128u ? 256u : 128u;
+        return p;
+    }
+    while (p.cs < 8u && tiles * p.cs * 2u <= sms && k_blocks >= p.cs * 2u) p.cs *= 2u;
+    return p;
+}
+
+}  // namespace fp8
+}  // namespace miori_b200

@@ -7,4 +7,6 @@
 #include "neighbors.cu"
 #include "pages.cu"
 #include "attention.cu"
+#include "fp8.cu"
+#include "moe.cu"
 #include "peers.cu"

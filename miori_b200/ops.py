@@ -18,9 +18,9 @@ from . import _native
 _native.bind(lib._handle, MioriError)
 
 from ._native import (argmax, attention_paged, attention_prompt, dequant4_cache, dequant4_rowmajor, dequant8_rowmajor, embed8,  # noqa: E402,F401
-                      gemm_bf16_cache, gemm_bf16_strided, gemv4, gemv4_post_norm_add, gemv4_rmsnorm,
+                      gemm_bf16_cache, gemm_bf16_strided, gemm_fp8, gemv4, gemv4_post_norm_add, gemv4_rmsnorm,
                       gemv4_rmsnorm_silu, gemv4_silu, gemv8, gemv8_rmsnorm, gemv_bf16_cache, linear4,
-                      page_slots, post_norm_add, rmsnorm, rope_kv, silu_mul)
+                      moe4, moe_fp8, page_slots, post_norm_add, quant_fp8, rmsnorm, rope_kv, silu_mul)
 
 
 def cache_to_rowmajor(cache, N, K):
@@ -43,6 +43,11 @@ def gemm_workspace(M, N, K, device):
 def attention_workspace(device):
     """Zeroed scratch tensor for attention_paged and attention_prompt: one per stream that may run them."""
     return torch.zeros(lib.miori_attention_workspace_bytes(), dtype=torch.uint8, device=device)
+
+
+def moe_workspace(tokens, top, ff, device):
+    """Zeroed scratch tensor for moe4 and moe_fp8 of up to `tokens` tokens: one per stream that may run them."""
+    return torch.zeros(lib.miori_moe_workspace_bytes(tokens, top, ff), dtype=torch.uint8, device=device)
 
 
 def rope_turns(rotary, theta=None, sections=None, interleaved=False, inv_freq=None, device=None):
