@@ -464,10 +464,10 @@ int miori_gemm_fp8(const void* a, int64_t lda, const float* sa, int64_t sa_row, 
  * score is not a number comes last.  x [tokens][hidden] and router [experts][hidden] bf16, bias fp32 [experts] or NULL, out
  * [tokens][hidden] fp32 (bf16 with MIORI_OUT_BF16), which may not be x.  1..32 tokens, 1..256 experts, top 1..16.  The choice is made from
  * fp32 sums; the chosen experts' weights are read once.  A token's result depends on the other tokens in the order of its sums only.
- * workspace: miori_moe_workspace_bytes, zeroed once by its owner, left so that the next launch may use it; launches that may run
- * concurrently need workspaces of their own.  One cooperative launch, whose CTAs wait for one another once; should the wait run
- * out (a second), miori_device_error_poll tells and the workspace has to be zeroed again. */
-size_t miori_moe_workspace_bytes(uint32_t tokens, uint32_t top, uint32_t ff);
+ * workspace: miori_moe_workspace_bytes of scratch; launches that may run concurrently need workspaces of their own.  Three launches, the first of
+ * which may begin while the launch before drains: it waits for that one before it reads x or writes anything (with MIORI_LAUNCH_PDL
+ * it reads the router ahead). */
+size_t miori_moe_workspace_bytes(uint32_t tokens, uint32_t experts, uint32_t top, uint32_t ff);
 /* Packed 4-bit weights as of miori_gemv4, the experts one behind the other: up [experts][2 ff][hidden], gate rows first; down
  * [experts][hidden][ff].  hidden and ff multiples of 128. */
 int miori_moe4(const void* x, const void* router, const float* bias, const void* q_up, const void* s_up,

@@ -89,6 +89,27 @@ inline cudaError_t launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
+// The same for clusters of `cluster` CTAs, always allowed to begin before the predecessor ends.
+template <class K, class... Args>
+inline cudaError_t launch_cluster(K kernel, uint32_t grid, uint32_t threads, size_t smem, uint32_t cluster, cudaStream_t stream, const Args&... args) {
+    cudaError_t e = set_up_kernel(reinterpret_cast<const void*>(kernel), Split::DRIVERS);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1u ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // Device-side record of kernel-internal failures (bounded waits that expired).
 // word 0: error count, word 1: code of the first failure, word 2/3: detail.
 __device__ unsigned int g_device_error[4];

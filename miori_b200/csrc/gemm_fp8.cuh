@@ -497,26 +497,6 @@ inline int bytes_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t
     return make_tmap_2d(map, base, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K, rows, KB_BYTES, box_rows, CU_TENSOR_MAP_SWIZZLE_128B, (uint64_t)pitch);
 }
 
-template <class K, class... Args>
-inline cudaError_t launch_cluster(K kernel, uint32_t grid, uint32_t threads, size_t smem, uint32_t cluster, cudaStream_t stream, const Args&... args) {
-    cudaError_t e = set_up_kernel(reinterpret_cast<const void*>(kernel), Split::DRIVERS);
-    if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = cluster;
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = cluster > 1u ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 template <int BN>
 inline int launch_pair(const GemmOperands& o, GemmArgs g, cudaStream_t stream) {
     CUtensorMap ma, mw, mc;

@@ -7,39 +7,8 @@
 namespace miori_b200 {
 namespace moe {
 
-constexpr size_t COUNTER_BYTES = 256;
-
-// Clusters of this kernel that the device holds at once: the launch's grid.  Asked once per context and kernel.
-static int resident_clusters(const void* kernel, size_t smem, uint32_t* out) {
-    struct Known { const void* kernel; unsigned long long context; uint32_t clusters; };
-    static thread_local Known known[16];
-    const unsigned long long context = context_id();
-    Known* slot = nullptr;
-    for (Known& k : known) {
-        if (k.kernel == kernel && k.context == context && context) {
-            *out = k.clusters;
-            return MIORI_OK;
-        }
-        if (!slot && !k.kernel) slot = &k;
-    }
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(CLUSTER);
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = smem;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = CLUSTER;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    int n = 0;
-    const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
-    if (e != cudaSuccess) return cuda_fail(e, "cudaOccupancyMaxActiveClusters");
-    if (n < 1) return fail(MIORI_E_CUDA, "the device holds no cluster of the kernel");
-    *out = (uint32_t)n;
-    if (slot) *slot = {kernel, context, *out};
-    return MIORI_OK;
-}
+// fp32 values of the workspace in front of the activations
+static size_t logits_room(uint32_t tokens, uint32_t experts) { return ((size_t)tokens * experts + 31) / 32 * 32; }
 
 // Warps over K in gate + up: as many as leave few of them without a unit, or with one less than others.
 static uint32_t slices_for(uint32_t units) {
@@ -53,32 +22,18 @@ static uint32_t slices_for(uint32_t units) {
 
 template <Format FMT, int NT>
 static int launch_moe(const char* op, Args a, cudaStream_t stream) {
-    const void* kernel = reinterpret_cast<const void*>(moe_kernel<FMT, NT>);
-    cudaError_t e = set_up_kernel(kernel, Split::DRIVERS);
-    if (e != cudaSuccess) return cuda_fail(e, "moe set-up");
     // all of an SM's shared memory: the ring, and partial sums in the rest
     constexpr size_t smem = 227 * 1024 - (sizeof(Tables) + 127) / 128 * 128;
     a.area = (uint32_t)(smem - Stage<FMT>::RING);
+    static_assert(smem - Stage<FMT>::RING >= WARPS * NT * 512u * 5u + MAX_TOKENS * 64u, "cells of a row tile for five entries a warp (288 of one unit each), and its sums");
     a.slices = slices_for(a.up.units);
-    const uint32_t per_tile = WARPS * a.tokens * 64u;
-    a.tiles_at_once = a.area / per_tile;
-    static_assert(smem > Stage<FMT>::RING + 2u * WARPS * MAX_TOKENS * 64u, "two row tiles of partial sums, and the logits' (96 KB at most)");
-    uint32_t clusters;
-    if (const int rc = resident_clusters(kernel, smem, &clusters)) return rc;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(clusters * CLUSTER);
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = CLUSTER;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeCooperative;
-    attr[1].val.cooperative = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    e = cudaLaunchKernelEx(&cfg, moe_kernel<FMT, NT>, a);
+    const uint32_t sms = (uint32_t)sm_count(), row_tiles = a.H / 16u;
+    // clusters of four whole SMs: an SM in nine has no place in one
+    const uint32_t most = sms * 8u / 9u / CLUSTER;
+    a.per = (row_tiles + most - 1u) / most;
+    cudaError_t e = launch(moe_router_kernel, dim3((a.experts + 15u) / 16u), dim3(THREADS), 0, stream, true, a);
+    if (e == cudaSuccess) e = launch(moe_up_kernel<FMT, NT>, dim3(sms), dim3(THREADS), smem, stream, true, a);
+    if (e == cudaSuccess) e = launch_cluster(moe_down_kernel<FMT, NT>, (row_tiles + a.per - 1u) / a.per * CLUSTER, THREADS, smem, CLUSTER, stream, a);
     return e == cudaSuccess ? MIORI_OK : cuda_fail(e, op);
 }
 
@@ -94,8 +49,8 @@ static int check_common(const char* op, const void* x, const void* router, const
     if (!std::isfinite(factor)) return fail(MIORI_E_INVALID, "%s: the factor must be finite", op);
     if (!aligned16(x) || !aligned16(router) || !aligned16(out) || !aligned16(workspace) || (reinterpret_cast<uintptr_t>(bias) & 3u))
         return fail(MIORI_E_INVALID, "%s: x, router, out and workspace must be 16-byte aligned, bias by its elements", op);
-    if (workspace_bytes < miori_moe_workspace_bytes(tokens, top, ff))
-        return fail(MIORI_E_INVALID, "%s: a workspace of %zu bytes is needed, got %zu", op, miori_moe_workspace_bytes(tokens, top, ff), workspace_bytes);
+    if (workspace_bytes < miori_moe_workspace_bytes(tokens, experts, top, ff))
+        return fail(MIORI_E_INVALID, "%s: a workspace of %zu bytes is needed, got %zu", op, miori_moe_workspace_bytes(tokens, experts, top, ff), workspace_bytes);
     return MIORI_OK;
 }
 
@@ -103,8 +58,9 @@ static Args common_args(const void* x, const void* router, const float* bias, vo
                         float factor, uint32_t flags, void* workspace) {
     Args a = {};
     a.x = static_cast<const uint16_t*>(x), a.router = static_cast<const uint16_t*>(router), a.bias = bias, a.out = out;
-    a.counters = static_cast<uint32_t*>(workspace);
-    a.h = reinterpret_cast<float*>(static_cast<char*>(workspace) + COUNTER_BYTES);
+    a.logits = static_cast<float*>(workspace);
+    a.h = a.logits + logits_room(tokens, experts);
+    a.ahead = flags & MIORI_LAUNCH_PDL ? 1u : 0u;
     a.factor = factor, a.tokens = tokens, a.experts = experts, a.top = top, a.H = hidden, a.F = ff;
     a.sigmoid = flags & MIORI_MOE_SIGMOID ? 1u : 0u, a.norm = flags & MIORI_MOE_NORM ? 1u : 0u, a.bf16 = flags & MIORI_OUT_BF16 ? 1u : 0u;
     auto matrix = [](Matrix& m, uint32_t rows, uint32_t K) { m.rows = rows, m.K = K, m.units = (K + UNIT - 1u) / UNIT; };
@@ -118,8 +74,8 @@ static Args common_args(const void* x, const void* router, const float* bias, vo
 
 using namespace miori_b200;
 
-MIORI_API size_t miori_moe_workspace_bytes(uint32_t tokens, uint32_t top, uint32_t ff) {
-    return moe::COUNTER_BYTES + (size_t)tokens * top * ff * sizeof(float);
+MIORI_API size_t miori_moe_workspace_bytes(uint32_t tokens, uint32_t experts, uint32_t top, uint32_t ff) {
+    return (moe::logits_room(tokens, experts) + (size_t)tokens * top * ff) * sizeof(float);
 }
 
 MIORI_API int miori_moe4(const void* x, const void* router, const float* bias, const void* q_up, const void* s_up, const void* b_up, const void* q_down,
