@@ -462,12 +462,13 @@ int miori_gemm_fp8(const void* a, int64_t lda, const float* sa, int64_t sa_row, 
  *   out[t] = sum_e w_e W_down,e (silu(g) * u),  g = W_up,e[0 .. ff) x[t],  u = W_up,e[ff .. 2 ff) x[t].
  * An expert whose bias is -inf is never chosen; a token left with fewer than `top` has fewer, with none its row is zeros.  An expert whose
  * score is not a number comes last.  x [tokens][hidden] and router [experts][hidden] bf16, bias fp32 [experts] or NULL, out
- * [tokens][hidden] fp32 (bf16 with MIORI_OUT_BF16), which may not be x.  1..32 tokens, 1..256 experts, top 1..16.  The choice is made from
+ * [tokens][hidden] fp32 (bf16 with MIORI_OUT_BF16), which may not be x.  1..32 tokens, 1..256 experts, top 1..16, hidden up to 7168, ff up
+ * to 65536.  The choice is made from
  * fp32 sums; the chosen experts' weights are read once.  A token's result depends on the other tokens in the order of its sums only.
  * workspace: miori_moe_workspace_bytes of scratch; launches that may run concurrently need workspaces of their own.  Three launches, the first of
  * which may begin while the launch before drains: it waits for that one before it reads x or writes anything (with MIORI_LAUNCH_PDL
  * it reads the router ahead). */
-size_t miori_moe_workspace_bytes(uint32_t tokens, uint32_t experts, uint32_t top, uint32_t ff);
+size_t miori_moe_workspace_bytes(uint32_t tokens, uint32_t top, uint32_t ff);
 /* Packed 4-bit weights as of miori_gemv4, the experts one behind the other: up [experts][2 ff][hidden], gate rows first; down
  * [experts][hidden][ff].  hidden and ff multiples of 128. */
 int miori_moe4(const void* x, const void* router, const float* bias, const void* q_up, const void* s_up,

@@ -91,7 +91,7 @@ _SIGS = {
     "miori_attention_prompt": (_i, [_p] * 4 + [_strides] + [_p] * 2 + [_u32] * 6 + [C.c_float, _u32, _p, _sz, _p]),
     "miori_quant_fp8": (_i, [_p, _i64, _p, _i64, _p, _i64, _i64, _u32, _u32, _u32, _u32, _p]),
     "miori_gemm_fp8": (_i, [_p, _i64, _p, _i64, _i64, _p, _i64, _p, _i64, _i64, _p, _i64, _u32, _u32, _u32, _u32, _p]),
-    "miori_moe_workspace_bytes": (_sz, [_u32] * 4),
+    "miori_moe_workspace_bytes": (_sz, [_u32] * 3),
     "miori_moe4": (_i, [_p] * 10 + [_u32] * 6 + [C.c_float, _u32, _p, _sz, _p]),
     "miori_moe_fp8": (_i, [_p] * 8 + [_u32] * 5 + [C.c_float, _u32, _p, _sz, _p]),
     "miori_device_error_poll": (_i, []),

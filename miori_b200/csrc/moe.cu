@@ -7,34 +7,40 @@
 namespace miori_b200 {
 namespace moe {
 
-// fp32 values of the workspace in front of the activations
-static size_t logits_room(uint32_t tokens, uint32_t experts) { return ((size_t)tokens * experts + 31) / 32 * 32; }
+constexpr size_t TOPS_BYTES = MAX_ROWS * sizeof(uint32_t), HEAD_BYTES = (sizeof(Tables) + TOPS_BYTES + 255) / 256 * 256;
 
-// Warps over K in gate + up: as many as leave few of them without a unit, or with one less than others.
-static uint32_t slices_for(uint32_t units) {
-    uint32_t best = 1, best_waste = ~0u;
-    for (uint32_t s = WARPS; s; s /= 2u) {
-        const uint32_t waste = ((units + s - 1u) / s * s - units) * 1000u / units;
-        if (waste < best_waste) best = s, best_waste = waste;
-    }
-    return best;
-}
-
+// Dynamic shared memory of both products: all of an SM's that the tables leave, a ring and B fragments or partial sums in the rest.
+constexpr size_t SMEM = 227 * 1024 - (sizeof(Tables) + 127) / 128 * 128;
 template <Format FMT, int NT>
+constexpr size_t frag_room(int depth) { return SMEM - Stage<FMT>::ring(depth) - 2 * WARPS * NT * 512; }
+
+template <Format FMT, int NT, int DEPTH>
 static int launch_moe(const char* op, Args a, cudaStream_t stream) {
-    // all of an SM's shared memory: the ring, and partial sums in the rest
-    constexpr size_t smem = 227 * 1024 - (sizeof(Tables) + 127) / 128 * 128;
-    a.area = (uint32_t)(smem - Stage<FMT>::RING);
-    static_assert(smem - Stage<FMT>::RING >= WARPS * NT * 512u * 5u + MAX_TOKENS * 64u, "cells of a row tile for five entries a warp (288 of one unit each), and its sums");
-    a.slices = slices_for(a.up.units);
+    a.slots = (uint32_t)(frag_room<FMT, NT>(DEPTH) / ((size_t)a.up.units * NT * FRAG_BYTES<FMT>));
+    a.area = (uint32_t)(SMEM - Stage<FMT>::ring(Stage<FMT>::DOWN));
+    static_assert(SMEM - Stage<FMT>::ring(Stage<FMT>::DOWN) >= WARPS * NT * 512u * 5u + MAX_TOKENS * 64u,
+                  "cells of a row tile for five entries a warp (288 of one unit each), and its sums");
+    a.columns = 8u * NT;
     const uint32_t sms = (uint32_t)sm_count(), row_tiles = a.H / 16u;
     // clusters of four whole SMs: an SM in nine has no place in one
     const uint32_t most = sms * 8u / 9u / CLUSTER;
     a.per = (row_tiles + most - 1u) / most;
-    cudaError_t e = launch(moe_router_kernel, dim3((a.experts + 15u) / 16u), dim3(THREADS), 0, stream, true, a);
-    if (e == cudaSuccess) e = launch(moe_up_kernel<FMT, NT>, dim3(sms), dim3(THREADS), smem, stream, true, a);
-    if (e == cudaSuccess) e = launch_cluster(moe_down_kernel<FMT, NT>, (row_tiles + a.per - 1u) / a.per * CLUSTER, THREADS, smem, CLUSTER, stream, a);
+    cudaError_t e = launch_cluster(moe_router_kernel, ROUTER_CLUSTER, THREADS, (size_t)a.tokens * 1024u, ROUTER_CLUSTER, stream, a);
+    if (e == cudaSuccess) e = launch(moe_up_kernel<FMT, NT, DEPTH>, dim3(sms), dim3(THREADS), SMEM, stream, true, a);
+    if (e == cudaSuccess) e = launch_cluster(moe_down_kernel<FMT, NT>, (row_tiles + a.per - 1u) / a.per * CLUSTER, THREADS, SMEM, CLUSTER, stream, a);
     return e == cudaSuccess ? MIORI_OK : cuda_fail(e, op);
+}
+// 16 columns an entry from nine tokens on, where two tiles' B fragments of a row have room: an expert of 9 to 16 tokens is read once then.  Rows too long
+// for the ring of e4m3 take one of two stages.
+template <Format FMT>
+static int launch_moe(const char* op, const Args& a, cudaStream_t stream) {
+    constexpr int DEPTH = Stage<FMT>::UP;
+    const size_t frag = (size_t)a.up.units * FRAG_BYTES<FMT>;
+    if (a.tokens > 8u && 2 * frag <= frag_room<FMT, 2>(DEPTH)) return launch_moe<FMT, 2, DEPTH>(op, a, stream);
+    if constexpr (FMT == E4M3)
+        if (frag > frag_room<FMT, 1>(DEPTH)) return launch_moe<FMT, 1, 2>(op, a, stream);
+    static_assert(MAX_HIDDEN / UNIT * FRAG_BYTES<FMT> <= frag_room<FMT, 1>(FMT == E4M3 ? 2 : DEPTH), "the longest rows fit");
+    return launch_moe<FMT, 1, DEPTH>(op, a, stream);
 }
 
 static int check_common(const char* op, const void* x, const void* router, const void* out, uint32_t tokens, uint32_t experts, uint32_t top, uint32_t hidden, uint32_t ff,
@@ -45,12 +51,12 @@ static int check_common(const char* op, const void* x, const void* router, const
     if (top == 0 || top > MAX_TOP || top > experts) return fail(MIORI_E_INVALID, "%s: 1..%u of %u experts for a token, got %u", op, MAX_TOP, experts, top);
     if (hidden == 0 || ff == 0 || hidden % step || ff % step)
         return fail(MIORI_E_INVALID, "%s: hidden and ff are multiples of %u, got %u and %u", op, step, hidden, ff);
-    if (hidden > 65536u || ff > 65536u) return fail(MIORI_E_INVALID, "%s: hidden and ff are at most 65536, got %u and %u", op, hidden, ff);
+    if (hidden > MAX_HIDDEN || ff > 65536u) return fail(MIORI_E_INVALID, "%s: hidden is at most %u and ff 65536, got %u and %u", op, MAX_HIDDEN, hidden, ff);
     if (!std::isfinite(factor)) return fail(MIORI_E_INVALID, "%s: the factor must be finite", op);
     if (!aligned16(x) || !aligned16(router) || !aligned16(out) || !aligned16(workspace) || (reinterpret_cast<uintptr_t>(bias) & 3u))
         return fail(MIORI_E_INVALID, "%s: x, router, out and workspace must be 16-byte aligned, bias by its elements", op);
-    if (workspace_bytes < miori_moe_workspace_bytes(tokens, experts, top, ff))
-        return fail(MIORI_E_INVALID, "%s: a workspace of %zu bytes is needed, got %zu", op, miori_moe_workspace_bytes(tokens, experts, top, ff), workspace_bytes);
+    if (workspace_bytes < miori_moe_workspace_bytes(tokens, top, ff))
+        return fail(MIORI_E_INVALID, "%s: a workspace of %zu bytes is needed, got %zu", op, miori_moe_workspace_bytes(tokens, top, ff), workspace_bytes);
     return MIORI_OK;
 }
 
@@ -58,8 +64,8 @@ static Args common_args(const void* x, const void* router, const float* bias, vo
                         float factor, uint32_t flags, void* workspace) {
     Args a = {};
     a.x = static_cast<const uint16_t*>(x), a.router = static_cast<const uint16_t*>(router), a.bias = bias, a.out = out;
-    a.logits = static_cast<float*>(workspace);
-    a.h = a.logits + logits_room(tokens, experts);
+    char* w = static_cast<char*>(workspace);
+    a.tables = reinterpret_cast<Tables*>(w), a.h_top = reinterpret_cast<uint32_t*>(w + sizeof(Tables)), a.h = reinterpret_cast<float*>(w + HEAD_BYTES);
     a.ahead = flags & MIORI_LAUNCH_PDL ? 1u : 0u;
     a.factor = factor, a.tokens = tokens, a.experts = experts, a.top = top, a.H = hidden, a.F = ff;
     a.sigmoid = flags & MIORI_MOE_SIGMOID ? 1u : 0u, a.norm = flags & MIORI_MOE_NORM ? 1u : 0u, a.bf16 = flags & MIORI_OUT_BF16 ? 1u : 0u;
@@ -74,9 +80,7 @@ static Args common_args(const void* x, const void* router, const float* bias, vo
 
 using namespace miori_b200;
 
-MIORI_API size_t miori_moe_workspace_bytes(uint32_t tokens, uint32_t experts, uint32_t top, uint32_t ff) {
-    return (moe::logits_room(tokens, experts) + (size_t)tokens * top * ff) * sizeof(float);
-}
+MIORI_API size_t miori_moe_workspace_bytes(uint32_t tokens, uint32_t top, uint32_t ff) { return moe::HEAD_BYTES + (size_t)tokens * top * ff * sizeof(float); }
 
 MIORI_API int miori_moe4(const void* x, const void* router, const float* bias, const void* q_up, const void* s_up, const void* b_up, const void* q_down,
                          const void* s_down, const void* b_down, void* out, uint32_t tokens, uint32_t experts, uint32_t top, uint32_t hidden, uint32_t ff,
@@ -92,8 +96,7 @@ MIORI_API int miori_moe4(const void* x, const void* router, const float* bias, c
     auto u8 = [](const void* p) { return static_cast<const uint8_t*>(p); };
     a.up.q = u8(q_up), a.up.s = u8(s_up), a.up.b = u8(b_up), a.down.q = u8(q_down), a.down.s = u8(s_down), a.down.b = u8(b_down);
     const cudaStream_t s = (cudaStream_t)stream;
-    if (group == 64) return tokens <= 8 ? launch_moe<GROUP64, 1>(op, a, s) : launch_moe<GROUP64, 2>(op, a, s);
-    return tokens <= 8 ? launch_moe<GROUP32, 1>(op, a, s) : launch_moe<GROUP32, 2>(op, a, s);
+    return group == 64 ? launch_moe<GROUP64>(op, a, s) : launch_moe<GROUP32>(op, a, s);
 }
 
 MIORI_API int miori_moe_fp8(const void* x, const void* router, const float* bias, const void* w_up, const float* s_up, const void* w_down, const float* s_down,
@@ -109,5 +112,5 @@ MIORI_API int miori_moe_fp8(const void* x, const void* router, const float* bias
     a.up.q = static_cast<const uint8_t*>(w_up), a.up.s = reinterpret_cast<const uint8_t*>(s_up);
     a.down.q = static_cast<const uint8_t*>(w_down), a.down.s = reinterpret_cast<const uint8_t*>(s_down);
     const cudaStream_t s = (cudaStream_t)stream;
-    return tokens <= 8 ? launch_moe<E4M3, 1>(op, a, s) : launch_moe<E4M3, 2>(op, a, s);
+    return launch_moe<E4M3>(op, a, s);
 }

@@ -3,29 +3,33 @@
 //   out[t] = sum_e w_e W_down,e (silu(g) * u),  [g; u] = W_up,e x[t]
 //
 // Bound by the chosen experts' weights, which are read once.  Three launches, each of which begins while the one before drains:
-//   moe_router  logits, 16 experts a CTA, K over its warps;
-//   moe_up      every CTA chooses for itself from the logits (the same sums in the same order: the same choice); the rows of all chosen experts'
-//               gate and up are dealt evenly to the CTAs, eight of each an MMA tile, K over the warps, whose partial sums meet in
-//               shared memory; silu(g) * u goes to the workspace in fp32.  At its end a CTA asks L2 for its share of the down weights;
+//   moe_router  one cluster: logits, K over its CTAs and warps, the choice of each token, and the lists that the others work from;
+//   moe_up      the rows of all chosen experts' gate and up are dealt evenly to the CTAs, eight of each an MMA tile, and a CTA's tiles times K
+//               evenly to its warps; a tile that several warps share meets in shared memory.  silu(g) * u goes to the workspace
+//               in fp32, the largest of each row beside it.  At its end a CTA asks L2 for its share of the down weights;
 //   moe_down    a cluster of four CTAs owns rows of the output.  The K axes of all experts, one behind the other, are dealt to its 64 warps,
 //               whose sums meet by token, times w, in a CTA and then over the cluster, always in the same order.
-// (As one cooperative launch with a meeting of the grid between the products the layer took 23 us for a token where this takes 11: such a
-// meeting costs 2.6 us, what it saves of a launch 0.7, and clusters of a whole SM's shared memory leave 16 SMs out.)
+// (As one cooperative launch with a meeting of the grid between the products, every CTA choosing for itself, a token took 23 us: such a meeting
+// costs 2.6, a launch's hand-over 0.7, a choice 2.)
 // Experts of more tokens than an MMA tile's columns (8, or 16 from nine tokens on) are listed once for every so many.
 //
 // Weights stream through a ring of cp.async stages that belongs to one warp: 16 rows x 128 of K and their scales, no CTA-wide wait.  They become
 // fp16 without a rounding: 4-bit codes as subnormals in the bits of a half, e4m3 by conversion; products by mma.sync.m16n8k16, sums in fp32, times
-// the scales after each group.  Activations, x and silu(g) * u, are fp16 times a power of two per token and 128 of K that puts the largest into
-// [2^14, 2^15): for bf16 x no rounding down to 2^-27 of that largest (4 bits) or 2^-31; for silu(g) * u 2^-11 of a value at most, an
-// eighth of what rounding it to bf16 costs where gate + up and down are two calls.
+// the scales after each group.  What bounds the stream is less HBM than the number of instructions a stage takes: B fragments are made once
+// a CTA and expert (moe_up) or once for several row tiles (moe_down), a row of activations has one power of two.
+// Activations, x and silu(g) * u, are fp16 times a power of two per row that puts its largest into [2^14, 2^15): bf16 x is not rounded down to
+// 2^-27 of that largest (4 bits) or 2^-31; silu(g) * u by 2^-11 of a value at most, an eighth of what rounding it to bf16 costs where
+// gate + up and down are two calls.
 #pragma once
 #include "common.cuh"
+
+#include <type_traits>
 
 namespace miori_b200 {
 namespace moe {
 
-constexpr uint32_t MAX_TOKENS = 32, MAX_EXPERTS = 256, MAX_TOP = 16, MAX_ROWS = MAX_TOKENS * MAX_TOP;
-constexpr uint32_t WARPS = 16, THREADS = WARPS * 32, CLUSTER = 4;
+constexpr uint32_t MAX_TOKENS = 32, MAX_EXPERTS = 256, MAX_TOP = 16, MAX_ROWS = MAX_TOKENS * MAX_TOP, MAX_HIDDEN = 7168;
+constexpr uint32_t WARPS = 16, THREADS = WARPS * 32, CLUSTER = 4, ROUTER_CLUSTER = 8;
 constexpr uint32_t UNIT = 128;  // of K: what a stage holds of 16 rows
 constexpr uint32_t MAX_ENTRIES = MAX_EXPERTS + 32;
 constexpr size_t PREFETCH = 192 * 1024;  // bytes of down weights that a CTA of moe_up asks L2 for
@@ -36,8 +40,9 @@ struct Stage {
     static constexpr uint32_t WEIGHTS = FMT == E4M3 ? 2048 : 1024;
     static constexpr uint32_t SCALES = FMT == GROUP32 ? 256 : 128;
     static constexpr uint32_t BYTES = WEIGHTS + SCALES;
-    static constexpr uint32_t DEPTH = FMT == E4M3 ? 4 : 5;
-    static constexpr uint32_t RING = BYTES * DEPTH * WARPS;
+    // stages of a warp's ring: in moe_up, where B fragments of 7168 elements have to fit beside it, and in moe_down
+    static constexpr int UP = FMT == E4M3 ? 3 : 4, DOWN = FMT == E4M3 ? 4 : 5;
+    __host__ __device__ static constexpr uint32_t ring(int depth) { return BYTES * depth * WARPS; }
 };
 
 struct Matrix {  // [experts][rows][K]
@@ -45,30 +50,34 @@ struct Matrix {  // [experts][rows][K]
     const uint8_t *s, *b;  // bf16 [experts][rows][K / group]; e4m3: s fp32 [experts][ceil(rows / 128)][ceil(K / 128)]
     uint32_t rows, K, units;
 };
+struct Tables {
+    uint32_t mask[MAX_EXPERTS];       // tokens that chose the expert
+    uint16_t entry_of[MAX_EXPERTS];   // its first entry
+    uint16_t entry_expert[MAX_ENTRIES], entry_row[MAX_ENTRIES + 2];
+    int32_t chosen[MAX_ROWS];         // [token][place], -1: nobody
+    float weight[MAX_ROWS];
+    uint16_t slot[MAX_ROWS];          // of a place: entry * 16 + column of the entry
+    uint8_t row_token[MAX_ROWS];
+    uint32_t x_top[MAX_TOKENS];       // the largest |x| of a token, as bits
+    uint32_t entries, pad[2];
+};
+static_assert(sizeof(Tables) % 16 == 0, "copied by 16 bytes");
+
 struct Args {
     const uint16_t *x, *router;
     const float* bias;
     Matrix up, down;
     void* out;
-    float* logits;  // [tokens][experts]
-    float* h;       // [rows][F], rows: the (expert, token) pairs in the experts' order
+    Tables* tables;  // the workspace: tables, h_top, h
+    uint32_t* h_top;  // the largest |h| of a row, as bits
+    float* h;         // [rows][F], rows: the (expert, token) pairs in the experts' order
     float factor;
     uint32_t tokens, experts, top, H, F;
     uint32_t sigmoid, norm, bf16, ahead;  // ahead: weights may be read before the launch before is done
-    uint32_t slices;   // moe_up: warps over K, a power of two
-    uint32_t area;     // bytes of partial sums
+    uint32_t columns;  // of an entry: 8 or 16
+    uint32_t slots;    // moe_up: entries whose B fragments shared memory takes
+    uint32_t area;     // moe_down: bytes of partial sums
     uint32_t per;      // moe_down: row tiles of a cluster
-};
-
-struct Tables {
-    uint32_t mask[MAX_EXPERTS];       // tokens that chose the expert
-    uint16_t entry_of[MAX_EXPERTS];   // its first entry
-    uint16_t entry_expert[MAX_ENTRIES], entry_row[MAX_ENTRIES + 1];
-    uint8_t row_token[MAX_ROWS];
-    int16_t chosen[MAX_ROWS];         // [token][place], -1: nobody
-    uint16_t slot[MAX_ROWS];          // of a place: entry * 16 + column of the entry
-    float weight[MAX_ROWS];
-    uint32_t entries;
 };
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool there) {
@@ -138,62 +147,52 @@ __device__ __forceinline__ uint32_t piece_k(uint32_t t, uint32_t i) {
 template <Format FMT>
 __device__ __forceinline__ uint32_t chunk_swizzle(uint32_t g) { return FMT == GROUP64 ? (g & 2u) : (g >> 1) & 3u; }
 
-// Activations of one unit as B fragments of up to NT tiles of eight columns.
-template <Format FMT, int NT>
-struct Frag {
-    static constexpr int GROUPS = FMT == GROUP64 ? 2 : FMT == GROUP32 ? 4 : 1;
-    uint32_t b[NT][16];
-    float scale[NT][2];                                   // of the columns 2 t, 2 t + 1 whose sums this thread gets
-    float sum[NT][FMT == E4M3 ? 1 : GROUPS][2];           // theirs, times 2^-24: what the biases multiply
-};
+template <Format FMT>
+constexpr int GROUPS = FMT == GROUP64 ? 2 : FMT == GROUP32 ? 4 : 1;  // scale groups of a unit
+// What a product with 4-bit codes lacks: they are taken as multiples of 2^-24.
+template <Format FMT>
+constexpr float WHOLE = FMT == E4M3 ? 1.0f : 16777216.0f;
 
-// v: the thread's 32 elements of column g, in pieces.
-template <Format FMT, int NT>
-__device__ __forceinline__ void make_frag(Frag<FMT, NT>& f, int n, const float (&v)[32], uint32_t lane) {
-    float m = fabsf(v[0]);
-#pragma unroll
-    for (int i = 1; i < 32; ++i) m = fmaxf(m, fabsf(v[i]));
-    m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
-    m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
-    // 2^(14 - exponent of m), no further than where its reciprocal is still a normal number
-    const uint32_t field = min(268u - (__float_as_uint(m) >> 23), 253u);
-    const float up = __uint_as_float(field << 23), down = __uint_as_float((254u - field) << 23);
-    const uint32_t c0 = (lane & 3u) * 8u, c1 = c0 + 4u;  // a lane of each of the two columns
+// 2^(14 - exponent of the largest), as far as its reciprocal is a normal number; and the reciprocal.
+__device__ __forceinline__ uint32_t scale_field(uint32_t top) { return min(268u - (top >> 23), 253u); }
+__device__ __forceinline__ float scale_up(uint32_t top) { return __uint_as_float(scale_field(top) << 23); }
+__device__ __forceinline__ float scale_down(uint32_t top) { return __uint_as_float((254u - scale_field(top)) << 23); }
+
+// B fragments of eight columns and one unit.  v: the thread's 32 elements of column g, in pieces; up: the column's power of two.
+template <Format FMT>
+__device__ __forceinline__ void make_frag(uint32_t (&b)[16], const float (&v)[32], float up) {
     if constexpr (FMT == E4M3) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) f.b[n][i] = pack_half(v[2 * i] * up, v[2 * i + 1] * up);
-        f.scale[n][0] = __shfl_sync(0xFFFFFFFFu, down, c0);
-        f.scale[n][1] = __shfl_sync(0xFFFFFFFFu, down, c1);
+        for (int i = 0; i < 16; ++i) b[i] = pack_half(v[2 * i] * up, v[2 * i + 1] * up);
     } else {
         // word i, codes 0..7: codes (0, 4) and (2, 6) are taken as multiples of 2^-24, (1, 5) and (3, 7) of 2^-20
         const float up16 = up * 0.0625f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            f.b[n][4 * i] = pack_half(v[8 * i] * up, v[8 * i + 4] * up);
-            f.b[n][4 * i + 1] = pack_half(v[8 * i + 1] * up16, v[8 * i + 5] * up16);
-            f.b[n][4 * i + 2] = pack_half(v[8 * i + 2] * up, v[8 * i + 6] * up);
-            f.b[n][4 * i + 3] = pack_half(v[8 * i + 3] * up16, v[8 * i + 7] * up16);
+            b[4 * i] = pack_half(v[8 * i] * up, v[8 * i + 4] * up);
+            b[4 * i + 1] = pack_half(v[8 * i + 1] * up16, v[8 * i + 5] * up16);
+            b[4 * i + 2] = pack_half(v[8 * i + 2] * up, v[8 * i + 6] * up);
+            b[4 * i + 3] = pack_half(v[8 * i + 3] * up16, v[8 * i + 7] * up16);
         }
-        // The sums are those of the rounded values, so that a rounding counts times the weight and not times the code; by MMAs with rows of
-        // 2^-24 and 2^-20, which leave them with the threads that need them.
-        constexpr int G = Frag<FMT, NT>::GROUPS, PIECES = 4 / G;
+    }
+}
+// The columns' sums over each scale group, which the biases multiply: of the rounded values, so that a rounding counts times the weight and not
+// times the code; by MMAs with rows of 2^-24 and 2^-20, which leave the sums of columns 2 t and 2 t + 1 with thread (g, t).
+template <Format FMT>
+__device__ __forceinline__ void make_sums(float (&sum)[GROUPS<FMT>][2], const uint32_t (&b)[16]) {
+    constexpr int G = GROUPS<FMT>, PIECES = 4 / G;
 #pragma unroll
-        for (int q = 0; q < G; ++q) {
-            float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int q = 0; q < G; ++q) {
+        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int i = q * PIECES * 2; i < (q + 1) * PIECES * 2; ++i) mma_f16(s, 0x00010001u, 0x00010001u, 0x00100010u, 0x00100010u, f.b[n][2 * i], f.b[n][2 * i + 1]);
-            f.sum[n][q][0] = s[0], f.sum[n][q][1] = s[1];
-        }
-        const float whole = down * 16777216.0f;  // 2^24
-        f.scale[n][0] = __shfl_sync(0xFFFFFFFFu, whole, c0);
-        f.scale[n][1] = __shfl_sync(0xFFFFFFFFu, whole, c1);
+        for (int i = q * PIECES * 2; i < (q + 1) * PIECES * 2; ++i) mma_f16(s, 0x00010001u, 0x00010001u, 0x00100010u, 0x00100010u, b[2 * i], b[2 * i + 1]);
+        sum[q][0] = s[0], sum[q][1] = s[1];
     }
 }
 
-// One stage times one unit of activations, COUNT tiles of columns: out[n] = (row g, column 2t), (g, 2t + 1), (g + 8, 2t), (g + 8, 2t + 1), scales
-// applied.
-template <Format FMT, int NT, int COUNT>
-__device__ __forceinline__ void multiply(uint32_t stage, const Frag<FMT, NT>& f, float (&out)[NT][4], uint32_t lane) {
+// One stage times one unit of COUNT tiles of columns, added to tot[n] = (row g, column 2t), (g, 2t + 1), (g + 8, 2t), (g + 8, 2t + 1).
+template <Format FMT, int COUNT>
+__device__ __forceinline__ void multiply(uint32_t stage, const uint32_t (&b)[COUNT][16], const float (&sum)[COUNT][GROUPS<FMT>][2], float (&tot)[COUNT][4], uint32_t lane) {
     const uint32_t g = lane >> 2, t = lane & 3u;
     if constexpr (FMT == E4M3) {
         float acc[COUNT][4] = {};
@@ -207,18 +206,17 @@ __device__ __forceinline__ void multiply(uint32_t stage, const Frag<FMT, NT>& f,
                 const uint32_t a0 = e4m3_half((uint16_t)wl[i]), a2 = e4m3_half((uint16_t)(wl[i] >> 16));
                 const uint32_t a1 = e4m3_half((uint16_t)wh[i]), a3 = e4m3_half((uint16_t)(wh[i] >> 16));
 #pragma unroll
-                for (int n = 0; n < COUNT; ++n)
-                    mma_f16(acc[n], a0, a1, a2, a3, f.b[n][c * 8 + i * 2], f.b[n][c * 8 + i * 2 + 1]);
+                for (int n = 0; n < COUNT; ++n) mma_f16(acc[n], a0, a1, a2, a3, b[n][c * 8 + i * 2], b[n][c * 8 + i * 2 + 1]);
             }
         }
         const float sl = __uint_as_float(sc.x), sh = __uint_as_float(sc.y);
 #pragma unroll
         for (int n = 0; n < COUNT; ++n) {
-            out[n][0] = acc[n][0] * sl * f.scale[n][0], out[n][1] = acc[n][1] * sl * f.scale[n][1];
-            out[n][2] = acc[n][2] * sh * f.scale[n][0], out[n][3] = acc[n][3] * sh * f.scale[n][1];
+            tot[n][0] = __fmaf_rn(sl, acc[n][0], tot[n][0]), tot[n][1] = __fmaf_rn(sl, acc[n][1], tot[n][1]);
+            tot[n][2] = __fmaf_rn(sh, acc[n][2], tot[n][2]), tot[n][3] = __fmaf_rn(sh, acc[n][3], tot[n][3]);
         }
     } else {
-        constexpr int G = Frag<FMT, NT>::GROUPS, PIECES = 4 / G;
+        constexpr int G = GROUPS<FMT>, PIECES = 4 / G;
         // scales and biases of rows g and g + 8, a pair of groups a word: s lo, s hi, b lo, b hi (twice as wide in groups of 32)
         uint32_t words[4 * (G / 2)];
         if constexpr (FMT == GROUP64) {
@@ -228,44 +226,44 @@ __device__ __forceinline__ void multiply(uint32_t stage, const Frag<FMT, NT>& f,
             const uint4 w = lds128(stage + 1024u + g * 32u), z = lds128(stage + 1024u + g * 32u + 16u);
             words[0] = w.x, words[1] = w.y, words[2] = w.z, words[3] = w.w, words[4] = z.x, words[5] = z.y, words[6] = z.z, words[7] = z.w;
         }
-#pragma unroll
-        for (int n = 0; n < COUNT; ++n) out[n][0] = out[n][1] = out[n][2] = out[n][3] = 0.0f;
+        uint32_t lo[4], hi[4];
 #pragma unroll
         for (int q = 0; q < G; ++q) {
-            uint32_t lo[PIECES], hi[PIECES];
             if constexpr (FMT == GROUP64) {
                 const uint32_t at = stage + (g * 4u + ((t >> 1) + 2u * q ^ chunk_swizzle<FMT>(g))) * 16u + (t & 1u) * 8u;
                 const uint2 l = lds64(at), h = lds64(at + 512u);
-                lo[0] = l.x, lo[1] = l.y, hi[0] = h.x, hi[1] = h.y;
+                lo[2 * q] = l.x, lo[2 * q + 1] = l.y, hi[2 * q] = h.x, hi[2 * q + 1] = h.y;
             } else {
                 const uint32_t at = stage + (g * 4u + ((uint32_t)q ^ chunk_swizzle<FMT>(g))) * 16u + t * 4u;
-                lo[0] = lds32(at), hi[0] = lds32(at + 512u);
+                lo[q] = lds32(at), hi[q] = lds32(at + 512u);
             }
-            float acc[COUNT][4] = {};
+        }
+        float acc[G][COUNT][4] = {};
+        // the groups' chains of MMAs take turns
 #pragma unroll
-            for (int p = 0; p < PIECES; ++p) {
-                const uint32_t l = lo[p], h = hi[p], l8 = l >> 8, h8 = h >> 8;
+        for (int p = 0; p < PIECES; ++p)
+#pragma unroll
+            for (int q = 0; q < G; ++q) {
+                const uint32_t l = lo[q * PIECES + p], h = hi[q * PIECES + p], l8 = l >> 8, h8 = h >> 8;
                 const int at = (q * PIECES + p) * 4;
 #pragma unroll
-                for (int n = 0; n < COUNT; ++n) {
-                    mma_f16(acc[n], l & 0x000F000Fu, h & 0x000F000Fu, l & 0x00F000F0u, h & 0x00F000F0u, f.b[n][at], f.b[n][at + 1]);
-                    mma_f16(acc[n], l8 & 0x000F000Fu, h8 & 0x000F000Fu, l8 & 0x00F000F0u, h8 & 0x00F000F0u, f.b[n][at + 2], f.b[n][at + 3]);
-                }
+                for (int n = 0; n < COUNT; ++n) mma_f16(acc[q][n], l & 0x000F000Fu, h & 0x000F000Fu, l & 0x00F000F0u, h & 0x00F000F0u, b[n][at], b[n][at + 1]);
+#pragma unroll
+                for (int n = 0; n < COUNT; ++n) mma_f16(acc[q][n], l8 & 0x000F000Fu, h8 & 0x000F000Fu, l8 & 0x00F000F0u, h8 & 0x00F000F0u, b[n][at + 2], b[n][at + 3]);
             }
+#pragma unroll
+        for (int q = 0; q < G; ++q) {
             const int pair = G / 2, at = q >> 1;
             auto value = [&](int which) { return q & 1 ? bf16hi(words[which * pair + at]) : bf16lo(words[which * pair + at]); };
             const float sl = value(0), sh = value(1), bl = value(2), bh = value(3);
 #pragma unroll
             for (int n = 0; n < COUNT; ++n) {
-                out[n][0] = __fmaf_rn(sl, acc[n][0], __fmaf_rn(bl, f.sum[n][q][0], out[n][0]));
-                out[n][1] = __fmaf_rn(sl, acc[n][1], __fmaf_rn(bl, f.sum[n][q][1], out[n][1]));
-                out[n][2] = __fmaf_rn(sh, acc[n][2], __fmaf_rn(bh, f.sum[n][q][0], out[n][2]));
-                out[n][3] = __fmaf_rn(sh, acc[n][3], __fmaf_rn(bh, f.sum[n][q][1], out[n][3]));
+                tot[n][0] = __fmaf_rn(sl, acc[q][n][0], __fmaf_rn(bl, sum[n][q][0], tot[n][0]));
+                tot[n][1] = __fmaf_rn(sl, acc[q][n][1], __fmaf_rn(bl, sum[n][q][1], tot[n][1]));
+                tot[n][2] = __fmaf_rn(sh, acc[q][n][2], __fmaf_rn(bh, sum[n][q][0], tot[n][2]));
+                tot[n][3] = __fmaf_rn(sh, acc[q][n][3], __fmaf_rn(bh, sum[n][q][1], tot[n][3]));
             }
         }
-#pragma unroll
-        for (int n = 0; n < COUNT; ++n)
-            out[n][0] *= f.scale[n][0], out[n][1] *= f.scale[n][1], out[n][2] *= f.scale[n][0], out[n][3] *= f.scale[n][1];
     }
 }
 
@@ -276,77 +274,16 @@ __device__ __forceinline__ uint32_t order_key(float v) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Logits [token][expert]: a CTA has 16 experts, its warps share K.
-__global__ void __launch_bounds__(THREADS)
-moe_router_kernel(const Args a) {
-    __shared__ float part[WARPS / 2][MAX_TOKENS][16];
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
-    const uint32_t units = (a.H + UNIT - 1u) / UNIT, columns = (a.tokens + 7u) / 8u;
-    const uint32_t e_lo = blockIdx.x * 16u + g, e_hi = e_lo + 8u;
-    uint4 lo[4], hi[4];
-    auto weights = [&](uint32_t u) {
-        const uint32_t k = u * UNIT + t * 32u;
-#pragma unroll
-        for (uint32_t i = 0; i < 4u; ++i) {
-            const bool there = u < units && k + i * 8u < a.H;
-            lo[i] = hi[i] = make_uint4(0u, 0u, 0u, 0u);
-            if (there && e_lo < a.experts) lo[i] = ld_fresh(reinterpret_cast<const uint4*>(a.router + (size_t)e_lo * a.H + k + i * 8u));
-            if (there && e_hi < a.experts) hi[i] = ld_fresh(reinterpret_cast<const uint4*>(a.router + (size_t)e_hi * a.H + k + i * 8u));
-        }
-    };
-    pdl_launch_dependents();
-    if (a.ahead) weights(warp);
-    pdl_wait_prior();
-    float acc[MAX_TOKENS / 8][4] = {};
-    for (uint32_t u = warp; u < units; u += WARPS) {
-        if (u != warp || !a.ahead) weights(u);
-        const uint32_t k = u * UNIT + t * 32u;
-#pragma unroll
-        for (uint32_t n = 0; n < MAX_TOKENS / 8u; ++n) {
-            if (n >= columns) break;
-            const uint32_t token = n * 8u + g;
-            uint4 x[4];
-#pragma unroll
-            for (uint32_t i = 0; i < 4u; ++i) {
-                x[i] = make_uint4(0u, 0u, 0u, 0u);
-                if (token < a.tokens && k + i * 8u < a.H) x[i] = ld_fresh(reinterpret_cast<const uint4*>(a.x + (size_t)token * a.H + k + i * 8u));
-            }
-#pragma unroll
-            for (uint32_t i = 0; i < 4u; ++i) {
-                mma_bf16(acc[n], lo[i].x, hi[i].x, lo[i].y, hi[i].y, x[i].x, x[i].y);
-                mma_bf16(acc[n], lo[i].z, hi[i].z, lo[i].w, hi[i].w, x[i].z, x[i].w);
-            }
-        }
-    }
-    // the upper half of the warps hands its sums to the lower half, then one thread adds up an output
-    for (int half = 1; half >= 0; --half) {
-        if ((warp >= WARPS / 2) == (half == 1)) {
-#pragma unroll
-            for (uint32_t n = 0; n < MAX_TOKENS / 8u; ++n) {
-                const uint32_t token = n * 8u + 2u * t;
-#pragma unroll
-                for (uint32_t i = 0; i < 4u; ++i)
-                    if (token + (i & 1u) < a.tokens) {
-                        float& p = part[warp % (WARPS / 2)][token + (i & 1u)][g + (i < 2u ? 0u : 8u)];
-                        p = half ? acc[n][i] : p + acc[n][i];
-                    }
-            }
-        }
-        __syncthreads();
-    }
-    for (uint32_t i = threadIdx.x; i < a.tokens * 16u; i += THREADS) {
-        const uint32_t token = i / 16u, e = blockIdx.x * 16u + i % 16u;
-        float s = part[0][token][i % 16u];
-#pragma unroll
-        for (uint32_t p = 1; p < WARPS / 2; ++p) s += part[p][token][i % 16u];
-        if (e < a.experts) a.logits[token * a.experts + e] = s;
-    }
+__device__ __forceinline__ uint32_t remote(uint32_t addr, uint32_t rank) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+    return a;
 }
 
-// The choice of one token by one warp.
-__device__ __forceinline__ void choose(const Args& a, Tables& tb, uint32_t token, uint32_t lane) {
+// The choice of one token by one warp.  logit(e): the token's logit of expert e.  The results go to the tables of the cluster's first CTA.
+template <class L>
+__device__ __forceinline__ void choose(const Args& a, Tables& tb, uint32_t token, uint32_t lane, L logit) {
     constexpr int PER = MAX_EXPERTS / 32;
-    const float* logits = a.logits + token * a.experts;
     float l[PER], r[PER];
     uint32_t key[PER];
     float most = -INFINITY, total = 0.0f;
@@ -354,8 +291,8 @@ __device__ __forceinline__ void choose(const Args& a, Tables& tb, uint32_t token
     for (int j = 0; j < PER; ++j) {
         if (j * 32u >= a.experts) break;
         const uint32_t e = j * 32u + lane;
-        l[j] = e < a.experts ? ld_fresh(logits + e) : -INFINITY;
         r[j] = a.bias && e < a.experts ? ld_fresh(a.bias + e) : 0.0f;
+        l[j] = e < a.experts ? logit(e) : -INFINITY;
     }
 #pragma unroll
     for (int j = 0; j < PER; ++j)
@@ -398,9 +335,10 @@ __device__ __forceinline__ void choose(const Args& a, Tables& tb, uint32_t token
 #pragma unroll
     for (int d = 8; d; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
     if (lane < a.top) {
-        tb.chosen[token * a.top + lane] = (int16_t)expert;
-        tb.weight[token * a.top + lane] = (a.norm ? p / sum : p) * a.factor;
-        if (expert >= 0) atomicOr(&tb.mask[expert], 1u << token);
+        const uint32_t at = token * a.top + lane;
+        asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(remote(smem_addr(&tb.chosen[at]), 0)), "r"(expert) : "memory");
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote(smem_addr(&tb.weight[at]), 0)), "f"((a.norm ? p / sum : p) * a.factor) : "memory");
+        if (expert >= 0) asm volatile("red.relaxed.cluster.shared::cluster.or.b32 [%0], %1;" ::"r"(remote(smem_addr(&tb.mask[expert]), 0)), "r"(1u << token) : "memory");
     }
 }
 
@@ -427,44 +365,137 @@ __device__ __forceinline__ void list_entries(const Args& a, Tables& tb, uint32_t
     if (lane == 0) tb.entries = entry, tb.entry_row[entry] = (uint16_t)row;
 }
 
-// Who works on what, in every CTA the same.
-__device__ __forceinline__ void make_tables(const Args& a, Tables& tb, uint32_t columns, uint32_t warp, uint32_t lane) {
-    for (uint32_t e = threadIdx.x; e < a.experts; e += THREADS) tb.mask[e] = 0u;
+// Logits and choices: a cluster of eight, whose CTAs have an eighth of K each for all tokens and experts, and then every eighth token.
+__global__ void __launch_bounds__(THREADS)
+moe_router_kernel(const Args a) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ __align__(16) Tables tb;
+    float* const part = reinterpret_cast<float*>(smem);  // [slice][token][expert]
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u, rank = blockIdx.x;
+    uint32_t wide = 1;  // tiles of 16 experts, up to a power of two
+    while (wide * 16u < a.experts) wide *= 2u;
+    const uint32_t split = WARPS / wide, tile = warp % wide, slice = warp / wide, width = wide * 16u, plane = a.tokens * width;
+    const uint32_t units = (a.H + UNIT - 1u) / UNIT, u0 = rank * units / ROUTER_CLUSTER, u1 = (rank + 1u) * units / ROUTER_CLUSTER;
+    const uint32_t columns = (a.tokens + 7u) / 8u, e_lo = tile * 16u + g, e_hi = e_lo + 8u;
+    uint4 lo[4], hi[4];
+    auto weights = [&](uint32_t u) {
+        const uint32_t k = u * UNIT + t * 32u;
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; ++i) {
+            const bool there = u < u1 && k + i * 8u < a.H;
+            lo[i] = hi[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (there && e_lo < a.experts) lo[i] = ld_fresh(reinterpret_cast<const uint4*>(a.router + (size_t)e_lo * a.H + k + i * 8u));
+            if (there && e_hi < a.experts) hi[i] = ld_fresh(reinterpret_cast<const uint4*>(a.router + (size_t)e_hi * a.H + k + i * 8u));
+        }
+    };
+    if (a.ahead) weights(u0 + slice);
+    for (uint32_t e = threadIdx.x; e < MAX_EXPERTS; e += THREADS) tb.mask[e] = 0u;
+    if (threadIdx.x < MAX_TOKENS) tb.x_top[threadIdx.x] = 0u;
+    cluster_barrier();  // the other CTAs run, and their tables are clear
+    pdl_wait_prior();
+    pdl_launch_dependents();
+    if (rank == 1u && threadIdx.x < a.tokens * a.top) a.h_top[threadIdx.x] = 0u;
+    float acc[MAX_TOKENS / 8][4] = {};
+    for (uint32_t u = u0 + slice; u < u1; u += split) {
+        if (u != u0 + slice || !a.ahead) weights(u);
+        const uint32_t k = u * UNIT + t * 32u;
+        uint4 x[MAX_TOKENS / 8][4];
+#pragma unroll
+        for (uint32_t n = 0; n < MAX_TOKENS / 8u; ++n) {
+            if (n >= columns) break;
+            const uint32_t token = n * 8u + g;
+#pragma unroll
+            for (uint32_t i = 0; i < 4u; ++i) {
+                x[n][i] = make_uint4(0u, 0u, 0u, 0u);
+                if (token < a.tokens && k + i * 8u < a.H) x[n][i] = ld_fresh(reinterpret_cast<const uint4*>(a.x + (size_t)token * a.H + k + i * 8u));
+            }
+        }
+#pragma unroll
+        for (uint32_t n = 0; n < MAX_TOKENS / 8u; ++n) {
+            if (n >= columns) break;
+#pragma unroll
+            for (uint32_t i = 0; i < 4u; ++i) {
+                mma_bf16(acc[n], lo[i].x, hi[i].x, lo[i].y, hi[i].y, x[n][i].x, x[n][i].y);
+                mma_bf16(acc[n], lo[i].z, hi[i].z, lo[i].w, hi[i].w, x[n][i].z, x[n][i].w);
+            }
+            if (tile == 0u) {
+                // magnitudes of bf16 are ordered as their bits are: the larger of each half of the words
+                uint32_t m = 0u;
+#pragma unroll
+                for (uint32_t i = 0; i < 4u; ++i)
+                    m = __vmaxu2(__vmaxu2(m, __vmaxu2(x[n][i].x & 0x7FFF7FFFu, x[n][i].y & 0x7FFF7FFFu)), __vmaxu2(x[n][i].z & 0x7FFF7FFFu, x[n][i].w & 0x7FFF7FFFu));
+                m = max(m & 0xFFFFu, m >> 16) << 16;
+                m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
+                m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
+                if (t == 0u && n * 8u + g < a.tokens)
+                    asm volatile("red.relaxed.cluster.shared::cluster.max.u32 [%0], %1;" ::"r"(remote(smem_addr(&tb.x_top[n * 8u + g]), 0)), "r"(m) : "memory");
+            }
+        }
+    }
+#pragma unroll
+    for (uint32_t n = 0; n < MAX_TOKENS / 8u; ++n) {
+        const uint32_t token = n * 8u + 2u * t;
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; ++i)
+            if (token + (i & 1u) < a.tokens) part[slice * plane + (token + (i & 1u)) * width + (i < 2u ? e_lo : e_hi)] = acc[n][i];
+    }
     __syncthreads();
-    for (uint32_t token = warp; token < a.tokens; token += WARPS) choose(a, tb, token, lane);
-    __syncthreads();
-    if (warp == 0) list_entries(a, tb, columns, lane);
+    for (uint32_t i = threadIdx.x; i < plane; i += THREADS) {
+        float s = part[i];
+        for (uint32_t p = 1; p < split; ++p) s += part[p * plane + i];
+        part[i] = s;
+    }
+    cluster_barrier();
+    for (uint32_t token = rank + ROUTER_CLUSTER * warp; token < a.tokens; token += ROUTER_CLUSTER * WARPS)
+        choose(a, tb, token, lane, [&](uint32_t e) {
+            const uint32_t at = smem_addr(part + token * width + e);
+            float v[ROUTER_CLUSTER], s = 0.0f;
+#pragma unroll
+            for (uint32_t r = 0; r < ROUTER_CLUSTER; ++r) v[r] = remote_f32(at, r);
+#pragma unroll
+            for (uint32_t r = 0; r < ROUTER_CLUSTER; ++r) s += v[r];
+            return s;
+        });
+    cluster_barrier();
+    if (rank) return;
+    if (warp == 0) list_entries(a, tb, a.columns, lane);
     __syncthreads();
     if (threadIdx.x < a.tokens * a.top) {
         const int e = tb.chosen[threadIdx.x];
         if (e >= 0) {
             const uint32_t token = threadIdx.x / a.top, at = __popc(tb.mask[e] & ((1u << token) - 1u)), first = tb.entry_of[e];
             tb.row_token[tb.entry_row[first] + at] = (uint8_t)token;
-            tb.slot[threadIdx.x] = (uint16_t)((first + at / columns) * 16u + at % columns);
+            tb.slot[threadIdx.x] = (uint16_t)((first + at / a.columns) * 16u + at % a.columns);
         }
     }
     __syncthreads();
+    for (uint32_t i = threadIdx.x; i < sizeof(Tables) / 16u; i += THREADS) reinterpret_cast<uint4*>(a.tables)[i] = reinterpret_cast<const uint4*>(&tb)[i];
 }
 
-// One warp's stages: a run of tiles whose rows lie evenly apart, of one expert and one unit of K.
+__device__ __forceinline__ void read_tables(const Args& a, Tables& tb) {
+#pragma unroll
+    for (uint32_t i = threadIdx.x; i < sizeof(Tables) / 16u; i += THREADS) reinterpret_cast<uint4*>(&tb)[i] = ld_fresh(reinterpret_cast<const uint4*>(a.tables) + i);
+    __syncthreads();
+}
+
+// Where a warp's next stages come from: a run of them that lie evenly apart, of one expert.
 template <Format FMT>
 struct Run {
-    const uint8_t *q, *s;   // this thread's piece of the next tile
-    uint32_t left = 0;      // tiles
-    bool hi_there, lo_there;  // e4m3: whether the pieces lie within K
+    const uint8_t *q, *s;  // this thread's piece of the next one
+    uint32_t left = 0;     // stages
+    uint32_t k;            // e4m3: where the piece begins in its row
 
     // row: the tile's first; part: what its second eight rows lie behind the first
-    __device__ __forceinline__ void begin(const Matrix& m, uint32_t e, uint32_t row, uint32_t part, uint32_t unit, uint32_t tiles, uint32_t lane) {
+    __device__ __forceinline__ void begin(const Matrix& m, uint32_t e, uint32_t row, uint32_t part, uint32_t unit, uint32_t stages, uint32_t lane) {
         const uint32_t g = lane >> 2, t = lane & 3u;
         const size_t base = (size_t)e * m.rows + row + g;
-        left = tiles;
+        left = stages;
         if constexpr (FMT == E4M3) {
-            const uint32_t k = unit * UNIT + t * 32u;
-            lo_there = k < m.K, hi_there = k + 16u < m.K;
+            k = unit * UNIT + t * 32u;
             q = m.q + base * m.K + k;
-            // lanes 0 and 1 fetch the scales of the tile's two halves, whose rows lie within a block each
+            // lanes 0 and 1 fetch the scales of the tile's halves, each of which lies within a block
             const uint32_t blocks = (m.rows + 127u) / 128u;
-            s = m.s + (((size_t)e * blocks) * m.units + unit) * 4u;
+            s = m.s + (((size_t)e * blocks + (row + (lane ? part : 0u)) / 128u) * m.units + unit) * 4u;
         } else {
             constexpr uint32_t GROUP = FMT == GROUP64 ? 64 : 32;
             q = m.q + base * (m.K / 2u) + unit * 64u + t * 16u;
@@ -472,130 +503,197 @@ struct Run {
             s = (t < 2u ? m.s : m.b) + ((base + (t & 1u ? part : 0u)) * (m.K / GROUP) + unit * (UNIT / GROUP)) * 2u;
         }
     }
-    // row: of the tile, for the scales of e4m3; then on by `step` rows
-    __device__ __forceinline__ void fetch(uint32_t stage, const Matrix& m, uint32_t row, uint32_t part, uint32_t step, uint32_t lane) {
-        const uint32_t g = lane >> 2, t = lane & 3u;
+    // part: bytes from a piece to that of the second eight rows; then on by so many bytes and, e4m3, elements of K
+    __device__ __forceinline__ void fetch(uint32_t stage, const Matrix& m, size_t part, uint32_t q_step, uint32_t s_step, uint32_t k_step, uint32_t lane) {
         if constexpr (FMT == E4M3) {
-            const uint8_t* second = q + (size_t)part * m.K;
-            cp16(stage + lane * 16u, lo_there ? q : m.q, lo_there);
-            cp16(stage + 512u + lane * 16u, hi_there ? q + 16 : m.q, hi_there);
-            cp16(stage + 1024u + lane * 16u, lo_there ? second : m.q, lo_there);
-            cp16(stage + 1536u + lane * 16u, hi_there ? second + 16 : m.q, hi_there);
-            if (lane < 2u) cp4(stage + 2048u + lane * 4u, s + (size_t)((row + (lane ? part : 0u)) / 128u) * m.units * 4u);
-            q += (size_t)step * m.K;
+            const bool lo = k < m.K, hi = k + 16u < m.K;
+            const uint8_t* second = q + part;
+            cp16(stage + lane * 16u, lo ? q : m.q, lo);
+            cp16(stage + 512u + lane * 16u, hi ? q + 16 : m.q, hi);
+            cp16(stage + 1024u + lane * 16u, lo ? second : m.q, lo);
+            cp16(stage + 1536u + lane * 16u, hi ? second + 16 : m.q, hi);
+            if (lane < 2u) cp4(stage + 2048u + lane * 4u, s);
+            k += k_step;
         } else {
-            const uint32_t slot = (g * 4u + (t ^ chunk_swizzle<FMT>(g))) * 16u;
-            constexpr uint32_t GROUP = FMT == GROUP64 ? 64 : 32;
+            const uint32_t g = lane >> 2, t = lane & 3u, slot = (g * 4u + (t ^ chunk_swizzle<FMT>(g))) * 16u;
             cp16(stage + slot, q, true);
-            cp16(stage + 512u + slot, q + (size_t)part * (m.K / 2u), true);
+            cp16(stage + 512u + slot, q + part, true);
             if constexpr (FMT == GROUP64) cp4(stage + 1024u + lane * 4u, s);
             else cp8(stage + 1024u + lane * 8u, s);
-            q += (size_t)step * (m.K / 2u);
-            s += (size_t)step * (m.K / GROUP) * 2u;
         }
+        q += q_step, s += s_step;
         --left;
     }
 };
 
-template <Format FMT, int NT>
+// B fragments in shared memory: four planes of 16 bytes a thread, and the sums [group][column].
+template <Format FMT>
+constexpr uint32_t FRAG_BYTES = 2048 + (FMT == E4M3 ? 0 : GROUPS<FMT> * 32);
+
+template <Format FMT, int NT, int DEPTH>
 __global__ void __launch_bounds__(THREADS, 1)
 moe_up_kernel(const Args a) {
     using S = Stage<FMT>;
-    constexpr uint32_t COLUMNS = 8u * NT, CELL = NT * 512u;  // a tile's partial sums: NT float4 a thread
-    constexpr int DEPTH = S::DEPTH;
+    constexpr uint32_t CELL = NT * 512u, RING = S::ring(DEPTH);  // a tile's partial sums: NT float4 a thread
+    constexpr int G = GROUPS<FMT>;
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ Tables tb;
+    __shared__ __align__(16) Tables tb;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
-    const uint32_t ring = smem_addr(smem) + warp * (S::BYTES * DEPTH);
-    float4* const cells = reinterpret_cast<float4*>(smem + S::RING);
+    const uint32_t ring = smem_addr(smem) + warp * (S::BYTES * DEPTH), ring_end = ring + S::BYTES * DEPTH;
+    float4* const cells = reinterpret_cast<float4*>(smem + RING);  // two a warp
+    const uint32_t frags = smem_addr(smem) + RING + 2u * WARPS * CELL;
 
     pdl_wait_prior();
-    pdl_launch_dependents();  // not sooner: moe_down reads the logits before its wait
-    make_tables(a, tb, COLUMNS, warp, lane);
-    const uint32_t f_tiles = a.F / 8u;
+    pdl_launch_dependents();  // not sooner: moe_down reads the tables before its wait
+    read_tables(a, tb);
+    const uint32_t f_tiles = a.F / 8u, units = a.up.units;
     const uint64_t items = (uint64_t)tb.entries * f_tiles;
     const uint32_t i0 = (uint32_t)(items * blockIdx.x / gridDim.x), i1 = (uint32_t)(items * (blockIdx.x + 1u) / gridDim.x);
-    const uint32_t slices = a.slices, groups = WARPS / slices, slice = warp % slices, group = warp / slices;
-    const uint32_t per_round = a.area / (slices * CELL) / groups * groups;  // items
-    // A warp goes through rounds, units of its slice, entries, items of its group.  Where the next stage to be asked for is:
-    uint32_t n_first = i0, n_unit = slice, n_item = i0 + group, n_row = 0;
+    // A pass: as many entries as have room for their B fragments (one token: all, since theirs are the same).  Its tiles times units are
+    // dealt to the warps.
+    const uint32_t slots = a.tokens == 1u ? 0x10000u : a.slots;
+    auto pass_end = [&](uint32_t from) { return min(i1, (from / f_tiles + slots) * f_tiles); };
+    auto share = [&](uint32_t from, uint32_t w) { return (uint32_t)((uint64_t)(pass_end(from) - from) * units * w / WARPS); };
+
+    uint32_t n_from = i0, n_stage = 0, n_end = 0;  // the pass, stages of it to be asked for
+    if (i0 < i1) n_stage = share(i0, warp), n_end = share(i0, warp + 1u);
     Run<FMT> run;
     uint32_t put = ring, got = ring;
-    const uint32_t ring_end = ring + S::BYTES * DEPTH;
-    auto seek = [&]() {  // to the next run, where there is one
-        while (n_first < i1) {
-            const uint32_t last = min(i1, n_first + per_round);
-            if (n_unit >= a.up.units) {
-                n_first += per_round, n_unit = slice, n_item = n_first + group;
-            } else if (n_item >= last) {
-                n_unit += slices, n_item = n_first + group;
-            } else {
-                const uint32_t entry = n_item / f_tiles, end = min(last, (entry + 1u) * f_tiles);
-                n_row = (n_item - entry * f_tiles) * 8u;
-                run.begin(a.up, tb.entry_expert[entry], n_row, a.F, n_unit, (end - n_item + groups - 1u) / groups, lane);
-                n_item += run.left * groups;
-                return;
+    const size_t part = (size_t)a.F * (FMT == E4M3 ? a.H : a.H / 2u);
+    auto fill = [&]() {
+        if (run.left == 0u) {
+            while (n_from < i1 && n_stage == n_end) {
+                n_from = pass_end(n_from);
+                if (n_from < i1) n_stage = share(n_from, warp), n_end = share(n_from, warp + 1u);
+            }
+            if (n_from < i1) {
+                const uint32_t in_pass = n_stage / units, unit = n_stage - in_pass * units, item = n_from + in_pass, entry = item / f_tiles;
+                run.begin(a.up, tb.entry_expert[entry], (item - entry * f_tiles) * 8u, a.F, unit, min(units - unit, n_end - n_stage), lane);
+                n_stage += run.left;
             }
         }
-    };
-    auto fill = [&]() {
-        if (run.left == 0u && n_first < i1) seek();
-        if (run.left) {
-            run.fetch(put, a.up, n_row, a.F, groups * 8u, lane);
-            n_row += groups * 8u;
-        }
+        if (run.left) run.fetch(put, a.up, part, FMT == E4M3 ? 128u : 64u, FMT == E4M3 ? 4u : FMT == GROUP64 ? 4u : 8u, UNIT, lane);
         cp_commit();
         put += S::BYTES;
         if (put == ring_end) put = ring;
     };
     for (int i = 0; i < DEPTH - 1; ++i) fill();
-    for (uint32_t first = i0; first < i1; first += per_round) {
-        const uint32_t last = min(i1, first + per_round);
-        for (uint32_t unit = slice; unit < a.up.units; unit += slices) {
-            for (uint32_t item = first + group; item < last;) {
-                const uint32_t entry = item / f_tiles, end = min(last, (entry + 1u) * f_tiles);
-                const uint32_t row0 = tb.entry_row[entry], count = tb.entry_row[entry + 1u] - row0, tiles = (count + 7u) / 8u;
-                Frag<FMT, NT> f;
+
+    // silu(g) * u of a tile, whose sums are whole
+    auto finish = [&](uint32_t item, const float (&tot)[NT][4]) {
+        const uint32_t entry = item / f_tiles, row0 = tb.entry_row[entry], count = tb.entry_row[entry + 1u] - row0;
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    if (n && (uint32_t)n >= tiles) break;
-                    float v[32];
-                    const bool there = n * 8u + g < count;
-                    const uint16_t* x = a.x + (size_t)(there ? tb.row_token[row0 + n * 8u + g] : 0u) * a.H;
+        for (int n = 0; n < NT; ++n) {
+            if (n && n * 8u >= count) break;
+            uint32_t most[2];
 #pragma unroll
-                    for (uint32_t i = 0; i < 4u; ++i) {
-                        const uint32_t k = unit * UNIT + piece_k<FMT>(t, i);
-                        uint4 w = make_uint4(0u, 0u, 0u, 0u);
-                        if (there && k < a.H) w = ld_fresh(reinterpret_cast<const uint4*>(x + k));
-                        v[8 * i] = bf16lo(w.x), v[8 * i + 1] = bf16hi(w.x), v[8 * i + 2] = bf16lo(w.y), v[8 * i + 3] = bf16hi(w.y);
-                        v[8 * i + 4] = bf16lo(w.z), v[8 * i + 5] = bf16hi(w.z), v[8 * i + 6] = bf16lo(w.w), v[8 * i + 7] = bf16hi(w.w);
-                    }
-                    make_frag(f, n, v, lane);
+            for (uint32_t c = 0; c < 2u; ++c) {
+                const uint32_t column = n * 8u + 2u * t + c;
+                most[c] = 0u;
+                if (column < count) {
+                    const float down = scale_down(tb.x_top[tb.row_token[row0 + column]]) * WHOLE<FMT>;
+                    const float gate = tot[n][c] * down, up = tot[n][2u + c] * down, h = gate / (1.0f + expf(-gate)) * up;
+                    a.h[(size_t)(row0 + column) * a.F + (item - entry * f_tiles) * 8u + g] = h;
+                    most[c] = __float_as_uint(fabsf(h));
                 }
-                float4* cell = cells + (((item - first) * slices + slice) * NT) * 32u + lane;
-                for (; item < end; item += groups, cell += groups * slices * NT * 32u) {
-                    cp_wait<DEPTH - 2>();
-                    __syncwarp();
-                    float o[NT][4];
-                    if (NT == 1 || tiles == 1u) multiply<FMT, NT, 1>(got, f, o, lane);
-                    else multiply<FMT, NT, NT>(got, f, o, lane);
-                    got += S::BYTES;
-                    if (got == ring_end) got = ring;
-                    fill();
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        if (n && (uint32_t)n >= tiles) break;
-                        float4 s = make_float4(o[n][0], o[n][1], o[n][2], o[n][3]);
-                        if (unit != slice) {
-                            const float4 p = cell[n * 32];
-                            s.x += p.x, s.y += p.y, s.z += p.z, s.w += p.w;
-                        }
-                        cell[n * 32] = s;
-                    }
+                for (int d = 4; d < 32; d <<= 1) most[c] = max(most[c], __shfl_xor_sync(0xFFFFFFFFu, most[c], d));
+                if (g == 0u && column < count) atomicMax(a.h_top + row0 + column, most[c]);
+            }
+        }
+    };
+
+    for (uint32_t from = i0; from < i1; from = pass_end(from)) {
+        const uint32_t to = pass_end(from), entry0 = from / f_tiles, entry1 = a.tokens == 1u ? entry0 + 1u : (to - 1u) / f_tiles + 1u;
+        for (uint32_t task = warp; task < (entry1 - entry0) * units * NT; task += WARPS) {
+            const uint32_t n = task % NT, at = task / NT, slot = at / units, unit = at - slot * units;
+            const uint32_t row0 = tb.entry_row[entry0 + slot], count = tb.entry_row[entry0 + slot + 1u] - row0;
+            if (n && n * 8u >= count) continue;
+            float v[32];
+            const bool there = n * 8u + g < count;
+            const uint32_t token = there ? tb.row_token[row0 + n * 8u + g] : 0u;
+            const uint16_t* x = a.x + (size_t)token * a.H;
+#pragma unroll
+            for (uint32_t i = 0; i < 4u; ++i) {
+                const uint32_t k = unit * UNIT + piece_k<FMT>(t, i);
+                uint4 w = make_uint4(0u, 0u, 0u, 0u);
+                if (there && k < a.H) w = ld_fresh(reinterpret_cast<const uint4*>(x + k));
+                v[8 * i] = bf16lo(w.x), v[8 * i + 1] = bf16hi(w.x), v[8 * i + 2] = bf16lo(w.y), v[8 * i + 3] = bf16hi(w.y);
+                v[8 * i + 4] = bf16lo(w.z), v[8 * i + 5] = bf16hi(w.z), v[8 * i + 6] = bf16lo(w.w), v[8 * i + 7] = bf16hi(w.w);
+            }
+            uint32_t b[16];
+            make_frag<FMT>(b, v, scale_up(tb.x_top[token]));
+            const uint32_t dst = frags + task * FRAG_BYTES<FMT>;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + i * 512u + lane * 16u), "r"(b[4 * i]), "r"(b[4 * i + 1]), "r"(b[4 * i + 2]), "r"(b[4 * i + 3]) : "memory");
+            if constexpr (FMT != E4M3) {
+                float sum[G][2];
+                make_sums<FMT>(sum, b);
+                if (g == 0u) {
+#pragma unroll
+                    for (int q = 0; q < G; ++q) asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(dst + 2048u + q * 32u + t * 8u), "f"(sum[q][0]), "f"(sum[q][1]) : "memory");
                 }
             }
         }
-        if (last == i1 && warp == 0 && lane == 0) {
+        __syncthreads();
+        const uint32_t s0 = share(from, warp), s1 = share(from, warp + 1u);
+        uint32_t item = from + s0 / units, unit = s0 % units;
+        bool whole = unit == 0u, first = true;  // this warp has the tile from its first unit on; it is the warp's first
+        float tot[NT][4];
+        uint32_t at = 0, tiles = 1;  // B fragments of the next unit
+        auto enter = [&]() {
+            const uint32_t entry = item / f_tiles;
+            tiles = (tb.entry_row[entry + 1u] - tb.entry_row[entry] + 7u) / 8u;
+            at = frags + ((a.tokens == 1u ? 0u : entry - entry0) * units + unit) * (NT * FRAG_BYTES<FMT>);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) tot[n][0] = tot[n][1] = tot[n][2] = tot[n][3] = 0.0f;
+        };
+        if (s0 < s1) enter();
+        for (uint32_t stage = s0; stage < s1; ++stage) {
+            cp_wait<DEPTH - 2>();
+            __syncwarp();
+            auto step = [&](auto count) {
+                constexpr int COUNT = decltype(count)::value;
+                uint32_t b[COUNT][16];
+                float sum[COUNT][G][2];
+#pragma unroll
+                for (int n = 0; n < COUNT; ++n) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint4 w = lds128(at + n * FRAG_BYTES<FMT> + i * 512u + lane * 16u);
+                        b[n][4 * i] = w.x, b[n][4 * i + 1] = w.y, b[n][4 * i + 2] = w.z, b[n][4 * i + 3] = w.w;
+                    }
+                    if constexpr (FMT != E4M3) {
+#pragma unroll
+                        for (int q = 0; q < G; ++q) {
+                            const uint2 w = lds64(at + n * FRAG_BYTES<FMT> + 2048u + q * 32u + t * 8u);
+                            sum[n][q][0] = __uint_as_float(w.x), sum[n][q][1] = __uint_as_float(w.y);
+                        }
+                    }
+                }
+                multiply<FMT, COUNT>(got, b, sum, reinterpret_cast<float(&)[COUNT][4]>(tot), lane);
+            };
+            if (NT == 1 || tiles == 1u) step(std::integral_constant<int, 1>());
+            else step(std::integral_constant<int, NT>());
+            at += NT * FRAG_BYTES<FMT>;
+            got += S::BYTES;
+            if (got == ring_end) got = ring;
+            fill();
+            const bool end = ++unit == units;
+            if (end || stage + 1u == s1) {
+                if (end && whole) {
+                    finish(item, tot);
+                } else {
+                    float4* cell = cells + ((warp * 2u + (first ? 0u : 1u)) * NT) * 32u + lane;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) cell[n * 32] = make_float4(tot[n][0], tot[n][1], tot[n][2], tot[n][3]);
+                }
+                first = false;
+                if (end && stage + 1u < s1) ++item, unit = 0u, whole = true, enter();
+            }
+        }
+        if (to == i1 && warp == 0 && lane == 0) {
             // this CTA's share of the down weights, on their way to L2 while the sums meet: whole experts' bytes, in pieces
             const size_t expert = (size_t)a.down.rows * a.down.K / (FMT == E4M3 ? 1u : 2u), all = expert * tb.entries;
             size_t at = all * blockIdx.x / gridDim.x & ~(size_t)15, to = all * (blockIdx.x + 1u) / gridDim.x & ~(size_t)15;
@@ -608,22 +706,25 @@ moe_up_kernel(const Args a) {
             }
         }
         __syncthreads();
-        const uint32_t used = min(slices, a.up.units);
-        for (uint32_t i = threadIdx.x; i < (last - first) * CELL / 16u; i += THREADS) {
-            const uint32_t at = i / (NT * 32u), n = i / 32u % NT, entry = (first + at) / f_tiles;
-            const uint32_t row0 = tb.entry_row[entry], count = tb.entry_row[entry + 1u] - row0, column = n * 8u + 2u * t;
-            if (column >= count) continue;
-            const float4* from = cells + (at * slices * NT + n) * 32u + lane;
-            float4 s = from[0];
-            for (uint32_t p = 1; p < used; ++p) {
-                const float4 v = from[p * NT * 32u];
-                s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+        // a tile that goes on beyond the end of the warp that began it: that warp adds up the others' cells, their first ones
+        if (s0 < s1 && s1 % units) {
+            const uint32_t begin = s1 / units * units, split = from + s1 / units;
+            if (begin >= s0) {
+                const float4* cell = cells + ((warp * 2u + (s0 / units == s1 / units ? 0u : 1u)) * NT) * 32u + lane;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) tot[n][0] = cell[n * 32].x, tot[n][1] = cell[n * 32].y, tot[n][2] = cell[n * 32].z, tot[n][3] = cell[n * 32].w;
+                for (uint32_t w = warp + 1u; w < WARPS && share(from, w) < begin + units; ++w) {
+                    if (share(from, w) == share(from, w + 1u)) continue;
+                    const float4* other = cells + w * 2u * NT * 32u + lane;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        const float4 v = other[n * 32];
+                        tot[n][0] += v.x, tot[n][1] += v.y, tot[n][2] += v.z, tot[n][3] += v.w;
+                    }
+                }
+                finish(split, tot);
             }
-            float* to = a.h + (size_t)(row0 + column) * a.F + (first + at - entry * f_tiles) * 8u + g;
-            to[0] = s.x / (1.0f + expf(-s.x)) * s.z;
-            if (column + 1u < count) to[a.F] = s.y / (1.0f + expf(-s.y)) * s.w;
         }
-        __syncthreads();
     }
     cp_wait<0>();
 }
@@ -632,17 +733,18 @@ template <Format FMT, int NT>
 __global__ void __launch_bounds__(THREADS, 1)
 moe_down_kernel(const Args a) {
     using S = Stage<FMT>;
-    constexpr uint32_t COLUMNS = 8u * NT, WORKERS = CLUSTER * WARPS;
-    constexpr int DEPTH = S::DEPTH;
+    constexpr uint32_t WORKERS = CLUSTER * WARPS;
+    constexpr int DEPTH = S::DOWN, G = GROUPS<FMT>;
+    constexpr uint32_t RING = S::ring(DEPTH);
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ Tables tb;
+    __shared__ __align__(16) Tables tb;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
     const uint32_t rank = blockIdx.x % CLUSTER, cluster = blockIdx.x / CLUSTER;
-    const uint32_t ring = smem_addr(smem) + warp * (S::BYTES * DEPTH), area = smem_addr(smem) + S::RING;
-    float4* const cells = reinterpret_cast<float4*>(smem + S::RING);
+    const uint32_t ring = smem_addr(smem) + warp * (S::BYTES * DEPTH), ring_end = ring + S::BYTES * DEPTH, area = smem_addr(smem) + RING;
+    float4* const cells = reinterpret_cast<float4*>(smem + RING);
 
     pdl_launch_dependents();
-    make_tables(a, tb, COLUMNS, warp, lane);  // the logits are those of a launch that was done before moe_up let this one start
+    read_tables(a, tb);  // of a launch that was done before moe_up let this one start
     const uint32_t units = a.down.units, all_units = tb.entries * units;
     const uint32_t r0 = cluster * a.per, r1 = min(a.H / 16u, r0 + a.per);
     // warp w of the cluster has the units [all w / 64, all (w + 1) / 64)
@@ -657,7 +759,8 @@ moe_down_kernel(const Args a) {
     uint32_t n_first = r0, n_unit = u0, n_row = 0;
     Run<FMT> run;
     uint32_t put = ring, got = ring;
-    const uint32_t ring_end = ring + S::BYTES * DEPTH;
+    const size_t part = (size_t)8 * (FMT == E4M3 ? a.F : a.F / 2u);
+    const uint32_t q_step = (uint32_t)part * 2u, s_step = FMT == E4M3 ? 0u : 16u * (a.F / (FMT == GROUP64 ? 64u : 32u)) * 2u;
     auto fill = [&]() {
         if (run.left == 0u && n_first < r1 && u0 < u1) {
             const uint32_t entry = n_unit / units;
@@ -666,8 +769,11 @@ moe_down_kernel(const Args a) {
             if (++n_unit == u1) n_unit = u0, n_first += at_once;
         }
         if (run.left) {
-            run.fetch(put, a.down, n_row, 8u, 16u, lane);
-            n_row += 16u;
+            run.fetch(put, a.down, part, q_step, s_step, 0u, lane);
+            if (FMT == E4M3) {  // the next block's scales every eighth tile
+                n_row += 16u;
+                if ((n_row & 127u) == 0u) run.s += units * 4u;
+            }
         }
         cp_commit();
         put += S::BYTES;
@@ -675,22 +781,42 @@ moe_down_kernel(const Args a) {
     };
     for (int i = 0; i < DEPTH - 1; ++i) fill();
     pdl_wait_prior();
+    // In place of a place's expert: this CTA's first warp that had units of its entry, the entry's number there, how many warps.  In place of its
+    // weight that times the row's power of two.
+    if (threadIdx.x < a.tokens * a.top) {
+        uint32_t what = 0;
+        if (tb.chosen[threadIdx.x] >= 0) {
+            const uint32_t entry = tb.slot[threadIdx.x] >> 4, column = tb.slot[threadIdx.x] & 15u, begin = entry * units;
+            // the warp that has unit u is ((u + 1) 64 - 1) / all
+            const uint32_t w0 = ((begin + 1u) * WORKERS - 1u) / all_units, w1 = ((begin + units) * WORKERS - 1u) / all_units;
+            const uint32_t lo = max(w0, rank * WARPS), hi = min(w1, rank * WARPS + WARPS - 1u);
+            if (lo <= hi) what = (lo - rank * WARPS) | (entry - all_units * lo / WORKERS / units) << 8 | (hi - lo + 1u) << 16;
+            tb.weight[threadIdx.x] *= scale_down(ld_fresh(a.h_top + tb.entry_row[entry] + column)) * WHOLE<FMT>;
+        }
+        tb.chosen[threadIdx.x] = (int)what;
+    }
 
     for (uint32_t first = r0; first < r1; first += at_once) {
         const uint32_t last = min(r1, first + at_once);
         uint32_t segment = 0;
+        if (u0 == u1) {  // fewer units than warps: nothing to add, but it is added
+            for (uint32_t i = 0; i < (last - first) * NT; ++i) mine[i * 32u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
         for (uint32_t unit = u0; unit < u1; ++unit) {
             const uint32_t entry = unit / units, k0 = (unit - entry * units) * UNIT;
             const uint32_t row0 = tb.entry_row[entry], count = tb.entry_row[entry + 1u] - row0, tiles = (count + 7u) / 8u;
             const bool fresh = unit == u0 || k0 == 0u;  // the first unit of its entry here
             if (fresh && unit != u0) ++segment;
-            Frag<FMT, NT> f;
+            uint32_t b[NT][16];
+            float sum[NT][G][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 if (n && (uint32_t)n >= tiles) break;
                 float v[32];
                 const bool there = n * 8u + g < count;
-                const float* h = a.h + (size_t)(row0 + (there ? n * 8u + g : 0u)) * a.F;
+                const uint32_t row = row0 + (there ? n * 8u + g : 0u);
+                const float* h = a.h + (size_t)row * a.F;
+                const float up = scale_up(ld_fresh(a.h_top + row));
 #pragma unroll
                 for (uint32_t i = 0; i < 4u; ++i) {
                     const uint32_t k = k0 + piece_k<FMT>(t, i);
@@ -698,52 +824,48 @@ moe_down_kernel(const Args a) {
                     if (there && k < a.F) p = ld_fresh(reinterpret_cast<const float4*>(h + k)), q = ld_fresh(reinterpret_cast<const float4*>(h + k + 4u));
                     v[8 * i] = p.x, v[8 * i + 1] = p.y, v[8 * i + 2] = p.z, v[8 * i + 3] = p.w, v[8 * i + 4] = q.x, v[8 * i + 5] = q.y, v[8 * i + 6] = q.z, v[8 * i + 7] = q.w;
                 }
-                make_frag(f, n, v, lane);
+                make_frag<FMT>(b[n], v, up);
+                if constexpr (FMT != E4M3) make_sums<FMT>(sum[n], b[n]);
             }
             float4* cell = mine + segment * (at_once * NT * 32u);
             for (uint32_t tile = first; tile < last; ++tile, cell += NT * 32u) {
                 cp_wait<DEPTH - 2>();
                 __syncwarp();
-                float o[NT][4];
-                if (NT == 1 || tiles == 1u) multiply<FMT, NT, 1>(got, f, o, lane);
-                else multiply<FMT, NT, NT>(got, f, o, lane);
+                auto step = [&](auto number) {
+                    constexpr int COUNT = decltype(number)::value;
+                    float tot[COUNT][4] = {};
+                    if (!fresh) {
+#pragma unroll
+                        for (int n = 0; n < COUNT; ++n) {
+                            const float4 p = cell[n * 32];
+                            tot[n][0] = p.x, tot[n][1] = p.y, tot[n][2] = p.z, tot[n][3] = p.w;
+                        }
+                    }
+                    multiply<FMT, COUNT>(got, reinterpret_cast<const uint32_t(&)[COUNT][16]>(b), reinterpret_cast<const float(&)[COUNT][G][2]>(sum), tot, lane);
+#pragma unroll
+                    for (int n = 0; n < COUNT; ++n) cell[n * 32] = make_float4(tot[n][0], tot[n][1], tot[n][2], tot[n][3]);
+                };
+                if (NT == 1 || tiles == 1u) step(std::integral_constant<int, 1>());
+                else step(std::integral_constant<int, NT>());
                 got += S::BYTES;
                 if (got == ring_end) got = ring;
                 fill();
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    if (n && (uint32_t)n >= tiles) break;
-                    float4 s = make_float4(o[n][0], o[n][1], o[n][2], o[n][3]);
-                    if (!fresh) {
-                        const float4 p = cell[n * 32];
-                        s.x += p.x, s.y += p.y, s.z += p.z, s.w += p.w;
-                    }
-                    cell[n * 32] = s;
-                }
             }
         }
         __syncthreads();
-        // a token's places, and of each the warps of this CTA that had units of its entry
-        const uint32_t outputs = (last - first) * a.tokens * 16u;
+        // a token's places, and of each the warps of this CTA that had units of its entry: all but the first began with it
+        const uint32_t outputs = (last - first) * a.tokens * 16u, warp_floats = segments * at_once * NT * 128u;
         const float* const parts = reinterpret_cast<const float*>(cells + at_once * out_tile / 16u);
         for (uint32_t i = threadIdx.x; i < outputs; i += THREADS) {
             const uint32_t row = i & 15u, rest = i >> 4, tile = rest / a.tokens, token = rest - tile * a.tokens;
             float total = 0.0f;
-            for (uint32_t place = 0; place < a.top; ++place) {
-                const uint32_t at = token * a.top + place;
-                if (tb.chosen[at] < 0) continue;
-                const uint32_t entry = tb.slot[at] >> 4, column = tb.slot[at] & 15u, begin = entry * units, end = begin + units;
-                // the warp that has unit u is ((u + 1) 64 - 1) / all
-                const uint32_t w0 = ((begin + 1u) * WORKERS - 1u) / all_units, w1 = (end * WORKERS - 1u) / all_units;
-                const uint32_t lo = max(w0, rank * WARPS), hi = min(w1, rank * WARPS + WARPS - 1u);
+            for (uint32_t at = token * a.top; at < (token + 1u) * a.top; ++at) {
+                const uint32_t what = (uint32_t)tb.chosen[at], warps = what >> 16;
+                if (warps == 0u) continue;
+                const uint32_t column = tb.slot[at] & 15u;
+                const float* from = parts + (what & 0xFFu) * warp_floats + ((tile * NT + column / 8u) * 32u + (row & 7u) * 4u + (column & 7u) / 2u) * 4u + (column & 1u) + (row >> 3) * 2u;
                 float s = 0.0f;
-                for (uint32_t w = lo; w <= hi && w0 <= w1; ++w) {
-                    const uint32_t from = all_units * w / WORKERS;
-                    if (from == all_units * (w + 1u) / WORKERS) continue;  // no units
-                    const uint32_t seg = entry - from / units;
-                    s += parts[(((((w - rank * WARPS) * segments + seg) * at_once + tile) * NT + column / 8u) * 32u + (row & 7u) * 4u + (column & 7u) / 2u) * 4u + (column & 1u) +
-                               (row >> 3) * 2u];
-                }
+                for (uint32_t w = 0; w < warps; ++w) s += from[w * warp_floats + (w == 0u ? (what >> 8 & 0xFFu) * (at_once * NT * 128u) : 0u)];
                 total = __fmaf_rn(tb.weight[at], s, total);
             }
             sums[i] = total;
@@ -751,9 +873,11 @@ moe_down_kernel(const Args a) {
         cluster_barrier();
         const uint32_t pieces = outputs / 16u, share0 = pieces * rank / CLUSTER * 16u, share1 = pieces * (rank + 1u) / CLUSTER * 16u;
         for (uint32_t i = share0 + threadIdx.x; i < share1; i += THREADS) {
-            float s = remote_f32(area + i * 4u, 0);
+            float v[CLUSTER], s = 0.0f;
 #pragma unroll
-            for (uint32_t r = 1; r < CLUSTER; ++r) s += remote_f32(area + i * 4u, r);
+            for (uint32_t r = 0; r < CLUSTER; ++r) v[r] = remote_f32(area + i * 4u, r);
+#pragma unroll
+            for (uint32_t r = 0; r < CLUSTER; ++r) s += v[r];
             const uint32_t rest = i >> 4, tile = rest / a.tokens, token = rest - tile * a.tokens;
             const size_t at = (size_t)token * a.H + (first + tile) * 16u + (i & 15u);
             if (a.bf16) static_cast<uint16_t*>(a.out)[at] = (uint16_t)pack_bf16(s, 0.0f);

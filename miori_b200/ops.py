@@ -45,9 +45,9 @@ def attention_workspace(device):
     return torch.zeros(lib.miori_attention_workspace_bytes(), dtype=torch.uint8, device=device)
 
 
-def moe_workspace(tokens, experts, top, ff, device):
+def moe_workspace(tokens, top, ff, device):
     """Scratch tensor for moe4 and moe_fp8 of up to `tokens` tokens: one per stream that may run them."""
-    return torch.empty(lib.miori_moe_workspace_bytes(tokens, experts, top, ff), dtype=torch.uint8, device=device)
+    return torch.empty(lib.miori_moe_workspace_bytes(tokens, top, ff), dtype=torch.uint8, device=device)
 
 
 def rope_turns(rotary, theta=None, sections=None, interleaved=False, inv_freq=None, device=None):

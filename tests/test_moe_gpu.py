@@ -83,7 +83,7 @@ def oracle(x, router, ws, bits, group, top, bias, sigmoid, norm, factor):
 
 def run(x, router, ws, bits, group, top, bias, flags, factor=1.0, workspace=None, out=None):
     F = ws[0].shape[1] // 2
-    workspace = mb.moe_workspace(x.shape[0], router.shape[0], top, F, DEV) if workspace is None else workspace
+    workspace = mb.moe_workspace(x.shape[0], top, F, DEV) if workspace is None else workspace
     if bits == 4:
         return mb.moe4(x, router, *ws, top, workspace, bias=bias, group=group, factor=factor, flags=flags, out=out)
     return mb.moe_fp8(x, router, *ws, top, workspace, bias=bias, factor=factor, flags=flags, out=out)
@@ -180,7 +180,7 @@ def test_activations_of_very_different_sizes(bits, group):
 def test_repeats_graphs_streams_and_a_workspace_used_again(bits, group, T):
     """The same bits from call to call; a graph replayed with new tokens; a workspace that a larger call has used."""
     x, router, ws, bias = make(bits, group, T, 16, 512, 384, 10)
-    workspace = mb.moe_workspace(32, 16, 4, 384, DEV)
+    workspace = mb.moe_workspace(32, 4, 384, DEV)
     first = run(x, router, ws, bits, group, 4, bias, 0, workspace=workspace)
     more = make(bits, group, 32, 16, 512, 384, 11)[0]
     run(more, router, ws, bits, group, 4, bias, 0, workspace=workspace)
@@ -211,7 +211,7 @@ def test_between_launches_that_may_begin_early():
     x, router, ws, bias = make(4, 64, 4, 16, 512, 384, 12)
     q, s, b = synth.make_weight(256, 512, 4, 64, seed=4, device=DEV)
     gamma = torch.ones(512, dtype=torch.bfloat16, device=DEV)
-    workspace = mb.moe_workspace(4, 16, 2, 384, DEV)
+    workspace = mb.moe_workspace(4, 2, 384, DEV)
     for i in range(20):
         r = torch.randn(4, 512, device=DEV, generator=torch.Generator(device=DEV).manual_seed(i))
         n = mb.rmsnorm(r, gamma, 1e-5, mb.LAUNCH_PDL)
