@@ -11,36 +11,38 @@ constexpr size_t TOPS_BYTES = MAX_ROWS * sizeof(uint32_t), HEAD_BYTES = (sizeof(
 
 // Dynamic shared memory of both products: all of an SM's that the tables leave, a ring and B fragments or partial sums in the rest.
 constexpr size_t SMEM = 227 * 1024 - (sizeof(Tables) + 127) / 128 * 128;
-template <Format FMT, int NT>
-constexpr size_t frag_room(int depth) { return SMEM - Stage<FMT>::ring(depth) - 2 * WARPS * NT * 512; }
+template <Format FMT>
+constexpr size_t frag_room(int depth) { return SMEM - Stage<FMT>::ring(depth) - 2 * WARPS * 512; }
 
-template <Format FMT, int NT, int DEPTH>
+template <Format FMT, int DEPTH>
 static int launch_moe(const char* op, Args a, cudaStream_t stream) {
-    a.slots = (uint32_t)(frag_room<FMT, NT>(DEPTH) / ((size_t)a.up.units * NT * FRAG_BYTES<FMT>));
+    a.slots = (uint32_t)(frag_room<FMT>(DEPTH) / ((size_t)a.up.units * Stage<FMT>::FRAG));
     a.area = (uint32_t)(SMEM - Stage<FMT>::ring(Stage<FMT>::DOWN));
-    static_assert(SMEM - Stage<FMT>::ring(Stage<FMT>::DOWN) >= WARPS * NT * 512u * 5u + MAX_TOKENS * 64u,
-                  "cells of a row tile for five entries a warp (288 of one unit each), and its sums");
-    a.columns = 8u * NT;
+    static_assert(SMEM - Stage<FMT>::ring(Stage<FMT>::DOWN) >= WARPS * 512u * ((MAX_ENTRIES + CLUSTER * WARPS - 1) / (CLUSTER * WARPS)) + MAX_TOKENS * 64u,
+                  "cells of a row tile, were every entry one unit, and its sums");
     const uint32_t sms = (uint32_t)sm_count(), row_tiles = a.H / 16u;
     // clusters of four whole SMs: an SM in nine has no place in one
     const uint32_t most = sms * 8u / 9u / CLUSTER;
     a.per = (row_tiles + most - 1u) / most;
     cudaError_t e = launch_cluster(moe_router_kernel, ROUTER_CLUSTER, THREADS, (size_t)a.tokens * 1024u, ROUTER_CLUSTER, stream, a);
-    if (e == cudaSuccess) e = launch(moe_up_kernel<FMT, NT, DEPTH>, dim3(sms), dim3(THREADS), SMEM, stream, true, a);
-    if (e == cudaSuccess) e = launch_cluster(moe_down_kernel<FMT, NT>, (row_tiles + a.per - 1u) / a.per * CLUSTER, THREADS, SMEM, CLUSTER, stream, a);
+    if (e == cudaSuccess) e = launch(moe_up_kernel<FMT, DEPTH>, dim3(sms), dim3(THREADS), SMEM, stream, true, a);
+    if (e == cudaSuccess) e = launch_cluster(moe_down_kernel<FMT>, (row_tiles + a.per - 1u) / a.per * CLUSTER, THREADS, SMEM, CLUSTER, stream, a);
     return e == cudaSuccess ? MIORI_OK : cuda_fail(e, op);
 }
-// 16 columns an entry from nine tokens on, where two tiles' B fragments of a row have room: an expert of 9 to 16 tokens is read once then.  Rows too long
-// for the ring of e4m3 take one of two stages.
+// Rows whose B fragments do not fit beside it take a ring of two stages.
 template <Format FMT>
-static int launch_moe(const char* op, const Args& a, cudaStream_t stream) {
+static int launch_moe(const char* op, Args a, cudaStream_t stream) {
     constexpr int DEPTH = Stage<FMT>::UP;
-    const size_t frag = (size_t)a.up.units * FRAG_BYTES<FMT>;
-    if (a.tokens > 8u && 2 * frag <= frag_room<FMT, 2>(DEPTH)) return launch_moe<FMT, 2, DEPTH>(op, a, stream);
-    if constexpr (FMT == E4M3)
-        if (frag > frag_room<FMT, 1>(DEPTH)) return launch_moe<FMT, 1, 2>(op, a, stream);
-    static_assert(MAX_HIDDEN / UNIT * FRAG_BYTES<FMT> <= frag_room<FMT, 1>(FMT == E4M3 ? 2 : DEPTH), "the longest rows fit");
-    return launch_moe<FMT, 1, DEPTH>(op, a, stream);
+    constexpr uint32_t UNIT = Stage<FMT>::UNIT;
+    auto matrix = [](Matrix& m, uint32_t rows, uint32_t K) {
+        m.rows = rows, m.K = K, m.units = (K + UNIT - 1u) / UNIT, m.whole = K % UNIT == 0u;
+        m.pitch = FMT == E4M3 ? K : K / 2u, m.scale_pitch = FMT == E4M3 ? 0u : K / (FMT == GROUP64 ? 64u : 32u) * 2u;
+    };
+    matrix(a.up, 2u * a.F, a.H);
+    matrix(a.down, a.H, a.F);
+    static_assert((MAX_HIDDEN + UNIT - 1) / UNIT * Stage<FMT>::FRAG <= frag_room<FMT>(2), "the longest rows fit");
+    if ((size_t)a.up.units * Stage<FMT>::FRAG > frag_room<FMT>(DEPTH)) return launch_moe<FMT, 2>(op, a, stream);
+    return launch_moe<FMT, DEPTH>(op, a, stream);
 }
 
 static int check_common(const char* op, const void* x, const void* router, const void* out, uint32_t tokens, uint32_t experts, uint32_t top, uint32_t hidden, uint32_t ff,
@@ -69,9 +71,6 @@ static Args common_args(const void* x, const void* router, const float* bias, vo
     a.ahead = flags & MIORI_LAUNCH_PDL ? 1u : 0u;
     a.factor = factor, a.tokens = tokens, a.experts = experts, a.top = top, a.H = hidden, a.F = ff;
     a.sigmoid = flags & MIORI_MOE_SIGMOID ? 1u : 0u, a.norm = flags & MIORI_MOE_NORM ? 1u : 0u, a.bf16 = flags & MIORI_OUT_BF16 ? 1u : 0u;
-    auto matrix = [](Matrix& m, uint32_t rows, uint32_t K) { m.rows = rows, m.K = K, m.units = (K + UNIT - 1u) / UNIT; };
-    matrix(a.up, 2u * ff, hidden);
-    matrix(a.down, hidden, ff);
     return a;
 }
 
@@ -89,7 +88,7 @@ MIORI_API int miori_moe4(const void* x, const void* router, const float* bias, c
     const char* op = "miori_moe4";
     if (!q_up || !s_up || !b_up || !q_down || !s_down || !b_down) return fail(MIORI_E_INVALID, "%s: null weight pointer", op);
     if (group != 32 && group != 64) return fail(MIORI_E_INVALID, "%s: group must be 32 or 64 (got %u)", op, group);
-    if (const int rc = check_common(op, x, router, out, tokens, experts, top, hidden, ff, UNIT, factor, bias, workspace, workspace_bytes)) return rc;
+    if (const int rc = check_common(op, x, router, out, tokens, experts, top, hidden, ff, 128u, factor, bias, workspace, workspace_bytes)) return rc;
     for (const void* p : {q_up, s_up, b_up, q_down, s_down, b_down})
         if (!aligned16(p)) return fail(MIORI_E_INVALID, "%s: weights must be 16-byte aligned", op);
     Args a = common_args(x, router, bias, out, tokens, experts, top, hidden, ff, factor, flags, workspace);

@@ -11,9 +11,9 @@
 //               whose sums meet by token, times w, in a CTA and then over the cluster, always in the same order.
 // (As one cooperative launch with a meeting of the grid between the products, every CTA choosing for itself, a token took 23 us: such a meeting
 // costs 2.6, a launch's hand-over 0.7, a choice 2.)
-// Experts of more tokens than an MMA tile's columns (8, or 16 from nine tokens on) are listed once for every so many.
+// Experts of more than eight tokens, the columns of an MMA tile, are listed once for every eight; L2 serves the second reading.
 //
-// Weights stream through a ring of cp.async stages that belongs to one warp: 16 rows x 128 of K and their scales, no CTA-wide wait.  They become
+// Weights stream through a ring of cp.async stages that belongs to one warp: 16 rows x 128 bytes and their scales, no CTA-wide wait.  They become
 // fp16 without a rounding: 4-bit codes as subnormals in the bits of a half, e4m3 by conversion; products by mma.sync.m16n8k16, sums in fp32, times
 // the scales after each group.  What bounds the stream is less HBM than the number of instructions a stage takes: B fragments are made once
 // a CTA and expert (moe_up) or once for several row tiles (moe_down), a row of activations has one power of two.
@@ -23,32 +23,38 @@
 #pragma once
 #include "common.cuh"
 
-#include <type_traits>
-
 namespace miori_b200 {
 namespace moe {
 
 constexpr uint32_t MAX_TOKENS = 32, MAX_EXPERTS = 256, MAX_TOP = 16, MAX_ROWS = MAX_TOKENS * MAX_TOP, MAX_HIDDEN = 7168;
 constexpr uint32_t WARPS = 16, THREADS = WARPS * 32, CLUSTER = 4, ROUTER_CLUSTER = 8;
-constexpr uint32_t UNIT = 128;  // of K: what a stage holds of 16 rows
-constexpr uint32_t MAX_ENTRIES = MAX_EXPERTS + 32;
+constexpr uint32_t ENTRY = 8;   // tokens of an entry: the columns of an MMA tile
+constexpr uint32_t MAX_ENTRIES = MAX_EXPERTS + MAX_ROWS / ENTRY;
 constexpr size_t PREFETCH = 192 * 1024;  // bytes of down weights that a CTA of moe_up asks L2 for
 enum Format { GROUP64, GROUP32, E4M3 };
 
+// A unit of K is what 128 bytes of a row hold; a stage is a unit of 16 rows.
 template <Format FMT>
 struct Stage {
-    static constexpr uint32_t WEIGHTS = FMT == E4M3 ? 2048 : 1024;
-    static constexpr uint32_t SCALES = FMT == GROUP32 ? 256 : 128;
-    static constexpr uint32_t BYTES = WEIGHTS + SCALES;
-    // stages of a warp's ring: in moe_up, where B fragments of 7168 elements have to fit beside it, and in moe_down
-    static constexpr int UP = FMT == E4M3 ? 3 : 4, DOWN = FMT == E4M3 ? 4 : 5;
+    static constexpr uint32_t UNIT = FMT == E4M3 ? 128 : 256;
+    static constexpr uint32_t CHUNK = UNIT / 8;             // elements in 16 bytes
+    static constexpr int HALVES = UNIT / 128;               // B fragments are made for 128 of K
+    static constexpr int GROUPS = FMT == GROUP64 ? 2 : FMT == GROUP32 ? 4 : 1;  // scale groups of a half
+    static constexpr uint32_t SCALES = FMT == GROUP32 ? 512 : FMT == GROUP64 ? 256 : 128;
+    static constexpr uint32_t BYTES = 2048 + SCALES;
+    static constexpr int UP = 3, DOWN = 4;                  // stages of a warp's ring in moe_up and moe_down
     __host__ __device__ static constexpr uint32_t ring(int depth) { return BYTES * depth * WARPS; }
+    // B fragments of a half in shared memory: four planes of 16 bytes a thread, and the sums [group][column]
+    static constexpr uint32_t HALF = 2048 + (FMT == E4M3 ? 0 : GROUPS * 32);
+    static constexpr uint32_t FRAG = HALVES * HALF;
 };
 
 struct Matrix {  // [experts][rows][K]
     const uint8_t* q;
     const uint8_t *s, *b;  // bf16 [experts][rows][K / group]; e4m3: s fp32 [experts][ceil(rows / 128)][ceil(K / 128)]
     uint32_t rows, K, units;
+    uint32_t pitch, scale_pitch;  // bytes of a row of q, of a row of s and b
+    uint32_t whole;               // rows are whole units
 };
 struct Tables {
     uint32_t mask[MAX_EXPERTS];       // tokens that chose the expert
@@ -56,7 +62,7 @@ struct Tables {
     uint16_t entry_expert[MAX_ENTRIES], entry_row[MAX_ENTRIES + 2];
     int32_t chosen[MAX_ROWS];         // [token][place], -1: nobody
     float weight[MAX_ROWS];
-    uint16_t slot[MAX_ROWS];          // of a place: entry * 16 + column of the entry
+    uint16_t slot[MAX_ROWS];          // of a place: entry * 8 + column of the entry
     uint8_t row_token[MAX_ROWS];
     uint32_t x_top[MAX_TOKENS];       // the largest |x| of a token, as bits
     uint32_t entries, pad[2];
@@ -74,7 +80,6 @@ struct Args {
     float factor;
     uint32_t tokens, experts, top, H, F;
     uint32_t sigmoid, norm, bf16, ahead;  // ahead: weights may be read before the launch before is done
-    uint32_t columns;  // of an entry: 8 or 16
     uint32_t slots;    // moe_up: entries whose B fragments shared memory takes
     uint32_t area;     // moe_down: bytes of partial sums
     uint32_t per;      // moe_down: row tiles of a cluster
@@ -83,8 +88,12 @@ struct Args {
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool there) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16u : 0u) : "memory");
 }
-__device__ __forceinline__ void cp8(uint32_t dst, const void* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory"); }
-__device__ __forceinline__ void cp4(uint32_t dst, const void* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory"); }
+__device__ __forceinline__ void cp8(uint32_t dst, const void* src, bool there) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(there ? 8u : 0u) : "memory");
+}
+__device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool there = true) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4u : 0u) : "memory");
+}
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -134,21 +143,17 @@ __device__ __forceinline__ float remote_f32(uint32_t addr, uint32_t rank) {
     return v;
 }
 
-// Where K lies in a thread's fragments.  Thread (g, t) of a warp, g = lane / 4, holds of a unit 32 elements, the same of rows g and g + 8 of the weights
-// and of column g of the activations, so that one MMA, whose k axis runs over t, stays inside a scale group.  Piece i (8 elements, word i of 4-bit codes):
+// Where K lies in a thread's fragments.  Thread (g, t) of a warp, g = lane / 4, holds of 128 of K 32 elements, the same of rows g and g + 8 of the
+// weights and of column g of the activations, so that one MMA, whose k axis runs over t, stays inside a scale group.  Piece i (8 elements):
 template <Format FMT>
 __device__ __forceinline__ uint32_t piece_k(uint32_t t, uint32_t i) {
-    if (FMT == GROUP64) return (i >> 1) * 64u + t * 16u + (i & 1u) * 8u;
-    if (FMT == GROUP32) return i * 32u + t * 8u;
-    return t * 32u + i * 8u;
+    return FMT == GROUP32 ? i * 32u + t * 8u : (i >> 1) * 64u + t * 16u + (i & 1u) * 8u;
 }
-// 4-bit stages: a row's 64 bytes are four 16-byte chunks, fetched by the four threads of the row; chunk c of row g lies at slot c ^ (this), so that the
-// words that a warp's threads read next lie in different banks.
+// Chunk c (16 bytes) of row r of a stage lies at c ^ swizzle(r % 8), so that what a warp's threads read at once lies in different banks: 8 bytes of a
+// quarter of the chunks and 4 rows, 4 bytes of a chunk and 8 rows, or 16 bytes of half the chunks and 2 rows.
 template <Format FMT>
-__device__ __forceinline__ uint32_t chunk_swizzle(uint32_t g) { return FMT == GROUP64 ? (g & 2u) : (g >> 1) & 3u; }
+__device__ __forceinline__ uint32_t swizzle(uint32_t r) { return FMT == E4M3 ? (r & 1u) << 2 | r >> 1 : (r & 3u) << 1 | r >> 2; }
 
-template <Format FMT>
-constexpr int GROUPS = FMT == GROUP64 ? 2 : FMT == GROUP32 ? 4 : 1;  // scale groups of a unit
 // What a product with 4-bit codes lacks: they are taken as multiples of 2^-24.
 template <Format FMT>
 constexpr float WHOLE = FMT == E4M3 ? 1.0f : 16777216.0f;
@@ -179,8 +184,8 @@ __device__ __forceinline__ void make_frag(uint32_t (&b)[16], const float (&v)[32
 // The columns' sums over each scale group, which the biases multiply: of the rounded values, so that a rounding counts times the weight and not
 // times the code; by MMAs with rows of 2^-24 and 2^-20, which leave the sums of columns 2 t and 2 t + 1 with thread (g, t).
 template <Format FMT>
-__device__ __forceinline__ void make_sums(float (&sum)[GROUPS<FMT>][2], const uint32_t (&b)[16]) {
-    constexpr int G = GROUPS<FMT>, PIECES = 4 / G;
+__device__ __forceinline__ void make_sums(float (&sum)[Stage<FMT>::GROUPS][2], const uint32_t (&b)[16]) {
+    constexpr int G = Stage<FMT>::GROUPS, PIECES = 4 / G;
 #pragma unroll
     for (int q = 0; q < G; ++q) {
         float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -190,78 +195,80 @@ __device__ __forceinline__ void make_sums(float (&sum)[GROUPS<FMT>][2], const ui
     }
 }
 
-// One stage times one unit of COUNT tiles of columns, added to tot[n] = (row g, column 2t), (g, 2t + 1), (g + 8, 2t), (g + 8, 2t + 1).
-template <Format FMT, int COUNT>
-__device__ __forceinline__ void multiply(uint32_t stage, const uint32_t (&b)[COUNT][16], const float (&sum)[COUNT][GROUPS<FMT>][2], float (&tot)[COUNT][4], uint32_t lane) {
-    const uint32_t g = lane >> 2, t = lane & 3u;
+// One stage times one unit of eight columns, added to tot = (row g, column 2t), (g, 2t + 1), (g + 8, 2t), (g + 8, 2t + 1).
+// frag(half, b, sum): the B fragments of a half.
+template <Format FMT, class F>
+__device__ __forceinline__ void multiply(uint32_t stage, float (&tot)[4], uint32_t lane, F frag) {
+    using S = Stage<FMT>;
+    const uint32_t g = lane >> 2, t = lane & 3u, row = stage + g * 128u, s = swizzle<FMT>(g);
+    uint32_t b[16];
+    float sum[S::GROUPS][2];
     if constexpr (FMT == E4M3) {
-        float acc[COUNT][4] = {};
+        float acc[2][4] = {};
         const uint2 sc = lds64(stage + 2048u);
+        frag(0, b, sum);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-            const uint4 lo = lds128(stage + (c * 32u + lane) * 16u), hi = lds128(stage + ((2u + c) * 32u + lane) * 16u);
+            const uint32_t at = row + ((c * 4u + t) ^ s) * 16u;
+            const uint4 lo = lds128(at), hi = lds128(at + 1024u);
             const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t a0 = e4m3_half((uint16_t)wl[i]), a2 = e4m3_half((uint16_t)(wl[i] >> 16));
-                const uint32_t a1 = e4m3_half((uint16_t)wh[i]), a3 = e4m3_half((uint16_t)(wh[i] >> 16));
-#pragma unroll
-                for (int n = 0; n < COUNT; ++n) mma_f16(acc[n], a0, a1, a2, a3, b[n][c * 8 + i * 2], b[n][c * 8 + i * 2 + 1]);
-            }
+            for (int i = 0; i < 4; ++i)
+                mma_f16(acc[c], e4m3_half((uint16_t)wl[i]), e4m3_half((uint16_t)wh[i]), e4m3_half((uint16_t)(wl[i] >> 16)), e4m3_half((uint16_t)(wh[i] >> 16)),
+                        b[c * 8 + i * 2], b[c * 8 + i * 2 + 1]);
         }
         const float sl = __uint_as_float(sc.x), sh = __uint_as_float(sc.y);
-#pragma unroll
-        for (int n = 0; n < COUNT; ++n) {
-            tot[n][0] = __fmaf_rn(sl, acc[n][0], tot[n][0]), tot[n][1] = __fmaf_rn(sl, acc[n][1], tot[n][1]);
-            tot[n][2] = __fmaf_rn(sh, acc[n][2], tot[n][2]), tot[n][3] = __fmaf_rn(sh, acc[n][3], tot[n][3]);
-        }
+        tot[0] = __fmaf_rn(sl, acc[0][0] + acc[1][0], tot[0]), tot[1] = __fmaf_rn(sl, acc[0][1] + acc[1][1], tot[1]);
+        tot[2] = __fmaf_rn(sh, acc[0][2] + acc[1][2], tot[2]), tot[3] = __fmaf_rn(sh, acc[0][3] + acc[1][3], tot[3]);
     } else {
-        constexpr int G = GROUPS<FMT>, PIECES = 4 / G;
-        // scales and biases of rows g and g + 8, a pair of groups a word: s lo, s hi, b lo, b hi (twice as wide in groups of 32)
-        uint32_t words[4 * (G / 2)];
+        constexpr int G = S::GROUPS, PIECES = 4 / G;
+        // rows g and g + 8: scales, scales, biases, biases, a pair of groups a word
+        uint32_t words[4][G];
         if constexpr (FMT == GROUP64) {
-            const uint4 w = lds128(stage + 1024u + g * 16u);
-            words[0] = w.x, words[1] = w.y, words[2] = w.z, words[3] = w.w;
+            const uint4 w = lds128(stage + 2048u + g * 32u), z = lds128(stage + 2048u + g * 32u + 16u);
+            words[0][0] = w.x, words[0][1] = w.y, words[1][0] = w.z, words[1][1] = w.w, words[2][0] = z.x, words[2][1] = z.y, words[3][0] = z.z, words[3][1] = z.w;
         } else {
-            const uint4 w = lds128(stage + 1024u + g * 32u), z = lds128(stage + 1024u + g * 32u + 16u);
-            words[0] = w.x, words[1] = w.y, words[2] = w.z, words[3] = w.w, words[4] = z.x, words[5] = z.y, words[6] = z.z, words[7] = z.w;
-        }
-        uint32_t lo[4], hi[4];
 #pragma unroll
-        for (int q = 0; q < G; ++q) {
-            if constexpr (FMT == GROUP64) {
-                const uint32_t at = stage + (g * 4u + ((t >> 1) + 2u * q ^ chunk_swizzle<FMT>(g))) * 16u + (t & 1u) * 8u;
-                const uint2 l = lds64(at), h = lds64(at + 512u);
-                lo[2 * q] = l.x, lo[2 * q + 1] = l.y, hi[2 * q] = h.x, hi[2 * q + 1] = h.y;
-            } else {
-                const uint32_t at = stage + (g * 4u + ((uint32_t)q ^ chunk_swizzle<FMT>(g))) * 16u + t * 4u;
-                lo[q] = lds32(at), hi[q] = lds32(at + 512u);
+            for (int i = 0; i < 4; ++i) {
+                const uint4 w = lds128(stage + 2048u + g * 64u + i * 16u);
+                words[i][0] = w.x, words[i][1] = w.y, words[i][2] = w.z, words[i][3] = w.w;
             }
         }
-        float acc[G][COUNT][4] = {};
-        // the groups' chains of MMAs take turns
 #pragma unroll
-        for (int p = 0; p < PIECES; ++p)
+        for (int half = 0; half < 2; ++half) {
+            frag(half, b, sum);
+            uint32_t lo[4], hi[4];
 #pragma unroll
             for (int q = 0; q < G; ++q) {
-                const uint32_t l = lo[q * PIECES + p], h = hi[q * PIECES + p], l8 = l >> 8, h8 = h >> 8;
-                const int at = (q * PIECES + p) * 4;
-#pragma unroll
-                for (int n = 0; n < COUNT; ++n) mma_f16(acc[q][n], l & 0x000F000Fu, h & 0x000F000Fu, l & 0x00F000F0u, h & 0x00F000F0u, b[n][at], b[n][at + 1]);
-#pragma unroll
-                for (int n = 0; n < COUNT; ++n) mma_f16(acc[q][n], l8 & 0x000F000Fu, h8 & 0x000F000Fu, l8 & 0x00F000F0u, h8 & 0x00F000F0u, b[n][at + 2], b[n][at + 3]);
+                if constexpr (FMT == GROUP64) {
+                    const uint32_t at = row + ((half * 4u + q * 2u + (t >> 1)) ^ s) * 16u + (t & 1u) * 8u;
+                    const uint2 l = lds64(at), h = lds64(at + 1024u);
+                    lo[2 * q] = l.x, lo[2 * q + 1] = l.y, hi[2 * q] = h.x, hi[2 * q + 1] = h.y;
+                } else {
+                    const uint32_t at = row + ((half * 4u + q) ^ s) * 16u + t * 4u;
+                    lo[q] = lds32(at), hi[q] = lds32(at + 1024u);
+                }
             }
+            float acc[G][4] = {};
+            // the groups' chains of MMAs take turns
 #pragma unroll
-        for (int q = 0; q < G; ++q) {
-            const int pair = G / 2, at = q >> 1;
-            auto value = [&](int which) { return q & 1 ? bf16hi(words[which * pair + at]) : bf16lo(words[which * pair + at]); };
-            const float sl = value(0), sh = value(1), bl = value(2), bh = value(3);
+            for (int p = 0; p < PIECES; ++p)
 #pragma unroll
-            for (int n = 0; n < COUNT; ++n) {
-                tot[n][0] = __fmaf_rn(sl, acc[q][n][0], __fmaf_rn(bl, sum[n][q][0], tot[n][0]));
-                tot[n][1] = __fmaf_rn(sl, acc[q][n][1], __fmaf_rn(bl, sum[n][q][1], tot[n][1]));
-                tot[n][2] = __fmaf_rn(sh, acc[q][n][2], __fmaf_rn(bh, sum[n][q][0], tot[n][2]));
-                tot[n][3] = __fmaf_rn(sh, acc[q][n][3], __fmaf_rn(bh, sum[n][q][1], tot[n][3]));
+                for (int q = 0; q < G; ++q) {
+                    const uint32_t l = lo[q * PIECES + p], h = hi[q * PIECES + p], l8 = l >> 8, h8 = h >> 8;
+                    const int at = (q * PIECES + p) * 4;
+                    mma_f16(acc[q], l & 0x000F000Fu, h & 0x000F000Fu, l & 0x00F000F0u, h & 0x00F000F0u, b[at], b[at + 1]);
+                    mma_f16(acc[q], l8 & 0x000F000Fu, h8 & 0x000F000Fu, l8 & 0x00F000F0u, h8 & 0x00F000F0u, b[at + 2], b[at + 3]);
+                }
+#pragma unroll
+            for (int q = 0; q < G; ++q) {
+                const int group = half * G + q;
+                auto value = [&](int which) { return group & 1 ? bf16hi(words[which][group >> 1]) : bf16lo(words[which][group >> 1]); };
+                const float sl = value(0), sh = value(1), bl = value(2), bh = value(3);
+                tot[0] = __fmaf_rn(sl, acc[q][0], __fmaf_rn(bl, sum[q][0], tot[0]));
+                tot[1] = __fmaf_rn(sl, acc[q][1], __fmaf_rn(bl, sum[q][1], tot[1]));
+                tot[2] = __fmaf_rn(sh, acc[q][2], __fmaf_rn(bh, sum[q][0], tot[2]));
+                tot[3] = __fmaf_rn(sh, acc[q][3], __fmaf_rn(bh, sum[q][1], tot[3]));
             }
         }
     }
@@ -342,11 +349,11 @@ __device__ __forceinline__ void choose(const Args& a, Tables& tb, uint32_t token
     }
 }
 
-// Entries: the chosen experts in order, one for every `columns` of their tokens.  By one warp.
-__device__ __forceinline__ void list_entries(const Args& a, Tables& tb, uint32_t columns, uint32_t lane) {
+// Entries: the chosen experts in order, one for every eight of their tokens.  By one warp.
+__device__ __forceinline__ void list_entries(const Args& a, Tables& tb, uint32_t lane) {
     uint32_t entry = 0, row = 0;
     for (uint32_t e0 = 0; e0 < a.experts; e0 += 32u) {
-        const uint32_t e = e0 + lane, count = e < a.experts ? __popc(tb.mask[e]) : 0u, mine = (count + columns - 1u) / columns;
+        const uint32_t e = e0 + lane, count = e < a.experts ? __popc(tb.mask[e]) : 0u, mine = (count + ENTRY - 1u) / ENTRY;
         uint32_t before = mine << 16 | count;  // both prefix sums in one
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -358,7 +365,7 @@ __device__ __forceinline__ void list_entries(const Args& a, Tables& tb, uint32_t
         if (e < a.experts) tb.entry_of[e] = (uint16_t)my_entry;
         for (uint32_t i = 0; i < mine; ++i) {
             tb.entry_expert[my_entry + i] = (uint16_t)e;
-            tb.entry_row[my_entry + i] = (uint16_t)(my_row + i * columns);
+            tb.entry_row[my_entry + i] = (uint16_t)(my_row + i * ENTRY);
         }
         entry += all >> 16, row += all & 0xFFFFu;
     }
@@ -375,11 +382,11 @@ moe_router_kernel(const Args a) {
     uint32_t wide = 1;  // tiles of 16 experts, up to a power of two
     while (wide * 16u < a.experts) wide *= 2u;
     const uint32_t split = WARPS / wide, tile = warp % wide, slice = warp / wide, width = wide * 16u, plane = a.tokens * width;
-    const uint32_t units = (a.H + UNIT - 1u) / UNIT, u0 = rank * units / ROUTER_CLUSTER, u1 = (rank + 1u) * units / ROUTER_CLUSTER;
+    const uint32_t units = (a.H + 127u) / 128u, u0 = rank * units / ROUTER_CLUSTER, u1 = (rank + 1u) * units / ROUTER_CLUSTER;
     const uint32_t columns = (a.tokens + 7u) / 8u, e_lo = tile * 16u + g, e_hi = e_lo + 8u;
     uint4 lo[4], hi[4];
     auto weights = [&](uint32_t u) {
-        const uint32_t k = u * UNIT + t * 32u;
+        const uint32_t k = u * 128u + t * 32u;
 #pragma unroll
         for (uint32_t i = 0; i < 4u; ++i) {
             const bool there = u < u1 && k + i * 8u < a.H;
@@ -398,7 +405,7 @@ moe_router_kernel(const Args a) {
     float acc[MAX_TOKENS / 8][4] = {};
     for (uint32_t u = u0 + slice; u < u1; u += split) {
         if (u != u0 + slice || !a.ahead) weights(u);
-        const uint32_t k = u * UNIT + t * 32u;
+        const uint32_t k = u * 128u + t * 32u;
         uint4 x[MAX_TOKENS / 8][4];
 #pragma unroll
         for (uint32_t n = 0; n < MAX_TOKENS / 8u; ++n) {
@@ -458,14 +465,14 @@ moe_router_kernel(const Args a) {
         });
     cluster_barrier();
     if (rank) return;
-    if (warp == 0) list_entries(a, tb, a.columns, lane);
+    if (warp == 0) list_entries(a, tb, lane);
     __syncthreads();
     if (threadIdx.x < a.tokens * a.top) {
         const int e = tb.chosen[threadIdx.x];
         if (e >= 0) {
             const uint32_t token = threadIdx.x / a.top, at = __popc(tb.mask[e] & ((1u << token) - 1u)), first = tb.entry_of[e];
             tb.row_token[tb.entry_row[first] + at] = (uint8_t)token;
-            tb.slot[threadIdx.x] = (uint16_t)((first + at / a.columns) * 16u + at % a.columns);
+            tb.slot[threadIdx.x] = (uint16_t)(first * ENTRY + at);
         }
     }
     __syncthreads();
@@ -481,61 +488,86 @@ __device__ __forceinline__ void read_tables(const Args& a, Tables& tb) {
 // Where a warp's next stages come from: a run of them that lie evenly apart, of one expert.
 template <Format FMT>
 struct Run {
+    using S = Stage<FMT>;
     const uint8_t *q, *s;  // this thread's piece of the next one
     uint32_t left = 0;     // stages
-    uint32_t k;            // e4m3: where the piece begins in its row
+    uint32_t k;            // where the unit begins
 
     // row: the tile's first; part: what its second eight rows lie behind the first
     __device__ __forceinline__ void begin(const Matrix& m, uint32_t e, uint32_t row, uint32_t part, uint32_t unit, uint32_t stages, uint32_t lane) {
-        const uint32_t g = lane >> 2, t = lane & 3u;
-        const size_t base = (size_t)e * m.rows + row + g;
+        const size_t base = (size_t)e * m.rows + row;
         left = stages;
+        k = unit * S::UNIT;
+        // a fetch takes four rows, eight threads a row
+        q = m.q + (base + (lane >> 3)) * m.pitch + unit * 128u + (lane & 7u) * 16u;
         if constexpr (FMT == E4M3) {
-            k = unit * UNIT + t * 32u;
-            q = m.q + base * m.K + k;
             // lanes 0 and 1 fetch the scales of the tile's halves, each of which lies within a block
             const uint32_t blocks = (m.rows + 127u) / 128u;
             s = m.s + (((size_t)e * blocks + (row + (lane ? part : 0u)) / 128u) * m.units + unit) * 4u;
         } else {
-            constexpr uint32_t GROUP = FMT == GROUP64 ? 64 : 32;
-            q = m.q + base * (m.K / 2u) + unit * 64u + t * 16u;
-            // thread t of a row fetches its s, its partner's s, its b, its partner's b
-            s = (t < 2u ? m.s : m.b) + ((base + (t & 1u ? part : 0u)) * (m.K / GROUP) + unit * (UNIT / GROUP)) * 2u;
+            // thread (g, t): s of row g, s of its partner, b of row g, b of its partner
+            const uint32_t g = lane >> 2, t = lane & 3u;
+            s = (t < 2u ? m.s : m.b) + (base + g + (t & 1u ? part : 0u)) * m.scale_pitch + unit * (S::SCALES / 32u);
         }
     }
-    // part: bytes from a piece to that of the second eight rows; then on by so many bytes and, e4m3, elements of K
+    // part: bytes from a row to its partner; then on by so many bytes, and elements of K
     __device__ __forceinline__ void fetch(uint32_t stage, const Matrix& m, size_t part, uint32_t q_step, uint32_t s_step, uint32_t k_step, uint32_t lane) {
+        const uint32_t r = lane >> 3, c = lane & 7u, at = stage + r * 128u;
+        const uint32_t d0 = at + ((c ^ swizzle<FMT>(r)) << 4), d1 = at + 512u + ((c ^ swizzle<FMT>(r + 4u)) << 4);
+        const bool there = k + c * S::CHUNK < m.K;
+        const uint8_t *first = there ? q : m.q, *second = there ? q + part : m.q;
+        const uint32_t four = there ? m.pitch * 4u : 0u;
+        cp16(d0, first, there);
+        cp16(d1, first + four, there);
+        cp16(d0 + 1024u, second, there);
+        cp16(d1 + 1024u, second + four, there);
         if constexpr (FMT == E4M3) {
-            const bool lo = k < m.K, hi = k + 16u < m.K;
-            const uint8_t* second = q + part;
-            cp16(stage + lane * 16u, lo ? q : m.q, lo);
-            cp16(stage + 512u + lane * 16u, hi ? q + 16 : m.q, hi);
-            cp16(stage + 1024u + lane * 16u, lo ? second : m.q, lo);
-            cp16(stage + 1536u + lane * 16u, hi ? second + 16 : m.q, hi);
             if (lane < 2u) cp4(stage + 2048u + lane * 4u, s);
-            k += k_step;
         } else {
-            const uint32_t g = lane >> 2, t = lane & 3u, slot = (g * 4u + (t ^ chunk_swizzle<FMT>(g))) * 16u;
-            cp16(stage + slot, q, true);
-            cp16(stage + 512u + slot, q + part, true);
-            if constexpr (FMT == GROUP64) cp4(stage + 1024u + lane * 4u, s);
-            else cp8(stage + 1024u + lane * 8u, s);
+            // the biases behind K have to be numbers: they are multiplied by sums that are zero
+            const uint32_t to = stage + 2048u + lane * (S::SCALES / 32u);
+            if (m.whole) {
+                if constexpr (FMT == GROUP64) cp8(to, s, true);
+                else cp16(to, s, true);
+            } else {  // rows of an odd number of 128 elements
+                const bool more = k + 128u < m.K;
+                if constexpr (FMT == GROUP64) cp4(to, s), cp4(to + 4u, more ? s + 4 : s, more);
+                else cp8(to, s, true), cp8(to + 8u, more ? s + 8 : s, more);
+            }
         }
-        q += q_step, s += s_step;
+        q += q_step, s += s_step, k += k_step;
         --left;
     }
 };
 
-// B fragments in shared memory: four planes of 16 bytes a thread, and the sums [group][column].
+// The 32 elements of 128 of K that a thread's B fragments hold of a row of x, bf16, or of h, fp32.  K, a multiple of 16, may end among them.
 template <Format FMT>
-constexpr uint32_t FRAG_BYTES = 2048 + (FMT == E4M3 ? 0 : GROUPS<FMT> * 32);
+__device__ __forceinline__ void read_x(float (&v)[32], const uint16_t* x, bool there, uint32_t k0, uint32_t K, uint32_t t) {
+#pragma unroll
+    for (uint32_t i = 0; i < 4u; ++i) {
+        const uint32_t k = k0 + piece_k<FMT>(t, i);
+        uint4 w = make_uint4(0u, 0u, 0u, 0u);
+        if (there && k < K) w = ld_fresh(reinterpret_cast<const uint4*>(x + k));
+        v[8 * i] = bf16lo(w.x), v[8 * i + 1] = bf16hi(w.x), v[8 * i + 2] = bf16lo(w.y), v[8 * i + 3] = bf16hi(w.y);
+        v[8 * i + 4] = bf16lo(w.z), v[8 * i + 5] = bf16hi(w.z), v[8 * i + 6] = bf16lo(w.w), v[8 * i + 7] = bf16hi(w.w);
+    }
+}
+template <Format FMT>
+__device__ __forceinline__ void read_h(float (&v)[32], const float* h, bool there, uint32_t k0, uint32_t K, uint32_t t) {
+#pragma unroll
+    for (uint32_t i = 0; i < 4u; ++i) {
+        const uint32_t k = k0 + piece_k<FMT>(t, i);
+        float4 p = make_float4(0.0f, 0.0f, 0.0f, 0.0f), q = p;
+        if (there && k < K) p = ld_fresh(reinterpret_cast<const float4*>(h + k)), q = ld_fresh(reinterpret_cast<const float4*>(h + k + 4u));
+        v[8 * i] = p.x, v[8 * i + 1] = p.y, v[8 * i + 2] = p.z, v[8 * i + 3] = p.w, v[8 * i + 4] = q.x, v[8 * i + 5] = q.y, v[8 * i + 6] = q.z, v[8 * i + 7] = q.w;
+    }
+}
 
-template <Format FMT, int NT, int DEPTH>
+template <Format FMT, int DEPTH>
 __global__ void __launch_bounds__(THREADS, 1)
 moe_up_kernel(const Args a) {
     using S = Stage<FMT>;
-    constexpr uint32_t CELL = NT * 512u, RING = S::ring(DEPTH);  // a tile's partial sums: NT float4 a thread
-    constexpr int G = GROUPS<FMT>;
+    constexpr uint32_t CELL = 512u, RING = S::ring(DEPTH);  // a tile's partial sums: a float4 a thread
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ __align__(16) Tables tb;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
@@ -559,7 +591,7 @@ moe_up_kernel(const Args a) {
     if (i0 < i1) n_stage = share(i0, warp), n_end = share(i0, warp + 1u);
     Run<FMT> run;
     uint32_t put = ring, got = ring;
-    const size_t part = (size_t)a.F * (FMT == E4M3 ? a.H : a.H / 2u);
+    const size_t part = (size_t)a.F * a.up.pitch;
     auto fill = [&]() {
         if (run.left == 0u) {
             while (n_from < i1 && n_stage == n_end) {
@@ -572,7 +604,7 @@ moe_up_kernel(const Args a) {
                 n_stage += run.left;
             }
         }
-        if (run.left) run.fetch(put, a.up, part, FMT == E4M3 ? 128u : 64u, FMT == E4M3 ? 4u : FMT == GROUP64 ? 4u : 8u, UNIT, lane);
+        if (run.left) run.fetch(put, a.up, part, 128u, FMT == E4M3 ? 4u : S::SCALES / 32u, S::UNIT, lane);
         cp_commit();
         put += S::BYTES;
         if (put == ring_end) put = ring;
@@ -580,59 +612,44 @@ moe_up_kernel(const Args a) {
     for (int i = 0; i < DEPTH - 1; ++i) fill();
 
     // silu(g) * u of a tile, whose sums are whole
-    auto finish = [&](uint32_t item, const float (&tot)[NT][4]) {
+    auto finish = [&](uint32_t item, const float (&tot)[4]) {
         const uint32_t entry = item / f_tiles, row0 = tb.entry_row[entry], count = tb.entry_row[entry + 1u] - row0;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            if (n && n * 8u >= count) break;
-            uint32_t most[2];
-#pragma unroll
-            for (uint32_t c = 0; c < 2u; ++c) {
-                const uint32_t column = n * 8u + 2u * t + c;
-                most[c] = 0u;
-                if (column < count) {
-                    const float down = scale_down(tb.x_top[tb.row_token[row0 + column]]) * WHOLE<FMT>;
-                    const float gate = tot[n][c] * down, up = tot[n][2u + c] * down, h = gate / (1.0f + expf(-gate)) * up;
-                    a.h[(size_t)(row0 + column) * a.F + (item - entry * f_tiles) * 8u + g] = h;
-                    most[c] = __float_as_uint(fabsf(h));
-                }
-#pragma unroll
-                for (int d = 4; d < 32; d <<= 1) most[c] = max(most[c], __shfl_xor_sync(0xFFFFFFFFu, most[c], d));
-                if (g == 0u && column < count) atomicMax(a.h_top + row0 + column, most[c]);
+        for (uint32_t c = 0; c < 2u; ++c) {
+            const uint32_t column = 2u * t + c;
+            uint32_t most = 0u;
+            if (column < count) {
+                const float down = scale_down(tb.x_top[tb.row_token[row0 + column]]) * WHOLE<FMT>;
+                const float gate = tot[c] * down, up = tot[2u + c] * down, h = gate / (1.0f + expf(-gate)) * up;
+                a.h[(size_t)(row0 + column) * a.F + (item - entry * f_tiles) * 8u + g] = h;
+                most = __float_as_uint(fabsf(h));
             }
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, d));
+            if (g == 0u && column < count) atomicMax(a.h_top + row0 + column, most);
         }
     };
 
     for (uint32_t from = i0; from < i1; from = pass_end(from)) {
         const uint32_t to = pass_end(from), entry0 = from / f_tiles, entry1 = a.tokens == 1u ? entry0 + 1u : (to - 1u) / f_tiles + 1u;
-        for (uint32_t task = warp; task < (entry1 - entry0) * units * NT; task += WARPS) {
-            const uint32_t n = task % NT, at = task / NT, slot = at / units, unit = at - slot * units;
+        for (uint32_t task = warp; task < (entry1 - entry0) * units * S::HALVES; task += WARPS) {
+            const uint32_t half = task % S::HALVES, at = task / S::HALVES, slot = at / units, unit = at - slot * units;
             const uint32_t row0 = tb.entry_row[entry0 + slot], count = tb.entry_row[entry0 + slot + 1u] - row0;
-            if (n && n * 8u >= count) continue;
+            const uint32_t token = g < count ? tb.row_token[row0 + g] : 0u;
             float v[32];
-            const bool there = n * 8u + g < count;
-            const uint32_t token = there ? tb.row_token[row0 + n * 8u + g] : 0u;
-            const uint16_t* x = a.x + (size_t)token * a.H;
-#pragma unroll
-            for (uint32_t i = 0; i < 4u; ++i) {
-                const uint32_t k = unit * UNIT + piece_k<FMT>(t, i);
-                uint4 w = make_uint4(0u, 0u, 0u, 0u);
-                if (there && k < a.H) w = ld_fresh(reinterpret_cast<const uint4*>(x + k));
-                v[8 * i] = bf16lo(w.x), v[8 * i + 1] = bf16hi(w.x), v[8 * i + 2] = bf16lo(w.y), v[8 * i + 3] = bf16hi(w.y);
-                v[8 * i + 4] = bf16lo(w.z), v[8 * i + 5] = bf16hi(w.z), v[8 * i + 6] = bf16lo(w.w), v[8 * i + 7] = bf16hi(w.w);
-            }
+            read_x<FMT>(v, a.x + (size_t)token * a.H, g < count, unit * S::UNIT + half * 128u, a.H, t);
             uint32_t b[16];
             make_frag<FMT>(b, v, scale_up(tb.x_top[token]));
-            const uint32_t dst = frags + task * FRAG_BYTES<FMT>;
+            const uint32_t dst = frags + task * S::HALF;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + i * 512u + lane * 16u), "r"(b[4 * i]), "r"(b[4 * i + 1]), "r"(b[4 * i + 2]), "r"(b[4 * i + 3]) : "memory");
             if constexpr (FMT != E4M3) {
-                float sum[G][2];
+                float sum[S::GROUPS][2];
                 make_sums<FMT>(sum, b);
                 if (g == 0u) {
 #pragma unroll
-                    for (int q = 0; q < G; ++q) asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(dst + 2048u + q * 32u + t * 8u), "f"(sum[q][0]), "f"(sum[q][1]) : "memory");
+                    for (int q = 0; q < S::GROUPS; ++q) asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(dst + 2048u + q * 32u + t * 8u), "f"(sum[q][0]), "f"(sum[q][1]) : "memory");
                 }
             }
         }
@@ -640,62 +657,43 @@ moe_up_kernel(const Args a) {
         const uint32_t s0 = share(from, warp), s1 = share(from, warp + 1u);
         uint32_t item = from + s0 / units, unit = s0 % units;
         bool whole = unit == 0u, first = true;  // this warp has the tile from its first unit on; it is the warp's first
-        float tot[NT][4];
-        uint32_t at = 0, tiles = 1;  // B fragments of the next unit
-        auto enter = [&]() {
-            const uint32_t entry = item / f_tiles;
-            tiles = (tb.entry_row[entry + 1u] - tb.entry_row[entry] + 7u) / 8u;
-            at = frags + ((a.tokens == 1u ? 0u : entry - entry0) * units + unit) * (NT * FRAG_BYTES<FMT>);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) tot[n][0] = tot[n][1] = tot[n][2] = tot[n][3] = 0.0f;
-        };
-        if (s0 < s1) enter();
+        float tot[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        auto frag_of = [&]() { return frags + ((a.tokens == 1u ? 0u : item / f_tiles - entry0) * units + unit) * S::FRAG; };
+        uint32_t at = frag_of();  // B fragments of the next unit
         for (uint32_t stage = s0; stage < s1; ++stage) {
             cp_wait<DEPTH - 2>();
             __syncwarp();
-            auto step = [&](auto count) {
-                constexpr int COUNT = decltype(count)::value;
-                uint32_t b[COUNT][16];
-                float sum[COUNT][G][2];
+            multiply<FMT>(got, tot, lane, [&](int half, uint32_t (&b)[16], float (&sum)[S::GROUPS][2]) {
+                const uint32_t src = at + half * S::HALF;
 #pragma unroll
-                for (int n = 0; n < COUNT; ++n) {
+                for (int i = 0; i < 4; ++i) {
+                    const uint4 w = lds128(src + i * 512u + lane * 16u);
+                    b[4 * i] = w.x, b[4 * i + 1] = w.y, b[4 * i + 2] = w.z, b[4 * i + 3] = w.w;
+                }
+                if constexpr (FMT != E4M3) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint4 w = lds128(at + n * FRAG_BYTES<FMT> + i * 512u + lane * 16u);
-                        b[n][4 * i] = w.x, b[n][4 * i + 1] = w.y, b[n][4 * i + 2] = w.z, b[n][4 * i + 3] = w.w;
-                    }
-                    if constexpr (FMT != E4M3) {
-#pragma unroll
-                        for (int q = 0; q < G; ++q) {
-                            const uint2 w = lds64(at + n * FRAG_BYTES<FMT> + 2048u + q * 32u + t * 8u);
-                            sum[n][q][0] = __uint_as_float(w.x), sum[n][q][1] = __uint_as_float(w.y);
-                        }
+                    for (int q = 0; q < S::GROUPS; ++q) {
+                        const uint2 w = lds64(src + 2048u + q * 32u + t * 8u);
+                        sum[q][0] = __uint_as_float(w.x), sum[q][1] = __uint_as_float(w.y);
                     }
                 }
-                multiply<FMT, COUNT>(got, b, sum, reinterpret_cast<float(&)[COUNT][4]>(tot), lane);
-            };
-            if (NT == 1 || tiles == 1u) step(std::integral_constant<int, 1>());
-            else step(std::integral_constant<int, NT>());
-            at += NT * FRAG_BYTES<FMT>;
+            });
+            at += S::FRAG;
             got += S::BYTES;
             if (got == ring_end) got = ring;
             fill();
             const bool end = ++unit == units;
             if (end || stage + 1u == s1) {
-                if (end && whole) {
-                    finish(item, tot);
-                } else {
-                    float4* cell = cells + ((warp * 2u + (first ? 0u : 1u)) * NT) * 32u + lane;
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) cell[n * 32] = make_float4(tot[n][0], tot[n][1], tot[n][2], tot[n][3]);
-                }
+                if (end && whole) finish(item, tot);
+                else cells[(warp * 2u + (first ? 0u : 1u)) * 32u + lane] = make_float4(tot[0], tot[1], tot[2], tot[3]);
                 first = false;
-                if (end && stage + 1u < s1) ++item, unit = 0u, whole = true, enter();
+                tot[0] = tot[1] = tot[2] = tot[3] = 0.0f;
+                if (end) ++item, unit = 0u, whole = true, at = frag_of();
             }
         }
         if (to == i1 && warp == 0 && lane == 0) {
             // this CTA's share of the down weights, on their way to L2 while the sums meet: whole experts' bytes, in pieces
-            const size_t expert = (size_t)a.down.rows * a.down.K / (FMT == E4M3 ? 1u : 2u), all = expert * tb.entries;
+            const size_t expert = (size_t)a.down.rows * a.down.pitch, all = expert * tb.entries;
             size_t at = all * blockIdx.x / gridDim.x & ~(size_t)15, to = all * (blockIdx.x + 1u) / gridDim.x & ~(size_t)15;
             if (to - at > PREFETCH) to = at + PREFETCH;
             while (at < to) {
@@ -708,33 +706,28 @@ moe_up_kernel(const Args a) {
         __syncthreads();
         // a tile that goes on beyond the end of the warp that began it: that warp adds up the others' cells, their first ones
         if (s0 < s1 && s1 % units) {
-            const uint32_t begin = s1 / units * units, split = from + s1 / units;
+            const uint32_t begin = s1 / units * units;
             if (begin >= s0) {
-                const float4* cell = cells + ((warp * 2u + (s0 / units == s1 / units ? 0u : 1u)) * NT) * 32u + lane;
-#pragma unroll
-                for (int n = 0; n < NT; ++n) tot[n][0] = cell[n * 32].x, tot[n][1] = cell[n * 32].y, tot[n][2] = cell[n * 32].z, tot[n][3] = cell[n * 32].w;
+                const float4 own = cells[(warp * 2u + (s0 / units == s1 / units ? 0u : 1u)) * 32u + lane];
+                tot[0] = own.x, tot[1] = own.y, tot[2] = own.z, tot[3] = own.w;
                 for (uint32_t w = warp + 1u; w < WARPS && share(from, w) < begin + units; ++w) {
                     if (share(from, w) == share(from, w + 1u)) continue;
-                    const float4* other = cells + w * 2u * NT * 32u + lane;
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        const float4 v = other[n * 32];
-                        tot[n][0] += v.x, tot[n][1] += v.y, tot[n][2] += v.z, tot[n][3] += v.w;
-                    }
+                    const float4 v = cells[w * 64u + lane];
+                    tot[0] += v.x, tot[1] += v.y, tot[2] += v.z, tot[3] += v.w;
                 }
-                finish(split, tot);
+                finish(from + s1 / units, tot);
             }
         }
     }
     cp_wait<0>();
 }
 
-template <Format FMT, int NT>
+template <Format FMT>
 __global__ void __launch_bounds__(THREADS, 1)
 moe_down_kernel(const Args a) {
     using S = Stage<FMT>;
     constexpr uint32_t WORKERS = CLUSTER * WARPS;
-    constexpr int DEPTH = S::DOWN, G = GROUPS<FMT>;
+    constexpr int DEPTH = S::DOWN;
     constexpr uint32_t RING = S::ring(DEPTH);
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ __align__(16) Tables tb;
@@ -752,15 +745,15 @@ moe_down_kernel(const Args a) {
     // partial sums: a cell for each entry that a warp meets and each row tile of a pass
     const uint32_t segments = ((all_units + WORKERS - 1u) / WORKERS + units - 2u) / units + 1u;
     const uint32_t out_tile = a.tokens * 64u;  // bytes of the CTA's sums of a row tile, [token][16 rows]
-    const uint32_t at_once = min(a.per, a.area / (WARPS * segments * NT * 512u + out_tile));
+    const uint32_t at_once = min(a.per, a.area / (WARPS * segments * 512u + out_tile));
     float* const sums = reinterpret_cast<float*>(cells);  // in front of the cells
-    float4* const mine = cells + at_once * out_tile / 16u + warp * (segments * at_once * NT * 32u) + lane;
+    float4* const mine = cells + at_once * out_tile / 16u + warp * (segments * at_once * 32u) + lane;
 
     uint32_t n_first = r0, n_unit = u0, n_row = 0;
     Run<FMT> run;
     uint32_t put = ring, got = ring;
-    const size_t part = (size_t)8 * (FMT == E4M3 ? a.F : a.F / 2u);
-    const uint32_t q_step = (uint32_t)part * 2u, s_step = FMT == E4M3 ? 0u : 16u * (a.F / (FMT == GROUP64 ? 64u : 32u)) * 2u;
+    const size_t part = (size_t)8 * a.down.pitch;
+    const uint32_t q_step = 16u * a.down.pitch, s_step = FMT == E4M3 ? 0u : 16u * a.down.scale_pitch;
     auto fill = [&]() {
         if (run.left == 0u && n_first < r1 && u0 < u1) {
             const uint32_t entry = n_unit / units;
@@ -786,7 +779,7 @@ moe_down_kernel(const Args a) {
     if (threadIdx.x < a.tokens * a.top) {
         uint32_t what = 0;
         if (tb.chosen[threadIdx.x] >= 0) {
-            const uint32_t entry = tb.slot[threadIdx.x] >> 4, column = tb.slot[threadIdx.x] & 15u, begin = entry * units;
+            const uint32_t entry = tb.slot[threadIdx.x] / ENTRY, column = tb.slot[threadIdx.x] % ENTRY, begin = entry * units;
             // the warp that has unit u is ((u + 1) 64 - 1) / all
             const uint32_t w0 = ((begin + 1u) * WORKERS - 1u) / all_units, w1 = ((begin + units) * WORKERS - 1u) / all_units;
             const uint32_t lo = max(w0, rank * WARPS), hi = min(w1, rank * WARPS + WARPS - 1u);
@@ -800,53 +793,42 @@ moe_down_kernel(const Args a) {
         const uint32_t last = min(r1, first + at_once);
         uint32_t segment = 0;
         if (u0 == u1) {  // fewer units than warps: nothing to add, but it is added
-            for (uint32_t i = 0; i < (last - first) * NT; ++i) mine[i * 32u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (uint32_t i = 0; i < last - first; ++i) mine[i * 32u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
         for (uint32_t unit = u0; unit < u1; ++unit) {
-            const uint32_t entry = unit / units, k0 = (unit - entry * units) * UNIT;
-            const uint32_t row0 = tb.entry_row[entry], count = tb.entry_row[entry + 1u] - row0, tiles = (count + 7u) / 8u;
+            const uint32_t entry = unit / units, k0 = (unit - entry * units) * S::UNIT;
+            const uint32_t row0 = tb.entry_row[entry], count = tb.entry_row[entry + 1u] - row0;
             const bool fresh = unit == u0 || k0 == 0u;  // the first unit of its entry here
             if (fresh && unit != u0) ++segment;
-            uint32_t b[NT][16];
-            float sum[NT][G][2];
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                if (n && (uint32_t)n >= tiles) break;
-                float v[32];
-                const bool there = n * 8u + g < count;
-                const uint32_t row = row0 + (there ? n * 8u + g : 0u);
-                const float* h = a.h + (size_t)row * a.F;
+            uint32_t b[S::HALVES][16];
+            float sum[S::HALVES][S::GROUPS][2];
+            {
+                const uint32_t row = row0 + (g < count ? g : 0u);
                 const float up = scale_up(ld_fresh(a.h_top + row));
 #pragma unroll
-                for (uint32_t i = 0; i < 4u; ++i) {
-                    const uint32_t k = k0 + piece_k<FMT>(t, i);
-                    float4 p = make_float4(0.0f, 0.0f, 0.0f, 0.0f), q = p;
-                    if (there && k < a.F) p = ld_fresh(reinterpret_cast<const float4*>(h + k)), q = ld_fresh(reinterpret_cast<const float4*>(h + k + 4u));
-                    v[8 * i] = p.x, v[8 * i + 1] = p.y, v[8 * i + 2] = p.z, v[8 * i + 3] = p.w, v[8 * i + 4] = q.x, v[8 * i + 5] = q.y, v[8 * i + 6] = q.z, v[8 * i + 7] = q.w;
+                for (int half = 0; half < S::HALVES; ++half) {
+                    float v[32];
+                    read_h<FMT>(v, a.h + (size_t)row * a.F, g < count, k0 + half * 128u, a.F, t);
+                    make_frag<FMT>(b[half], v, up);
+                    if constexpr (FMT != E4M3) make_sums<FMT>(sum[half], b[half]);
                 }
-                make_frag<FMT>(b[n], v, up);
-                if constexpr (FMT != E4M3) make_sums<FMT>(sum[n], b[n]);
             }
-            float4* cell = mine + segment * (at_once * NT * 32u);
-            for (uint32_t tile = first; tile < last; ++tile, cell += NT * 32u) {
+            float4* cell = mine + segment * (at_once * 32u);
+            for (uint32_t tile = first; tile < last; ++tile, cell += 32u) {
                 cp_wait<DEPTH - 2>();
                 __syncwarp();
-                auto step = [&](auto number) {
-                    constexpr int COUNT = decltype(number)::value;
-                    float tot[COUNT][4] = {};
-                    if (!fresh) {
+                float tot[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                if (!fresh) {
+                    const float4 p = *cell;
+                    tot[0] = p.x, tot[1] = p.y, tot[2] = p.z, tot[3] = p.w;
+                }
+                multiply<FMT>(got, tot, lane, [&](int half, uint32_t (&to)[16], float (&sums_to)[S::GROUPS][2]) {
 #pragma unroll
-                        for (int n = 0; n < COUNT; ++n) {
-                            const float4 p = cell[n * 32];
-                            tot[n][0] = p.x, tot[n][1] = p.y, tot[n][2] = p.z, tot[n][3] = p.w;
-                        }
-                    }
-                    multiply<FMT, COUNT>(got, reinterpret_cast<const uint32_t(&)[COUNT][16]>(b), reinterpret_cast<const float(&)[COUNT][G][2]>(sum), tot, lane);
+                    for (int i = 0; i < 16; ++i) to[i] = b[half][i];
 #pragma unroll
-                    for (int n = 0; n < COUNT; ++n) cell[n * 32] = make_float4(tot[n][0], tot[n][1], tot[n][2], tot[n][3]);
-                };
-                if (NT == 1 || tiles == 1u) step(std::integral_constant<int, 1>());
-                else step(std::integral_constant<int, NT>());
+                    for (int q = 0; q < S::GROUPS; ++q) sums_to[q][0] = sum[half][q][0], sums_to[q][1] = sum[half][q][1];
+                });
+                *cell = make_float4(tot[0], tot[1], tot[2], tot[3]);
                 got += S::BYTES;
                 if (got == ring_end) got = ring;
                 fill();
@@ -854,7 +836,7 @@ moe_down_kernel(const Args a) {
         }
         __syncthreads();
         // a token's places, and of each the warps of this CTA that had units of its entry: all but the first began with it
-        const uint32_t outputs = (last - first) * a.tokens * 16u, warp_floats = segments * at_once * NT * 128u;
+        const uint32_t outputs = (last - first) * a.tokens * 16u, warp_floats = segments * at_once * 128u;
         const float* const parts = reinterpret_cast<const float*>(cells + at_once * out_tile / 16u);
         for (uint32_t i = threadIdx.x; i < outputs; i += THREADS) {
             const uint32_t row = i & 15u, rest = i >> 4, tile = rest / a.tokens, token = rest - tile * a.tokens;
@@ -862,10 +844,10 @@ moe_down_kernel(const Args a) {
             for (uint32_t at = token * a.top; at < (token + 1u) * a.top; ++at) {
                 const uint32_t what = (uint32_t)tb.chosen[at], warps = what >> 16;
                 if (warps == 0u) continue;
-                const uint32_t column = tb.slot[at] & 15u;
-                const float* from = parts + (what & 0xFFu) * warp_floats + ((tile * NT + column / 8u) * 32u + (row & 7u) * 4u + (column & 7u) / 2u) * 4u + (column & 1u) + (row >> 3) * 2u;
+                const uint32_t column = tb.slot[at] % ENTRY;
+                const float* from = parts + (what & 0xFFu) * warp_floats + (tile * 32u + (row & 7u) * 4u + column / 2u) * 4u + (column & 1u) + (row >> 3) * 2u;
                 float s = 0.0f;
-                for (uint32_t w = 0; w < warps; ++w) s += from[w * warp_floats + (w == 0u ? (what >> 8 & 0xFFu) * (at_once * NT * 128u) : 0u)];
+                for (uint32_t w = 0; w < warps; ++w) s += from[w * warp_floats + (w == 0u ? (what >> 8 & 0xFFu) * (at_once * 128u) : 0u)];
                 total = __fmaf_rn(tb.weight[at], s, total);
             }
             sums[i] = total;
