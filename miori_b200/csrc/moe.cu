@@ -24,7 +24,12 @@ static int launch_moe(const char* op, Args a, cudaStream_t stream) {
     // clusters of four whole SMs: an SM in nine has no place in one
     const uint32_t most = sms * 8u / 9u / CLUSTER;
     a.per = (row_tiles + most - 1u) / most;
-    cudaError_t e = launch_cluster(moe_router_kernel, ROUTER_CLUSTER, THREADS, (size_t)a.tokens * 1024u, ROUTER_CLUSTER, stream, a);
+    a.by_tokens = Div::by(a.tokens), a.by_tiles = Div::by(a.F / 8u), a.by_ctas = Div::by(sms);
+    // Of the experts that T tokens choose `top` of, evenly, a share of about exp(-T top / E) is nobody's; less than a sixth, and their weights are asked for
+    // ahead: what HBM delivers while the router runs
+    a.guess = a.tokens * a.top * 5u >= a.experts * 9u ? GUESS : 0u;
+    auto router = a.experts <= 32u ? moe_router_kernel<1> : a.experts <= 128u ? moe_router_kernel<4> : moe_router_kernel<8>;
+    cudaError_t e = launch_cluster(router, ROUTER_CLUSTER, THREADS, (size_t)a.tokens * 1024u, ROUTER_CLUSTER, stream, a);
     if (e == cudaSuccess) e = launch(moe_up_kernel<FMT, DEPTH>, dim3(sms), dim3(THREADS), SMEM, stream, true, a);
     if (e == cudaSuccess) e = launch_cluster(moe_down_kernel<FMT>, (row_tiles + a.per - 1u) / a.per * CLUSTER, THREADS, SMEM, CLUSTER, stream, a);
     return e == cudaSuccess ? MIORI_OK : cuda_fail(e, op);
@@ -35,7 +40,7 @@ static int launch_moe(const char* op, Args a, cudaStream_t stream) {
     constexpr int DEPTH = Stage<FMT>::UP;
     constexpr uint32_t UNIT = Stage<FMT>::UNIT;
     auto matrix = [](Matrix& m, uint32_t rows, uint32_t K) {
-        m.rows = rows, m.K = K, m.units = (K + UNIT - 1u) / UNIT, m.whole = K % UNIT == 0u;
+        m.rows = rows, m.K = K, m.units = (K + UNIT - 1u) / UNIT, m.by_units = Div::by(m.units), m.whole = K % UNIT == 0u;
         m.pitch = FMT == E4M3 ? K : K / 2u, m.scale_pitch = FMT == E4M3 ? 0u : K / (FMT == GROUP64 ? 64u : 32u) * 2u;
     };
     matrix(a.up, 2u * a.F, a.H);

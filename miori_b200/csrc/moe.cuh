@@ -31,6 +31,7 @@ constexpr uint32_t WARPS = 16, THREADS = WARPS * 32, CLUSTER = 4, ROUTER_CLUSTER
 constexpr uint32_t ENTRY = 8;   // tokens of an entry: the columns of an MMA tile
 constexpr uint32_t MAX_ENTRIES = MAX_EXPERTS + MAX_ROWS / ENTRY;
 constexpr size_t PREFETCH = 192 * 1024;  // bytes of down weights that a CTA of moe_up asks L2 for
+constexpr uint32_t GUESS = 320 * 1024;      // and of up weights, before the choice is known: what all CTAs' share of L2 holds beside them
 enum Format { GROUP64, GROUP32, E4M3 };
 
 // A unit of K is what 128 bytes of a row hold; a stage is a unit of 16 rows.
@@ -49,10 +50,21 @@ struct Stage {
     static constexpr uint32_t FRAG = HALVES * HALF;
 };
 
+// Division by a number that the host knows: a dozen instructions less, of which the kernels' beginnings, on every warp, were mostly made.
+struct Div {
+    uint32_t d, m;
+    __host__ __device__ static Div by(uint32_t d) { return {d, d > 1u ? (uint32_t)((1ull << 32) / d) + 1u : 0xFFFFFFFFu}; }
+    __device__ __forceinline__ uint32_t operator()(uint32_t n) const {
+        const uint32_t q = __umulhi(n, m), r = n - q * d;
+        return (int32_t)r < 0 ? q - 1u : r >= d ? q + 1u : q;
+    }
+};
+
 struct Matrix {  // [experts][rows][K]
     const uint8_t* q;
     const uint8_t *s, *b;  // bf16 [experts][rows][K / group]; e4m3: s fp32 [experts][ceil(rows / 128)][ceil(K / 128)]
     uint32_t rows, K, units;
+    Div by_units;
     uint32_t pitch, scale_pitch;  // bytes of a row of q, of a row of s and b
     uint32_t whole;               // rows are whole units
 };
@@ -80,6 +92,8 @@ struct Args {
     float factor;
     uint32_t tokens, experts, top, H, F;
     uint32_t sigmoid, norm, bf16, ahead;  // ahead: weights may be read before the launch before is done
+    Div by_tokens, by_tiles, by_ctas;  // tokens, F / 8, CTAs of moe_up
+    uint32_t guess;    // moe_up: bytes of up weights that a CTA asks L2 for before it knows the choice
     uint32_t slots;    // moe_up: entries whose B fragments shared memory takes
     uint32_t area;     // moe_down: bytes of partial sums
     uint32_t per;      // moe_down: row tiles of a cluster
@@ -195,21 +209,34 @@ __device__ __forceinline__ void make_sums(float (&sum)[Stage<FMT>::GROUPS][2], c
     }
 }
 
+// What a thread adds to a stage's address, made once: where its first chunk lies (others by exclusive or, since stages begin on 128-byte boundaries), its
+// rows' scales, and where it puts what it fetches.
+template <Format FMT>
+struct Places {
+    uint32_t chunk, scale, d0, d1;
+    __device__ __forceinline__ explicit Places(uint32_t lane) {
+        const uint32_t g = lane >> 2, t = lane & 3u, r = lane >> 3, c = lane & 7u;
+        chunk = g * 128u + (FMT == GROUP64 ? (((t >> 1) ^ swizzle<FMT>(g)) << 4) + (t & 1u) * 8u : FMT == GROUP32 ? (swizzle<FMT>(g) << 4) + t * 4u : (t ^ swizzle<FMT>(g)) << 4);
+        scale = 2048u + (FMT == E4M3 ? 0u : g * (FMT == GROUP64 ? 32u : 64u));
+        d0 = r * 128u + ((c ^ swizzle<FMT>(r)) << 4), d1 = r * 128u + 512u + ((c ^ swizzle<FMT>(r + 4u)) << 4);
+    }
+};
+
 // One stage times one unit of eight columns, added to tot = (row g, column 2t), (g, 2t + 1), (g + 8, 2t), (g + 8, 2t + 1).
 // frag(half, b, sum): the B fragments of a half.
 template <Format FMT, class F>
-__device__ __forceinline__ void multiply(uint32_t stage, float (&tot)[4], uint32_t lane, F frag) {
+__device__ __forceinline__ void multiply(uint32_t stage, const Places<FMT>& places, float (&tot)[4], F frag) {
     using S = Stage<FMT>;
-    const uint32_t g = lane >> 2, t = lane & 3u, row = stage + g * 128u, s = swizzle<FMT>(g);
+    const uint32_t chunk = stage + places.chunk, scale = stage + places.scale;
     uint32_t b[16];
     float sum[S::GROUPS][2];
     if constexpr (FMT == E4M3) {
         float acc[2][4] = {};
-        const uint2 sc = lds64(stage + 2048u);
+        const uint2 sc = lds64(scale);
         frag(0, b, sum);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-            const uint32_t at = row + ((c * 4u + t) ^ s) * 16u;
+            const uint32_t at = chunk ^ (c * 64u);
             const uint4 lo = lds128(at), hi = lds128(at + 1024u);
             const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
@@ -225,12 +252,12 @@ __device__ __forceinline__ void multiply(uint32_t stage, float (&tot)[4], uint32
         // rows g and g + 8: scales, scales, biases, biases, a pair of groups a word
         uint32_t words[4][G];
         if constexpr (FMT == GROUP64) {
-            const uint4 w = lds128(stage + 2048u + g * 32u), z = lds128(stage + 2048u + g * 32u + 16u);
+            const uint4 w = lds128(scale), z = lds128(scale + 16u);
             words[0][0] = w.x, words[0][1] = w.y, words[1][0] = w.z, words[1][1] = w.w, words[2][0] = z.x, words[2][1] = z.y, words[3][0] = z.z, words[3][1] = z.w;
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const uint4 w = lds128(stage + 2048u + g * 64u + i * 16u);
+                const uint4 w = lds128(scale + i * 16u);
                 words[i][0] = w.x, words[i][1] = w.y, words[i][2] = w.z, words[i][3] = w.w;
             }
         }
@@ -241,11 +268,11 @@ __device__ __forceinline__ void multiply(uint32_t stage, float (&tot)[4], uint32
 #pragma unroll
             for (int q = 0; q < G; ++q) {
                 if constexpr (FMT == GROUP64) {
-                    const uint32_t at = row + ((half * 4u + q * 2u + (t >> 1)) ^ s) * 16u + (t & 1u) * 8u;
+                    const uint32_t at = chunk ^ (half * 64u + q * 32u);
                     const uint2 l = lds64(at), h = lds64(at + 1024u);
                     lo[2 * q] = l.x, lo[2 * q + 1] = l.y, hi[2 * q] = h.x, hi[2 * q + 1] = h.y;
                 } else {
-                    const uint32_t at = row + ((half * 4u + q) ^ s) * 16u + t * 4u;
+                    const uint32_t at = chunk ^ (half * 64u + q * 16u);
                     lo[q] = lds32(at), hi[q] = lds32(at + 1024u);
                 }
             }
@@ -288,9 +315,9 @@ __device__ __forceinline__ uint32_t remote(uint32_t addr, uint32_t rank) {
 }
 
 // The choice of one token by one warp.  logit(e): the token's logit of expert e.  The results go to the tables of the cluster's first CTA.
-template <class L>
+// PER: experts of a lane.
+template <int PER, class L>
 __device__ __forceinline__ void choose(const Args& a, Tables& tb, uint32_t token, uint32_t lane, L logit) {
-    constexpr int PER = MAX_EXPERTS / 32;
     float l[PER], r[PER];
     uint32_t key[PER];
     float most = -INFINITY, total = 0.0f;
@@ -372,16 +399,16 @@ __device__ __forceinline__ void list_entries(const Args& a, Tables& tb, uint32_t
     if (lane == 0) tb.entries = entry, tb.entry_row[entry] = (uint16_t)row;
 }
 
-// Logits and choices: a cluster of eight, whose CTAs have an eighth of K each for all tokens and experts, and then every eighth token.
+// Logits and choices: one cluster, whose CTAs have a share of K each for all tokens and experts, and then each their tokens.
+template <int PER>
 __global__ void __launch_bounds__(THREADS)
 moe_router_kernel(const Args a) {
-    extern __shared__ __align__(16) uint8_t smem[];
+    constexpr uint32_t WIDE = PER * 2, SPLIT = WARPS / WIDE, WIDTH = PER * 32;  // tiles of 16 experts; warps over K; experts of a plane
+    extern __shared__ __align__(128) uint8_t smem[];
     __shared__ __align__(16) Tables tb;
     float* const part = reinterpret_cast<float*>(smem);  // [slice][token][expert]
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u, rank = blockIdx.x;
-    uint32_t wide = 1;  // tiles of 16 experts, up to a power of two
-    while (wide * 16u < a.experts) wide *= 2u;
-    const uint32_t split = WARPS / wide, tile = warp % wide, slice = warp / wide, width = wide * 16u, plane = a.tokens * width;
+    const uint32_t tile = warp % WIDE, slice = warp / WIDE, plane = a.tokens * WIDTH;
     const uint32_t units = (a.H + 127u) / 128u, u0 = rank * units / ROUTER_CLUSTER, u1 = (rank + 1u) * units / ROUTER_CLUSTER;
     const uint32_t columns = (a.tokens + 7u) / 8u, e_lo = tile * 16u + g, e_hi = e_lo + 8u;
     uint4 lo[4], hi[4];
@@ -395,15 +422,15 @@ moe_router_kernel(const Args a) {
             if (there && e_hi < a.experts) hi[i] = ld_fresh(reinterpret_cast<const uint4*>(a.router + (size_t)e_hi * a.H + k + i * 8u));
         }
     };
+    pdl_launch_dependents();
     if (a.ahead) weights(u0 + slice);
     for (uint32_t e = threadIdx.x; e < MAX_EXPERTS; e += THREADS) tb.mask[e] = 0u;
     if (threadIdx.x < MAX_TOKENS) tb.x_top[threadIdx.x] = 0u;
-    cluster_barrier();  // the other CTAs run, and their tables are clear
+    __syncthreads();
     pdl_wait_prior();
-    pdl_launch_dependents();
-    if (rank == 1u && threadIdx.x < a.tokens * a.top) a.h_top[threadIdx.x] = 0u;
+    if (rank == 0u && threadIdx.x < a.tokens * a.top) a.h_top[threadIdx.x] = 0u;
     float acc[MAX_TOKENS / 8][4] = {};
-    for (uint32_t u = u0 + slice; u < u1; u += split) {
+    for (uint32_t u = u0 + slice; u < u1; u += SPLIT) {
         if (u != u0 + slice || !a.ahead) weights(u);
         const uint32_t k = u * 128u + t * 32u;
         uint4 x[MAX_TOKENS / 8][4];
@@ -434,28 +461,35 @@ moe_router_kernel(const Args a) {
                 m = max(m & 0xFFFFu, m >> 16) << 16;
                 m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
                 m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
-                if (t == 0u && n * 8u + g < a.tokens)
-                    asm volatile("red.relaxed.cluster.shared::cluster.max.u32 [%0], %1;" ::"r"(remote(smem_addr(&tb.x_top[n * 8u + g]), 0)), "r"(m) : "memory");
+                if (t == 0u && n * 8u + g < a.tokens) atomicMax(&tb.x_top[n * 8u + g], m);
             }
         }
     }
 #pragma unroll
     for (uint32_t n = 0; n < MAX_TOKENS / 8u; ++n) {
+        if (n >= columns) break;
         const uint32_t token = n * 8u + 2u * t;
 #pragma unroll
         for (uint32_t i = 0; i < 4u; ++i)
-            if (token + (i & 1u) < a.tokens) part[slice * plane + (token + (i & 1u)) * width + (i < 2u ? e_lo : e_hi)] = acc[n][i];
+            if (token + (i & 1u) < a.tokens) part[slice * plane + (token + (i & 1u)) * WIDTH + (i < 2u ? e_lo : e_hi)] = acc[n][i];
     }
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < plane; i += THREADS) {
         float s = part[i];
-        for (uint32_t p = 1; p < split; ++p) s += part[p * plane + i];
+#pragma unroll
+        for (uint32_t p = 1; p < SPLIT; ++p) s += part[p * plane + i];
         part[i] = s;
     }
     cluster_barrier();
+    if (rank == 0u && threadIdx.x < a.tokens) {
+        uint32_t m = tb.x_top[threadIdx.x];
+#pragma unroll
+        for (uint32_t r = 1; r < ROUTER_CLUSTER; ++r) m = max(m, __float_as_uint(remote_f32(smem_addr(&tb.x_top[threadIdx.x]), r)));
+        tb.x_top[threadIdx.x] = m;
+    }
     for (uint32_t token = rank + ROUTER_CLUSTER * warp; token < a.tokens; token += ROUTER_CLUSTER * WARPS)
-        choose(a, tb, token, lane, [&](uint32_t e) {
-            const uint32_t at = smem_addr(part + token * width + e);
+        choose<PER>(a, tb, token, lane, [&](uint32_t e) {
+            const uint32_t at = smem_addr(part + token * WIDTH + e);
             float v[ROUTER_CLUSTER], s = 0.0f;
 #pragma unroll
             for (uint32_t r = 0; r < ROUTER_CLUSTER; ++r) v[r] = remote_f32(at, r);
@@ -477,6 +511,12 @@ moe_router_kernel(const Args a) {
     }
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < sizeof(Tables) / 16u; i += THREADS) reinterpret_cast<uint4*>(a.tables)[i] = reinterpret_cast<const uint4*>(&tb)[i];
+}
+
+// Asks L2 for bytes [from, to) of an array, from and to multiples of 16.
+__device__ __forceinline__ void ask(const uint8_t* p, size_t from, size_t to) {
+    for (; from < to; from += 16384u)
+        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p + from), "r"((uint32_t)min((size_t)16384u, to - from)) : "memory");
 }
 
 __device__ __forceinline__ void read_tables(const Args& a, Tables& tb) {
@@ -511,31 +551,32 @@ struct Run {
         }
     }
     // part: bytes from a row to its partner; then on by so many bytes, and elements of K
-    __device__ __forceinline__ void fetch(uint32_t stage, const Matrix& m, size_t part, uint32_t q_step, uint32_t s_step, uint32_t k_step, uint32_t lane) {
-        const uint32_t r = lane >> 3, c = lane & 7u, at = stage + r * 128u;
-        const uint32_t d0 = at + ((c ^ swizzle<FMT>(r)) << 4), d1 = at + 512u + ((c ^ swizzle<FMT>(r + 4u)) << 4);
-        const bool there = k + c * S::CHUNK < m.K;
-        const uint8_t *first = there ? q : m.q, *second = there ? q + part : m.q;
-        const uint32_t four = there ? m.pitch * 4u : 0u;
-        cp16(d0, first, there);
-        cp16(d1, first + four, there);
-        cp16(d0 + 1024u, second, there);
-        cp16(d1 + 1024u, second + four, there);
-        if constexpr (FMT == E4M3) {
-            if (lane < 2u) cp4(stage + 2048u + lane * 4u, s);
-        } else {
+    __device__ __forceinline__ void fetch(uint32_t stage, const Places<FMT>& places, const Matrix& m, size_t part, uint32_t q_step, uint32_t s_step, uint32_t k_step, uint32_t lane) {
+        const uint32_t d0 = stage + places.d0, d1 = stage + places.d1, to = stage + 2048u + lane * (S::SCALES / 32u);
+        const uint32_t four = m.pitch * 4u;
+        if (m.whole) {
+            cp16(d0, q, true);
+            cp16(d1, q + four, true);
+            cp16(d0 + 1024u, q + part, true);
+            cp16(d1 + 1024u, q + part + four, true);
+            if constexpr (FMT == GROUP64) cp8(to, s, true);
+            if constexpr (FMT == GROUP32) cp16(to, s, true);
+        } else {  // rows may end inside the unit
+            const bool there = k + (lane & 7u) * S::CHUNK < m.K;
+            const uint8_t *first = there ? q : m.q, *second = there ? q + part : m.q;
+            cp16(d0, first, there);
+            cp16(d1, there ? first + four : first, there);
+            cp16(d0 + 1024u, second, there);
+            cp16(d1 + 1024u, there ? second + four : second, there);
             // the biases behind K have to be numbers: they are multiplied by sums that are zero
-            const uint32_t to = stage + 2048u + lane * (S::SCALES / 32u);
-            if (m.whole) {
-                if constexpr (FMT == GROUP64) cp8(to, s, true);
-                else cp16(to, s, true);
-            } else {  // rows of an odd number of 128 elements
-                const bool more = k + 128u < m.K;
-                if constexpr (FMT == GROUP64) cp4(to, s), cp4(to + 4u, more ? s + 4 : s, more);
-                else cp8(to, s, true), cp8(to + 8u, more ? s + 8 : s, more);
-            }
+            const bool more = k + 128u < m.K;
+            if constexpr (FMT == GROUP64) cp4(to, s), cp4(to + 4u, more ? s + 4 : s, more);
+            if constexpr (FMT == GROUP32) cp8(to, s, true), cp8(to + 8u, more ? s + 8 : s, more);
+            k += k_step;
         }
-        q += q_step, s += s_step, k += k_step;
+        if constexpr (FMT == E4M3)
+            if (lane < 2u) cp4(stage + 2048u + lane * 4u, s);
+        q += q_step, s += s_step;
         --left;
     }
 };
@@ -568,52 +609,56 @@ __global__ void __launch_bounds__(THREADS, 1)
 moe_up_kernel(const Args a) {
     using S = Stage<FMT>;
     constexpr uint32_t CELL = 512u, RING = S::ring(DEPTH);  // a tile's partial sums: a float4 a thread
-    extern __shared__ __align__(16) uint8_t smem[];
+    extern __shared__ __align__(128) uint8_t smem[];
     __shared__ __align__(16) Tables tb;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
     const uint32_t ring = smem_addr(smem) + warp * (S::BYTES * DEPTH), ring_end = ring + S::BYTES * DEPTH;
     float4* const cells = reinterpret_cast<float4*>(smem + RING);  // two a warp
     const uint32_t frags = smem_addr(smem) + RING + 2u * WARPS * CELL;
 
+    // Where most experts will be somebody's choice, HBM need not wait for it: this CTA's share of all of them, a part of which may be for nothing.
+    if (a.guess && threadIdx.x == 0) {
+        const size_t all = (size_t)a.experts * a.up.rows * a.up.pitch, from = all / gridDim.x * blockIdx.x & ~(size_t)15;
+        ask(a.up.q, from, min(from + a.guess, all));
+    }
     pdl_wait_prior();
     pdl_launch_dependents();  // not sooner: moe_down reads the tables before its wait
     read_tables(a, tb);
-    const uint32_t f_tiles = a.F / 8u, units = a.up.units;
-    const uint64_t items = (uint64_t)tb.entries * f_tiles;
-    const uint32_t i0 = (uint32_t)(items * blockIdx.x / gridDim.x), i1 = (uint32_t)(items * (blockIdx.x + 1u) / gridDim.x);
+    const uint32_t f_tiles = a.F / 8u, units = a.up.units, items = tb.entries * f_tiles;
+    const uint32_t i0 = a.by_ctas(items * blockIdx.x), i1 = a.by_ctas(items * (blockIdx.x + 1u));
     // A pass: as many entries as have room for their B fragments (one token: all, since theirs are the same).  Its tiles times units are
     // dealt to the warps.
     const uint32_t slots = a.tokens == 1u ? 0x10000u : a.slots;
-    auto pass_end = [&](uint32_t from) { return min(i1, (from / f_tiles + slots) * f_tiles); };
-    auto share = [&](uint32_t from, uint32_t w) { return (uint32_t)((uint64_t)(pass_end(from) - from) * units * w / WARPS); };
+    auto pass_end = [&](uint32_t from) { return min(i1, (a.by_tiles(from) + slots) * f_tiles); };
+    auto share = [&](uint32_t from, uint32_t w) { return (pass_end(from) - from) * units * w / WARPS; };
 
     uint32_t n_from = i0, n_stage = 0, n_end = 0;  // the pass, stages of it to be asked for
     if (i0 < i1) n_stage = share(i0, warp), n_end = share(i0, warp + 1u);
     Run<FMT> run;
-    uint32_t put = ring, got = ring;
+    const Places<FMT> places(lane);
+    uint32_t got = ring;
     const size_t part = (size_t)a.F * a.up.pitch;
-    auto fill = [&]() {
+    auto fill = [&](uint32_t put) {
         if (run.left == 0u) {
             while (n_from < i1 && n_stage == n_end) {
                 n_from = pass_end(n_from);
                 if (n_from < i1) n_stage = share(n_from, warp), n_end = share(n_from, warp + 1u);
             }
             if (n_from < i1) {
-                const uint32_t in_pass = n_stage / units, unit = n_stage - in_pass * units, item = n_from + in_pass, entry = item / f_tiles;
+                const uint32_t in_pass = a.up.by_units(n_stage), unit = n_stage - in_pass * units, item = n_from + in_pass, entry = a.by_tiles(item);
                 run.begin(a.up, tb.entry_expert[entry], (item - entry * f_tiles) * 8u, a.F, unit, min(units - unit, n_end - n_stage), lane);
                 n_stage += run.left;
             }
         }
-        if (run.left) run.fetch(put, a.up, part, 128u, FMT == E4M3 ? 4u : S::SCALES / 32u, S::UNIT, lane);
+        if (run.left) run.fetch(put, places, a.up, part, 128u, FMT == E4M3 ? 4u : S::SCALES / 32u, S::UNIT, lane);
         cp_commit();
-        put += S::BYTES;
-        if (put == ring_end) put = ring;
     };
-    for (int i = 0; i < DEPTH - 1; ++i) fill();
+#pragma unroll 1
+    for (uint32_t put = ring; put < ring_end; put += S::BYTES) fill(put);
 
     // silu(g) * u of a tile, whose sums are whole
     auto finish = [&](uint32_t item, const float (&tot)[4]) {
-        const uint32_t entry = item / f_tiles, row0 = tb.entry_row[entry], count = tb.entry_row[entry + 1u] - row0;
+        const uint32_t entry = a.by_tiles(item), row0 = tb.entry_row[entry], count = tb.entry_row[entry + 1u] - row0;
 #pragma unroll
         for (uint32_t c = 0; c < 2u; ++c) {
             const uint32_t column = 2u * t + c;
@@ -631,9 +676,9 @@ moe_up_kernel(const Args a) {
     };
 
     for (uint32_t from = i0; from < i1; from = pass_end(from)) {
-        const uint32_t to = pass_end(from), entry0 = from / f_tiles, entry1 = a.tokens == 1u ? entry0 + 1u : (to - 1u) / f_tiles + 1u;
+        const uint32_t to = pass_end(from), entry0 = a.by_tiles(from), entry1 = a.tokens == 1u ? entry0 + 1u : a.by_tiles(to - 1u) + 1u;
         for (uint32_t task = warp; task < (entry1 - entry0) * units * S::HALVES; task += WARPS) {
-            const uint32_t half = task % S::HALVES, at = task / S::HALVES, slot = at / units, unit = at - slot * units;
+            const uint32_t half = task % S::HALVES, at = task / S::HALVES, slot = a.up.by_units(at), unit = at - slot * units;
             const uint32_t row0 = tb.entry_row[entry0 + slot], count = tb.entry_row[entry0 + slot + 1u] - row0;
             const uint32_t token = g < count ? tb.row_token[row0 + g] : 0u;
             float v[32];
@@ -655,67 +700,67 @@ moe_up_kernel(const Args a) {
         }
         __syncthreads();
         const uint32_t s0 = share(from, warp), s1 = share(from, warp + 1u);
-        uint32_t item = from + s0 / units, unit = s0 % units;
+        const uint32_t t0 = a.up.by_units(s0), t1 = a.up.by_units(s1);  // its first tile of the pass, and the one that the next warp begins in
+        uint32_t item = from + t0, unit = s0 - t0 * units;
         bool whole = unit == 0u, first = true;  // this warp has the tile from its first unit on; it is the warp's first
         float tot[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        auto frag_of = [&]() { return frags + ((a.tokens == 1u ? 0u : item / f_tiles - entry0) * units + unit) * S::FRAG; };
-        uint32_t at = frag_of();  // B fragments of the next unit
-        for (uint32_t stage = s0; stage < s1; ++stage) {
-            cp_wait<DEPTH - 2>();
-            __syncwarp();
-            multiply<FMT>(got, tot, lane, [&](int half, uint32_t (&b)[16], float (&sum)[S::GROUPS][2]) {
-                const uint32_t src = at + half * S::HALF;
+        for (uint32_t stage = s0; stage < s1;) {
+            const uint32_t count = min(units - unit, s1 - stage);
+            uint32_t at = frags + ((a.tokens == 1u ? 0u : a.by_tiles(item) - entry0) * units + unit) * S::FRAG + lane * 16u;  // B fragments of the next unit
+#pragma unroll 1
+            for (uint32_t i = 0; i < count; ++i) {
+                cp_wait<DEPTH - 1>();
+                __syncwarp();
+                multiply<FMT>(got, places, tot, [&](int half, uint32_t (&b)[16], float (&sum)[S::GROUPS][2]) {
+                    const uint32_t src = at + half * S::HALF;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint4 w = lds128(src + i * 512u + lane * 16u);
-                    b[4 * i] = w.x, b[4 * i + 1] = w.y, b[4 * i + 2] = w.z, b[4 * i + 3] = w.w;
-                }
-                if constexpr (FMT != E4M3) {
-#pragma unroll
-                    for (int q = 0; q < S::GROUPS; ++q) {
-                        const uint2 w = lds64(src + 2048u + q * 32u + t * 8u);
-                        sum[q][0] = __uint_as_float(w.x), sum[q][1] = __uint_as_float(w.y);
+                    for (int i = 0; i < 4; ++i) {
+                        const uint4 w = lds128(src + i * 512u);
+                        b[4 * i] = w.x, b[4 * i + 1] = w.y, b[4 * i + 2] = w.z, b[4 * i + 3] = w.w;
                     }
-                }
-            });
-            at += S::FRAG;
-            got += S::BYTES;
-            if (got == ring_end) got = ring;
-            fill();
-            const bool end = ++unit == units;
-            if (end || stage + 1u == s1) {
-                if (end && whole) finish(item, tot);
-                else cells[(warp * 2u + (first ? 0u : 1u)) * 32u + lane] = make_float4(tot[0], tot[1], tot[2], tot[3]);
-                first = false;
-                tot[0] = tot[1] = tot[2] = tot[3] = 0.0f;
-                if (end) ++item, unit = 0u, whole = true, at = frag_of();
+                    if constexpr (FMT != E4M3) {
+                        const uint32_t sums = src + (2048u + t * 8u - lane * 16u);
+#pragma unroll
+                        for (int q = 0; q < S::GROUPS; ++q) {
+                            const uint2 w = lds64(sums + q * 32u);
+                            sum[q][0] = __uint_as_float(w.x), sum[q][1] = __uint_as_float(w.y);
+                        }
+                    }
+                });
+                at += S::FRAG;
+                __syncwarp();  // everybody has read the stage
+                fill(got);
+                got += S::BYTES;
+                if (got == ring_end) got = ring;
             }
+            stage += count, unit += count;
+            if (unit == units && whole) finish(item, tot);
+            else cells[(warp * 2u + (first ? 0u : 1u)) * 32u + lane] = make_float4(tot[0], tot[1], tot[2], tot[3]);
+            first = false;
+            tot[0] = tot[1] = tot[2] = tot[3] = 0.0f;
+            if (unit == units) ++item, unit = 0u, whole = true;
         }
         if (to == i1 && warp == 0 && lane == 0) {
-            // this CTA's share of the down weights, on their way to L2 while the sums meet: whole experts' bytes, in pieces
-            const size_t expert = (size_t)a.down.rows * a.down.pitch, all = expert * tb.entries;
-            size_t at = all * blockIdx.x / gridDim.x & ~(size_t)15, to = all * (blockIdx.x + 1u) / gridDim.x & ~(size_t)15;
-            if (to - at > PREFETCH) to = at + PREFETCH;
-            while (at < to) {
-                const size_t entry = at / expert, offset = at - entry * expert;
-                const uint32_t bytes = (uint32_t)min((size_t)16384, min(to - at, expert - offset));
-                asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(a.down.q + tb.entry_expert[entry] * expert + offset), "r"(bytes) : "memory");
-                at += bytes;
-            }
+            // this CTA's share of the down weights, on their way to L2 while the sums meet: an entry's expert's, in pieces
+            const uint32_t expert = a.down.rows * a.down.pitch;
+            const size_t all = (size_t)expert * tb.entries, from_byte = all / gridDim.x * blockIdx.x & ~(size_t)15;
+            const uint32_t entry = (uint32_t)(from_byte / expert), offset = (uint32_t)(from_byte - (size_t)entry * expert);
+            const uint32_t bytes = (uint32_t)min(PREFETCH, all / gridDim.x) & ~15u, here = min(bytes, expert - offset);
+            ask(a.down.q + (size_t)tb.entry_expert[entry] * expert, offset, offset + here);
+            if (here < bytes && entry + 1u < tb.entries) ask(a.down.q + (size_t)tb.entry_expert[entry + 1u] * expert, 0, min(bytes - here, expert));
         }
         __syncthreads();
         // a tile that goes on beyond the end of the warp that began it: that warp adds up the others' cells, their first ones
-        if (s0 < s1 && s1 % units) {
-            const uint32_t begin = s1 / units * units;
-            if (begin >= s0) {
-                const float4 own = cells[(warp * 2u + (s0 / units == s1 / units ? 0u : 1u)) * 32u + lane];
+        if (const uint32_t begin = t1 * units; begin >= s0 && begin < s1) {
+            {
+                const float4 own = cells[(warp * 2u + (t0 == t1 ? 0u : 1u)) * 32u + lane];
                 tot[0] = own.x, tot[1] = own.y, tot[2] = own.z, tot[3] = own.w;
                 for (uint32_t w = warp + 1u; w < WARPS && share(from, w) < begin + units; ++w) {
                     if (share(from, w) == share(from, w + 1u)) continue;
                     const float4 v = cells[w * 64u + lane];
                     tot[0] += v.x, tot[1] += v.y, tot[2] += v.z, tot[3] += v.w;
                 }
-                finish(from + s1 / units, tot);
+                finish(from + t1, tot);
             }
         }
     }
@@ -729,7 +774,7 @@ moe_down_kernel(const Args a) {
     constexpr uint32_t WORKERS = CLUSTER * WARPS;
     constexpr int DEPTH = S::DOWN;
     constexpr uint32_t RING = S::ring(DEPTH);
-    extern __shared__ __align__(16) uint8_t smem[];
+    extern __shared__ __align__(128) uint8_t smem[];
     __shared__ __align__(16) Tables tb;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
     const uint32_t rank = blockIdx.x % CLUSTER, cluster = blockIdx.x / CLUSTER;
@@ -751,28 +796,28 @@ moe_down_kernel(const Args a) {
 
     uint32_t n_first = r0, n_unit = u0, n_row = 0;
     Run<FMT> run;
-    uint32_t put = ring, got = ring;
+    const Places<FMT> places(lane);
+    uint32_t got = ring;
     const size_t part = (size_t)8 * a.down.pitch;
     const uint32_t q_step = 16u * a.down.pitch, s_step = FMT == E4M3 ? 0u : 16u * a.down.scale_pitch;
-    auto fill = [&]() {
+    auto fill = [&](uint32_t put) {
         if (run.left == 0u && n_first < r1 && u0 < u1) {
-            const uint32_t entry = n_unit / units;
+            const uint32_t entry = a.down.by_units(n_unit);
             n_row = n_first * 16u;
             run.begin(a.down, tb.entry_expert[entry], n_row, 8u, n_unit - entry * units, min(at_once, r1 - n_first), lane);
             if (++n_unit == u1) n_unit = u0, n_first += at_once;
         }
         if (run.left) {
-            run.fetch(put, a.down, part, q_step, s_step, 0u, lane);
+            run.fetch(put, places, a.down, part, q_step, s_step, 0u, lane);
             if (FMT == E4M3) {  // the next block's scales every eighth tile
                 n_row += 16u;
                 if ((n_row & 127u) == 0u) run.s += units * 4u;
             }
         }
         cp_commit();
-        put += S::BYTES;
-        if (put == ring_end) put = ring;
     };
-    for (int i = 0; i < DEPTH - 1; ++i) fill();
+#pragma unroll 1
+    for (uint32_t put = ring; put < ring_end; put += S::BYTES) fill(put);
     pdl_wait_prior();
     // In place of a place's expert: this CTA's first warp that had units of its entry, the entry's number there, how many warps.  In place of its
     // weight that times the row's power of two.
@@ -796,7 +841,7 @@ moe_down_kernel(const Args a) {
             for (uint32_t i = 0; i < last - first; ++i) mine[i * 32u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
         for (uint32_t unit = u0; unit < u1; ++unit) {
-            const uint32_t entry = unit / units, k0 = (unit - entry * units) * S::UNIT;
+            const uint32_t entry = a.down.by_units(unit), k0 = (unit - entry * units) * S::UNIT;
             const uint32_t row0 = tb.entry_row[entry], count = tb.entry_row[entry + 1u] - row0;
             const bool fresh = unit == u0 || k0 == 0u;  // the first unit of its entry here
             if (fresh && unit != u0) ++segment;
@@ -814,43 +859,51 @@ moe_down_kernel(const Args a) {
                 }
             }
             float4* cell = mine + segment * (at_once * 32u);
+#pragma unroll 1
             for (uint32_t tile = first; tile < last; ++tile, cell += 32u) {
-                cp_wait<DEPTH - 2>();
+                cp_wait<DEPTH - 1>();
                 __syncwarp();
                 float tot[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                 if (!fresh) {
                     const float4 p = *cell;
                     tot[0] = p.x, tot[1] = p.y, tot[2] = p.z, tot[3] = p.w;
                 }
-                multiply<FMT>(got, tot, lane, [&](int half, uint32_t (&to)[16], float (&sums_to)[S::GROUPS][2]) {
+                multiply<FMT>(got, places, tot, [&](int half, uint32_t (&to)[16], float (&sums_to)[S::GROUPS][2]) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) to[i] = b[half][i];
 #pragma unroll
                     for (int q = 0; q < S::GROUPS; ++q) sums_to[q][0] = sum[half][q][0], sums_to[q][1] = sum[half][q][1];
                 });
                 *cell = make_float4(tot[0], tot[1], tot[2], tot[3]);
+                __syncwarp();  // everybody has read the stage
+                fill(got);
                 got += S::BYTES;
                 if (got == ring_end) got = ring;
-                fill();
             }
         }
         __syncthreads();
-        // a token's places, and of each the warps of this CTA that had units of its entry: all but the first began with it
-        const uint32_t outputs = (last - first) * a.tokens * 16u, warp_floats = segments * at_once * 128u;
+        // A token's places, and of each the warps of this CTA that had units of its entry: all but the first began with it.  Few outputs are
+        // eight threads' work each.
+        const uint32_t outputs = (last - first) * a.tokens * 16u, warp_floats = segments * at_once * 128u, lanes = outputs * 8u <= THREADS ? 8u : 1u;
         const float* const parts = reinterpret_cast<const float*>(cells + at_once * out_tile / 16u);
-        for (uint32_t i = threadIdx.x; i < outputs; i += THREADS) {
-            const uint32_t row = i & 15u, rest = i >> 4, tile = rest / a.tokens, token = rest - tile * a.tokens;
+        for (uint32_t i = threadIdx.x / lanes; i < outputs; i += THREADS / lanes) {
+            const uint32_t row = i & 15u, rest = i >> 4, tile = a.by_tokens(rest), token = rest - tile * a.tokens, w0 = threadIdx.x & (lanes - 1u);
             float total = 0.0f;
             for (uint32_t at = token * a.top; at < (token + 1u) * a.top; ++at) {
                 const uint32_t what = (uint32_t)tb.chosen[at], warps = what >> 16;
                 if (warps == 0u) continue;
                 const uint32_t column = tb.slot[at] % ENTRY;
                 const float* from = parts + (what & 0xFFu) * warp_floats + (tile * 32u + (row & 7u) * 4u + column / 2u) * 4u + (column & 1u) + (row >> 3) * 2u;
-                float s = 0.0f;
-                for (uint32_t w = 0; w < warps; ++w) s += from[w * warp_floats + (w == 0u ? (what >> 8 & 0xFFu) * (at_once * 128u) : 0u)];
+                float s = w0 == 0u ? from[(what >> 8 & 0xFFu) * (at_once * 128u)] : w0 < warps ? from[w0 * warp_floats] : 0.0f;
+                for (uint32_t w = w0 + lanes; w < warps; w += lanes) s += from[w * warp_floats];
                 total = __fmaf_rn(tb.weight[at], s, total);
             }
-            sums[i] = total;
+            if (lanes == 8u) {  // whole warps: outputs are a multiple of 16
+                total += __shfl_xor_sync(0xFFFFFFFFu, total, 1);
+                total += __shfl_xor_sync(0xFFFFFFFFu, total, 2);
+                total += __shfl_xor_sync(0xFFFFFFFFu, total, 4);
+            }
+            if (w0 == 0u) sums[i] = total;
         }
         cluster_barrier();
         const uint32_t pieces = outputs / 16u, share0 = pieces * rank / CLUSTER * 16u, share1 = pieces * (rank + 1u) / CLUSTER * 16u;
@@ -860,7 +913,7 @@ moe_down_kernel(const Args a) {
             for (uint32_t r = 0; r < CLUSTER; ++r) v[r] = remote_f32(area + i * 4u, r);
 #pragma unroll
             for (uint32_t r = 0; r < CLUSTER; ++r) s += v[r];
-            const uint32_t rest = i >> 4, tile = rest / a.tokens, token = rest - tile * a.tokens;
+            const uint32_t rest = i >> 4, tile = a.by_tokens(rest), token = rest - tile * a.tokens;
             const size_t at = (size_t)token * a.H + (first + tile) * 16u + (i & 15u);
             if (a.bf16) static_cast<uint16_t*>(a.out)[at] = (uint16_t)pack_bf16(s, 0.0f);
             else static_cast<float*>(a.out)[at] = s;
