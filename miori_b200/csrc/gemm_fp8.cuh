@@ -58,7 +58,7 @@ __device__ __forceinline__ void commit_both(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
 }
 __device__ __forceinline__ void arrive_leader(uint32_t bar) {
-    asm volatile("{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %0, 0;\n\tmbarrier.arrive.release.cluster.shared::cluster.b64 _, [ra];\n\t}" ::"r"(bar) : "memory");
+    asm volatile("{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %0, 0;\n\tmbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [ra];\n\t}" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void load_pair(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
@@ -82,26 +82,57 @@ __device__ __forceinline__ void tmem_wait16(uint32_t (&r)[16]) {
                  : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
                    "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]) :: "memory");
 }
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
+          "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]) : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait32(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
+                   "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),
+                   "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]) :: "memory");
+    asm volatile("" : "+r"(r[29]), "+r"(r[30]), "+r"(r[31]));
+}
 __device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
     uint64_t v;
     asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
     return v;
 }
+// mbar_wait by a whole warp, with one answer for it.  (By one lane, that tells the others: 100 cycles more a wait.)
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile uint32_t* abort, uint32_t where) {
+    if (__all_sync(0xFFFFFFFFu, mbar_try(bar, parity))) return true;
+    return __all_sync(0xFFFFFFFFu, mbar_wait<false>(bar, parity, abort, where));
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0u;
+}
+// A value that all lanes hold, for the compiler to know that they do.
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xFFFFFFFFu, x, 0); }
 // (acc.x + v.x s, acc.y + v.y s)
 __device__ __forceinline__ void fma2(uint64_t& acc, uint64_t v, uint64_t s) { asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(v), "l"(s)); }
 
 // ---- 256-row tiles on SM pairs ----------------------------------------------------------------------------
 
+// BN: columns of a tile, 256 or 128; it is worked on in halves of 128, the columns of a block of w, so that four of a half's sums fit tensor
+// memory and a half is read while the unit works on the next.
 template <int BN>
 struct PairCfg {
-    static constexpr int A_BYTES = 128 * KB_BYTES, B_BYTES = BN / 2 * KB_BYTES, STAGE_BYTES = A_BYTES + B_BYTES;
+    static constexpr int HALVES = BN / 128;
+    static constexpr int A_BYTES = 128 * KB_BYTES, HALF_BYTES = 64 * KB_BYTES, STAGE_BYTES = A_BYTES + HALVES * HALF_BYTES;  // a CTA's: 128 rows of a, 64 of each half of w
     static constexpr int STAGES = BN == 256 ? 5 : 6;
-    static constexpr int BUFS = 512 / BN;        // sums of k-blocks in tensor memory
-    static constexpr int COLS = BN / 2;          // columns of an epilogue warp
+    static constexpr int BUFS = 4;
     static constexpr int OUT_BYTES = 8 * 2 * 32 * 128;  // two buffers of 32 rows x 128 bytes an epilogue warp
     static constexpr int SMEM = STAGES * STAGE_BYTES + OUT_BYTES + 1024 + 256;
 };
-constexpr int PAIR_THREADS = 320;
+// A warpgroup that copies and issues and two that read: at 168 registers a thread when launched, 24 and 240 then (128 x 24 + 256 x 240 = 384 x 168).  Sixteen
+// reading warps of 112 registers had to wait for each other's sums and spilled (16384 x 16384 x 2048: 749 us).
+constexpr int PAIR_THREADS = 384;
 constexpr uint32_t GROUP_TILES = 8;  // row tiles that share what L2 holds of w
 
 struct Tile {
@@ -118,7 +149,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
 gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_c,
                      const GemmArgs g) {
     using C = PairCfg<BN>;
-    constexpr int STAGES = C::STAGES, STAGE_BYTES = C::STAGE_BYTES, BUFS = C::BUFS, COLS = C::COLS;
+    constexpr int STAGES = C::STAGES, STAGE_BYTES = C::STAGE_BYTES, BUFS = C::BUFS, HALVES = C::HALVES;
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint32_t tmem_slot;
     __shared__ volatile uint32_t abort_flag;
@@ -139,7 +170,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     if (threadIdx.x == 0) {
         abort_flag = 0u;
         for (int s = 0; s < STAGES; ++s) mbar_init(full(s), 1), mbar_init(empty(s), 1);
-        for (int b = 0; b < BUFS; ++b) mbar_init(summed(b), 1), mbar_init(taken(b), 16);  // the leader's: eight epilogue warps of each CTA
+        for (int b = 0; b < BUFS; ++b) mbar_init(summed(b), 1), mbar_init(taken(b), rank == 0u ? 9 : 8);  // eight epilogue warps; the leader's: and the other CTA's word for its own
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w) : "memory");
@@ -156,138 +187,167 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     const uint32_t tmem = tmem_slot;
     pdl_wait_prior();
 
-    if (warp == 0) {
-        if (lane == 0) {
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 24;");
+        if (warp == 0 && lane == 0) {
             uint32_t s = 0, parity = 1u;
             bool ok = true;
             for (uint32_t t = pair; t < tiles && ok; t += pairs) {
                 const Tile tc = tile_at(t, m_tiles, n_tiles);
-                const int m = (int)(tc.m * 256u + rank * 128u), n = (int)(tc.n * BN + rank * (BN / 2));
+                const int m = (int)(tc.m * 256u + rank * 128u), n = (int)(tc.n * BN + rank * 64u);
                 for (uint32_t kb = 0; kb < k_blocks; ++kb) {
                     if (!(ok = mbar_wait(empty(s), parity, &abort_flag, 0x71))) break;
                     const uint32_t at = ring + s * STAGE_BYTES, bar = full(s) & PEER_MASK;
                     if (rank == 0) mbar_expect_tx(full(s), 2u * STAGE_BYTES);
                     load_pair(at, &map_a, (int)(kb * KB_BYTES), m, bar);
-                    load_pair(at + C::A_BYTES, &map_w, (int)(kb * KB_BYTES), n, bar);
+#pragma unroll
+                    for (int h = 0; h < HALVES; ++h) load_pair(at + C::A_BYTES + h * C::HALF_BYTES, &map_w, (int)(kb * KB_BYTES), n + h * 128, bar);
                     if (++s == STAGES) s = 0u, parity ^= 1u;
                 }
             }
-        }
-    } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
-            constexpr uint32_t idesc = idesc_e4m3(256, BN);
+        } else if (warp == 1 && lane == 0 && rank != 0) {
+            // one arrival from CTA to CTA a half: eight of them, each of which waits for what its thread wrote before, took longer than the MMAs
+            uint32_t b = 0, b_parity = 0u;
+            bool ok = true;
+            for (uint32_t t = pair; t < tiles && ok; t += pairs)
+                for (uint32_t i = 0; i < k_blocks * HALVES; ++i) {
+                    if (!(ok = mbar_wait(taken(b), b_parity, &abort_flag, 0x79))) break;
+                    arrive_leader(taken(b));
+                    if (++b == BUFS) b = 0u, b_parity ^= 1u;
+                }
+        } else if (warp == 1 && rank == 0) {
+            // The whole warp walks the loop and one elected thread issues: descriptors and addresses stay in uniform registers.
+            constexpr uint32_t idesc = idesc_e4m3(256, 128);
+            const uint32_t tm = uniform(tmem);
+            const uint64_t first = desc_sw128(uniform(ring));
             uint32_t s = 0, parity = 0u, b = 0, b_parity = 1u;
             bool ok = true;
             for (uint32_t t = pair; t < tiles && ok; t += pairs) {
                 for (uint32_t kb = 0; kb < k_blocks; ++kb) {
-                    if (!(ok = mbar_wait(taken(b), b_parity, &abort_flag, 0x72))) break;
-                    if (!(ok = mbar_wait(full(s), parity, &abort_flag, 0x73))) break;
-                    fence_after();
-                    const uint64_t ad = desc_sw128(ring + s * STAGE_BYTES), wd = desc_sw128(ring + s * STAGE_BYTES + C::A_BYTES);
+                    if (!(ok = warp_wait(full(s), parity, &abort_flag, 0x73))) break;
+                    const uint64_t ad = first + s * (STAGE_BYTES / 16u);
 #pragma unroll
-                    for (uint32_t k = 0; k < KB_BYTES / UMMA_KB; ++k) umma_e4m3<2>(tmem + b * BN, ad + 2u * k, wd + 2u * k, idesc, k != 0u);
-                    commit_both(empty(s));
-                    commit_both(summed(b));
+                    for (int h = 0; h < HALVES; ++h) {
+                        if (!(ok = warp_wait(taken(b), b_parity, &abort_flag, 0x72))) break;
+                        fence_after();
+                        if (elect_one()) {
+                            const uint64_t wd = ad + (C::A_BYTES + h * C::HALF_BYTES) / 16u;
+#pragma unroll
+                            for (uint32_t k = 0; k < KB_BYTES / UMMA_KB; ++k) umma_e4m3<2>(tm + b * 128u, ad + 2u * k, wd + 2u * k, idesc, k != 0u);
+                            commit_both(summed(b));
+                            if (h + 1 == HALVES) commit_both(empty(s));
+                        }
+                        __syncwarp();
+                        if (++b == BUFS) b = 0u, b_parity ^= 1u;
+                    }
+                    if (!ok) break;
                     if (++s == STAGES) s = 0u, parity ^= 1u;
-                    if (++b == BUFS) b = 0u, b_parity ^= 1u;
                 }
             }
         }
     } else {
-        const uint32_t quad = warp & 3u, half = (warp - 2u) >> 2;  // TMEM lanes and columns of this warp
-        const uint32_t bufs = out_stage + (warp - 2u) * 2u * 4096u, sw_lane = lane & 7u;
-        uint32_t b = 0, b_parity = 0u;
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 240;");
+        const uint32_t quad = warp & 3u, part = (warp - 4u) >> 2;  // TMEM lanes of this warp, and which 64 columns of a half
+        const uint32_t bufs = out_stage + (warp - 4u) * 8192u, sw_lane = lane & 7u;
+        uint32_t b = 0, b_parity = 0u, fills = 0;
         bool ok = true;
         for (uint32_t t = pair; t < tiles && ok; t += pairs) {
             const Tile tc = tile_at(t, m_tiles, n_tiles);
-            const uint32_t row0 = tc.m * 256u + rank * 128u + quad * 32u, col0 = tc.n * BN + half * COLS;
+            const uint32_t row0 = tc.m * 256u + rank * 128u + quad * 32u;
             const float* sa = g.sa + (int64_t)min(row0 + lane, g.M - 1u) * g.sa_row;
-            const float* sw = g.sw + (int64_t)(min(col0, g.N - 1u) / 128u) * g.sw_row;
-            uint64_t acc[COLS / 2];
-            float scale = __fmul_rn(ld_fresh(sa), ld_fresh(sw));
-            for (uint32_t kb = 0; kb < k_blocks; ++kb) {
-                float next_a = 0.0f, next_w = 0.0f;
-                if (kb + 1u < k_blocks) next_a = ld_fresh(sa + (int64_t)(kb + 1u) * g.sa_col), next_w = ld_fresh(sw + (int64_t)(kb + 1u) * g.sw_col);
-                ok = __all_sync(0xFFFFFFFFu, mbar_wait(summed(b), b_parity, &abort_flag, 0x74));
-                if (!ok) break;
-                fence_after();
-                const uint32_t from = tmem + ((quad * 32u) << 16) + b * BN + half * COLS;
-                const uint64_t s2 = pack2(__float_as_uint(scale), __float_as_uint(scale));
-                uint32_t r[2][16];
-                tmem_ld16(from, r[0]);
-                tmem_wait16(r[0]);
-                if (kb == 0) {
+            const float* sw[HALVES];
+            float next_a = ld_fresh(sa), next_w[HALVES];
 #pragma unroll
-                    for (int i = 0; i < COLS / 2; ++i) acc[i] = 0ull;
+            for (int h = 0; h < HALVES; ++h) {
+                sw[h] = g.sw + (int64_t)(min(tc.n * BN + h * 128u, g.N - 1u) / 128u) * g.sw_row;
+                next_w[h] = ld_fresh(sw[h]);
+            }
+            uint64_t acc[HALVES][32];
+#pragma unroll
+            for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+                for (int i = 0; i < 32; ++i) acc[h][i] = 0ull;
+            for (uint32_t kb = 0; kb < k_blocks && ok; ++kb) {
+                float scale[HALVES];
+#pragma unroll
+                for (int h = 0; h < HALVES; ++h) scale[h] = __fmul_rn(next_a, next_w[h]);
+                if (kb + 1u < k_blocks) {
+                    next_a = ld_fresh(sa + (int64_t)(kb + 1u) * g.sa_col);
+#pragma unroll
+                    for (int h = 0; h < HALVES; ++h) next_w[h] = ld_fresh(sw[h] + (int64_t)(kb + 1u) * g.sw_col);
                 }
 #pragma unroll
-                for (int c = 0; c < COLS / 16; ++c) {
-                    if (c + 1 < COLS / 16) tmem_ld16(from + (c + 1) * 16, r[(c + 1) & 1]);
+                for (int h = 0; h < HALVES; ++h) {
+                    if (!(ok = warp_wait(summed(b), b_parity, &abort_flag, 0x74))) break;
+                    fence_after();
+                    const uint32_t from = tmem + ((quad * 32u) << 16) + b * 128u + part * 64u;
+                    uint32_t r[2][32];
+                    tmem_ld32(from, r[0]);
+                    tmem_ld32(from + 32u, r[1]);
+                    tmem_wait32(r[0]);
+                    tmem_wait32(r[1]);
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(taken(b));  // before the sums are used
+                    if (++b == BUFS) b = 0u, b_parity ^= 1u;
+                    const uint64_t s2 = pack2(__float_as_uint(scale[h]), __float_as_uint(scale[h]));
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) fma2(acc[c * 8 + j], pack2(r[c & 1][2 * j], r[c & 1][2 * j + 1]), s2);
-                    if (c + 1 < COLS / 16) tmem_wait16(r[(c + 1) & 1]);
+                    for (int j = 0; j < 32; ++j) fma2(acc[h][j], pack2(r[j >> 4][2 * (j & 15)], r[j >> 4][2 * (j & 15) + 1]), s2);
                 }
-                fence_before();
-                __syncwarp();
-                if (lane == 0) arrive_leader(taken(b));
-                if (++b == BUFS) b = 0u, b_parity ^= 1u;
-                scale = __fmul_rn(next_a, next_w);
             }
             if (!ok) break;
             // 32 rows x 128 bytes at a time through shared memory, in the 128-byte swizzle
             if (row0 >= g.M) continue;
-            const uint32_t per = g.bf16 ? 64u : 32u;  // columns of a buffer
-            auto word = [&](int i) { return (uint32_t)(i & 1 ? acc[i >> 1] >> 32 : acc[i >> 1]); };
 #pragma unroll
-            for (int f = 0; f < COLS / 32; ++f) {
-                if (g.bf16 && f >= COLS / 64) break;
-                if (col0 + f * per >= g.N) break;
-                const uint32_t buf = bufs + (f & 1) * 4096u, rowp = buf + lane * 128u;
-                if (lane == 0) tma_store_wait_read<1>();  // the store issued two buffers ago has read this one
-                __syncwarp();
-                if (g.bf16) {
-                    if (f < COLS / 64) {
+            for (int h = 0; h < HALVES; ++h) {
+                const uint32_t col0 = tc.n * BN + h * 128u + part * 64u;
+                auto word = [&](int i) { return (uint32_t)(i & 1 ? acc[h][i >> 1] >> 32 : acc[h][i >> 1]); };
+#pragma unroll
+                for (int f = 0; f < 2; ++f) {
+                    if (g.bf16 && f > 0) break;  // 64 columns are 128 bytes
+                    if (col0 + f * 32u >= g.N) break;
+                    const uint32_t buf = bufs + (fills++ & 1u) * 4096u, rowp = buf + lane * 128u;
+                    if (lane == 0) tma_store_wait_read<1>();  // the store issued two buffers ago has read this one
+                    __syncwarp();
+                    if (g.bf16) {
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
                             uint32_t v[4];
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const int at = (f * 64 + j * 8 + e * 2) % COLS;
-                                v[e] = pack_bf16(__uint_as_float(word(at)), __uint_as_float(word(at + 1)));
-                            }
+                            for (int e = 0; e < 4; ++e) v[e] = pack_bf16(__uint_as_float(word(j * 8 + e * 2)), __uint_as_float(word(j * 8 + e * 2 + 1)));
                             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
                                          ::"r"(rowp + (((uint32_t)j ^ sw_lane) << 4)), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
                         }
-                    }
-                } else {
+                    } else {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
-                                     ::"r"(rowp + (((uint32_t)j ^ sw_lane) << 4)), "r"(word(f * 32 + j * 4)), "r"(word(f * 32 + j * 4 + 1)),
-                                       "r"(word(f * 32 + j * 4 + 2)), "r"(word(f * 32 + j * 4 + 3)) : "memory");
-                }
-                if (g.by_tma) {
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) {
-                        tma_store_3d(&map_c, (int)(col0 + f * per), (int)row0, 0, buf);
-                        tma_store_commit();
+                        for (int j = 0; j < 8; ++j)
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};"
+                                         ::"r"(rowp + (((uint32_t)j ^ sw_lane) << 4)), "r"(word(f * 32 + j * 4)), "r"(word(f * 32 + j * 4 + 1)),
+                                           "r"(word(f * 32 + j * 4 + 2)), "r"(word(f * 32 + j * 4 + 3)) : "memory");
                     }
-                } else {
-                    __syncwarp();
-                    const uint32_t rows = min(32u, g.M - row0), col = col0 + f * per + lane * (g.bf16 ? 2u : 1u);
-                    for (uint32_t r = 0; r < rows; ++r) {
-                        uint32_t w;
-                        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(buf + r * 128u + (((lane >> 2) ^ (r & 7u)) << 4) + (lane & 3u) * 4u) : "memory");
-                        const int64_t at = (int64_t)(row0 + r) * g.ldc + col;
-                        if (g.bf16) {
-                            if (col < g.N) static_cast<uint16_t*>(g.c)[at] = (uint16_t)w;
-                            if (col + 1u < g.N) static_cast<uint16_t*>(g.c)[at + 1] = (uint16_t)(w >> 16);
-                        } else if (col < g.N) {
-                            static_cast<uint32_t*>(g.c)[at] = w;
+                    if (g.by_tma) {
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) {
+                            tma_store_3d(&map_c, (int)(col0 + f * 32u), (int)row0, 0, buf);
+                            tma_store_commit();
                         }
+                    } else {
+                        __syncwarp();
+                        const uint32_t rows = min(32u, g.M - row0), col = col0 + f * 32u + lane * (g.bf16 ? 2u : 1u);
+                        for (uint32_t r = 0; r < rows; ++r) {
+                            uint32_t w;
+                            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(buf + r * 128u + (((lane >> 2) ^ (r & 7u)) << 4) + (lane & 3u) * 4u) : "memory");
+                            const int64_t at = (int64_t)(row0 + r) * g.ldc + col;
+                            if (g.bf16) {
+                                if (col < g.N) static_cast<uint16_t*>(g.c)[at] = (uint16_t)w;
+                                if (col + 1u < g.N) static_cast<uint16_t*>(g.c)[at + 1] = (uint16_t)(w >> 16);
+                            } else if (col < g.N) {
+                                static_cast<uint32_t*>(g.c)[at] = w;
+                            }
+                        }
+                        __syncwarp();
                     }
-                    __syncwarp();
                 }
             }
         }
@@ -374,21 +434,24 @@ gemm_fp8_swap_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            constexpr uint32_t idesc = idesc_e4m3(128, MP);
-            uint32_t s = 0, parity = 0u, b = 0, b_parity = 1u;
-            for (uint32_t i = 0; i < nkb; ++i) {
-                if (!(ok = mbar_wait(taken(b), b_parity, &abort_flag, 0x76))) break;
-                if (!(ok = mbar_wait(full(s), parity, &abort_flag, 0x77))) break;
-                fence_after();
-                const uint64_t wd = desc_sw128(ring + s * STAGE_BYTES), ad = desc_sw128(ring + s * STAGE_BYTES + W_BYTES);
+        constexpr uint32_t idesc = idesc_e4m3(128, MP);
+        const uint32_t tm = uniform(tmem);
+        const uint64_t first = desc_sw128(uniform(ring));
+        uint32_t s = 0, parity = 0u, b = 0, b_parity = 1u;
+        for (uint32_t i = 0; i < nkb; ++i) {
+            if (!(ok = warp_wait(taken(b), b_parity, &abort_flag, 0x76))) break;
+            if (!(ok = warp_wait(full(s), parity, &abort_flag, 0x77))) break;
+            fence_after();
+            if (elect_one()) {
+                const uint64_t wd = first + s * (STAGE_BYTES / 16u), ad = wd + W_BYTES / 16u;
 #pragma unroll
-                for (uint32_t k = 0; k < KB_BYTES / UMMA_KB; ++k) umma_e4m3<1>(tmem + b * MP, wd + 2u * k, ad + 2u * k, idesc, k != 0u);
-                commit_one(empty(s));
+                for (uint32_t k = 0; k < KB_BYTES / UMMA_KB; ++k) umma_e4m3<1>(tm + b * MP, wd + 2u * k, ad + 2u * k, idesc, k != 0u);
                 commit_one(summed(b));
-                if (++s == geo.stages) s = 0u, parity ^= 1u;
-                if (++b == (uint32_t)BUFS) b = 0u, b_parity ^= 1u;
+                commit_one(empty(s));
             }
+            __syncwarp();
+            if (++s == geo.stages) s = 0u, parity ^= 1u;
+            if (++b == (uint32_t)BUFS) b = 0u, b_parity ^= 1u;
         }
     } else {
         // the slice's scales, multiplied out: no row's weight is read twice
@@ -404,7 +467,7 @@ gemm_fp8_swap_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
         for (int j = 0; j < MP; ++j) acc[j] = 0.0f;
         uint32_t b = 0, b_parity = 0u;
         for (uint32_t i = 0; i < nkb; ++i) {
-            ok = __all_sync(0xFFFFFFFFu, mbar_wait(summed(b), b_parity, &abort_flag, 0x78));
+            ok = warp_wait(summed(b), b_parity, &abort_flag, 0x78);
             if (!ok) break;
             fence_after();
 #pragma unroll
@@ -501,7 +564,7 @@ template <int BN>
 inline int launch_pair(const GemmOperands& o, GemmArgs g, cudaStream_t stream) {
     CUtensorMap ma, mw, mc;
     if (const int rc = bytes_map(&ma, o.a, g.M, g.K, 128, o.lda)) return rc;
-    if (const int rc = bytes_map(&mw, o.w, g.N, g.K, BN / 2, o.ldw)) return rc;
+    if (const int rc = bytes_map(&mw, o.w, g.N, g.K, 64, o.ldw)) return rc;
     mc = ma;  // unused where C is stored otherwise
     if (g.by_tma) {
         const int rc = g.bf16 ? make_tmap_3d(&mc, g.c, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, g.N, g.M, 1, 64, 32, CU_TENSOR_MAP_SWIZZLE_128B, (uint64_t)g.ldc)
@@ -543,9 +606,13 @@ struct GemmPlan {
     uint32_t pair_n;  // columns of a pair's tile, 0: the kernel of few rows
     uint32_t mp, cs;
 };
-inline GemmPlan plan_gemm_fp8(uint32_t M, uint32_t N, uint32_t K) {
+inline GemmPlan plan_gemm_fp8(uint32_t M, uint32_t N, uint32_t K, uint32_t flags) {
     const uint32_t sms = (uint32_t)sm_count(), k_blocks = (K + KB_BYTES - 1u) / KB_BYTES;
     GemmPlan p = {0, 16, 1};
+    if (const uint32_t f = flags >> MIORI_TUNE_FP8_SHIFT & 7u) {
+        if (f >= 5u) return {f == 5u ? 128u : 256u, 0, 0};
+        return {0, 8u << f, 1u << (flags >> (MIORI_TUNE_FP8_SHIFT + 3) & 3u)};
+    }
     while (p.mp < M && p.mp < 128u) p.mp *= 2u;
     const uint64_t tiles = (uint64_t)((N + 127u) / 128u) * ((M + p.mp - 1u) / p.mp);
     if ((M > 128u && tiles > sms) || k_blocks > 128u) {  // the kernel of few rows keeps its scales in shared memory

@@ -130,6 +130,11 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// The first of a chain: its sum begins at zero.
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
 __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -231,7 +236,7 @@ __device__ __forceinline__ void multiply(uint32_t stage, const Places<FMT>& plac
     uint32_t b[16];
     float sum[S::GROUPS][2];
     if constexpr (FMT == E4M3) {
-        float acc[2][4] = {};
+        float acc[2][4];
         const uint2 sc = lds64(scale);
         frag(0, b, sum);
 #pragma unroll
@@ -240,9 +245,11 @@ __device__ __forceinline__ void multiply(uint32_t stage, const Places<FMT>& plac
             const uint4 lo = lds128(at), hi = lds128(at + 1024u);
             const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                mma_f16(acc[c], e4m3_half((uint16_t)wl[i]), e4m3_half((uint16_t)wh[i]), e4m3_half((uint16_t)(wl[i] >> 16)), e4m3_half((uint16_t)(wh[i] >> 16)),
-                        b[c * 8 + i * 2], b[c * 8 + i * 2 + 1]);
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t a0 = e4m3_half((uint16_t)wl[i]), a1 = e4m3_half((uint16_t)wh[i]), a2 = e4m3_half((uint16_t)(wl[i] >> 16)), a3 = e4m3_half((uint16_t)(wh[i] >> 16));
+                if (i == 0) mma_f16_first(acc[c], a0, a1, a2, a3, b[c * 8], b[c * 8 + 1]);
+                else mma_f16(acc[c], a0, a1, a2, a3, b[c * 8 + i * 2], b[c * 8 + i * 2 + 1]);
+            }
         }
         const float sl = __uint_as_float(sc.x), sh = __uint_as_float(sc.y);
         tot[0] = __fmaf_rn(sl, acc[0][0] + acc[1][0], tot[0]), tot[1] = __fmaf_rn(sl, acc[0][1] + acc[1][1], tot[1]);
@@ -276,7 +283,7 @@ __device__ __forceinline__ void multiply(uint32_t stage, const Places<FMT>& plac
                     lo[q] = lds32(at), hi[q] = lds32(at + 1024u);
                 }
             }
-            float acc[G][4] = {};
+            float acc[G][4];
             // the groups' chains of MMAs take turns
 #pragma unroll
             for (int p = 0; p < PIECES; ++p)
@@ -284,7 +291,8 @@ __device__ __forceinline__ void multiply(uint32_t stage, const Places<FMT>& plac
                 for (int q = 0; q < G; ++q) {
                     const uint32_t l = lo[q * PIECES + p], h = hi[q * PIECES + p], l8 = l >> 8, h8 = h >> 8;
                     const int at = (q * PIECES + p) * 4;
-                    mma_f16(acc[q], l & 0x000F000Fu, h & 0x000F000Fu, l & 0x00F000F0u, h & 0x00F000F0u, b[at], b[at + 1]);
+                    if (p == 0) mma_f16_first(acc[q], l & 0x000F000Fu, h & 0x000F000Fu, l & 0x00F000F0u, h & 0x00F000F0u, b[at], b[at + 1]);
+                    else mma_f16(acc[q], l & 0x000F000Fu, h & 0x000F000Fu, l & 0x00F000F0u, h & 0x00F000F0u, b[at], b[at + 1]);
                     mma_f16(acc[q], l8 & 0x000F000Fu, h8 & 0x000F000Fu, l8 & 0x00F000F0u, h8 & 0x00F000F0u, b[at + 2], b[at + 3]);
                 }
 #pragma unroll
