@@ -169,7 +169,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     pdl_launch_dependents();
     if (threadIdx.x == 0) {
         abort_flag = 0u;
-        for (int s = 0; s < STAGES; ++s) mbar_init(full(s), 1), mbar_init(empty(s), 1);
+        for (int s = 0; s < STAGES; ++s) mbar_init(full(s), 1), mbar_init(empty(s), HALVES);
         for (int b = 0; b < BUFS; ++b) mbar_init(summed(b), 1), mbar_init(taken(b), rank == 0u ? 9 : 8);  // eight epilogue warps; the leader's: and the other CTA's word for its own
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
@@ -205,42 +205,40 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                     if (++s == STAGES) s = 0u, parity ^= 1u;
                 }
             }
-        } else if (warp == 1 && lane == 0 && rank != 0) {
+        } else if (warp >= 1 && warp <= HALVES && rank != 0) {
             // one arrival from CTA to CTA a half: eight of them, each of which waits for what its thread wrote before, took longer than the MMAs
-            uint32_t b = 0, b_parity = 0u;
-            bool ok = true;
-            for (uint32_t t = pair; t < tiles && ok; t += pairs)
-                for (uint32_t i = 0; i < k_blocks * HALVES; ++i) {
-                    if (!(ok = mbar_wait(taken(b), b_parity, &abort_flag, 0x79))) break;
-                    arrive_leader(taken(b));
-                    if (++b == BUFS) b = 0u, b_parity ^= 1u;
-                }
-        } else if (warp == 1 && rank == 0) {
-            // The whole warp walks the loop and one elected thread issues: descriptors and addresses stay in uniform registers.
+            if (lane == 0) {
+                uint32_t b = warp - 1u, b_parity = 0u;
+                bool ok = true;
+                for (uint32_t t = pair; t < tiles && ok; t += pairs)
+                    for (uint32_t i = 0; i < k_blocks; ++i) {
+                        if (!(ok = mbar_wait(taken(b), b_parity, &abort_flag, 0x79))) break;
+                        arrive_leader(taken(b));
+                        if ((b += HALVES) >= BUFS) b -= BUFS, b_parity ^= 1u;
+                    }
+            }
+        } else if (warp >= 1 && warp <= HALVES) {
+            // A warp for each half.  The whole warp walks the loop and one elected thread issues: descriptors and addresses stay in uniform
+            // registers (a k-block's eight MMAs, three waits and three commits by one thread: 1300 cycles, by one warp so 800).
             constexpr uint32_t idesc = idesc_e4m3(256, 128);
-            const uint32_t tm = uniform(tmem);
+            const uint32_t tm = uniform(tmem), half = uniform(warp - 1u);
             const uint64_t first = desc_sw128(uniform(ring));
-            uint32_t s = 0, parity = 0u, b = 0, b_parity = 1u;
+            uint32_t s = 0, parity = 0u, b = half, b_parity = 1u;
             bool ok = true;
             for (uint32_t t = pair; t < tiles && ok; t += pairs) {
                 for (uint32_t kb = 0; kb < k_blocks; ++kb) {
+                    if (!(ok = warp_wait(taken(b), b_parity, &abort_flag, 0x72))) break;
                     if (!(ok = warp_wait(full(s), parity, &abort_flag, 0x73))) break;
-                    const uint64_t ad = first + s * (STAGE_BYTES / 16u);
+                    fence_after();
+                    if (elect_one()) {
+                        const uint64_t ad = first + s * (STAGE_BYTES / 16u), wd = ad + (C::A_BYTES + half * C::HALF_BYTES) / 16u;
 #pragma unroll
-                    for (int h = 0; h < HALVES; ++h) {
-                        if (!(ok = warp_wait(taken(b), b_parity, &abort_flag, 0x72))) break;
-                        fence_after();
-                        if (elect_one()) {
-                            const uint64_t wd = ad + (C::A_BYTES + h * C::HALF_BYTES) / 16u;
-#pragma unroll
-                            for (uint32_t k = 0; k < KB_BYTES / UMMA_KB; ++k) umma_e4m3<2>(tm + b * 128u, ad + 2u * k, wd + 2u * k, idesc, k != 0u);
-                            commit_both(summed(b));
-                            if (h + 1 == HALVES) commit_both(empty(s));
-                        }
-                        __syncwarp();
-                        if (++b == BUFS) b = 0u, b_parity ^= 1u;
+                        for (uint32_t k = 0; k < KB_BYTES / UMMA_KB; ++k) umma_e4m3<2>(tm + b * 128u, ad + 2u * k, wd + 2u * k, idesc, k != 0u);
+                        commit_both(summed(b));
+                        commit_both(empty(s));
                     }
-                    if (!ok) break;
+                    __syncwarp();
+                    if ((b += HALVES) >= BUFS) b -= BUFS, b_parity ^= 1u;
                     if (++s == STAGES) s = 0u, parity ^= 1u;
                 }
             }
@@ -254,46 +252,61 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
         for (uint32_t t = pair; t < tiles && ok; t += pairs) {
             const Tile tc = tile_at(t, m_tiles, n_tiles);
             const uint32_t row0 = tc.m * 256u + rank * 128u + quad * 32u;
+            // scales two k-blocks ahead
             const float* sa = g.sa + (int64_t)min(row0 + lane, g.M - 1u) * g.sa_row;
-            const float* sw[HALVES];
-            float next_a = ld_fresh(sa), next_w[HALVES];
-#pragma unroll
-            for (int h = 0; h < HALVES; ++h) {
-                sw[h] = g.sw + (int64_t)(min(tc.n * BN + h * 128u, g.N - 1u) / 128u) * g.sw_row;
-                next_w[h] = ld_fresh(sw[h]);
-            }
+            const float* sw = g.sw + (int64_t)(tc.n * HALVES) * g.sw_row;
+            const int64_t next_half = HALVES == 2 && tc.n * BN + 128u < g.N ? g.sw_row : 0;  // a half behind N has no scale
+            float x[2], y[2][HALVES];
+            auto scales = [&](int to) {
+                x[to] = ld_fresh(sa), y[to][0] = ld_fresh(sw);
+                if (HALVES == 2) y[to][HALVES - 1] = ld_fresh(sw + next_half);
+                sa += g.sa_col, sw += g.sw_col;
+            };
+            scales(0);
+            if (k_blocks > 1u) scales(1);
             uint64_t acc[HALVES][32];
 #pragma unroll
             for (int h = 0; h < HALVES; ++h)
 #pragma unroll
                 for (int i = 0; i < 32; ++i) acc[h][i] = 0ull;
-            for (uint32_t kb = 0; kb < k_blocks && ok; ++kb) {
+            // A step is a half of a k-block; the next one's sums are on their way while this one's are added.
+            const uint32_t from = tmem + ((quad * 32u) << 16) + part * 64u;
+            uint32_t r[2][32];
+            if (!(ok = warp_wait(summed(b), b_parity, &abort_flag, 0x74))) break;
+            fence_after();
+            tmem_ld32(from + b * 128u, r[0]);
+            tmem_ld32(from + b * 128u + 32u, r[1]);
+            auto block = [&](int at, uint32_t kb) {
                 float scale[HALVES];
 #pragma unroll
-                for (int h = 0; h < HALVES; ++h) scale[h] = __fmul_rn(next_a, next_w[h]);
-                if (kb + 1u < k_blocks) {
-                    next_a = ld_fresh(sa + (int64_t)(kb + 1u) * g.sa_col);
-#pragma unroll
-                    for (int h = 0; h < HALVES; ++h) next_w[h] = ld_fresh(sw[h] + (int64_t)(kb + 1u) * g.sw_col);
-                }
+                for (int h = 0; h < HALVES; ++h) scale[h] = __fmul_rn(x[at], y[at][h]);
+                if (kb + 2u < k_blocks) scales(at);
 #pragma unroll
                 for (int h = 0; h < HALVES; ++h) {
-                    if (!(ok = warp_wait(summed(b), b_parity, &abort_flag, 0x74))) break;
-                    fence_after();
-                    const uint32_t from = tmem + ((quad * 32u) << 16) + b * 128u + part * 64u;
-                    uint32_t r[2][32];
-                    tmem_ld32(from, r[0]);
-                    tmem_ld32(from + 32u, r[1]);
                     tmem_wait32(r[0]);
                     tmem_wait32(r[1]);
                     fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(taken(b));  // before the sums are used
                     if (++b == BUFS) b = 0u, b_parity ^= 1u;
+                    const bool more = h + 1 < HALVES || kb + 1u < k_blocks;
                     const uint64_t s2 = pack2(__float_as_uint(scale[h]), __float_as_uint(scale[h]));
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) fma2(acc[h][j], pack2(r[j >> 4][2 * (j & 15)], r[j >> 4][2 * (j & 15) + 1]), s2);
+                    for (int j = 0; j < 16; ++j) fma2(acc[h][j], pack2(r[0][2 * j], r[0][2 * j + 1]), s2);
+                    if (more) {
+                        ok = warp_wait(summed(b), b_parity, &abort_flag, 0x74);
+                        if (!ok) return;
+                        fence_after();
+                        tmem_ld32(from + b * 128u, r[0]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) fma2(acc[h][16 + j], pack2(r[1][2 * j], r[1][2 * j + 1]), s2);
+                    if (more) tmem_ld32(from + b * 128u + 32u, r[1]);
                 }
+            };
+            for (uint32_t kb = 0; kb < k_blocks && ok; kb += 2u) {
+                block(0, kb);
+                if (ok && kb + 1u < k_blocks) block(1, kb + 1u);
             }
             if (!ok) break;
             // 32 rows x 128 bytes at a time through shared memory, in the 128-byte swizzle
