@@ -384,7 +384,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
 
 // ---- few rows: w's rows as the MMA's M, K over a cluster ------------------------------------------------------
 
-constexpr int SWAP_THREADS = 192;
+constexpr int SWAP_THREADS = 224;  // a copying, two MMA and four epilogue warps
 constexpr int SWAP_MAX_STAGES = 8;
 __host__ __device__ constexpr int SWAP_BUFS(int mp) { return mp >= 128 ? 2 : 4; }  // at most 256 columns: two CTAs an SM fit
 
@@ -446,12 +446,13 @@ gemm_fp8_swap_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
                 if (++s == geo.stages) s = 0u, parity ^= 1u;
             }
         }
-    } else if (warp == 1) {
+    } else if (warp < 3) {
+        // Two warps take the k-blocks in turns: a block's waits, MMAs and commits are 500 cycles of one of them, more than its bytes take.
         constexpr uint32_t idesc = idesc_e4m3(128, MP);
-        const uint32_t tm = uniform(tmem);
+        const uint32_t tm = uniform(tmem), turn = uniform(warp - 1u);
         const uint64_t first = desc_sw128(uniform(ring));
-        uint32_t s = 0, parity = 0u, b = 0, b_parity = 1u;
-        for (uint32_t i = 0; i < nkb; ++i) {
+        uint32_t s = turn % geo.stages, parity = turn / geo.stages & 1u, b = turn, b_parity = 1u;
+        for (uint32_t i = turn; i < nkb; i += 2u) {
             if (!(ok = warp_wait(taken(b), b_parity, &abort_flag, 0x76))) break;
             if (!(ok = warp_wait(full(s), parity, &abort_flag, 0x77))) break;
             fence_after();
@@ -463,13 +464,15 @@ gemm_fp8_swap_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
                 commit_one(empty(s));
             }
             __syncwarp();
-            if (++s == geo.stages) s = 0u, parity ^= 1u;
-            if (++b == (uint32_t)BUFS) b = 0u, b_parity ^= 1u;
+            for (uint32_t n = 0; n < 2u; ++n)
+                if (++s == geo.stages) s = 0u, parity ^= 1u;
+            b ^= 2u % BUFS;
+            if (BUFS == 2 || b < 2u) b_parity ^= 1u;
         }
     } else {
         // the slice's scales, multiplied out: no row's weight is read twice
         const float* sw = g.sw + (int64_t)n_tile * g.sw_row + (int64_t)kb0 * g.sw_col;
-        for (uint32_t i = threadIdx.x - 64u; i < nkb * MP; i += 128u) {
+        for (uint32_t i = threadIdx.x - 96u; i < nkb * MP; i += 128u) {
             const uint32_t kb = i / MP, m = m0 + i % MP;
             float v = 0.0f;
             if (m < g.M) v = __fmul_rn(ld_fresh(g.sa + (int64_t)m * g.sa_row + (int64_t)(kb0 + kb) * g.sa_col), ld_fresh(sw + (int64_t)kb * g.sw_col));
@@ -514,7 +517,7 @@ gemm_fp8_swap_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
         else static_cast<float*>(g.c)[at] = v;
     };
     if (geo.cs == 1u) {
-        if (warp >= 2u && ok) {
+        if (warp >= 3u && ok) {
 #pragma unroll
             for (int j = 0; j < MP; ++j)
                 if ((uint32_t)j < rows) store((uint32_t)j, acc[j]);
@@ -524,7 +527,7 @@ gemm_fp8_swap_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
         // take the partial sums, [source][row / cs][row of w].
         cluster_barrier();
         const uint32_t share = (rows + geo.cs - 1u) / geo.cs;
-        if (warp >= 2u) {
+        if (warp >= 3u) {
             uint32_t to_rank = 0, at = 0;
 #pragma unroll
             for (int j = 0; j < MP; ++j) {
@@ -537,7 +540,7 @@ gemm_fp8_swap_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
             }
         }
         cluster_barrier();
-        if (warp >= 2u && ok) {
+        if (warp >= 3u && ok) {
             for (uint32_t at = 0, m = rank; m < rows; ++at, m += geo.cs) {
                 float v = 0.0f;
 #pragma unroll 4
@@ -619,21 +622,40 @@ struct GemmPlan {
     uint32_t pair_n;  // columns of a pair's tile, 0: the kernel of few rows
     uint32_t mp, cs;
 };
+// The cheapest by a small model (us), whose numbers are what the kernels take a k-block once they run: 0.31 and 0.56 the tiles of pairs, of 128 and 256
+// columns; 0.2, 0.3, 0.5 and 0.95 the kernel of few rows with 16, 32, 64 and 128 of them; a wave's beginning and end on top; what HBM takes to deliver w is
+// a floor.  A split of K costs the clusters' meeting, which grows with the rows that are exchanged.
 inline GemmPlan plan_gemm_fp8(uint32_t M, uint32_t N, uint32_t K, uint32_t flags) {
-    const uint32_t sms = (uint32_t)sm_count(), k_blocks = (K + KB_BYTES - 1u) / KB_BYTES;
-    GemmPlan p = {0, 16, 1};
     if (const uint32_t f = flags >> MIORI_TUNE_FP8_SHIFT & 7u) {
         if (f >= 5u) return {f == 5u ? 128u : 256u, 0, 0};
         return {0, 8u << f, 1u << (flags >> (MIORI_TUNE_FP8_SHIFT + 3) & 3u)};
     }
-    while (p.mp < M && p.mp < 128u) p.mp *= 2u;
-    const uint64_t tiles = (uint64_t)((N + 127u) / 128u) * ((M + p.mp - 1u) / p.mp);
-    if ((M > 128u && tiles > sms) || k_blocks > 128u) {  // the kernel of few rows keeps its scales in shared memory
-        p.pair_n = N > 128u ? 256u : 128u;
-        return p;
+    const uint32_t sms = (uint32_t)sm_count(), k_blocks = (K + KB_BYTES - 1u) / KB_BYTES;
+    auto waves = [](uint64_t n, uint32_t at_once) { return (double)((n + at_once - 1u) / at_once); };
+    const double floor = (double)N * K / 5.5e6;
+    GemmPlan best = {128, 0, 0};
+    double best_t = 1e30;
+    auto consider = [&](const GemmPlan& p, double t) {
+        if (t < floor) t = floor;
+        if (t < best_t) best_t = t, best = p;
+    };
+    const uint64_t m256 = (M + 255u) / 256u;
+    consider({128, 0, 0}, waves(m256 * ((N + 127u) / 128u), sms / 2) * (k_blocks * 0.31 + 1.0) + 0.8);
+    consider({256, 0, 0}, waves(m256 * ((N + 255u) / 256u), sms / 2) * (k_blocks * 0.56 + 1.4) + 0.8);
+    if (k_blocks > 128u) return best;  // the kernel of few rows keeps its scales in shared memory
+    static const double per_block[4] = {0.2, 0.3, 0.5, 0.95};
+    for (uint32_t i = 0; i < 4u; ++i) {
+        const uint32_t mp = 16u << i;
+        if (mp >= 2u * M && mp > 16u) break;
+        const uint64_t tiles = (uint64_t)((N + 127u) / 128u) * ((M + mp - 1u) / mp);
+        for (uint32_t cs = 1; cs <= 8u && k_blocks >= cs; cs *= 2u) {
+            if (cs > 1u && tiles * cs > sms) break;
+            const uint32_t rows = M < mp ? M : mp;
+            const double t = waves(tiles * cs, sms) * ((k_blocks + cs - 1u) / cs * per_block[i] + 0.4) + (cs > 1u ? 0.5 + rows * 0.04 : 0.0);
+            consider({0, mp, cs}, t);
+        }
     }
-    while (p.cs < 8u && tiles * p.cs * 2u <= sms && k_blocks >= p.cs * 2u) p.cs *= 2u;
-    return p;
+    return best;
 }
 
 }  // namespace fp8
