@@ -110,6 +110,18 @@ inline cudaError_t launch_cluster(K kernel, uint32_t grid, uint32_t threads, siz
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
+// Division of a number below 2^31 by one that the host knows: five instructions for some twenty.
+struct Div {
+    uint32_t d, m;
+    static Div by(uint32_t d) { return {d, d > 1u ? (uint32_t)((1ull << 32) / d) + 1u : 0xFFFFFFFFu}; }
+#ifdef __CUDACC__
+    __device__ __forceinline__ uint32_t operator()(uint32_t n) const {
+        const uint32_t q = __umulhi(n, m), r = n - q * d;  // one too many at most, or with d = 1 one too few
+        return (int32_t)r < 0 ? q - 1u : r >= d ? q + 1u : q;
+    }
+#endif
+};
+
 // Device-side record of kernel-internal failures (bounded waits that expired).
 // word 0: error count, word 1: code of the first failure, word 2/3: detail.
 __device__ unsigned int g_device_error[4];

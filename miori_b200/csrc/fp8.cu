@@ -34,8 +34,8 @@ MIORI_API int miori_quant_fp8(const void* x, int64_t x_row, void* q, int64_t q_r
     a.x = x, a.q = static_cast<uint8_t*>(q), a.scales = scales;
     a.x_row = x_row, a.q_row = q_row, a.s_row = scale_row, a.s_col = scale_col;
     a.rows = rows, a.K = K, a.k_blocks = (K + BLOCK - 1u) / BLOCK;
-    const uint64_t ctas = tile == 1 ? ((uint64_t)rows * a.k_blocks + ROW_GROUPS - 1) / ROW_GROUPS : (uint64_t)((rows + BLOCK - 1u) / BLOCK) * a.k_blocks;
-    if (ctas > 0x7FFFFFFFull) return fail(MIORI_E_INVALID, "%s: too many blocks (rows=%u K=%u)", op, rows, K);
+    a.by_blocks = Div::by(a.k_blocks);
+    if ((uint64_t)(tile == 1 ? rows : (rows + BLOCK - 1u) / BLOCK) * a.k_blocks > 0x7FFFFF00ull) return fail(MIORI_E_INVALID, "%s: too many blocks (rows=%u K=%u)", op, rows, K);
     const bool vec = aligned16(x) && x_row % (f32 ? 4 : 8) == 0;
     const cudaStream_t s = (cudaStream_t)stream;
     const cudaError_t e = f32 ? (vec ? launch_quant<true, true>(a, tile != 1, s) : launch_quant<true, false>(a, tile != 1, s))

@@ -50,16 +50,6 @@ struct Stage {
     static constexpr uint32_t FRAG = HALVES * HALF;
 };
 
-// Division by a number that the host knows: a dozen instructions less, of which the kernels' beginnings, on every warp, were mostly made.
-struct Div {
-    uint32_t d, m;
-    __host__ __device__ static Div by(uint32_t d) { return {d, d > 1u ? (uint32_t)((1ull << 32) / d) + 1u : 0xFFFFFFFFu}; }
-    __device__ __forceinline__ uint32_t operator()(uint32_t n) const {
-        const uint32_t q = __umulhi(n, m), r = n - q * d;
-        return (int32_t)r < 0 ? q - 1u : r >= d ? q + 1u : q;
-    }
-};
-
 struct Matrix {  // [experts][rows][K]
     const uint8_t* q;
     const uint8_t *s, *b;  // bf16 [experts][rows][K / group]; e4m3: s fp32 [experts][ceil(rows / 128)][ceil(K / 128)]

@@ -23,38 +23,79 @@ __device__ __forceinline__ uint32_t pack_e4m3(float lo, float hi) {
     return r;
 }
 
-// Eight neighbouring elements from column k on; those behind K are zeros.  VEC: rows begin on 16-byte boundaries.
+// Eight neighbouring elements of a row, as they lie in memory.
+template <bool F32>
+struct Eight;
+template <>
+struct Eight<false> {
+    uint4 w;
+    __device__ __forceinline__ void value(float (&v)[8]) const {
+        v[0] = bf16lo(w.x), v[1] = bf16hi(w.x), v[2] = bf16lo(w.y), v[3] = bf16hi(w.y), v[4] = bf16lo(w.z), v[5] = bf16hi(w.z), v[6] = bf16lo(w.w), v[7] = bf16hi(w.w);
+    }
+};
+template <>
+struct Eight<true> {
+    float4 a, b;
+    __device__ __forceinline__ void value(float (&v)[8]) const { v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w; }
+};
+// From column k on; those behind K are zeros.  VEC: rows begin on 16-byte boundaries.
 template <bool F32, bool VEC>
-__device__ __forceinline__ void load8(const void* x, size_t row_at, uint32_t k, uint32_t K, float (&v)[8]) {
+__device__ __forceinline__ Eight<F32> load8(const void* x, size_t row_at, uint32_t k, uint32_t K) {
+    Eight<F32> e;
     if (VEC && k + 8u <= K) {
         if constexpr (F32) {
             const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(x) + row_at + k);
-            const float4 a = ld_fresh<float4, true>(p), b = ld_fresh<float4, true>(p + 1);
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+            e.a = ld_fresh<float4, true>(p), e.b = ld_fresh<float4, true>(p + 1);
         } else {
-            const uint4 a = ld_fresh<uint4, true>(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + row_at + k));
-            v[0] = bf16lo(a.x), v[1] = bf16hi(a.x), v[2] = bf16lo(a.y), v[3] = bf16hi(a.y);
-            v[4] = bf16lo(a.z), v[5] = bf16hi(a.z), v[6] = bf16lo(a.w), v[7] = bf16hi(a.w);
+            e.w = ld_fresh<uint4, true>(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x) + row_at + k));
         }
-        return;
+        return e;
     }
+    uint32_t v[8];
 #pragma unroll
     for (uint32_t i = 0; i < 8u; ++i) {
-        v[i] = 0.0f;
-        if (k + i < K)
-            v[i] = F32 ? ld_fresh(static_cast<const float*>(x) + row_at + k + i)
-                       : bf16_bits_to_float(ld_fresh(static_cast<const uint16_t*>(x) + row_at + k + i));
+        v[i] = 0u;
+        if (k + i < K) {
+            if constexpr (F32) v[i] = ld_fresh(static_cast<const uint32_t*>(x) + row_at + k + i);
+            else v[i] = ld_fresh(static_cast<const uint16_t*>(x) + row_at + k + i);
+        }
     }
+    if constexpr (F32) {
+        e.a = make_float4(__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]), __uint_as_float(v[3]));
+        e.b = make_float4(__uint_as_float(v[4]), __uint_as_float(v[5]), __uint_as_float(v[6]), __uint_as_float(v[7]));
+    } else {
+        e.w = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+    }
+    return e;
 }
-__device__ __forceinline__ float max8(const float (&v)[8]) {
-    float m = fabsf(v[0]);
+// The largest magnitude of N such pieces, NaN left out.  Magnitudes of bf16 are ordered as their bits are, two at a time; a NaN's lie above all
+// others', and where there is one they are looked at one by one.
+template <bool F32, int N>
+__device__ __forceinline__ float largest(const Eight<F32> (&e)[N]) {
+    if constexpr (!F32) {
+        uint32_t m = 0u;
 #pragma unroll
-    for (int i = 1; i < 8; ++i) m = fmaxf(m, fabsf(v[i]));
+        for (int i = 0; i < N; ++i)
+            m = __vmaxu2(__vmaxu2(m, __vmaxu2(e[i].w.x & 0x7FFF7FFFu, e[i].w.y & 0x7FFF7FFFu)), __vmaxu2(e[i].w.z & 0x7FFF7FFFu, e[i].w.w & 0x7FFF7FFFu));
+        m = max(m & 0xFFFFu, m >> 16);
+        if (m <= 0x7F80u) return bf16_bits_to_float(m);
+    }
+    float m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        float v[8];
+        e[i].value(v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(v[j]));
+    }
     return m;
 }
 // Rows of q begin on 16-byte boundaries and k is a multiple of eight; what lies behind K is left as it was.
-__device__ __forceinline__ void store8(uint8_t* q, size_t row_at, uint32_t k, uint32_t K, const float (&v)[8], float inv) {
+template <bool F32>
+__device__ __forceinline__ void store8(uint8_t* q, size_t row_at, uint32_t k, uint32_t K, const Eight<F32>& e, float inv) {
     if (k >= K) return;
+    float v[8];
+    e.value(v);
     uint32_t w[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -74,43 +115,34 @@ struct QuantArgs {
     float* scales;
     int64_t x_row, q_row, s_row, s_col;  // elements
     uint32_t rows, K, k_blocks;
+    Div by_blocks;
 };
 
-// A block of 1 x 128: 16 lanes, eight elements each.  UNITS blocks a lane group, their loads all under way before the first
-// maximum.
-constexpr uint32_t ROW_THREADS = 256, ROW_GROUPS = ROW_THREADS / 16;
-template <bool F32, bool VEC, int UNITS>
+// A block of 1 x 128: LANES lanes, 128 / LANES elements each in pieces of eight, the lanes' pieces side by side.  Four lanes, so that what a block costs (two
+// divisions, a maximum's shuffles) is shared by 32 elements a thread; sixteen where that leaves the SMs without a warp.
+constexpr uint32_t ROW_THREADS = 128;
+template <bool F32, bool VEC, int LANES>
 __global__ void __launch_bounds__(ROW_THREADS)
 quant_rows_kernel(const QuantArgs a) {
+    constexpr int PIECES = 16 / LANES;
     pdl_launch_dependents();
     pdl_wait_prior();
-    const uint32_t group = threadIdx.x >> 4, lane = threadIdx.x & 15u;
-    const uint64_t total = (uint64_t)a.rows * a.k_blocks, first = (uint64_t)blockIdx.x * (ROW_GROUPS * UNITS) + group;
-    float v[UNITS][8];
-    uint32_t row[UNITS], block[UNITS];
+    const uint32_t lane = threadIdx.x % LANES, i = blockIdx.x * (ROW_THREADS / LANES) + threadIdx.x / LANES;
+    const bool there = i < a.rows * a.k_blocks;
+    const uint32_t row = there ? a.by_blocks(i) : 0u, block = there ? i - row * a.k_blocks : 0u, k = block * BLOCK + lane * 8u;
+    const size_t from = (size_t)row * (size_t)a.x_row, to = (size_t)row * (size_t)a.q_row;
+    Eight<F32> e[PIECES];
 #pragma unroll
-    for (int u = 0; u < UNITS; ++u) {
-        const uint64_t i = first + (uint64_t)u * ROW_GROUPS;
-        // 64-bit division only where 32 do not do
-        row[u] = total <= 0xFFFFFFFFull ? (uint32_t)i / a.k_blocks : (uint32_t)(i / a.k_blocks);
-        block[u] = (uint32_t)(i - (uint64_t)row[u] * a.k_blocks);
-        if (i < total) {
-            load8<F32, VEC>(a.x, (size_t)row[u] * (size_t)a.x_row, block[u] * BLOCK + lane * 8u, a.K, v[u]);
-        } else {
+    for (int p = 0; p < PIECES; ++p) e[p] = load8<F32, VEC>(a.x, from, k + p * (LANES * 8u), there ? a.K : 0u);
+    float m = largest<F32, PIECES>(e);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[u][e] = 0.0f;
-        }
-    }
+    for (int d = LANES / 2; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
+    m = fmaxf(m, LEAST);
+    if (!there) return;
+    const float inv = __fdiv_rn(TOP, m);
 #pragma unroll
-    for (int u = 0; u < UNITS; ++u) {
-        float m = max8(v[u]);
-#pragma unroll
-        for (int d = 8; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
-        m = fmaxf(m, LEAST);
-        if (first + (uint64_t)u * ROW_GROUPS >= total) continue;
-        store8(a.q, (size_t)row[u] * (size_t)a.q_row, block[u] * BLOCK + lane * 8u, a.K, v[u], __fdiv_rn(TOP, m));
-        if (lane == 0) a.scales[(int64_t)row[u] * a.s_row + (int64_t)block[u] * a.s_col] = __fdiv_rn(m, TOP);
-    }
+    for (int p = 0; p < PIECES; ++p) store8<F32>(a.q, to, k + p * (LANES * 8u), a.K, e[p], inv);
+    if (lane == 0) a.scales[(int64_t)row * a.s_row + (int64_t)block * a.s_col] = __fdiv_rn(m, TOP);
 }
 
 // A block of 128 x 128: one CTA, everything in registers between the maximum and the store.
@@ -122,21 +154,15 @@ quant_tiles_kernel(const QuantArgs a) {
     pdl_launch_dependents();
     pdl_wait_prior();
     constexpr uint32_t STEPS = BLOCK * BLOCK / 8 / TILE_THREADS, STEP_ROWS = TILE_THREADS / 16;
-    const uint32_t tile_row = blockIdx.x / a.k_blocks, block = blockIdx.x - tile_row * a.k_blocks;
+    const uint32_t tile_row = a.by_blocks(blockIdx.x), block = blockIdx.x - tile_row * a.k_blocks;
     const uint32_t k = block * BLOCK + (threadIdx.x & 15u) * 8u, row0 = tile_row * BLOCK + (threadIdx.x >> 4);
-    float v[STEPS][8], m = LEAST;
+    Eight<F32> e[STEPS];
 #pragma unroll
     for (uint32_t s = 0; s < STEPS; ++s) {
         const uint32_t row = row0 + s * STEP_ROWS;
-        if (row < a.rows) {
-            load8<F32, VEC>(a.x, (size_t)row * (size_t)a.x_row, k, a.K, v[s]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[s][e] = 0.0f;
-        }
+        e[s] = load8<F32, VEC>(a.x, (size_t)min(row, a.rows - 1u) * (size_t)a.x_row, k, row < a.rows ? a.K : 0u);
     }
-#pragma unroll
-    for (uint32_t s = 0; s < STEPS; ++s) m = fmaxf(m, max8(v[s]));
+    float m = fmaxf(largest<F32, STEPS>(e), LEAST);
 #pragma unroll
     for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
     if ((threadIdx.x & 31u) == 0) part[threadIdx.x >> 5] = m;
@@ -147,7 +173,7 @@ quant_tiles_kernel(const QuantArgs a) {
 #pragma unroll
     for (uint32_t s = 0; s < STEPS; ++s) {
         const uint32_t row = row0 + s * STEP_ROWS;
-        if (row < a.rows) store8(a.q, (size_t)row * (size_t)a.q_row, k, a.K, v[s], inv);
+        if (row < a.rows) store8<F32>(a.q, (size_t)row * (size_t)a.q_row, k, a.K, e[s], inv);
     }
     if (threadIdx.x == 0) a.scales[(int64_t)tile_row * a.s_row + (int64_t)block * a.s_col] = __fdiv_rn(m, TOP);
 }
@@ -155,11 +181,11 @@ quant_tiles_kernel(const QuantArgs a) {
 template <bool F32, bool VEC>
 inline cudaError_t launch_quant(const QuantArgs& a, bool tiles, cudaStream_t stream) {
     if (tiles) return launch(quant_tiles_kernel<F32, VEC>, dim3((a.rows + BLOCK - 1) / BLOCK * a.k_blocks), dim3(TILE_THREADS), 0, stream, true, a);
-    const uint64_t total = (uint64_t)a.rows * a.k_blocks;
-    // four blocks a lane group once the SMs have enough groups with that
-    if (total >= (uint64_t)sm_count() * ROW_GROUPS * 16u)
-        return launch(quant_rows_kernel<F32, VEC, 4>, dim3((unsigned)((total + ROW_GROUPS * 4 - 1) / (ROW_GROUPS * 4))), dim3(ROW_THREADS), 0, stream, true, a);
-    return launch(quant_rows_kernel<F32, VEC, 1>, dim3((unsigned)((total + ROW_GROUPS - 1) / ROW_GROUPS)), dim3(ROW_THREADS), 0, stream, true, a);
+    const uint32_t total = a.rows * a.k_blocks;
+    // four lanes a block once every SM has 16 warps with that
+    if (total >= (uint32_t)sm_count() * 128u)
+        return launch(quant_rows_kernel<F32, VEC, 4>, dim3((total + ROW_THREADS / 4u - 1u) / (ROW_THREADS / 4u)), dim3(ROW_THREADS), 0, stream, true, a);
+    return launch(quant_rows_kernel<F32, VEC, 16>, dim3((total + ROW_THREADS / 16u - 1u) / (ROW_THREADS / 16u)), dim3(ROW_THREADS), 0, stream, true, a);
 }
 
 }  // namespace fp8
