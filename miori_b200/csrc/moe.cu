@@ -10,7 +10,7 @@ namespace moe {
 constexpr size_t TOPS_BYTES = MAX_ROWS * sizeof(uint32_t), HEAD_BYTES = (sizeof(Tables) + TOPS_BYTES + 255) / 256 * 256;
 
 // Dynamic shared memory of both products: all of an SM's that the tables leave, a ring and B fragments or partial sums in the rest.
-constexpr size_t SMEM = 227 * 1024 - (sizeof(Tables) + 127) / 128 * 128;
+constexpr size_t SMEM = 227 * 1024 - (sizeof(Tables) + 32 + 127) / 128 * 128;
 template <Format FMT>
 constexpr size_t frag_room(int depth) { return SMEM - Stage<FMT>::ring(depth) - 2 * WARPS * 512; }
 
@@ -18,8 +18,8 @@ template <Format FMT, int DEPTH>
 static int launch_moe(const char* op, Args a, cudaStream_t stream) {
     a.slots = (uint32_t)(frag_room<FMT>(DEPTH) / ((size_t)a.up.units * Stage<FMT>::FRAG));
     a.area = (uint32_t)(SMEM - Stage<FMT>::ring(Stage<FMT>::DOWN));
-    static_assert(SMEM - Stage<FMT>::ring(Stage<FMT>::DOWN) >= WARPS * 512u * ((MAX_ENTRIES + CLUSTER * WARPS - 1) / (CLUSTER * WARPS)) + MAX_TOKENS * 64u,
-                  "cells of a row tile, were every entry one unit, and its sums");
+    static_assert(SMEM - Stage<FMT>::ring(Stage<FMT>::DOWN) >= WARPS * 512u * ((MAX_ENTRIES + CLUSTER * WARPS - 1) / (CLUSTER * WARPS)) + 4u * MAX_TOKENS * 64u,
+                  "cells of a row tile, were every entry one unit, and the cluster's sums");
     const uint32_t sms = (uint32_t)sm_count(), row_tiles = a.H / 16u;
     // clusters of four whole SMs: an SM in nine has no place in one
     const uint32_t most = sms * 8u / 9u / CLUSTER;

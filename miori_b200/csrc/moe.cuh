@@ -401,14 +401,17 @@ __device__ __forceinline__ void list_entries(const Args& a, Tables& tb, uint32_t
 template <int PER>
 __global__ void __launch_bounds__(THREADS)
 moe_router_kernel(const Args a) {
-    constexpr uint32_t WIDE = PER * 2, SPLIT = WARPS / WIDE, WIDTH = PER * 32;  // tiles of 16 experts; warps over K; experts of a plane
+    constexpr uint32_t WIDE = PER * 2, REST = WARPS / WIDE, WIDTH = PER * 32;  // tiles of 16 experts; warps of each; experts of a plane
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ __align__(16) Tables tb;
     float* const part = reinterpret_cast<float*>(smem);  // [slice][token][expert]
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u, rank = blockIdx.x;
-    const uint32_t tile = warp % WIDE, slice = warp / WIDE, plane = a.tokens * WIDTH;
+    const uint32_t columns = (a.tokens + 7u) / 8u, plane = a.tokens * WIDTH;
+    // a tile's warps are dealt to the tiles of eight tokens, and what is left of them to K
+    const uint32_t spread = min(columns > 2u ? 4u : columns, REST), split = REST / spread;
+    const uint32_t tile = warp % WIDE, turn = warp / WIDE % spread, slice = warp / WIDE / spread;
     const uint32_t units = (a.H + 127u) / 128u, u0 = rank * units / ROUTER_CLUSTER, u1 = (rank + 1u) * units / ROUTER_CLUSTER;
-    const uint32_t columns = (a.tokens + 7u) / 8u, e_lo = tile * 16u + g, e_hi = e_lo + 8u;
+    const uint32_t e_lo = tile * 16u + g, e_hi = e_lo + 8u;
     uint4 lo[4], hi[4];
     auto weights = [&](uint32_t u) {
         const uint32_t k = u * 128u + t * 32u;
@@ -427,55 +430,43 @@ moe_router_kernel(const Args a) {
     __syncthreads();
     pdl_wait_prior();
     if (rank == 0u && threadIdx.x < a.tokens * a.top) a.h_top[threadIdx.x] = 0u;
-    float acc[MAX_TOKENS / 8][4] = {};
-    for (uint32_t u = u0 + slice; u < u1; u += SPLIT) {
-        if (u != u0 + slice || !a.ahead) weights(u);
-        const uint32_t k = u * 128u + t * 32u;
-        uint4 x[MAX_TOKENS / 8][4];
-#pragma unroll
-        for (uint32_t n = 0; n < MAX_TOKENS / 8u; ++n) {
-            if (n >= columns) break;
-            const uint32_t token = n * 8u + g;
-#pragma unroll
-            for (uint32_t i = 0; i < 4u; ++i) {
-                x[n][i] = make_uint4(0u, 0u, 0u, 0u);
-                if (token < a.tokens && k + i * 8u < a.H) x[n][i] = ld_fresh(reinterpret_cast<const uint4*>(a.x + (size_t)token * a.H + k + i * 8u));
-            }
-        }
-#pragma unroll
-        for (uint32_t n = 0; n < MAX_TOKENS / 8u; ++n) {
-            if (n >= columns) break;
+    for (uint32_t n = turn; n < columns; n += spread) {
+        const uint32_t token = n * 8u + g, in = min(token, a.tokens - 1u);  // those behind the last are computed and not stored
+        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        uint32_t most = 0u;
+        for (uint32_t u = u0 + slice; u < u1; u += split) {
+            if (n != turn || u != u0 + slice || !a.ahead) weights(u);
+            const uint32_t k = u * 128u + t * 32u;
+            uint4 x[4];
 #pragma unroll
             for (uint32_t i = 0; i < 4u; ++i) {
-                mma_bf16(acc[n], lo[i].x, hi[i].x, lo[i].y, hi[i].y, x[n][i].x, x[n][i].y);
-                mma_bf16(acc[n], lo[i].z, hi[i].z, lo[i].w, hi[i].w, x[n][i].z, x[n][i].w);
+                x[i] = make_uint4(0u, 0u, 0u, 0u);
+                if (k + i * 8u < a.H) x[i] = ld_fresh(reinterpret_cast<const uint4*>(a.x + (size_t)in * a.H + k + i * 8u));
             }
-            if (tile == 0u) {
+#pragma unroll
+            for (uint32_t i = 0; i < 4u; ++i) {
+                mma_bf16(acc, lo[i].x, hi[i].x, lo[i].y, hi[i].y, x[i].x, x[i].y);
+                mma_bf16(acc, lo[i].z, hi[i].z, lo[i].w, hi[i].w, x[i].z, x[i].w);
                 // magnitudes of bf16 are ordered as their bits are: the larger of each half of the words
-                uint32_t m = 0u;
-#pragma unroll
-                for (uint32_t i = 0; i < 4u; ++i)
-                    m = __vmaxu2(__vmaxu2(m, __vmaxu2(x[n][i].x & 0x7FFF7FFFu, x[n][i].y & 0x7FFF7FFFu)), __vmaxu2(x[n][i].z & 0x7FFF7FFFu, x[n][i].w & 0x7FFF7FFFu));
-                m = max(m & 0xFFFFu, m >> 16) << 16;
-                m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
-                m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
-                if (t == 0u && n * 8u + g < a.tokens) atomicMax(&tb.x_top[n * 8u + g], m);
+                most = __vmaxu2(__vmaxu2(most, __vmaxu2(x[i].x & 0x7FFF7FFFu, x[i].y & 0x7FFF7FFFu)), __vmaxu2(x[i].z & 0x7FFF7FFFu, x[i].w & 0x7FFF7FFFu));
             }
         }
-    }
+        if (tile == 0u) {
+            most = max(most & 0xFFFFu, most >> 16) << 16;
+            most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, 1));
+            most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, 2));
+            if (t == 0u && token < a.tokens) atomicMax(&tb.x_top[token], most);
+        }
 #pragma unroll
-    for (uint32_t n = 0; n < MAX_TOKENS / 8u; ++n) {
-        if (n >= columns) break;
-        const uint32_t token = n * 8u + 2u * t;
-#pragma unroll
-        for (uint32_t i = 0; i < 4u; ++i)
-            if (token + (i & 1u) < a.tokens) part[slice * plane + (token + (i & 1u)) * WIDTH + (i < 2u ? e_lo : e_hi)] = acc[n][i];
+        for (uint32_t i = 0; i < 4u; ++i) {
+            const uint32_t of = n * 8u + 2u * t + (i & 1u);
+            if (of < a.tokens) part[slice * plane + of * WIDTH + (i < 2u ? e_lo : e_hi)] = acc[i];
+        }
     }
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < plane; i += THREADS) {
         float s = part[i];
-#pragma unroll
-        for (uint32_t p = 1; p < SPLIT; ++p) s += part[p * plane + i];
+        for (uint32_t p = 1; p < split; ++p) s += part[p * plane + i];
         part[i] = s;
     }
     cluster_barrier();
@@ -774,12 +765,19 @@ moe_down_kernel(const Args a) {
     constexpr uint32_t RING = S::ring(DEPTH);
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ __align__(16) Tables tb;
+    __shared__ __align__(8) uint64_t arrived;  // the cluster's sums of this CTA's tiles
+    __shared__ volatile uint32_t abort_flag;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
     const uint32_t rank = blockIdx.x % CLUSTER, cluster = blockIdx.x / CLUSTER;
     const uint32_t ring = smem_addr(smem) + warp * (S::BYTES * DEPTH), ring_end = ring + S::BYTES * DEPTH, area = smem_addr(smem) + RING;
     float4* const cells = reinterpret_cast<float4*>(smem + RING);
 
     pdl_launch_dependents();
+    if (threadIdx.x == 0) {
+        abort_flag = 0u;
+        mbar_init(smem_addr(&arrived), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
     read_tables(a, tb);  // of a launch that was done before moe_up let this one start
     const uint32_t units = a.down.units, all_units = tb.entries * units;
     const uint32_t r0 = cluster * a.per, r1 = min(a.H / 16u, r0 + a.per);
@@ -787,10 +785,12 @@ moe_down_kernel(const Args a) {
     const uint32_t worker = rank * WARPS + warp, u0 = all_units * worker / WORKERS, u1 = all_units * (worker + 1u) / WORKERS;
     // partial sums: a cell for each entry that a warp meets and each row tile of a pass
     const uint32_t segments = ((all_units + WORKERS - 1u) / WORKERS + units - 2u) / units + 1u;
-    const uint32_t out_tile = a.tokens * 64u;  // bytes of the CTA's sums of a row tile, [token][16 rows]
-    const uint32_t at_once = min(a.per, a.area / (WARPS * segments * 512u + out_tile));
-    float* const sums = reinterpret_cast<float*>(cells);  // in front of the cells
-    float4* const mine = cells + at_once * out_tile / 16u + warp * (segments * at_once * 32u) + lane;
+    const uint32_t out_tile = a.tokens * 64u;  // bytes of a CTA's sums of a row tile, [token][16 rows]
+    // in front of the cells: the four CTAs' sums of this one's tiles, every fourth of a pass
+    uint32_t at_once = min(a.per, a.area / (WARPS * segments * 512u + out_tile));
+    while ((at_once + CLUSTER - 1u) / CLUSTER * CLUSTER * out_tile + at_once * (WARPS * segments * 512u) > a.area) --at_once;
+    const uint32_t own = (at_once + CLUSTER - 1u) / CLUSTER, front = own * CLUSTER * out_tile;
+    float4* const mine = cells + front / 16u + warp * (segments * at_once * 32u) + lane;
 
     uint32_t n_first = r0, n_unit = u0, n_row = 0;
     Run<FMT> run;
@@ -816,7 +816,9 @@ moe_down_kernel(const Args a) {
     };
 #pragma unroll 1
     for (uint32_t put = ring; put < ring_end; put += S::BYTES) fill(put);
+    asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
     pdl_wait_prior();
+    asm volatile("barrier.cluster.wait;" ::: "memory");  // the cluster's barriers exist
     // In place of a place's expert: this CTA's first warp that had units of its entry, the entry's number there, how many warps.  In place of its
     // weight that times the row's power of two.
     if (threadIdx.x < a.tokens * a.top) {
@@ -832,6 +834,7 @@ moe_down_kernel(const Args a) {
         tb.chosen[threadIdx.x] = (int)what;
     }
 
+    uint32_t parity = 0u;
     for (uint32_t first = r0; first < r1; first += at_once) {
         const uint32_t last = min(r1, first + at_once);
         uint32_t segment = 0;
@@ -880,43 +883,67 @@ moe_down_kernel(const Args a) {
             }
         }
         __syncthreads();
-        // A token's places, and of each the warps of this CTA that had units of its entry: all but the first began with it.  Few outputs are
-        // eight threads' work each.
-        const uint32_t outputs = (last - first) * a.tokens * 16u, warp_floats = segments * at_once * 128u, lanes = outputs * 8u <= THREADS ? 8u : 1u;
-        const float* const parts = reinterpret_cast<const float*>(cells + at_once * out_tile / 16u);
-        for (uint32_t i = threadIdx.x / lanes; i < outputs; i += THREADS / lanes) {
-            const uint32_t row = i & 15u, rest = i >> 4, tile = a.by_tokens(rest), token = rest - tile * a.tokens, w0 = threadIdx.x & (lanes - 1u);
-            float total = 0.0f;
-            for (uint32_t at = token * a.top; at < (token + 1u) * a.top; ++at) {
-                const uint32_t what = (uint32_t)tb.chosen[at], warps = what >> 16;
-                if (warps == 0u) continue;
-                const uint32_t column = tb.slot[at] % ENTRY;
-                const float* from = parts + (what & 0xFFu) * warp_floats + (tile * 32u + (row & 7u) * 4u + column / 2u) * 4u + (column & 1u) + (row >> 3) * 2u;
-                float s = w0 == 0u ? from[(what >> 8 & 0xFFu) * (at_once * 128u)] : w0 < warps ? from[w0 * warp_floats] : 0.0f;
-                for (uint32_t w = w0 + lanes; w < warps; w += lanes) s += from[w * warp_floats];
-                total = __fmaf_rn(tb.weight[at], s, total);
-            }
-            if (lanes == 8u) {  // whole warps: outputs are a multiple of 16
-                total += __shfl_xor_sync(0xFFFFFFFFu, total, 1);
-                total += __shfl_xor_sync(0xFFFFFFFFu, total, 2);
-                total += __shfl_xor_sync(0xFFFFFFFFu, total, 4);
-            }
-            if (w0 == 0u) sums[i] = total;
-        }
-        cluster_barrier();
-        const uint32_t pieces = outputs / 16u, share0 = pieces * rank / CLUSTER * 16u, share1 = pieces * (rank + 1u) / CLUSTER * 16u;
-        for (uint32_t i = share0 + threadIdx.x; i < share1; i += THREADS) {
-            float v[CLUSTER], s = 0.0f;
+        // A row of a token's sums in all tiles of the pass: its places, and of each the warps of this CTA that had units of its entry, all but the first
+        // of which began with it.  Few tokens' are eight threads' work each.  The sums go straight to the CTA that owns the tile.
+        const uint32_t tiles = last - first, lanes = a.tokens <= 4u ? 8u : 1u, warp_floats = segments * at_once * 128u;
+        const uint32_t mine_now = (tiles + CLUSTER - 1u - rank) / CLUSTER;  // of the tiles, those that are this CTA's
+        const float* const parts = reinterpret_cast<const float*>(cells + front / 16u);
+        if (threadIdx.x == 0) mbar_expect_tx(smem_addr(&arrived), mine_now * CLUSTER * out_tile);
+        for (uint32_t i = threadIdx.x / lanes; i < a.tokens * 16u; i += THREADS / lanes) {
+            const uint32_t row = i & 15u, token = i >> 4, w0 = threadIdx.x & (lanes - 1u);
+            for (uint32_t t0 = 0; t0 < tiles; t0 += CLUSTER) {
+                float total[CLUSTER] = {};
+                for (uint32_t at = token * a.top; at < (token + 1u) * a.top; ++at) {
+                    const uint32_t what = (uint32_t)tb.chosen[at], warps = what >> 16, column = tb.slot[at] % ENTRY;
+                    const float* from = parts + (what & 0xFFu) * warp_floats + (t0 * 32u + (row & 7u) * 4u + column / 2u) * 4u + (column & 1u) + (row >> 3) * 2u;
+                    const float weight = tb.weight[at];
+                    float s[CLUSTER] = {};
+                    for (uint32_t w = w0; w < warps; w += lanes) {
+                        const float* p = from + w * warp_floats + (w == 0u ? (what >> 8 & 0xFFu) * (at_once * 128u) : 0u);
 #pragma unroll
-            for (uint32_t r = 0; r < CLUSTER; ++r) v[r] = remote_f32(area + i * 4u, r);
+                        for (uint32_t j = 0; j < CLUSTER; ++j)
+                            if (t0 + j < tiles) s[j] += p[j * 128u];
+                    }
+                    if (warps) {
 #pragma unroll
-            for (uint32_t r = 0; r < CLUSTER; ++r) s += v[r];
-            const uint32_t rest = i >> 4, tile = a.by_tokens(rest), token = rest - tile * a.tokens;
-            const size_t at = (size_t)token * a.H + (first + tile) * 16u + (i & 15u);
-            if (a.bf16) static_cast<uint16_t*>(a.out)[at] = (uint16_t)pack_bf16(s, 0.0f);
-            else static_cast<float*>(a.out)[at] = s;
+                        for (uint32_t j = 0; j < CLUSTER; ++j) total[j] = __fmaf_rn(weight, s[j], total[j]);
+                    }
+                }
+                if (lanes == 8u) {  // whole warps: 16 rows a token
+#pragma unroll
+                    for (uint32_t d = 1; d < 8u; d *= 2u)
+#pragma unroll
+                        for (uint32_t j = 0; j < CLUSTER; ++j) total[j] += __shfl_xor_sync(0xFFFFFFFFu, total[j], d);
+                }
+                if (w0 == 0u) {
+#pragma unroll
+                    for (uint32_t j = 0; j < CLUSTER; ++j)
+                        if (t0 + j < tiles)
+                            asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.u32 [%0], %1, [%2];"
+                                         ::"r"(remote(area + ((rank * own + t0 / CLUSTER) * a.tokens * 16u + i) * 4u, j)), "r"(__float_as_uint(total[j])), "r"(remote(smem_addr(&arrived), j)) : "memory");
+                }
+            }
         }
-        cluster_barrier();
+        // No CTA leaves, or sends a next pass's sums, before all have come this far; on the last pass that is said before they are waited for.
+        if (last >= r1) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
+        if (mine_now) {
+            const bool ok = mbar_wait(smem_addr(&arrived), parity, &abort_flag, 0x81);
+            for (uint32_t i = threadIdx.x; ok && i < mine_now * a.tokens * 16u; i += THREADS) {
+                const uint32_t rest = i >> 4, q = a.by_tokens(rest), token = rest - q * a.tokens;
+                float v = 0.0f;
+#pragma unroll
+                for (uint32_t r = 0; r < CLUSTER; ++r) {
+                    const float w = reinterpret_cast<const float*>(cells)[r * own * a.tokens * 16u + i];
+                    v = r ? v + w : w;
+                }
+                const size_t at = (size_t)token * a.H + (first + q * CLUSTER + rank) * 16u + (i & 15u);
+                if (a.bf16) static_cast<uint16_t*>(a.out)[at] = (uint16_t)pack_bf16(v, 0.0f);
+                else static_cast<float*>(a.out)[at] = v;
+            }
+        }
+        parity ^= 1u;
+        if (last < r1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+        asm volatile("barrier.cluster.wait;" ::: "memory");
     }
     cp_wait<0>();
 }
