@@ -68,6 +68,7 @@ MIORI_API int miori_gemm_fp8(const void* a, int64_t lda, const float* sa, int64_
     g.by_tma = aligned16(C) && ldc * size % 16 == 0 && (uint64_t)N * size % 16 == 0 ? 1u : 0u;
     const GemmOperands o = {a, w, lda, ldw};
     const GemmPlan p = plan_gemm_fp8(M, N, K, flags);
+    if (!p.pair_n && K > 128u * KB_BYTES) return fail(MIORI_E_INVALID, "%s: the kernel of few rows takes K up to 16384, got %u", op, K);  // by a tuning flag
     const cudaStream_t s = (cudaStream_t)stream;
     if (p.pair_n) return p.pair_n == 256u ? launch_pair<256>(o, g, s) : launch_pair<128>(o, g, s);
     switch (p.mp) {

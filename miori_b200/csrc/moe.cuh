@@ -362,14 +362,20 @@ __device__ __forceinline__ void choose(const Args& a, Tables& tb, uint32_t token
             if (j * 32u + lane == e) key[j] = 0u;
         if (lane == place) mine = w, expert = (int)e;
     }
-    const float p = expert >= 0 ? score(mine) : 0.0f;
-    float sum = p;
+    float p = expert >= 0 ? score(mine) : 0.0f, sum = 1.0f;
+    if (a.norm) {  // as shares of the largest chosen one, e^(l - m) [/ (1 + e^l)]: scores that underflow have a sum all the same
+        float m = expert >= 0 ? mine : -INFINITY;
 #pragma unroll
-    for (int d = 8; d; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+        for (int d = 8; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
+        if (expert >= 0) p = a.sigmoid ? expf(fminf(mine, 0.0f) - fminf(m, 0.0f)) / (1.0f + expf(-fabsf(mine))) : expf(mine - m);
+        sum = p;
+#pragma unroll
+        for (int d = 8; d; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+    }
     if (lane < a.top) {
         const uint32_t at = token * a.top + lane;
         asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(remote(smem_addr(&tb.chosen[at]), 0)), "r"(expert) : "memory");
-        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote(smem_addr(&tb.weight[at]), 0)), "f"((a.norm ? p / sum : p) * a.factor) : "memory");
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote(smem_addr(&tb.weight[at]), 0)), "f"(p / sum * a.factor) : "memory");
         if (expert >= 0) asm volatile("red.relaxed.cluster.shared::cluster.or.b32 [%0], %1;" ::"r"(remote(smem_addr(&tb.mask[expert]), 0)), "r"(1u << token) : "memory");
     }
 }

@@ -204,3 +204,63 @@ def test_a_projection_in_blocks():
         # each factor off by 2^-4 of itself at most, 2^-4 / sqrt(3) on average over a binade, of either sign
         assert float((C.double() - want).norm() / want.norm()) < 2 ** 0.5 * 2.0 ** -4
     assert mb.lib.miori_device_error_poll() == 0
+
+
+FEW, PAIRS = [(mp, cs) for mp in (1, 2, 3, 4) for cs in (0, 1, 2, 3)], [(5, 0), (6, 0)]  # as the tuning bits have them
+
+
+@pytest.mark.parametrize("kind,log_slices", FEW + PAIRS)
+def test_every_kernel_takes_every_size(kind, log_slices):
+    """Each tile and split, chosen by the tuning bits rather than by size: the same products within the same tolerance."""
+    tune = kind << 20 | log_slices << 23
+    for M, N, K in ((1, 1, 16), (9, 130, 1100), (70, 300, 1440), (140, 257, 2000), (300, 128, 1024)):
+        ops = operands(M, N, K, M + kind)
+        close(mb.gemm_fp8(*ops, flags=tune), *ops)
+        close(mb.gemm_fp8(*ops, flags=tune | mb.OUT_BF16), *ops)
+    assert mb.lib.miori_device_error_poll() == 0
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 100, 16384), (3, 200, 16385), (70, 130, 16400), (300, 300, 20000)])
+def test_long_sums(M, N, K):
+    """On both sides of the longest K of the kernel of few rows, and a refusal where it is asked for more."""
+    ops = operands(M, N, K, 9)
+    close(mb.gemm_fp8(*ops), *ops)
+    if K > 16384:
+        with pytest.raises(mb.MioriError, match="K up to 16384"):
+            mb.gemm_fp8(*ops, flags=1 << 20)
+
+
+def test_scales_that_are_broadcast():
+    """One scale for all of a, or for all of w: strides of zero."""
+    a, _, w, _ = operands(40, 300, 500, 10)
+    one = torch.full((1, 1), 0.25, device=DEV)
+    sa, sw = one.expand(40, blocks(500)), one.expand(blocks(300), blocks(500))
+    close(mb.gemm_fp8(a, sa, w, sw), a, sa, w, sw)
+
+
+def test_gemm_to_memory_past_32_bits():
+    """Rows of C that begin more than 2^32 bytes behind the first, by both kernels."""
+    for M, N in ((600, 200), (70, 130)):
+        a, sa, w, sw = operands(M, N, 256, 11)
+        pitch = 2 ** 32 // M // 2 // 8 * 8 + 4096  # bf16
+        out = torch.full((M, pitch), 2.0, dtype=torch.bfloat16, device=DEV)
+        got = mb.gemm_fp8(a, sa, w, sw, flags=mb.OUT_BF16, out=out[:, :N])
+        close(got, a, sa, w, sw)
+        assert bool((out[-1, N:] == 2).all()) and bool((out[0, N:] == 2).all())
+        del out, got
+
+
+def test_quant_of_memory_past_32_bits():
+    x = torch.zeros((3, 2 ** 30 + 64), dtype=torch.float32, device=DEV)[:, :700]
+    x.copy_(torch.randn(3, 700, device=DEV, generator=torch.Generator(device=DEV).manual_seed(12)))
+    for tile in (1, 128):
+        same(mb.quant_fp8(x, tile=tile), oracle_quant(x, tile))
+
+
+def test_quant_rows_do_not_depend_on_one_another():
+    """A row's codes and scales in blocks of one row are the same alone, in a small and in a large batch (other numbers of lanes a block)."""
+    x = torch.randn(5000, 1440, device=DEV, generator=torch.Generator(device=DEV).manual_seed(13))
+    q, s = mb.quant_fp8(x)
+    for rows in (1, 2, 7, 33, 600):
+        part, ps = mb.quant_fp8(x[100:100 + rows])
+        assert torch.equal(bits(part), bits(q)[100:100 + rows]) and torch.equal(ps, s[100:100 + rows])

@@ -223,3 +223,60 @@ def test_between_launches_that_may_begin_early():
         y2 = run(n2, router, ws, 4, 64, 2, bias, mb.OUT_BF16, workspace=workspace)
         torch.cuda.synchronize()
         assert torch.equal(y, y2) and torch.equal(z, mb.gemv4(q, s, b, y2, 64))
+
+
+@pytest.mark.parametrize("bits,group,T,E,top,H,F", [
+    (4, 64, 3, 4, 2, 7168, 256), (4, 32, 20, 4, 2, 7168, 128), (8, 128, 9, 4, 3, 7168, 144),  # rows whose B fragments take a shorter ring
+    (4, 64, 32, 128, 16, 2048, 128), (4, 32, 32, 256, 8, 7168, 128), (8, 128, 32, 256, 16, 1024, 128),  # so many entries that rows of the output are worked on in parts
+    (4, 64, 2, 2, 1, 128, 65536), (8, 128, 2, 1, 1, 16, 65536), (8, 128, 32, 3, 2, 16, 16)])
+def test_the_largest_and_the_smallest(bits, group, T, E, top, H, F):
+    x, router, ws, bias = make(bits, group, T, E, H, F, T + E + 1)
+    check(x, router, ws, bits, group, top, bias, mb.MOE_SIGMOID)
+
+
+@pytest.mark.parametrize("flags", [0, 1 << 10])
+def test_logits_far_from_zero(flags):
+    """Scores that are one, or underflow: shares of them stay shares.  (Logits of a single product, which fp32 holds: only the exponentials round.)"""
+    assert mb.MOE_NORM == 1 << 10
+    x, router, ws, bias = make(4, 64, 6, 12, 256, 128, 14)
+    column = (router[:, 0].float() * 16 * 60).to(torch.bfloat16)
+    router = torch.zeros_like(router)
+    router[:, 0] = column
+    x[:, 0] = torch.tensor([1.0, -1.0, 0.5, 2.0, -2.0, 0.25], device=DEV).to(torch.bfloat16)
+    check(x, router, ws, 4, 64, 3, None, flags)
+    check(x, router, ws, 4, 64, 3, None, flags | mb.MOE_SIGMOID)
+    # a bias that picks experts whose scores are nothing in fp32; with logits of -200 and so on a 64-bit oracle still has them
+    x[:, 0] = 1.0
+    low = torch.zeros_like(router)
+    low[:, 0] = torch.arange(12, device=DEV) * -2.0 - 200.0
+    low[5] = 0.0
+    bias = torch.zeros(12, device=DEV)
+    bias[[2, 3, 4]] = 5.0
+    if flags & mb.MOE_NORM:
+        check(x, low, ws, 4, 64, 3, bias, flags)
+        check(x, low, ws, 4, 64, 3, bias, flags | mb.MOE_SIGMOID)
+
+
+@pytest.mark.parametrize("bits,group", [(4, 64), (8, 128)])
+def test_in_place(bits, group):
+    x, router, ws, bias = make(bits, group, 7, 8, 256, 256, 15)
+    want = run(x, router, ws, bits, group, 2, bias, mb.OUT_BF16)
+    got = run(x, router, ws, bits, group, 2, bias, mb.OUT_BF16, out=x)
+    assert got is x and torch.equal(got, want)
+
+
+def test_two_streams_at_once():
+    """Layers that overlap, each with a workspace of its own."""
+    sides, results = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    problems = [make(4, 64, 32, 16, 1024, 512, 16), make(8, 128, 5, 16, 1024, 512, 17)]
+    want = [run(problems[0][0], *problems[0][1:3], 4, 64, 2, problems[0][3], 0), run(problems[1][0], *problems[1][1:3], 8, 128, 2, problems[1][3], 0)]
+    torch.cuda.synchronize()
+    spaces = [mb.moe_workspace(32, 2, 512, DEV) for _ in range(2)]
+    for _ in range(20):
+        for i, (x, router, ws, bias) in enumerate(problems):
+            with torch.cuda.stream(sides[i]):
+                results[i].append(run(x, router, ws, (4, 8)[i], (64, 128)[i], 2, bias, mb.LAUNCH_PDL, workspace=spaces[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(r, want[i]) for r in results[i])
+    assert mb.lib.miori_device_error_poll() == 0
