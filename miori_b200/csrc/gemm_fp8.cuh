@@ -31,7 +31,7 @@ struct GemmArgs {
     int64_t ldc, sa_row, sa_col, sw_row, sw_col;  // elements
     uint32_t M, N, K;
     uint32_t bf16;
-    uint32_t by_tma;  // C's rows begin on 16-byte boundaries: stored by TMA
+    uint32_t by_tma;  // C's rows begin and end on 16-byte boundaries: stored by TMA, or by words
 };
 
 // K-major, 128-byte swizzle: rows of 128 bytes, eight of them an atom of 1024 bytes.
@@ -509,50 +509,51 @@ gemm_fp8_swap_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     }
     __syncwarp();
 
-    const uint32_t row = (warp & 3u) * 32u + lane, n = n_tile * 128u + row, rows = min((uint32_t)MP, g.M - m0);
-    auto store = [&](uint32_t m, float v) {  // 32 lanes: neighbouring elements of a row of C
+    // The sums go to shared memory, [row of a][row of w]: all MMAs are done and, after a barrier of their readers, the scales are read.  From there
+    // CTA r of the cluster takes rows r, r + cs, ... of a, each by a warp, and adds them up in rank order.  (Stored by the threads that hold them
+    // a row was 160 cycles: its instructions, which nothing had run before, took that long to come.)
+    if (warp >= 3u) {
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        const uint32_t to = ring + ((warp & 3u) * 32u + lane) * 4u;
+#pragma unroll
+        for (int j = 0; j < MP; ++j) asm volatile("st.shared.f32 [%0], %1;" ::"r"(to + j * 512u), "f"(acc[j]) : "memory");
+    }
+    if (geo.cs > 1u) cluster_barrier();
+    else __syncthreads();
+    const uint32_t rows = min((uint32_t)MP, g.M - m0), n = n_tile * 128u + lane * 4u;
+#pragma unroll 1
+    for (uint32_t m = rank + geo.cs * warp; m < rows && !abort_flag; m += geo.cs * (SWAP_THREADS / 32u)) {
+        const uint32_t from = ring + m * 512u + lane * 16u;
+        float4 v[8];
+#pragma unroll
+        for (uint32_t p = 0; p < 8u; ++p) {
+            if (p >= geo.cs) break;
+            uint32_t at;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(from), "r"(p));
+            asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[p].x), "=f"(v[p].y), "=f"(v[p].z), "=f"(v[p].w) : "r"(at) : "memory");
+        }
+        float4 t = v[0];
+#pragma unroll
+        for (uint32_t p = 1; p < 8u; ++p) {
+            if (p >= geo.cs) break;
+            t.x += v[p].x, t.y += v[p].y, t.z += v[p].z, t.w += v[p].w;
+        }
         const int64_t at = (int64_t)(m0 + m) * g.ldc + n;
-        if (n >= g.N) return;
-        if (g.bf16) static_cast<uint16_t*>(g.c)[at] = (uint16_t)pack_bf16(v, 0.0f);
-        else static_cast<float*>(g.c)[at] = v;
-    };
-    if (geo.cs == 1u) {
-        if (warp >= 3u && ok) {
+        if (g.by_tma) {  // rows begin and end on 16-byte boundaries: four columns are all there or none is
+            if (n >= g.N) continue;
+            if (g.bf16) *reinterpret_cast<uint2*>(static_cast<uint16_t*>(g.c) + at) = make_uint2(pack_bf16(t.x, t.y), pack_bf16(t.z, t.w));
+            else *reinterpret_cast<float4*>(static_cast<float*>(g.c) + at) = t;
+        } else {
+            const float e[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
-            for (int j = 0; j < MP; ++j)
-                if ((uint32_t)j < rows) store((uint32_t)j, acc[j]);
-        }
-    } else {
-        // CTA r of the cluster adds up rows r, r + cs, ... of a, in rank order.  All MMAs are done (their sums have been read): the rings
-        // take the partial sums, [source][row / cs][row of w].
-        cluster_barrier();
-        const uint32_t share = (rows + geo.cs - 1u) / geo.cs;
-        if (warp >= 3u) {
-            uint32_t to_rank = 0, at = 0;
-#pragma unroll
-            for (int j = 0; j < MP; ++j) {
-                if ((uint32_t)j < rows) {
-                    uint32_t to;
-                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(ring + ((rank * share + at) * 128u + row) * 4u), "r"(to_rank));
-                    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(acc[j]) : "memory");
-                    if (++to_rank == geo.cs) to_rank = 0u, ++at;
-                }
-            }
-        }
-        cluster_barrier();
-        if (warp >= 3u && ok) {
-            for (uint32_t at = 0, m = rank; m < rows; ++at, m += geo.cs) {
-                float v = 0.0f;
-#pragma unroll 4
-                for (uint32_t p = 0; p < geo.cs; ++p) {
-                    float w;
-                    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(w) : "r"(ring + ((p * share + at) * 128u + row) * 4u) : "memory");
-                    v = p == 0u ? w : v + w;
-                }
-                store(m, v);
+            for (uint32_t i = 0; i < 4u; ++i) {
+                if (n + i >= g.N) break;
+                if (g.bf16) static_cast<uint16_t*>(g.c)[at + i] = (uint16_t)pack_bf16(e[i], 0.0f);
+                else static_cast<float*>(g.c)[at + i] = e[i];
             }
         }
     }
+    if (geo.cs > 1u) cluster_barrier();  // nobody leaves while its sums are read
 
     if (abort_flag) {
         const long long t0 = clock64();
@@ -610,9 +611,7 @@ inline int launch_swap(const GemmOperands& o, const GemmArgs& g, uint32_t cs, cu
     if (geo.stages > (uint32_t)SWAP_MAX_STAGES) geo.stages = SWAP_MAX_STAGES;
     if (geo.stages > slice) geo.stages = slice;
     size_t smem = (size_t)geo.stages * STAGE_BYTES + scale_bytes;
-    const uint32_t rows = g.M < (uint32_t)MP ? g.M : (uint32_t)MP;
-    const size_t recv = cs > 1u ? (size_t)(rows + cs) * 512u : 0;
-    if (smem < recv) smem = recv;
+    if (smem < MP * 512u) smem = MP * 512u;  // the sums
     const cudaError_t e = launch_cluster(gemm_fp8_swap_kernel<MP>, (g.N + 127u) / 128u * geo.m_tiles * cs, SWAP_THREADS, smem + 1024, cs, stream, mw, ma, g, geo);
     return e == cudaSuccess ? MIORI_OK : cuda_fail(e, "gemm_fp8 (few rows) launch");
 }
@@ -623,8 +622,8 @@ struct GemmPlan {
     uint32_t mp, cs;
 };
 // The cheapest by a small model (us), whose numbers are what the kernels take a k-block once they run: 0.31 and 0.56 the tiles of pairs, of 128 and 256
-// columns; 0.2, 0.3, 0.5 and 0.95 the kernel of few rows with 16, 32, 64 and 128 of them; a wave's beginning and end on top; what HBM takes to deliver w is
-// a floor.  A split of K costs the clusters' meeting, which grows with the rows that are exchanged.
+// columns; 0.2, 0.23, 0.33 and 0.6 the kernel of few rows with 16, 32, 64 and 128 of them, which has 0.025 a row at its end and 0.7 where K is split; a
+// wave's beginning and end on top; what HBM takes to deliver w is a floor.
 inline GemmPlan plan_gemm_fp8(uint32_t M, uint32_t N, uint32_t K, uint32_t flags) {
     if (const uint32_t f = flags >> MIORI_TUNE_FP8_SHIFT & 7u) {
         if (f >= 5u) return {f == 5u ? 128u : 256u, 0, 0};
@@ -643,16 +642,14 @@ inline GemmPlan plan_gemm_fp8(uint32_t M, uint32_t N, uint32_t K, uint32_t flags
     consider({128, 0, 0}, waves(m256 * ((N + 127u) / 128u), sms / 2) * (k_blocks * 0.31 + 1.0) + 0.8);
     consider({256, 0, 0}, waves(m256 * ((N + 255u) / 256u), sms / 2) * (k_blocks * 0.56 + 1.4) + 0.8);
     if (k_blocks > 128u) return best;  // the kernel of few rows keeps its scales in shared memory
-    static const double per_block[4] = {0.2, 0.3, 0.5, 0.95};
+    static const double per_block[4] = {0.2, 0.23, 0.33, 0.6};
     for (uint32_t i = 0; i < 4u; ++i) {
         const uint32_t mp = 16u << i;
         if (mp >= 2u * M && mp > 16u) break;
         const uint64_t tiles = (uint64_t)((N + 127u) / 128u) * ((M + mp - 1u) / mp);
-        for (uint32_t cs = 1; cs <= 8u && k_blocks >= cs; cs *= 2u) {
+        for (uint32_t cs = 1; cs <= (mp == 128u ? 4u : 8u) && k_blocks >= cs; cs *= 2u) {  // 128 rows are an SM's registers: eight such SMs side by side are rare
             if (cs > 1u && tiles * cs > sms) break;
-            const uint32_t rows = M < mp ? M : mp;
-            const double t = waves(tiles * cs, sms) * ((k_blocks + cs - 1u) / cs * per_block[i] + 0.4) + (cs > 1u ? 0.5 + rows * 0.04 : 0.0);
-            consider({0, mp, cs}, t);
+            consider({0, mp, cs}, waves(tiles * cs, sms) * ((k_blocks + cs - 1u) / cs * per_block[i] + mp * 0.025) + (cs > 1u ? 0.7 : 0.0));
         }
     }
     return best;
