@@ -790,7 +790,7 @@ moe_down_kernel(const Args a) {
     // warp w of the cluster has the units [all w / 64, all (w + 1) / 64)
     const uint32_t worker = rank * WARPS + warp, u0 = all_units * worker / WORKERS, u1 = all_units * (worker + 1u) / WORKERS;
     // partial sums: a cell for each entry that a warp meets and each row tile of a pass
-    const uint32_t segments = ((all_units + WORKERS - 1u) / WORKERS + units - 2u) / units + 1u;
+    const uint32_t segments = (max((all_units + WORKERS - 1u) / WORKERS, 1u) + units - 2u) / units + 1u;
     const uint32_t out_tile = a.tokens * 64u;  // bytes of a CTA's sums of a row tile, [token][16 rows]
     // in front of the cells: the four CTAs' sums of this one's tiles, every fourth of a pass
     uint32_t at_once = min(a.per, a.area / (WARPS * segments * 512u + out_tile));
