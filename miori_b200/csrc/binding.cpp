@@ -11,6 +11,7 @@
 #include <Python.h>
 
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -562,6 +563,23 @@ OP(attention_prompt, 4, "q", "k", "v", "cu", "cu_k", "scale", "flags", "out", "w
     return o.result();
 }
 
+// An optional argument for the next function; one that is not on a GPU is refused, or taken where it is pinned, by its own check.
+const at::Tensor* or_first(const Args& a, int i) { return a.given(i) && a.tensor(i).is_cuda() ? &a.tensor(i) : &a.tensor(0); }
+// A call on a device that need not be the current one, on its current stream.
+void* stream(c10::Device d) { return (void*)c10::cuda::getCurrentCUDAStream(d.index()).stream(); }
+template <class... P, class... A>
+void call_on(c10::Device d, int (*fn)(P...), A... args) {
+    const c10::cuda::CUDAGuard guard(d);
+    call(fn, args...);
+}
+// The device of these tensors, which have to share one.
+c10::Device device_of(std::initializer_list<const at::Tensor*> ts) {
+    const c10::Device d = (*ts.begin())->device();
+    for (const at::Tensor* t : ts)
+        if (t->device() != d) raise(PyExc_ValueError, "tensors of one device are expected, got some of %s and of %s", d.str().c_str(), t->device().str().c_str());
+    return d;
+}
+
 // A matrix of 8-bit floating point: rows may lie apart, on 16-byte boundaries (the library checks those).
 void need_fp8(const at::Tensor& t, const char* what, int64_t dims) {
     if (!t.is_cuda()) raise(PyExc_ValueError, "miori_b200 ops need CUDA tensors (there is no CPU path)");
@@ -596,6 +614,7 @@ OP(quant_fp8, 1, "x", "tile", "flags", "out", "scales") {
     const int64_t row_blocks = (R + tile - 1) / tile;
     const uint32_t flags = (a.u32(2, 0) & ~MIORI_QUANT_F32) | (fp32 ? MIORI_QUANT_F32 : 0u);
     at::Tensor q, s;
+    const c10::Device on = device_of({&x, or_first(a, 3), or_first(a, 4)});
     if (a.given(3)) {
         q = a.tensor(3);
         need_fp8(q, "out", 2);
@@ -611,8 +630,8 @@ OP(quant_fp8, 1, "x", "tile", "flags", "out", "scales") {
     } else {
         s = empty({row_blocks, blocks(K)}, at::kFloat, x);
     }
-    call(abi.quant_fp8, x.data_ptr(), R == 1 ? K : x.stride(0), q.data_ptr(), pitch(q, 16), static_cast<float*>(s.data_ptr()), s.stride(0), s.stride(1), R, K, tile,
-         flags, stream());
+    call_on(on, abi.quant_fp8, x.data_ptr(), R == 1 ? K : x.stride(0), q.data_ptr(), pitch(q, 16), static_cast<float*>(s.data_ptr()), s.stride(0), s.stride(1), R, K, tile,
+         flags, stream(on));
     return tuple_of({&q, &s});
 }
 
@@ -627,6 +646,7 @@ OP(gemm_fp8, 4, "a", "sa", "w", "sw", "flags", "out") {
     need_scales(sw, "sw", blocks(N), blocks(K));
     const uint32_t flags = a.u32(4, 0);
     const at::ScalarType dt = out_type(flags);
+    const c10::Device on = device_of({&x, &sa, &w, &sw, or_first(a, 5)});
     Out o;  // rows of a caller's output may lie apart
     if (a.given(5)) a.tensor(5), o.given = a.v[5];
     else o.made = empty({M, N}, dt, x);
@@ -634,8 +654,8 @@ OP(gemm_fp8, 4, "a", "sa", "w", "sw", "flags", "out") {
     if (!c.is_cuda()) raise(PyExc_ValueError, "out: a CUDA tensor is expected");
     if (c.scalar_type() != dt || c.dim() != 2 || c.size(0) != M || c.size(1) != N || (N != 1 && c.stride(1) != 1))
         raise(PyExc_ValueError, "out: [%lld][%lld] of the output's type with contiguous rows expected", (long long)M, (long long)N);
-    call(abi.gemm_fp8, x.data_ptr(), pitch(x, 16), static_cast<const float*>(sa.data_ptr()), sa.stride(0), sa.stride(1), w.data_ptr(), pitch(w, 16),
-         static_cast<const float*>(sw.data_ptr()), sw.stride(0), sw.stride(1), c.data_ptr(), M == 1 ? N : c.stride(0), M, N, K, flags, stream());
+    call_on(on, abi.gemm_fp8, x.data_ptr(), pitch(x, 16), static_cast<const float*>(sa.data_ptr()), sa.stride(0), sa.stride(1), w.data_ptr(), pitch(w, 16),
+         static_cast<const float*>(sw.data_ptr()), sw.stride(0), sw.stride(1), c.data_ptr(), M == 1 ? N : c.stride(0), M, N, K, flags, stream(on));
     return o.result();
 }
 
@@ -688,10 +708,12 @@ OP(moe4, 10, "x", "router", "q_up", "s_up", "b_up", "q_down", "s_down", "b_down"
                *bu = weights(a.tensor(4), "b_up", at::kBFloat16, l.E, 2 * F, l.H / group), *qd = weights(a.tensor(5), "q_down", at::kInt, l.E, l.H, F / 8),
                *sd = weights(a.tensor(6), "s_down", at::kBFloat16, l.E, l.H, F / group), *bd = weights(a.tensor(7), "b_down", at::kBFloat16, l.E, l.H, F / group);
     const uint32_t top = a.u32(8, 0), flags = a.u32(13, 0);
+    const c10::Device on = device_of({&a.tensor(0), &a.tensor(1), &a.tensor(2), &a.tensor(3), &a.tensor(4), &a.tensor(5), &a.tensor(6), &a.tensor(7), &a.tensor(9),
+                                             or_first(a, 10), or_first(a, 14)});
     const float factor = a.given(12) ? a.f32(12) : 1.0f;
     Out o = output(a, 14, {l.T, l.H}, out_type(flags), a.tensor(0));
-    call(abi.moe4, a.tensor(0).data_ptr(), a.tensor(1).data_ptr(), l.bias, qu, su, bu, qd, sd, bd, o.ptr(), l.T, l.E, top, l.H, F, group, factor, flags, l.workspace,
-         l.bytes, stream());
+    call_on(on, abi.moe4, a.tensor(0).data_ptr(), a.tensor(1).data_ptr(), l.bias, qu, su, bu, qd, sd, bd, o.ptr(), l.T, l.E, top, l.H, F, group, factor, flags, l.workspace,
+         l.bytes, stream(on));
     return o.result();
 }
 
@@ -701,10 +723,12 @@ OP(moe_fp8, 8, "x", "router", "w_up", "s_up", "w_down", "s_down", "top", "worksp
     const void *wu = weights(a.tensor(2), "w_up", at::kFloat8_e4m3fn, l.E, 2 * F, l.H), *su = weights(a.tensor(3), "s_up", at::kFloat, l.E, blocks(2 * F), blocks(l.H)),
                *wd = weights(a.tensor(4), "w_down", at::kFloat8_e4m3fn, l.E, l.H, F), *sd = weights(a.tensor(5), "s_down", at::kFloat, l.E, blocks(l.H), blocks(F));
     const uint32_t top = a.u32(6, 0), flags = a.u32(10, 0);
+    const c10::Device on = device_of({&a.tensor(0), &a.tensor(1), &a.tensor(2), &a.tensor(3), &a.tensor(4), &a.tensor(5), &a.tensor(7),
+                                             or_first(a, 8), or_first(a, 11)});
     const float factor = a.given(9) ? a.f32(9) : 1.0f;
     Out o = output(a, 11, {l.T, l.H}, out_type(flags), a.tensor(0));
-    call(abi.moe_fp8, a.tensor(0).data_ptr(), a.tensor(1).data_ptr(), l.bias, wu, static_cast<const float*>(su), wd, static_cast<const float*>(sd), o.ptr(), l.T, l.E,
-         top, l.H, F, factor, flags, l.workspace, l.bytes, stream());
+    call_on(on, abi.moe_fp8, a.tensor(0).data_ptr(), a.tensor(1).data_ptr(), l.bias, wu, static_cast<const float*>(su), wd, static_cast<const float*>(sd), o.ptr(), l.T, l.E,
+         top, l.H, F, factor, flags, l.workspace, l.bytes, stream(on));
     return o.result();
 }
 

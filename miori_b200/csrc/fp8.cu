@@ -27,6 +27,7 @@ MIORI_API int miori_quant_fp8(const void* x, int64_t x_row, void* q, int64_t q_r
     if (!fine_pitch(x_row) || x_row < (int64_t)K || !fine_pitch(q_row) || q_row < (int64_t)K)
         return fail(MIORI_E_INVALID, "%s: a row pitch is shorter than its row, or too long (x_row=%lld q_row=%lld K=%u)", op, (long long)x_row, (long long)q_row, K);
     if (!fine_stride(scale_row) || !fine_stride(scale_col)) return fail(MIORI_E_INVALID, "%s: strides of the scales must be below 2^40", op);
+    if ((scale_row == 0 && (rows + tile - 1) / tile > 1) || (scale_col == 0 && K > BLOCK)) return fail(MIORI_E_INVALID, "%s: scales of several blocks would lie on one another", op);
     if (!aligned16(q) || q_row % 16) return fail(MIORI_E_INVALID, "%s: rows of q must begin on 16-byte boundaries", op);
     if ((reinterpret_cast<uintptr_t>(x) & (f32 ? 3u : 1u)) || (reinterpret_cast<uintptr_t>(scales) & 3u))
         return fail(MIORI_E_INVALID, "%s: x or scales is not aligned to its elements", op);

@@ -27,7 +27,7 @@ def test_quant_refuses_bad_arguments():
                        (lambda: quant(q_row=240), b"pitch"), (lambda: quant(q_row=264), b"16-byte"), (lambda: quant(q=OK + 8), b"16-byte"),
                        (lambda: quant(x=OK + 1), b"aligned"), (lambda: quant(x=OK + 2, flags=64), b"aligned"), (lambda: quant(s=OK + 2), b"aligned"),
                        (lambda: quant(x_row=1 << 41), b"pitch"), (lambda: quant(s_row=1 << 41), b"strides"), (lambda: quant(s_col=-(1 << 41)), b"strides"),
-                       (lambda: quant(rows=0x80000000), b"2^31"), (lambda: quant(rows=1 << 30, K=256), b"blocks")):
+                       (lambda: quant(s_row=0), b"on one another"), (lambda: quant(s_col=0), b"on one another"), (lambda: quant(rows=0x80000000), b"2^31"), (lambda: quant(rows=1 << 30, K=256), b"blocks")):
         refused(call, text)
 
 
@@ -141,3 +141,26 @@ def test_tensors_of_other_shapes_and_types():
     case(TypeError, "another type", ops.moe_fp8, "xb", "router", "up", "s", "down", "sd", 2, "ws")
     case(ValueError, "group", ops.moe4, "xb", "router", "q", "s", "s", "qd", "ds", "ds", 2, "ws", group=48)
     case(ValueError, "s_up", ops.moe4, "xb", "router", "q", "s", "s", "qd", "ds", "ds", 2, "ws")  # scales of groups of 64 where 32 are meant
+
+
+def test_tensors_of_several_devices():
+    """Refused before anything is launched."""
+    f = fakes()
+    from torch._subclasses import FakeTensorMode
+    with FakeTensorMode():
+        far = torch.empty((4, 256), dtype=torch.float8_e4m3fn, device="cuda:1")
+        far_ws, far_out = torch.empty(1 << 20, dtype=torch.uint8, device="cuda:1"), torch.empty((4, 2), device="cuda:1")
+    fp8 = [f[k] for k in ("up", "su", "down", "sd")]
+    for call in (lambda: ops.quant_fp8(f["x"], out=far), lambda: ops.quant_fp8(f["x"], out=f["a"], scales=far_out), lambda: ops.gemm_fp8(far, f["sa"], f["w"], f["sw"]),
+                 lambda: ops.moe_fp8(f["xb"], f["router"], *fp8, 2, far_ws)):
+        with pytest.raises((ValueError, RuntimeError), match="one device|storage"):
+            call()
+
+
+def test_weights_of_experts_are_contiguous():
+    f = fakes()
+    from torch._subclasses import FakeTensorMode
+    with FakeTensorMode():
+        turned = torch.empty((8, 256, 512), dtype=torch.float8_e4m3fn, device="cuda").transpose(1, 2)
+    with pytest.raises(ValueError, match="contiguous"):
+        ops.moe_fp8(f["xb"], f["router"], turned, f["su"], f["down"], f["sd"], 2, f["ws"])
