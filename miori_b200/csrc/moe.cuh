@@ -15,7 +15,8 @@
 //
 // Weights stream through a ring of cp.async stages that belongs to one warp: 16 rows x 128 bytes and their scales, no CTA-wide wait.  They become
 // fp16 without a rounding: 4-bit codes as subnormals in the bits of a half, e4m3 by conversion; products by mma.sync.m16n8k16, sums in fp32, times
-// the scales after each group.  What bounds the stream is less HBM than the number of instructions a stage takes: B fragments are made once
+// the scales after each group.  Experts of 2048 x 1536 in 4 bits, 4 of 32 a token: 18.3 us for one token, of which 3.3 are the bytes' and the rest latency; 55 for 32 (25.6); in e4m3, 8 of
+// 64 of 2048 x 768, 4 tokens: 38.5 (19).  What bounds the stream of many tokens is less HBM than the number of instructions a stage takes: B fragments are made once
 // a CTA and expert (moe_up) or once for several row tiles (moe_down), a row of activations has one power of two.
 // Activations, x and silu(g) * u, are fp16 times a power of two per row that puts its largest into [2^14, 2^15): bf16 x is not rounded down to
 // 2^-27 of that largest (4 bits) or 2^-31; silu(g) * u by 2^-11 of a value at most, an eighth of what rounding it to bf16 costs where
