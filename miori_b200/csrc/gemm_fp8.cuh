@@ -292,11 +292,12 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
                     if (lane == 0) mbar_arrive(taken(b));  // before the sums are used
                     if (++b == BUFS) b = 0u, b_parity ^= 1u;
                     const bool more = h + 1 < HALVES || kb + 1u < k_blocks;
+                    const bool there = mbar_test(summed(b), b_parity);  // asked for now, looked at when these sums have been added: an answer takes 100 cycles
                     const uint64_t s2 = pack2(__float_as_uint(scale[h]), __float_as_uint(scale[h]));
 #pragma unroll
                     for (int j = 0; j < 16; ++j) fma2(acc[h][j], pack2(r[0][2 * j], r[0][2 * j + 1]), s2);
                     if (more) {
-                        ok = warp_wait(summed(b), b_parity, &abort_flag, 0x74);
+                        if (!__all_sync(0xFFFFFFFFu, there)) ok = warp_wait(summed(b), b_parity, &abort_flag, 0x74);
                         if (!ok) return;
                         fence_after();
                         tmem_ld32(from + b * 128u, r[0]);
