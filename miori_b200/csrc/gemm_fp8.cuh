@@ -10,8 +10,8 @@
 //
 // Two kernels:
 //   pair   more than a hundred rows or so: 256 x 256 or 256 x 128 tiles on SM pairs (cta_group::2), persistent; each CTA pulls 32 KB a
-//          block through L2 for 512 cycles of its matrix unit, and takes some 650 for them.  16384 x 16384 x 2048: 572 us in a burst, 1.92 PFLOP/s
-//          (660 under the power limit); 1024 x 2048 x 8192: 20.4 us in a chain.
+//          block through L2 for 512 cycles of its matrix unit, and takes some 650 for them.  16384 x 16384 x 2048: 550 us in a burst, 2.0 PFLOP/s
+//          (624 under the power limit, which holds the clock at 1.58 GHz in the one and 1.39 in the other); 1024 x 2048 x 8192: 20.4 us in a chain.
 //   swap   few rows, or few tiles: 128 rows of w are the MMA's M, up to 128 rows of a its N; K is split over the CTAs of a
 //          cluster and the partial sums meet in distributed shared memory, in rank order.  8 x 16384 x 2048: 7.2 us, 4.7 TB/s; one row of 2048 x 2048: 3.4 us
 //          in a chain; 64 x 16384 x 2048: 10.2 us.
