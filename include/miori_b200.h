@@ -445,7 +445,8 @@ int miori_attention_prompt(const void* q, const void* k, const void* v, void* ou
 /* q = e4m3(x * (448 / a)), scale = a / 448, a = max(largest |x| of the block, 2^-100), each operation in fp32 and rounded
  * once.  tile: 1 or 128 rows a block.  x bf16 (fp32 with MIORI_QUANT_F32), rows x_row elements apart (whole 16 bytes, and x
  * 16-byte aligned, is the fast case).  A NaN stays one and does not count for the largest; a block with an infinity gets an infinite
- * scale.  What lies behind K in a row of q is left as it was. */
+ * scale.  What lies behind K in a row of q is left as it was; q and the scales may not lie on x, nor the scales of several blocks on
+ * one another. */
 int miori_quant_fp8(const void* x, int64_t x_row, void* q, int64_t q_row, float* scales, int64_t scale_row,
                     int64_t scale_col, uint32_t rows, uint32_t K, uint32_t tile, uint32_t flags, void* stream);
 /* C[m][n] (fp32, or bf16 with MIORI_OUT_BF16; rows ldc elements apart) = sum_b sa[m][b] sw[n / 128][b] sum_{k in block b} a[m][k]
