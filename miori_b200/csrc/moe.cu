@@ -25,9 +25,6 @@ static int launch_moe(const char* op, Args a, cudaStream_t stream) {
     const uint32_t most = sms * 8u / 9u / CLUSTER;
     a.per = (row_tiles + most - 1u) / most;
     a.by_tokens = Div::by(a.tokens), a.by_tiles = Div::by(a.F / 8u), a.by_ctas = Div::by(sms);
-    // Of the experts that T tokens choose `top` of, evenly, a share of about exp(-T top / E) is nobody's; less than a sixth, and their weights are asked for
-    // ahead: what HBM delivers while the router runs
-    a.guess = a.tokens * a.top * 5u >= a.experts * 9u ? GUESS : 0u;
     auto router = a.experts <= 32u ? moe_router_kernel<1> : a.experts <= 128u ? moe_router_kernel<4> : moe_router_kernel<8>;
     cudaError_t e = launch_cluster(router, ROUTER_CLUSTER, THREADS, (size_t)a.tokens * 1024u, ROUTER_CLUSTER, stream, a);
     if (e == cudaSuccess) e = launch(moe_up_kernel<FMT, DEPTH>, dim3(sms), dim3(THREADS), SMEM, stream, true, a);

@@ -32,7 +32,6 @@ constexpr uint32_t WARPS = 16, THREADS = WARPS * 32, CLUSTER = 4, ROUTER_CLUSTER
 constexpr uint32_t ENTRY = 8;   // tokens of an entry: the columns of an MMA tile
 constexpr uint32_t MAX_ENTRIES = MAX_EXPERTS + MAX_ROWS / ENTRY;
 constexpr size_t PREFETCH = 192 * 1024;  // bytes of down weights that a CTA of moe_up asks L2 for
-constexpr uint32_t GUESS = 320 * 1024;      // and of up weights, before the choice is known: what all CTAs' share of L2 holds beside them
 enum Format { GROUP64, GROUP32, E4M3 };
 
 // A unit of K is what 128 bytes of a row hold; a stage is a unit of 16 rows.
@@ -84,7 +83,6 @@ struct Args {
     uint32_t tokens, experts, top, H, F;
     uint32_t sigmoid, norm, bf16, ahead;  // ahead: weights may be read before the launch before is done
     Div by_tokens, by_tiles, by_ctas;  // tokens, F / 8, CTAs of moe_up
-    uint32_t guess;    // moe_up: bytes of up weights that a CTA asks L2 for before it knows the choice
     uint32_t slots;    // moe_up: entries whose B fragments shared memory takes
     uint32_t area;     // moe_down: bytes of partial sums
     uint32_t per;      // moe_down: row tiles of a cluster
@@ -612,11 +610,6 @@ moe_up_kernel(const Args a) {
     float4* const cells = reinterpret_cast<float4*>(smem + RING);  // two a warp
     const uint32_t frags = smem_addr(smem) + RING + 2u * WARPS * CELL;
 
-    // Where most experts will be somebody's choice, HBM need not wait for it: this CTA's share of all of them, a part of which may be for nothing.
-    if (a.guess && threadIdx.x == 0) {
-        const size_t all = (size_t)a.experts * a.up.rows * a.up.pitch, from = all / gridDim.x * blockIdx.x & ~(size_t)15;
-        ask(a.up.q, from, min(from + a.guess, all));
-    }
     pdl_wait_prior();
     pdl_launch_dependents();  // not sooner: moe_down reads the tables before its wait
     read_tables(a, tb);
