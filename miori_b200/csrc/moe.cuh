@@ -6,16 +6,17 @@
 //   moe_router  one cluster: logits, K over its CTAs and warps, the choice of each token, and the lists that the others work from;
 //   moe_up      the rows of all chosen experts' gate and up are dealt evenly to the CTAs, eight of each an MMA tile, and a CTA's tiles times K
 //               evenly to its warps; a tile that several warps share meets in shared memory.  silu(g) * u goes to the workspace
-//               in fp32, the largest of each row beside it.  At its end a CTA asks L2 for its share of the down weights;
+//               in fp32, the largest of each row beside it;
 //   moe_down    a cluster of four CTAs owns rows of the output.  The K axes of all experts, one behind the other, are dealt to its 64 warps,
 //               whose sums meet by token, times w, in a CTA and then over the cluster, always in the same order.
 // (As one cooperative launch with a meeting of the grid between the products, every CTA choosing for itself, a token took 23 us: such a meeting
-// costs 2.6, a launch's hand-over 0.7, a choice 2.)
+// costs 2.6, a launch's hand-over 0.7, a choice 2.  Weights asked of L2 ahead of their kernel, up's before the choice or down's at the end of moe_up, are nobody's gain
+// any more: 18.0 us for one token without, 18.6 with.)
 // Experts of more than eight tokens, the columns of an MMA tile, are listed once for every eight; L2 serves the second reading.
 //
 // Weights stream through a ring of cp.async stages that belongs to one warp: 16 rows x 128 bytes and their scales, no CTA-wide wait.  They become
 // fp16 without a rounding: 4-bit codes as subnormals in the bits of a half, e4m3 by conversion; products by mma.sync.m16n8k16, sums in fp32, times
-// the scales after each group.  Experts of 2048 x 1536 in 4 bits, 4 of 32 a token: 18.3 us for one token, of which 3.3 are the bytes' and the rest latency; 55 for 32 (25.6); in e4m3, 8 of
+// the scales after each group.  Experts of 2048 x 1536 in 4 bits, 4 of 32 a token: 18.0 us for one token, of which 3.3 are the bytes' and the rest latency; 54 for 32 (25.6); in e4m3, 8 of
 // 64 of 2048 x 768, 4 tokens: 38.5 (19).  What bounds the stream of many tokens is less HBM than the number of instructions a stage takes: B fragments are made once
 // a CTA and expert (moe_up) or once for several row tiles (moe_down), a row of activations has one power of two.
 // Activations, x and silu(g) * u, are fp16 times a power of two per row that puts its largest into [2^14, 2^15): bf16 x is not rounded down to
@@ -31,7 +32,6 @@ constexpr uint32_t MAX_TOKENS = 32, MAX_EXPERTS = 256, MAX_TOP = 16, MAX_ROWS = 
 constexpr uint32_t WARPS = 16, THREADS = WARPS * 32, CLUSTER = 4, ROUTER_CLUSTER = 8;
 constexpr uint32_t ENTRY = 8;   // tokens of an entry: the columns of an MMA tile
 constexpr uint32_t MAX_ENTRIES = MAX_EXPERTS + MAX_ROWS / ENTRY;
-constexpr size_t PREFETCH = 192 * 1024;  // bytes of down weights that a CTA of moe_up asks L2 for
 enum Format { GROUP64, GROUP32, E4M3 };
 
 // A unit of K is what 128 bytes of a row hold; a stage is a unit of 16 rows.
@@ -507,12 +507,6 @@ moe_router_kernel(const Args a) {
     for (uint32_t i = threadIdx.x; i < sizeof(Tables) / 16u; i += THREADS) reinterpret_cast<uint4*>(a.tables)[i] = reinterpret_cast<const uint4*>(&tb)[i];
 }
 
-// Asks L2 for bytes [from, to) of an array, from and to multiples of 16.
-__device__ __forceinline__ void ask(const uint8_t* p, size_t from, size_t to) {
-    for (; from < to; from += 16384u)
-        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p + from), "r"((uint32_t)min((size_t)16384u, to - from)) : "memory");
-}
-
 __device__ __forceinline__ void read_tables(const Args& a, Tables& tb) {
 #pragma unroll
     for (uint32_t i = threadIdx.x; i < sizeof(Tables) / 16u; i += THREADS) reinterpret_cast<uint4*>(&tb)[i] = ld_fresh(reinterpret_cast<const uint4*>(a.tables) + i);
@@ -728,15 +722,6 @@ moe_up_kernel(const Args a) {
             first = false;
             tot[0] = tot[1] = tot[2] = tot[3] = 0.0f;
             if (unit == units) ++item, unit = 0u, whole = true;
-        }
-        if (to == i1 && warp == 0 && lane == 0) {
-            // this CTA's share of the down weights, on their way to L2 while the sums meet: an entry's expert's, in pieces
-            const uint32_t expert = a.down.rows * a.down.pitch;
-            const size_t all = (size_t)expert * tb.entries, from_byte = all / gridDim.x * blockIdx.x & ~(size_t)15;
-            const uint32_t entry = (uint32_t)(from_byte / expert), offset = (uint32_t)(from_byte - (size_t)entry * expert);
-            const uint32_t bytes = (uint32_t)min(PREFETCH, all / gridDim.x) & ~15u, here = min(bytes, expert - offset);
-            ask(a.down.q + (size_t)tb.entry_expert[entry] * expert, offset, offset + here);
-            if (here < bytes && entry + 1u < tb.entries) ask(a.down.q + (size_t)tb.entry_expert[entry + 1u] * expert, 0, min(bytes - here, expert));
         }
         __syncthreads();
         // a tile that goes on beyond the end of the warp that began it: that warp adds up the others' cells, their first ones
