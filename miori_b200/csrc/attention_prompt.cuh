@@ -338,7 +338,6 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     const uint32_t s_free = bar(4 * ST + 10);                          // D = 128: S has been loaded
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
 
-    pdl_launch_dependents();
     if (threadIdx.x == 0) {
         abort_flag = 0u;
         for (uint32_t i = 0; i < ST; ++i) mbar_init(full(i), 1), mbar_init(empty(i), 1), mbar_init(raw(i), 1), mbar_init(checked(i), 2);
@@ -354,6 +353,7 @@ attention_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     if (warp == 9) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&tmem_slot)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        pdl_launch_dependents();  // with its columns in hand
     }
     pdl_wait_prior();
     const uint32_t group = a.group, per_tile = ROW_TILE / group, per_item = 2u * per_tile;

@@ -136,6 +136,8 @@ __device__ __forceinline__ void device_error(unsigned code, unsigned d0, unsigne
 }
 
 // Programmatic dependent launch controls (no-ops when the launch is not programmatic).
+// A kernel with tensor memory lets its dependents start from the warp that allocates, after it has: a dependent that took the columns first would keep them
+// until this grid is done, and an allocation that waits for them has no limit.
 __device__ __forceinline__ void pdl_launch_dependents() {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }

@@ -168,7 +168,6 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     const uint32_t m_tiles = (g.M + 255u) / 256u, n_tiles = (g.N + BN - 1u) / BN, tiles = m_tiles * n_tiles;
     const uint32_t k_blocks = (g.K + KB_BYTES - 1u) / KB_BYTES;
 
-    pdl_launch_dependents();
     if (threadIdx.x == 0) {
         abort_flag = 0u;
         for (int s = 0; s < STAGES; ++s) mbar_init(full(s), 1), mbar_init(empty(s), HALVES);
@@ -181,6 +180,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        pdl_launch_dependents();  // with its columns in hand
     }
     fence_before();
     __syncthreads();
@@ -418,7 +418,6 @@ gemm_fp8_swap_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     const uint32_t k_blocks = (g.K + KB_BYTES - 1u) / KB_BYTES;
     const uint32_t kb0 = rank * k_blocks / geo.cs, nkb = (rank + 1u) * k_blocks / geo.cs - kb0;
 
-    pdl_launch_dependents();
     if (threadIdx.x == 0) {
         abort_flag = 0u;
         for (uint32_t s = 0; s < geo.stages; ++s) mbar_init(full(s), 1), mbar_init(empty(s), 1);
@@ -428,6 +427,7 @@ gemm_fp8_swap_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)), "r"(TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        pdl_launch_dependents();  // with its columns in hand
     }
     fence_before();
     __syncthreads();

@@ -71,7 +71,6 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
     const uint32_t k_blocks = (g.K + BK - 1) / BK;  // TMA zero-fills a ragged last block
     const uint32_t kb0 = rank * k_blocks / g.cs, nkb = (rank + 1u) * k_blocks / g.cs - kb0;
 
-    pdl_launch_dependents();
     if (threadIdx.x == 0) {
         abort_flag = 0u;
         for (uint32_t s = 0; s < g.stages; ++s) {
@@ -90,6 +89,7 @@ gemm_skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                      ::"r"(smem_addr(&tmem_base_slot)), "r"(g.tmem_cols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        pdl_launch_dependents();  // with its columns in hand
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();

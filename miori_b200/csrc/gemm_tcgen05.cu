@@ -199,8 +199,6 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a,
     const uint32_t tiles = m_blocks * n_blocks * splits;
     const uint32_t k_blocks = (K + BK - 1) / BK;  // TMA zero-fills a ragged last block
 
-    pdl_launch_dependents();
-
     if (threadIdx.x == 0) {
         abort_flag = 0u;
         for (int s = 0; s < C::STAGES; ++s) {
@@ -221,6 +219,7 @@ gemm_bf16_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_a,
                      ::"r"(smem_addr(&tmem_base_slot)), "r"((uint32_t)C::TMEM_COLS)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        pdl_launch_dependents();  // with its columns in hand
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -430,8 +429,6 @@ gemm_bf16_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap tmap_a,
     const uint32_t tiles = m_blocks * n_blocks * splits;
     const uint32_t k_blocks = (K + BK - 1) / BK;  // TMA zero-fills a ragged last block
 
-    pdl_launch_dependents();
-
     if (threadIdx.x == 0) {
         abort_flag = 0u;
         for (int s = 0; s < STAGES; ++s) {
@@ -452,6 +449,7 @@ gemm_bf16_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap tmap_a,
                      ::"r"(smem_addr(&tmem_base_slot)), "r"((uint32_t)TMEM_COLS)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        pdl_launch_dependents();  // with its columns in hand
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();

@@ -1,0 +1,40 @@
+"""What the kernels with tensor memory owe one another and cannot show by running: an allocation waits without a limit, and tensor memory that another
+CTA's MMAs write is handed over by barriers.  Read from the sources."""
+import glob
+import os
+import re
+
+import pytest
+
+from conftest import ROOT
+
+CSRC = os.path.join(ROOT, "miori_b200", "csrc")
+
+
+def code(path):
+    return re.sub(r"//[^\n]*", "", open(path).read())
+
+
+def kernels():
+    """(name, body) of every kernel that allocates tensor memory."""
+    found = []
+    for path in sorted(glob.glob(os.path.join(CSRC, "*.cu")) + glob.glob(os.path.join(CSRC, "*.cuh"))):
+        for part in code(path).split("__global__")[1:]:
+            if "tcgen05.alloc" in part:
+                found.append((re.search(r"(\w+_kernel)\(", part).group(1), part))
+    return found
+
+
+def test_they_are_found():
+    assert {name for name, _ in kernels()} >= {"gemm_fp8_pair_kernel", "gemm_fp8_swap_kernel", "gemm_skinny_kernel", "attention_prompt_kernel"}
+    assert len(kernels()) >= 6
+
+
+@pytest.mark.parametrize("name,body", kernels(), ids=[name for name, _ in kernels()])
+def test_dependents_start_behind_the_allocation(name, body):
+    """A dependent grid may take an SM's free columns as soon as it is let go, and keeps them until this grid is done: a CTA that has yet to allocate would wait for it, and
+    it for the CTA.  One warp allocates and then lets go, and nobody else does."""
+    assert body.count("pdl_launch_dependents") == 1 and body.count("tcgen05.alloc") == 1
+    assert body.index("tcgen05.alloc") < body.index("pdl_launch_dependents")
+    between = body[body.index("tcgen05.alloc"):body.index("pdl_launch_dependents")]
+    assert "}" not in re.sub(r'"[^"]*"', "", between), "in the allocating warp's own block"
