@@ -38,3 +38,17 @@ def test_dependents_start_behind_the_allocation(name, body):
     assert body.index("tcgen05.alloc") < body.index("pdl_launch_dependents")
     between = body[body.index("tcgen05.alloc"):body.index("pdl_launch_dependents")]
     assert "}" not in re.sub(r'"[^"]*"', "", between), "in the allocating warp's own block"
+
+
+def test_hand_overs_between_ctas_are_released_and_acquired_by_the_cluster():
+    """The second CTA of a pair tells the leader that its sums are read, and the leader's MMAs write over them: an arrival that releases nothing, or a wait
+    whose scope ends at its own CTA, orders neither."""
+    fp8 = code(os.path.join(CSRC, "gemm_fp8.cuh"))
+    remote = re.findall(r"mapa\.shared::cluster\.u32 ra.*?\[ra\]", fp8)
+    assert remote and all("mbarrier.arrive.release.cluster" in a for a in remote)
+    assert "warp_wait<true>(taken(b)" in fp8  # the leader's
+    relay = fp8[:fp8.index("arrive_leader(taken(b))")].rsplit("mbar_wait(taken(b)", 1)[1]
+    assert "fence_after();" in relay and "fence_before();" in relay
+    assert "mbar_wait<true, true>(smem_addr(&arrived)" in code(os.path.join(CSRC, "moe.cuh"))  # sums that other CTAs store
+    wait = code(os.path.join(CSRC, "common.cuh"))
+    assert wait.count("mbarrier.try_wait.parity.acquire.cluster") == 2
