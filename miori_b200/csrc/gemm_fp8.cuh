@@ -380,6 +380,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
         const long long t0 = clock64();
         while (clock64() - t0 < 2000000LL) __nanosleep(1000);
     }
+    __syncwarp();
     fence_before();
     __syncthreads();
     cluster_barrier();  // the other CTA may still signal this one's barriers or read its shared memory
@@ -485,6 +486,7 @@ gemm_fp8_swap_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
             if (m < g.M) v = __fmul_rn(ld_fresh(g.sa + (int64_t)m * g.sa_row + (int64_t)(kb0 + kb) * g.sa_col), ld_fresh(sw + (int64_t)kb * g.sw_col));
             asm volatile("st.shared.f32 [%0], %1;" ::"r"(scales + i * 4u), "f"(v) : "memory");
         }
+        __syncwarp();
         asm volatile("bar.sync 1, 128;" ::: "memory");
 #pragma unroll
         for (int j = 0; j < MP; ++j) acc[j] = 0.0f;
@@ -560,12 +562,14 @@ gemm_fp8_swap_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
             }
         }
     }
+    __syncwarp();  // lanes leave the stores at different times, and the barrier is one of whole warps
     if (geo.cs > 1u) cluster_barrier();  // nobody leaves while its sums are read
 
     if (abort_flag) {
         const long long t0 = clock64();
         while (clock64() - t0 < 2000000LL) __nanosleep(1000);
     }
+    __syncwarp();
     fence_before();
     __syncthreads();
     if (warp == 1) {

@@ -52,3 +52,20 @@ def test_hand_overs_between_ctas_are_released_and_acquired_by_the_cluster():
     assert "mbar_wait<true, true>(smem_addr(&arrived)" in code(os.path.join(CSRC, "moe.cuh"))  # sums that other CTAs store
     wait = code(os.path.join(CSRC, "common.cuh"))
     assert wait.count("mbarrier.try_wait.parity.acquire.cluster") == 2
+
+
+def test_whole_warps_come_to_barriers_of_whole_warps():
+    """barrier.cluster and bar.sync in their aligned forms take warps whose lanes are together.  Behind code whose lanes part, a loop over columns or one that leaves at an abort,
+    they are brought together first."""
+    fp8 = code(os.path.join(CSRC, "gemm_fp8.cuh"))
+    swap = fp8[fp8.index("gemm_fp8_swap_kernel("):fp8.index("struct GemmOperands")]
+    barriers = [m.start() for m in re.finditer(r"if \(geo\.cs > 1u\) cluster_barrier\(\);|asm volatile\(\"bar\.sync 1, 128;", swap)]
+    assert len(barriers) == 4
+    for at in barriers:
+        before = [line.strip() for line in swap[:at].splitlines() if line.strip()]
+        # ... or nothing lies between it and such a place but stores that every lane makes
+        tail = "\n".join(before[-9:])
+        assert "__syncwarp();" in tail and "continue" not in tail.rsplit("__syncwarp();", 1)[1] and "break" not in tail.rsplit("__syncwarp();", 1)[1], tail
+    for part in (fp8[:fp8.index("gemm_fp8_swap_kernel(")], swap):
+        leaving = part[part.index("__nanosleep"):]
+        assert leaving.index("__syncwarp();") < leaving.index("__syncthreads();")
