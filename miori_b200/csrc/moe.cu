@@ -14,12 +14,21 @@ constexpr size_t SMEM = 227 * 1024 - (sizeof(Tables) + 32 + 127) / 128 * 128;
 template <Format FMT>
 constexpr size_t frag_room(int depth) { return SMEM - Stage<FMT>::ring(depth) - 2 * WARPS * 512; }
 
+// Of moe_down, were there as many entries as there can be: cells of one row tile for every warp, and the cluster's sums of one.
+constexpr uint32_t most_segments(uint32_t most_units) {
+    uint32_t most = 0;
+    for (uint32_t units = 1; units <= most_units; ++units)
+        if (segments_of(MAX_ENTRIES * units, units) > most) most = segments_of(MAX_ENTRIES * units, units);
+    return most;
+}
+template <Format FMT>
+constexpr uint32_t ONE_TILE = WARPS * 512u * most_segments(MAX_FF / Stage<FMT>::UNIT) + CLUSTER * MAX_TOKENS * 64u;
+
 template <Format FMT, int DEPTH>
 static int launch_moe(const char* op, Args a, cudaStream_t stream) {
     a.slots = (uint32_t)(frag_room<FMT>(DEPTH) / ((size_t)a.up.units * Stage<FMT>::FRAG));
     a.area = (uint32_t)(SMEM - Stage<FMT>::ring(Stage<FMT>::DOWN));
-    static_assert(SMEM - Stage<FMT>::ring(Stage<FMT>::DOWN) >= WARPS * 512u * ((MAX_ENTRIES + CLUSTER * WARPS - 1) / (CLUSTER * WARPS)) + 4u * MAX_TOKENS * 64u,
-                  "cells of a row tile, were every entry one unit, and the cluster's sums");
+    static_assert(SMEM - Stage<FMT>::ring(Stage<FMT>::DOWN) >= ONE_TILE<FMT>, "moe_down works on one row tile at a time at least");
     const uint32_t sms = (uint32_t)sm_count(), row_tiles = a.H / 16u;
     // clusters of four whole SMs: an SM in nine has no place in one
     const uint32_t most = sms * 8u / 9u / CLUSTER;
@@ -55,7 +64,7 @@ static int check_common(const char* op, const void* x, const void* router, const
     if (top == 0 || top > MAX_TOP || top > experts) return fail(MIORI_E_INVALID, "%s: 1..%u of %u experts for a token, got %u", op, MAX_TOP, experts, top);
     if (hidden == 0 || ff == 0 || hidden % step || ff % step)
         return fail(MIORI_E_INVALID, "%s: hidden and ff are multiples of %u, got %u and %u", op, step, hidden, ff);
-    if (hidden > MAX_HIDDEN || ff > 65536u) return fail(MIORI_E_INVALID, "%s: hidden is at most %u and ff 65536, got %u and %u", op, MAX_HIDDEN, hidden, ff);
+    if (hidden > MAX_HIDDEN || ff > MAX_FF) return fail(MIORI_E_INVALID, "%s: hidden is at most %u and ff %u, got %u and %u", op, MAX_HIDDEN, MAX_FF, hidden, ff);
     if (!std::isfinite(factor)) return fail(MIORI_E_INVALID, "%s: the factor must be finite", op);
     if (!aligned16(x) || !aligned16(router) || !aligned16(out) || !aligned16(workspace) || (reinterpret_cast<uintptr_t>(bias) & 3u))
         return fail(MIORI_E_INVALID, "%s: x, router, out and workspace must be 16-byte aligned, bias by its elements", op);

@@ -28,10 +28,16 @@
 namespace miori_b200 {
 namespace moe {
 
-constexpr uint32_t MAX_TOKENS = 32, MAX_EXPERTS = 256, MAX_TOP = 16, MAX_ROWS = MAX_TOKENS * MAX_TOP, MAX_HIDDEN = 7168;
+constexpr uint32_t MAX_TOKENS = 32, MAX_EXPERTS = 256, MAX_TOP = 16, MAX_ROWS = MAX_TOKENS * MAX_TOP, MAX_HIDDEN = 7168, MAX_FF = 65536;
 constexpr uint32_t WARPS = 16, THREADS = WARPS * 32, CLUSTER = 4, ROUTER_CLUSTER = 8;
 constexpr uint32_t ENTRY = 8;   // tokens of an entry: the columns of an MMA tile
 constexpr uint32_t MAX_ENTRIES = MAX_EXPERTS + MAX_ROWS / ENTRY;
+constexpr uint32_t WORKERS = CLUSTER * WARPS;  // warps of moe_down that share the entries' units
+// The most entries that one of them meets: its units are neighbours, and may begin with an entry's last.
+__host__ __device__ constexpr uint32_t segments_of(uint32_t all_units, uint32_t units) {
+    const uint32_t mine = (all_units + WORKERS - 1u) / WORKERS;
+    return ((mine ? mine : 1u) + units - 2u) / units + 1u;
+}
 enum Format { GROUP64, GROUP32, E4M3 };
 
 // A unit of K is what 128 bytes of a row hold; a stage is a unit of 16 rows.
@@ -745,7 +751,6 @@ template <Format FMT>
 __global__ void __launch_bounds__(THREADS, 1)
 moe_down_kernel(const Args a) {
     using S = Stage<FMT>;
-    constexpr uint32_t WORKERS = CLUSTER * WARPS;
     constexpr int DEPTH = S::DOWN;
     constexpr uint32_t RING = S::ring(DEPTH);
     extern __shared__ __align__(128) uint8_t smem[];
@@ -769,7 +774,7 @@ moe_down_kernel(const Args a) {
     // warp w of the cluster has the units [all w / 64, all (w + 1) / 64)
     const uint32_t worker = rank * WARPS + warp, u0 = all_units * worker / WORKERS, u1 = all_units * (worker + 1u) / WORKERS;
     // partial sums: a cell for each entry that a warp meets and each row tile of a pass
-    const uint32_t segments = (max((all_units + WORKERS - 1u) / WORKERS, 1u) + units - 2u) / units + 1u;
+    const uint32_t segments = segments_of(all_units, units);
     const uint32_t out_tile = a.tokens * 64u;  // bytes of a CTA's sums of a row tile, [token][16 rows]
     // in front of the cells: the four CTAs' sums of this one's tiles, every fourth of a pass
     uint32_t at_once = min(a.per, a.area / (WARPS * segments * 512u + out_tile));
