@@ -59,9 +59,9 @@ __device__ __forceinline__ void commit_one(uint32_t bar) {
 __device__ __forceinline__ void commit_both(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
 }
-// For the pair's leader to see what this CTA's warps have done, it is released, and there acquired, at the cluster's scope.
+// Hands over tensor memory and nothing else: behind fence_before, and waited for with Order TENSOR in front of fence_after.
 __device__ __forceinline__ void arrive_leader(uint32_t bar) {
-    asm volatile("{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %0, 0;\n\tmbarrier.arrive.release.cluster.shared::cluster.b64 _, [ra];\n\t}" ::"r"(bar) : "memory");
+    asm volatile("{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %0, 0;\n\tmbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [ra];\n\t}" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void load_pair(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
@@ -106,10 +106,10 @@ __device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
     return v;
 }
 // mbar_wait by a whole warp, with one answer for it.  (By one lane, that tells the others: 100 cycles more a wait.)
-template <bool CLUSTER = false>
+template <Order O = OWN>
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile uint32_t* abort, uint32_t where) {
-    if (__all_sync(0xFFFFFFFFu, mbar_try<CLUSTER>(bar, parity))) return true;
-    return __all_sync(0xFFFFFFFFu, mbar_wait<false, CLUSTER>(bar, parity, abort, where));
+    if (__all_sync(0xFFFFFFFFu, mbar_try<O>(bar, parity))) return true;
+    return __all_sync(0xFFFFFFFFu, mbar_wait<false, O>(bar, parity, abort, where));
 }
 __device__ __forceinline__ bool elect_one() {
     uint32_t one;
@@ -233,7 +233,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             bool ok = true;
             for (uint32_t t = pair; t < tiles && ok; t += pairs) {
                 for (uint32_t kb = 0; kb < k_blocks; ++kb) {
-                    if (!(ok = warp_wait<true>(taken(b), b_parity, &abort_flag, 0x72))) break;
+                    if (!(ok = warp_wait<TENSOR>(taken(b), b_parity, &abort_flag, 0x72))) break;
                     if (!(ok = warp_wait(full(s), parity, &abort_flag, 0x73))) break;
                     fence_after();
                     if (elect_one()) {

@@ -40,18 +40,19 @@ def test_dependents_start_behind_the_allocation(name, body):
     assert "}" not in re.sub(r'"[^"]*"', "", between), "in the allocating warp's own block"
 
 
-def test_hand_overs_between_ctas_are_released_and_acquired_by_the_cluster():
-    """The second CTA of a pair tells the leader that its sums are read, and the leader's MMAs write over them: an arrival that releases nothing, or a wait
-    whose scope ends at its own CTA, orders neither."""
+def test_hand_overs_between_ctas():
+    """The second CTA of a pair tells the leader that its sums are read, and the leader's MMAs write over them.  Of tensor memory: fences on either side of a barrier whose
+    arrival and wait reach over the cluster, in the thread that passes the word on too.  Sums in shared memory: released, and acquired, by the cluster."""
     fp8 = code(os.path.join(CSRC, "gemm_fp8.cuh"))
     remote = re.findall(r"mapa\.shared::cluster\.u32 ra.*?\[ra\]", fp8)
-    assert remote and all("mbarrier.arrive.release.cluster" in a for a in remote)
-    assert "warp_wait<true>(taken(b)" in fp8  # the leader's
+    assert remote and all("mbarrier.arrive.relaxed.cluster" in a for a in remote)
     relay = fp8[:fp8.index("arrive_leader(taken(b))")].rsplit("mbar_wait(taken(b)", 1)[1]
-    assert "fence_after();" in relay and "fence_before();" in relay
-    assert "mbar_wait<true, true>(smem_addr(&arrived)" in code(os.path.join(CSRC, "moe.cuh"))  # sums that other CTAs store
+    assert relay.index("fence_after();") < relay.index("fence_before();")
+    leader = fp8[fp8.index("warp_wait<TENSOR>(taken(b)"):]
+    assert leader.index("fence_after();") < leader.index("umma_e4m3<2>")
     wait = code(os.path.join(CSRC, "common.cuh"))
-    assert wait.count("mbarrier.try_wait.parity.acquire.cluster") == 2
+    assert wait.count("mbarrier.try_wait.parity.relaxed.cluster") == 1 and wait.count("mbarrier.try_wait.parity.acquire.cluster") == 1
+    assert "mbar_wait<true, miori_b200::CLUSTER>(smem_addr(&arrived)" in code(os.path.join(CSRC, "moe.cuh"))
 
 
 def test_whole_warps_come_to_barriers_of_whole_warps():
