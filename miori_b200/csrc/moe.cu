@@ -10,7 +10,8 @@ namespace moe {
 constexpr size_t TOPS_BYTES = MAX_ROWS * sizeof(uint32_t), HEAD_BYTES = (sizeof(Tables) + TOPS_BYTES + 255) / 256 * 256;
 
 // Dynamic shared memory of both products: all of an SM's that the tables leave, a ring and B fragments or partial sums in the rest.
-constexpr size_t SMEM = 227 * 1024 - (sizeof(Tables) + 32 + 127) / 128 * 128;
+static_assert(sizeof(UpTables) <= sizeof(DownTables), "");
+constexpr size_t SMEM = 227 * 1024 - (sizeof(DownTables) + 32 + 127) / 128 * 128;
 template <Format FMT>
 constexpr size_t frag_room(int depth) { return SMEM - Stage<FMT>::ring(depth) - 2 * WARPS * 512; }
 
@@ -18,7 +19,7 @@ constexpr size_t frag_room(int depth) { return SMEM - Stage<FMT>::ring(depth) - 
 constexpr uint32_t most_segments(uint32_t most_units) {
     uint32_t most = 0;
     for (uint32_t units = 1; units <= most_units; ++units)
-        if (segments_of(MAX_ENTRIES * units, units) > most) most = segments_of(MAX_ENTRIES * units, units);
+        if (segments_of(MAX_DOWN_ENTRIES * units, units) > most) most = segments_of(MAX_DOWN_ENTRIES * units, units);
     return most;
 }
 template <Format FMT>

@@ -12,7 +12,8 @@
 // (As one cooperative launch with a meeting of the grid between the products, every CTA choosing for itself, a token took 23 us: such a meeting
 // costs 2.6, a launch's hand-over 0.7, a choice 2.  Weights asked of L2 ahead of their kernel, up's before the choice or down's at the end of moe_up, are nobody's gain
 // any more: 18.0 us for one token without, 18.6 with.)
-// Experts of more than eight tokens, the columns of an MMA tile, are listed once for every eight; L2 serves the second reading.
+// An MMA tile has eight columns: moe_up's are eight tokens, moe_down's four, each twice (below).  An expert of more tokens is listed, and read, once for every
+// eight or four of them; L2 serves the further readings.
 //
 // Weights stream through a ring of cp.async stages that belongs to one warp: 16 rows x 128 bytes and their scales, no CTA-wide wait.  They become
 // fp16 without a rounding: 4-bit codes as subnormals in the bits of a half, e4m3 by conversion; products by mma.sync.m16n8k16, sums in fp32, times
@@ -20,8 +21,8 @@
 // 64 of 2048 x 768, 4 tokens: 38.5 (19).  What bounds the stream of many tokens is less HBM than the number of instructions a stage takes: B fragments are made once
 // a CTA and expert (moe_up) or once for several row tiles (moe_down), a row of activations has one power of two.
 // Activations, x and silu(g) * u, are fp16 times a power of two per row that puts its largest into [2^14, 2^15): bf16 x is not rounded down to
-// 2^-27 of that largest (4 bits) or 2^-31; silu(g) * u by 2^-11 of a value at most, an eighth of what rounding it to bf16 costs where
-// gate + up and down are two calls.
+// 2^-27 of that largest (4 bits) or 2^-31.  silu(g) * u, fp32, is a pair of fp16, a value and what it has beyond that, in two columns of one tile: 2^-22 of a value at most, where one
+// fp16 would be off by 2^-11.
 #pragma once
 #include "common.cuh"
 
@@ -30,8 +31,10 @@ namespace moe {
 
 constexpr uint32_t MAX_TOKENS = 32, MAX_EXPERTS = 256, MAX_TOP = 16, MAX_ROWS = MAX_TOKENS * MAX_TOP, MAX_HIDDEN = 7168, MAX_FF = 65536;
 constexpr uint32_t WARPS = 16, THREADS = WARPS * 32, CLUSTER = 4, ROUTER_CLUSTER = 8;
-constexpr uint32_t ENTRY = 8;   // tokens of an entry: the columns of an MMA tile
-constexpr uint32_t MAX_ENTRIES = MAX_EXPERTS + MAX_ROWS / ENTRY;
+// Tokens of an entry: the columns of an MMA tile, of which moe_down takes two a token.
+constexpr uint32_t UP_ENTRY = 8, DOWN_ENTRY = 4;
+constexpr uint32_t most_entries(uint32_t of) { return MAX_EXPERTS + (MAX_ROWS - MAX_EXPERTS) / of; }  // every expert one, and one more for every `of` rows beyond
+constexpr uint32_t MAX_UP_ENTRIES = most_entries(UP_ENTRY), MAX_DOWN_ENTRIES = most_entries(DOWN_ENTRY);
 constexpr uint32_t WORKERS = CLUSTER * WARPS;  // warps of moe_down that share the entries' units
 // The most entries that one of them meets: its units are neighbours, and may begin with an entry's last.
 __host__ __device__ constexpr uint32_t segments_of(uint32_t all_units, uint32_t units) {
@@ -64,18 +67,24 @@ struct Matrix {  // [experts][rows][K]
     uint32_t pitch, scale_pitch;  // bytes of a row of q, of a row of s and b
     uint32_t whole;               // rows are whole units
 };
-struct Tables {
-    uint32_t mask[MAX_EXPERTS];       // tokens that chose the expert
-    uint16_t entry_of[MAX_EXPERTS];   // its first entry
-    uint16_t entry_expert[MAX_ENTRIES], entry_row[MAX_ENTRIES + 2];
-    int32_t chosen[MAX_ROWS];         // [token][place], -1: nobody
-    float weight[MAX_ROWS];
-    uint16_t slot[MAX_ROWS];          // of a place: entry * 8 + column of the entry
+// What moe_router tells the products.
+struct alignas(16) UpTables {
+    uint16_t entry_expert[MAX_UP_ENTRIES], entry_row[MAX_UP_ENTRIES + 2];
     uint8_t row_token[MAX_ROWS];
     uint32_t x_top[MAX_TOKENS];       // the largest |x| of a token, as bits
-    uint32_t entries, pad[2];
+    uint32_t entries;
 };
-static_assert(sizeof(Tables) % 16 == 0, "copied by 16 bytes");
+struct alignas(16) DownTables {
+    uint16_t entry_expert[MAX_DOWN_ENTRIES], entry_row[MAX_DOWN_ENTRIES + 2];
+    int32_t chosen[MAX_ROWS];         // [token][place], -1: nobody
+    float weight[MAX_ROWS];
+    uint16_t slot[MAX_ROWS];          // of a place: entry * 4 + its token's number in the entry
+    uint32_t entries;
+};
+struct Tables {
+    UpTables up;
+    DownTables down;
+};
 
 struct Args {
     const uint16_t *x, *router;
@@ -177,21 +186,29 @@ __device__ __forceinline__ uint32_t scale_field(uint32_t top) { return min(268u 
 __device__ __forceinline__ float scale_up(uint32_t top) { return __uint_as_float(scale_field(top) << 23); }
 __device__ __forceinline__ float scale_down(uint32_t top) { return __uint_as_float((254u - scale_field(top)) << 23); }
 
-// B fragments of eight columns and one unit.  v: the thread's 32 elements of column g, in pieces; up: the column's power of two.
-template <Format FMT>
-__device__ __forceinline__ void make_frag(uint32_t (&b)[16], const float (&v)[32], float up) {
+// Two numbers as fp16, or what they have beyond that: exactly, before it is rounded itself.  Not two paths: a warp's lanes want both.
+__device__ __forceinline__ uint32_t pack_part(float lo, float hi, bool rest) {
+    const uint32_t w = pack_half(lo, hi);
+    float l, h;
+    asm("{\n\t.reg .f16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}" : "=f"(l), "=f"(h) : "r"(w));
+    const uint32_t r = pack_half(lo - l, hi - h);
+    return rest ? r : w;
+}
+// B fragments of eight columns and one unit.  v: the thread's 32 elements of column g, in pieces; up: the column's power of two; pack: makes fp16 of two.
+template <Format FMT, class P>
+__device__ __forceinline__ void make_frag(uint32_t (&b)[16], const float (&v)[32], float up, P pack) {
     if constexpr (FMT == E4M3) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) b[i] = pack_half(v[2 * i] * up, v[2 * i + 1] * up);
+        for (int i = 0; i < 16; ++i) b[i] = pack(v[2 * i] * up, v[2 * i + 1] * up);
     } else {
         // word i, codes 0..7: codes (0, 4) and (2, 6) are taken as multiples of 2^-24, (1, 5) and (3, 7) of 2^-20
         const float up16 = up * 0.0625f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            b[4 * i] = pack_half(v[8 * i] * up, v[8 * i + 4] * up);
-            b[4 * i + 1] = pack_half(v[8 * i + 1] * up16, v[8 * i + 5] * up16);
-            b[4 * i + 2] = pack_half(v[8 * i + 2] * up, v[8 * i + 6] * up);
-            b[4 * i + 3] = pack_half(v[8 * i + 3] * up16, v[8 * i + 7] * up16);
+            b[4 * i] = pack(v[8 * i] * up, v[8 * i + 4] * up);
+            b[4 * i + 1] = pack(v[8 * i + 1] * up16, v[8 * i + 5] * up16);
+            b[4 * i + 2] = pack(v[8 * i + 2] * up, v[8 * i + 6] * up);
+            b[4 * i + 3] = pack(v[8 * i + 3] * up16, v[8 * i + 7] * up16);
         }
     }
 }
@@ -317,10 +334,16 @@ __device__ __forceinline__ uint32_t remote(uint32_t addr, uint32_t rank) {
     return a;
 }
 
-// The choice of one token by one warp.  logit(e): the token's logit of expert e.  The results go to the tables of the cluster's first CTA.
+// What only moe_router works with.
+struct Lists {
+    Tables to;
+    uint32_t mask[MAX_EXPERTS];      // tokens that chose the expert
+    uint16_t entry_of[MAX_EXPERTS];  // its first entry of moe_down
+};
+// The choice of one token by one warp.  logit(e): the token's logit of expert e.  The results go to the lists of the cluster's first CTA.
 // PER: experts of a lane.
 template <int PER, class L>
-__device__ __forceinline__ void choose(const Args& a, Tables& tb, uint32_t token, uint32_t lane, L logit) {
+__device__ __forceinline__ void choose(const Args& a, Lists& lists, uint32_t token, uint32_t lane, L logit) {
     float l[PER], r[PER];
     uint32_t key[PER];
     float most = -INFINITY, total = 0.0f;
@@ -379,33 +402,40 @@ __device__ __forceinline__ void choose(const Args& a, Tables& tb, uint32_t token
     }
     if (lane < a.top) {
         const uint32_t at = token * a.top + lane;
-        asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(remote(smem_addr(&tb.chosen[at]), 0)), "r"(expert) : "memory");
-        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote(smem_addr(&tb.weight[at]), 0)), "f"(p / sum * a.factor) : "memory");
-        if (expert >= 0) asm volatile("red.relaxed.cluster.shared::cluster.or.b32 [%0], %1;" ::"r"(remote(smem_addr(&tb.mask[expert]), 0)), "r"(1u << token) : "memory");
+        asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(remote(smem_addr(&lists.to.down.chosen[at]), 0)), "r"(expert) : "memory");
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote(smem_addr(&lists.to.down.weight[at]), 0)), "f"(p / sum * a.factor) : "memory");
+        if (expert >= 0) asm volatile("red.relaxed.cluster.shared::cluster.or.b32 [%0], %1;" ::"r"(remote(smem_addr(&lists.mask[expert]), 0)), "r"(1u << token) : "memory");
     }
 }
 
-// Entries: the chosen experts in order, one for every eight of their tokens.  By one warp.
-__device__ __forceinline__ void list_entries(const Args& a, Tables& tb, uint32_t lane) {
-    uint32_t entry = 0, row = 0;
+// Entries: the chosen experts in order, one for every eight of their tokens (moe_up) and every four (moe_down).  By one warp.
+__device__ __forceinline__ void list_entries(const Args& a, Lists& lists, uint32_t lane) {
+    UpTables& up = lists.to.up;
+    DownTables& down = lists.to.down;
+    uint32_t up_entry = 0, down_entry = 0, row = 0;
     for (uint32_t e0 = 0; e0 < a.experts; e0 += 32u) {
-        const uint32_t e = e0 + lane, count = e < a.experts ? __popc(tb.mask[e]) : 0u, mine = (count + ENTRY - 1u) / ENTRY;
-        uint32_t before = mine << 16 | count;  // both prefix sums in one
+        const uint32_t e = e0 + lane, count = e < a.experts ? __popc(lists.mask[e]) : 0u;
+        const uint32_t my_up = (count + UP_ENTRY - 1u) / UP_ENTRY, my_down = (count + DOWN_ENTRY - 1u) / DOWN_ENTRY;
+        uint32_t before = my_up << 22 | my_down << 12 | count;  // three prefix sums in one: 32 experts have up to 128 and 256 entries and 512 rows
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
             const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, before, d);
             if (lane >= (uint32_t)d) before += v;
         }
         const uint32_t all = __shfl_sync(0xFFFFFFFFu, before, 31);
-        const uint32_t my_entry = entry + (before >> 16) - mine, my_row = row + (before & 0xFFFFu) - count;
-        if (e < a.experts) tb.entry_of[e] = (uint16_t)my_entry;
-        for (uint32_t i = 0; i < mine; ++i) {
-            tb.entry_expert[my_entry + i] = (uint16_t)e;
-            tb.entry_row[my_entry + i] = (uint16_t)(my_row + i * ENTRY);
+        const uint32_t at_up = up_entry + (before >> 22) - my_up, at_down = down_entry + (before >> 12 & 0x3FFu) - my_down, my_row = row + (before & 0xFFFu) - count;
+        if (e < a.experts) lists.entry_of[e] = (uint16_t)at_down;
+        for (uint32_t i = 0; i < my_down; ++i) {
+            down.entry_expert[at_down + i] = (uint16_t)e;
+            down.entry_row[at_down + i] = (uint16_t)(my_row + i * DOWN_ENTRY);
         }
-        entry += all >> 16, row += all & 0xFFFFu;
+        for (uint32_t i = 0; i < my_up; ++i) {
+            up.entry_expert[at_up + i] = (uint16_t)e;
+            up.entry_row[at_up + i] = (uint16_t)(my_row + i * UP_ENTRY);
+        }
+        up_entry += all >> 22, down_entry += all >> 12 & 0x3FFu, row += all & 0xFFFu;
     }
-    if (lane == 0) tb.entries = entry, tb.entry_row[entry] = (uint16_t)row;
+    if (lane == 0) up.entries = up_entry, up.entry_row[up_entry] = (uint16_t)row, down.entries = down_entry, down.entry_row[down_entry] = (uint16_t)row;
 }
 
 // Logits and choices: one cluster, whose CTAs have a share of K each for all tokens and experts, and then each their tokens.
@@ -414,7 +444,7 @@ __global__ void __launch_bounds__(THREADS)
 moe_router_kernel(const Args a) {
     constexpr uint32_t WIDE = PER * 2, REST = WARPS / WIDE, WIDTH = PER * 32;  // tiles of 16 experts; warps of each; experts of a plane
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ __align__(16) Tables tb;
+    __shared__ Lists lists;
     float* const part = reinterpret_cast<float*>(smem);  // [slice][token][expert]
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u, rank = blockIdx.x;
     const uint32_t columns = (a.tokens + 7u) / 8u, plane = a.tokens * WIDTH;
@@ -436,8 +466,9 @@ moe_router_kernel(const Args a) {
     };
     pdl_launch_dependents();
     if (a.ahead) weights(u0 + slice);
-    for (uint32_t e = threadIdx.x; e < MAX_EXPERTS; e += THREADS) tb.mask[e] = 0u;
-    if (threadIdx.x < MAX_TOKENS) tb.x_top[threadIdx.x] = 0u;
+    uint32_t* const x_top = lists.to.up.x_top;
+    for (uint32_t e = threadIdx.x; e < MAX_EXPERTS; e += THREADS) lists.mask[e] = 0u;
+    if (threadIdx.x < MAX_TOKENS) x_top[threadIdx.x] = 0u;
     __syncthreads();
     pdl_wait_prior();
     if (rank == 0u && threadIdx.x < a.tokens * a.top) a.h_top[threadIdx.x] = 0u;
@@ -466,7 +497,7 @@ moe_router_kernel(const Args a) {
             most = max(most & 0xFFFFu, most >> 16) << 16;
             most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, 1));
             most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, 2));
-            if (t == 0u && token < a.tokens) atomicMax(&tb.x_top[token], most);
+            if (t == 0u && token < a.tokens) atomicMax(&x_top[token], most);
         }
 #pragma unroll
         for (uint32_t i = 0; i < 4u; ++i) {
@@ -482,13 +513,13 @@ moe_router_kernel(const Args a) {
     }
     cluster_barrier();
     if (rank == 0u && threadIdx.x < a.tokens) {
-        uint32_t m = tb.x_top[threadIdx.x];
+        uint32_t m = x_top[threadIdx.x];
 #pragma unroll
-        for (uint32_t r = 1; r < ROUTER_CLUSTER; ++r) m = max(m, __float_as_uint(remote_f32(smem_addr(&tb.x_top[threadIdx.x]), r)));
-        tb.x_top[threadIdx.x] = m;
+        for (uint32_t r = 1; r < ROUTER_CLUSTER; ++r) m = max(m, __float_as_uint(remote_f32(smem_addr(&x_top[threadIdx.x]), r)));
+        x_top[threadIdx.x] = m;
     }
     for (uint32_t token = rank + ROUTER_CLUSTER * warp; token < a.tokens; token += ROUTER_CLUSTER * WARPS)
-        choose<PER>(a, tb, token, lane, [&](uint32_t e) {
+        choose<PER>(a, lists, token, lane, [&](uint32_t e) {
             const uint32_t at = smem_addr(part + token * WIDTH + e);
             float v[ROUTER_CLUSTER], s = 0.0f;
 #pragma unroll
@@ -499,23 +530,25 @@ moe_router_kernel(const Args a) {
         });
     cluster_barrier();
     if (rank) return;
-    if (warp == 0) list_entries(a, tb, lane);
+    if (warp == 0) list_entries(a, lists, lane);
     __syncthreads();
     if (threadIdx.x < a.tokens * a.top) {
-        const int e = tb.chosen[threadIdx.x];
+        const int e = lists.to.down.chosen[threadIdx.x];
         if (e >= 0) {
-            const uint32_t token = threadIdx.x / a.top, at = __popc(tb.mask[e] & ((1u << token) - 1u)), first = tb.entry_of[e];
-            tb.row_token[tb.entry_row[first] + at] = (uint8_t)token;
-            tb.slot[threadIdx.x] = (uint16_t)(first * ENTRY + at);
+            const uint32_t token = threadIdx.x / a.top, at = __popc(lists.mask[e] & ((1u << token) - 1u)), first = lists.entry_of[e];
+            lists.to.up.row_token[lists.to.down.entry_row[first] + at] = (uint8_t)token;
+            lists.to.down.slot[threadIdx.x] = (uint16_t)(first * DOWN_ENTRY + at);
         }
     }
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < sizeof(Tables) / 16u; i += THREADS) reinterpret_cast<uint4*>(a.tables)[i] = reinterpret_cast<const uint4*>(&tb)[i];
+    for (uint32_t i = threadIdx.x; i < sizeof(Tables) / 16u; i += THREADS) reinterpret_cast<uint4*>(a.tables)[i] = reinterpret_cast<const uint4*>(&lists.to)[i];
 }
 
-__device__ __forceinline__ void read_tables(const Args& a, Tables& tb) {
+template <class T>
+__device__ __forceinline__ void read_tables(const T* from, T& to) {
+    static_assert(sizeof(T) % 16 == 0, "copied by 16 bytes");
 #pragma unroll
-    for (uint32_t i = threadIdx.x; i < sizeof(Tables) / 16u; i += THREADS) reinterpret_cast<uint4*>(&tb)[i] = ld_fresh(reinterpret_cast<const uint4*>(a.tables) + i);
+    for (uint32_t i = threadIdx.x; i < sizeof(T) / 16u; i += THREADS) reinterpret_cast<uint4*>(&to)[i] = ld_fresh(reinterpret_cast<const uint4*>(from) + i);
     __syncthreads();
 }
 
@@ -604,7 +637,7 @@ moe_up_kernel(const Args a) {
     using S = Stage<FMT>;
     constexpr uint32_t CELL = 512u, RING = S::ring(DEPTH);  // a tile's partial sums: a float4 a thread
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ __align__(16) Tables tb;
+    __shared__ UpTables tb;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
     const uint32_t ring = smem_addr(smem) + warp * (S::BYTES * DEPTH), ring_end = ring + S::BYTES * DEPTH;
     float4* const cells = reinterpret_cast<float4*>(smem + RING);  // two a warp
@@ -612,7 +645,7 @@ moe_up_kernel(const Args a) {
 
     pdl_wait_prior();
     pdl_launch_dependents();  // not sooner: moe_down reads the tables before its wait
-    read_tables(a, tb);
+    read_tables(&a.tables->up, tb);
     const uint32_t f_tiles = a.F / 8u, units = a.up.units, items = tb.entries * f_tiles;
     const uint32_t i0 = a.by_ctas(items * blockIdx.x), i1 = a.by_ctas(items * (blockIdx.x + 1u));
     // A pass: as many entries as have room for their B fragments (one token: all, since theirs are the same).  Its tiles times units are
@@ -673,7 +706,7 @@ moe_up_kernel(const Args a) {
             float v[32];
             read_x<FMT>(v, a.x + (size_t)token * a.H, g < count, unit * S::UNIT + half * 128u, a.H, t);
             uint32_t b[16];
-            make_frag<FMT>(b, v, scale_up(tb.x_top[token]));
+            make_frag<FMT>(b, v, scale_up(tb.x_top[token]), pack_half);
             const uint32_t dst = frags + task * S::HALF;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
@@ -751,10 +784,11 @@ template <Format FMT>
 __global__ void __launch_bounds__(THREADS, 1)
 moe_down_kernel(const Args a) {
     using S = Stage<FMT>;
+    constexpr uint32_t REST = DOWN_ENTRY / 2u * 4u;  // floats of a cell from a column to that of the rest: a float4 holds two
     constexpr int DEPTH = S::DOWN;
     constexpr uint32_t RING = S::ring(DEPTH);
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ __align__(16) Tables tb;
+    __shared__ DownTables tb;
     __shared__ __align__(8) uint64_t arrived;  // the cluster's sums of this CTA's tiles
     __shared__ volatile uint32_t abort_flag;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
@@ -768,7 +802,7 @@ moe_down_kernel(const Args a) {
         mbar_init(smem_addr(&arrived), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    read_tables(a, tb);  // of a launch that was done before moe_up let this one start
+    read_tables(&a.tables->down, tb);  // of a launch that was done before moe_up let this one start
     const uint32_t units = a.down.units, all_units = tb.entries * units;
     const uint32_t r0 = cluster * a.per, r1 = min(a.H / 16u, r0 + a.per);
     // warp w of the cluster has the units [all w / 64, all (w + 1) / 64)
@@ -814,7 +848,7 @@ moe_down_kernel(const Args a) {
     if (threadIdx.x < a.tokens * a.top) {
         uint32_t what = 0;
         if (tb.chosen[threadIdx.x] >= 0) {
-            const uint32_t entry = tb.slot[threadIdx.x] / ENTRY, column = tb.slot[threadIdx.x] % ENTRY, begin = entry * units;
+            const uint32_t entry = tb.slot[threadIdx.x] / DOWN_ENTRY, column = tb.slot[threadIdx.x] % DOWN_ENTRY, begin = entry * units;
             // the warp that has unit u is ((u + 1) 64 - 1) / all
             const uint32_t w0 = ((begin + 1u) * WORKERS - 1u) / all_units, w1 = ((begin + units) * WORKERS - 1u) / all_units;
             const uint32_t lo = max(w0, rank * WARPS), hi = min(w1, rank * WARPS + WARPS - 1u);
@@ -839,13 +873,15 @@ moe_down_kernel(const Args a) {
             uint32_t b[S::HALVES][16];
             float sum[S::HALVES][S::GROUPS][2];
             {
-                const uint32_t row = row0 + (g < count ? g : 0u);
-                const float up = scale_up(ld_fresh(a.h_top + row));
+                // columns 0..3: the tokens' activations as fp16; 4..7: what they have beyond that, nothing where a row has an infinity
+                const uint32_t token = g % DOWN_ENTRY, row = row0 + (token < count ? token : 0u), top = ld_fresh(a.h_top + row);
+                const bool rest = g >= DOWN_ENTRY, there = token < count && !(rest && top >= 0x7F800000u);
+                const float up = scale_up(top);
 #pragma unroll
                 for (int half = 0; half < S::HALVES; ++half) {
                     float v[32];
-                    read_h<FMT>(v, a.h + (size_t)row * a.F, g < count, k0 + half * 128u, a.F, t);
-                    make_frag<FMT>(b[half], v, up);
+                    read_h<FMT>(v, a.h + (size_t)row * a.F, there, k0 + half * 128u, a.F, t);
+                    make_frag<FMT>(b[half], v, up, [rest](float lo, float hi) { return pack_part(lo, hi, rest); });
                     if constexpr (FMT != E4M3) make_sums<FMT>(sum[half], b[half]);
                 }
             }
@@ -884,7 +920,7 @@ moe_down_kernel(const Args a) {
             for (uint32_t t0 = 0; t0 < tiles; t0 += CLUSTER) {
                 float total[CLUSTER] = {};
                 for (uint32_t at = token * a.top; at < (token + 1u) * a.top; ++at) {
-                    const uint32_t what = (uint32_t)tb.chosen[at], warps = what >> 16, column = tb.slot[at] % ENTRY;
+                    const uint32_t what = (uint32_t)tb.chosen[at], warps = what >> 16, column = tb.slot[at] % DOWN_ENTRY;
                     const float* from = parts + (what & 0xFFu) * warp_floats + (t0 * 32u + (row & 7u) * 4u + column / 2u) * 4u + (column & 1u) + (row >> 3) * 2u;
                     const float weight = tb.weight[at];
                     float s[CLUSTER] = {};
@@ -892,7 +928,7 @@ moe_down_kernel(const Args a) {
                         const float* p = from + w * warp_floats + (w == 0u ? (what >> 8 & 0xFFu) * (at_once * 128u) : 0u);
 #pragma unroll
                         for (uint32_t j = 0; j < CLUSTER; ++j)
-                            if (t0 + j < tiles) s[j] += p[j * 128u];
+                            if (t0 + j < tiles) s[j] += p[j * 128u] + p[j * 128u + REST];
                     }
                     if (warps) {
 #pragma unroll
