@@ -177,9 +177,10 @@ __device__ __forceinline__ uint32_t piece_k(uint32_t t, uint32_t i) {
 template <Format FMT>
 __device__ __forceinline__ uint32_t swizzle(uint32_t r) { return FMT == E4M3 ? (r & 1u) << 2 | r >> 1 : (r & 3u) << 1 | r >> 2; }
 
-// What a product with 4-bit codes lacks: they are taken as multiples of 2^-24.
+// What a product with 4-bit codes lacks, which are taken as multiples of 2^-24: half of its exponent goes to the sums and half to their row's power of two, whose
+// exponent alone has no room for all of it where the row's largest is 2^118 or more.
 template <Format FMT>
-constexpr float WHOLE = FMT == E4M3 ? 1.0f : 16777216.0f;
+constexpr float WHOLE_ROOT = FMT == E4M3 ? 1.0f : 4096.0f;
 
 // 2^(14 - exponent of the largest), as far as its reciprocal is a normal number; and the reciprocal.
 __device__ __forceinline__ uint32_t scale_field(uint32_t top) { return min(268u - (top >> 23), 253u); }
@@ -686,8 +687,8 @@ moe_up_kernel(const Args a) {
             const uint32_t column = 2u * t + c;
             uint32_t most = 0u;
             if (column < count) {
-                const float down = scale_down(tb.x_top[tb.row_token[row0 + column]]) * WHOLE<FMT>;
-                const float gate = tot[c] * down, up = tot[2u + c] * down, h = gate / (1.0f + expf(-gate)) * up;
+                const float down = scale_down(tb.x_top[tb.row_token[row0 + column]]) * WHOLE_ROOT<FMT>;
+                const float gate = tot[c] * WHOLE_ROOT<FMT> * down, up = tot[2u + c] * WHOLE_ROOT<FMT> * down, h = gate / (1.0f + expf(-gate)) * up;
                 a.h[(size_t)(row0 + column) * a.F + (item - entry * f_tiles) * 8u + g] = h;
                 most = __float_as_uint(fabsf(h));
             }
@@ -853,7 +854,7 @@ moe_down_kernel(const Args a) {
             const uint32_t w0 = ((begin + 1u) * WORKERS - 1u) / all_units, w1 = ((begin + units) * WORKERS - 1u) / all_units;
             const uint32_t lo = max(w0, rank * WARPS), hi = min(w1, rank * WARPS + WARPS - 1u);
             if (lo <= hi) what = (lo - rank * WARPS) | (entry - all_units * lo / WORKERS / units) << 8 | (hi - lo + 1u) << 16;
-            tb.weight[threadIdx.x] *= scale_down(ld_fresh(a.h_top + tb.entry_row[entry] + column)) * WHOLE<FMT>;
+            tb.weight[threadIdx.x] *= scale_down(ld_fresh(a.h_top + tb.entry_row[entry] + column)) * WHOLE_ROOT<FMT>;
         }
         tb.chosen[threadIdx.x] = (int)what;
     }
@@ -932,7 +933,7 @@ moe_down_kernel(const Args a) {
                     }
                     if (warps) {
 #pragma unroll
-                        for (uint32_t j = 0; j < CLUSTER; ++j) total[j] = __fmaf_rn(weight, s[j], total[j]);
+                        for (uint32_t j = 0; j < CLUSTER; ++j) total[j] = __fmaf_rn(weight, s[j] * WHOLE_ROOT<FMT>, total[j]);
                     }
                 }
                 if (lanes == 8u) {  // whole warps: 16 rows a token
