@@ -396,7 +396,7 @@ __device__ __forceinline__ void choose(const Args& a, Lists& lists, uint32_t tok
         float m = expert >= 0 ? mine : -INFINITY;
 #pragma unroll
         for (int d = 8; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
-        if (expert >= 0) p = a.sigmoid ? expf(fminf(mine, 0.0f) - fminf(m, 0.0f)) / (1.0f + expf(-fabsf(mine))) : expf(mine - m);
+        if (expert >= 0) p = a.sigmoid ? expf(fminf(mine, 0.0f) - fminf(m, 0.0f)) / (1.0f + expf(-fabsf(mine))) : total == total ? expf(mine - m) : total;
         sum = p;
 #pragma unroll
         for (int d = 8; d; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
