@@ -462,7 +462,8 @@ int miori_gemm_fp8(const void* a, int64_t lda, const float* sa, int64_t sa_row, 
  * (of largest l without a bias; ties: lowest index), their weights w = p, divided by their sum with MIORI_MOE_NORM, times factor;
  *   out[t] = sum_e w_e W_down,e (silu(g) * u),  g = W_up,e[0 .. ff) x[t],  u = W_up,e[ff .. 2 ff) x[t].
  * An expert whose bias is -inf is never chosen; a token left with fewer than `top` has fewer, with none its row is zeros.  An expert whose
- * score is not a number comes last; a softmax over a logit that is none, or infinite, is of no numbers, and so is its token's row.  x [tokens][hidden] and router [experts][hidden] bf16, bias fp32 [experts] or NULL, out
+ * score is not a number comes last; a softmax over a logit that is none, or +inf, is of no numbers, and so is its
+ * token's row.  x [tokens][hidden] and router [experts][hidden] bf16, bias fp32 [experts] or NULL, out
  * [tokens][hidden] fp32 (bf16 with MIORI_OUT_BF16; that may be x).  1..32 tokens, 1..256 experts, top 1..16, hidden up to 7168, ff up
  * to 65536.  The choice is made from
  * fp32 sums; the chosen experts' weights are read once.  A token's result depends on the other tokens in the order of its sums only.
