@@ -615,22 +615,11 @@ OP(quant_fp8, 1, "x", "tile", "flags", "out", "scales") {
     const uint32_t flags = (a.u32(2, 0) & ~MIORI_QUANT_F32) | (fp32 ? MIORI_QUANT_F32 : 0u);
     at::Tensor q, s;
     const c10::Device on = device_of({&x, or_first(a, 3), or_first(a, 4)});
-    const int64_t pitch_made = (K + 15) / 16 * 16;  // rows of new codes begin on 16-byte boundaries
-    const int64_t code_bytes = (R * pitch_made + 255) / 256 * 256, k_blocks = blocks(K);
-    at::Tensor both;  // new codes and new scales are one allocation, which costs as much as a launch's share of the call does
-    if (!a.given(3) && !a.given(4)) both = empty({code_bytes + row_blocks * k_blocks * 4}, at::kByte, x);
-    auto make = [&](at::ScalarType dt, int64_t from, std::initializer_list<int64_t> sizes, std::initializer_list<int64_t> strides) {
-        at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(both.storage()), both.key_set(), c10::scalarTypeToTypeMeta(dt));
-        t.unsafeGetTensorImpl()->set_storage_offset(from);
-        t.unsafeGetTensorImpl()->set_sizes_and_strides(sizes, strides);
-        return t;
-    };
+    const int64_t pitch_made = (K + 15) / 16 * 16, k_blocks = blocks(K);  // rows of new codes begin on 16-byte boundaries
     if (a.given(3)) {
         q = a.tensor(3);
         need_fp8(q, "out", 2);
         if (q.size(0) != R || q.size(1) != K) raise(PyExc_ValueError, "out: the shape of x is expected");
-    } else if (both.defined()) {
-        q = make(at::kFloat8_e4m3fn, 0, {R, K}, {pitch_made, 1});
     } else {
         q = empty({R, pitch_made}, at::kFloat8_e4m3fn, x);
         q.unsafeGetTensorImpl()->set_sizes_and_strides(std::vector<int64_t>{R, K}, std::vector<int64_t>{pitch_made, 1});
@@ -638,8 +627,6 @@ OP(quant_fp8, 1, "x", "tile", "flags", "out", "scales") {
     if (a.given(4)) {
         s = a.tensor(4);
         need_scales(s, "scales", row_blocks, k_blocks);
-    } else if (both.defined()) {
-        s = make(at::kFloat, code_bytes / 4, {row_blocks, k_blocks}, {k_blocks, 1});
     } else {
         s = empty({row_blocks, k_blocks}, at::kFloat, x);
     }
