@@ -521,7 +521,19 @@ gemm_fp8_swap_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     // The sums go to shared memory, [row of a][row of w]: all MMAs are done and, after a barrier of their readers, the scales are read.  From there
     // CTA r of the cluster takes rows r, r + cs, ... of a, each by a warp, and adds them up in rank order.  (Stored by the threads that hold them
     // a row was 160 cycles: its instructions, which nothing had run before, took that long to come.)
+    // Tensor memory is free before other CTAs are waited for: one of the cluster may still wait for columns that somebody holds who waits in turn.
+    bool freed = false;
+    if (warp == 1u) {
+        asm volatile("bar.sync 2, 160;" ::: "memory");  // its readers
+        freed = __all_sync(0xFFFFFFFFu, abort_flag == 0u);
+        if (freed) {
+            fence_after();
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+        }
+    }
     if (warp >= 3u) {
+        fence_before();
+        asm volatile("bar.arrive 2, 160;" ::: "memory");
         asm volatile("bar.sync 1, 128;" ::: "memory");
         const uint32_t to = ring + ((warp & 3u) * 32u + lane) * 4u;
 #pragma unroll
@@ -572,7 +584,7 @@ gemm_fp8_swap_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     __syncwarp();
     fence_before();
     __syncthreads();
-    if (warp == 1) {
+    if (warp == 1 && !freed) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
     }

@@ -65,8 +65,21 @@ def test_whole_warps_come_to_barriers_of_whole_warps():
     for at in barriers:
         before = [line.strip() for line in swap[:at].splitlines() if line.strip()]
         # ... or nothing lies between it and such a place but stores that every lane makes
-        tail = "\n".join(before[-9:])
+        tail = "\n".join(before[-26:])
         assert "__syncwarp();" in tail and "continue" not in tail.rsplit("__syncwarp();", 1)[1] and "break" not in tail.rsplit("__syncwarp();", 1)[1], tail
     for part in (fp8[:fp8.index("gemm_fp8_swap_kernel(")], swap):
         leaving = part[part.index("__nanosleep"):]
         assert leaving.index("__syncwarp();") < leaving.index("__syncthreads();")
+
+
+def test_a_cluster_is_waited_for_without_tensor_memory():
+    """A CTA of gemm_fp8's few-row kernel frees its columns in front of its first wait for others of its cluster: theirs may be waiting for columns, without a limit, that a CTA
+    holds which waits for this one.  (Pairs allocate together, and their registers leave an SM to them alone.)"""
+    swap = code(os.path.join(CSRC, "gemm_fp8.cuh"))
+    swap = swap[swap.index("gemm_fp8_swap_kernel("):swap.index("struct GemmOperands")]
+    freed, meeting = swap.index("tcgen05.dealloc"), swap.index("cluster_barrier()")
+    assert freed < meeting
+    before = swap[:freed]
+    assert before.rindex('"bar.sync 2, 160;"') < before.rindex("fence_after();")  # behind the warps that read it
+    readers = swap[:swap.index('"bar.arrive 2, 160;"')]
+    assert readers.rindex("tmem_wait16") < readers.rindex("fence_before();")
