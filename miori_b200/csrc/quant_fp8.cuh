@@ -7,8 +7,6 @@
 #pragma once
 #include "common.cuh"
 
-#include <cuda_fp8.h>
-
 namespace miori_b200 {
 namespace fp8 {
 
