@@ -451,7 +451,8 @@ int miori_quant_fp8(const void* x, int64_t x_row, void* q, int64_t q_row, float*
                     int64_t scale_col, uint32_t rows, uint32_t K, uint32_t tile, uint32_t flags, void* stream);
 /* C[m][n] (fp32, or bf16 with MIORI_OUT_BF16; rows ldc elements apart) = sum_b sa[m][b] sw[n / 128][b] sum_{k in block b} a[m][k]
  * w[n][k]: activations in blocks of one row times weights in blocks of 128, any M, N, K >= 1, fp32 sums.  What lies behind N in
- * a row of C is left as it was. */
+ * a row of C is left as it was; C may lie on none of the others.  Few rows have a kernel of their own up to K = 16384; beyond that they take as long as
+ * two hundred and fifty-six. */
 int miori_gemm_fp8(const void* a, int64_t lda, const float* sa, int64_t sa_row, int64_t sa_col, const void* w,
                    int64_t ldw, const float* sw, int64_t sw_row, int64_t sw_col, void* C, int64_t ldc, uint32_t M,
                    uint32_t N, uint32_t K, uint32_t flags, void* stream);
@@ -466,7 +467,9 @@ int miori_gemm_fp8(const void* a, int64_t lda, const float* sa, int64_t sa_row, 
  * token's row.  x [tokens][hidden] and router [experts][hidden] bf16, bias fp32 [experts] or NULL, out
  * [tokens][hidden] fp32 (bf16 with MIORI_OUT_BF16; that may be x).  1..32 tokens, 1..256 experts, top 1..16, hidden up to 7168, ff up
  * to 65536.  The choice is made from
- * fp32 sums; the chosen experts' weights are read once.  A token's result depends on the other tokens in the order of its sums only.
+ * fp32 sums (scores closer than those tell apart may go either way).  x is multiplied as it is, down to 2^-27 of its row's largest; silu(g) * u is
+ * fp32, and within 2^-22 of that where it is multiplied.  A chosen expert's W_up is read once for every eight of its tokens, W_down once for every four.  A token's result depends on the other
+ * tokens in the order of its sums only.
  * workspace: miori_moe_workspace_bytes of scratch; launches that may run concurrently need workspaces of their own.  Three launches, the first of
  * which may begin while the launch before drains: it waits for that one before it reads x or writes anything (with MIORI_LAUNCH_PDL
  * it reads the router ahead). */

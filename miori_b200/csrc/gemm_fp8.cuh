@@ -5,16 +5,18 @@
 // so what it has summed leaves tensor memory once a block and is added, times the block's scale, to fp32
 // accumulators in registers.  That is one tcgen05.ld and half a packed FMA (fma.rn.f32x2) an element and block: of the 512 cycles that the
 // matrix unit takes for a 128 x 256 x 128 block, 256 of the tensor memory's reading and 128 to 256 of issue, beside it.  Two
-// or four blocks' sums fit tensor memory, so that the unit never waits for the readers.
+// or four blocks' sums fit tensor memory, so that the unit works on some while others are read.  It waits for the readers all the same: half of
+// its cycles are busy in the largest products, and those take a fifth less time without the additions.
 // (Scales that are powers of two could ride along inside the MMA; a checkpoint's are any fp32.)
 //
 // Two kernels:
 //   pair   more than a hundred rows or so: 256 x 256 or 256 x 128 tiles on SM pairs (cta_group::2), persistent; each CTA pulls 32 KB a
-//          block through L2 for 512 cycles of its matrix unit, and takes some 650 for them.  16384 x 16384 x 2048: 550 us in a burst, 2.0 PFLOP/s
-//          (624 under the power limit, which holds the clock at 1.58 GHz in the one and 1.39 in the other); 1024 x 2048 x 8192: 20.4 us in a chain.
+//          block through L2 for 512 cycles of its matrix unit, and takes some 800 for them.  16384 x 16384 x 2048: 557 us in a burst, 1.97 PFLOP/s
+//          (633 under the power limit, which holds the clock at 1.58 GHz in the one and 1.39 in the other); 1024 x 2048 x 8192: 23 us.
 //   swap   few rows, or few tiles: 128 rows of w are the MMA's M, up to 128 rows of a its N; K is split over the CTAs of a
 //          cluster and the partial sums meet in distributed shared memory, in rank order.  8 x 16384 x 2048: 7.2 us, 4.7 TB/s; one row of 2048 x 2048: 3.4 us
-//          in a chain; 64 x 16384 x 2048: 10.2 us.
+//          in a chain; 64 x 16384 x 2048: 10.2 us.  A slice's scales lie in shared memory, which has room for K of 16384; beyond that few rows go through
+//          tiles of 256 too (1 x 8192 x 16384 27 us, x 28672 100; 8 rows 72).
 // Ends of M, N and K are zeros by TMA; what lies behind N in a row of C is left as it was.  Every wait is bounded.
 #pragma once
 #include "common.cuh"

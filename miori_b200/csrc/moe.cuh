@@ -10,19 +10,20 @@
 //   moe_down    a cluster of four CTAs owns rows of the output.  The K axes of all experts, one behind the other, are dealt to its 64 warps,
 //               whose sums meet by token, times w, in a CTA and then over the cluster, always in the same order.
 // (As one cooperative launch with a meeting of the grid between the products, every CTA choosing for itself, a token took 23 us: such a meeting
-// costs 2.6, a launch's hand-over 0.7, a choice 2.  Weights asked of L2 ahead of their kernel, up's before the choice or down's at the end of moe_up, are nobody's gain
-// any more: 18.0 us for one token without, 18.6 with.)
+// costs 2.6, a launch's hand-over 0.7, a choice 2.  Weights asked of L2 ahead of their kernel, up's before the choice or down's at the end of moe_up, are nobody's gain:
+// a token took 18.0 us without, 18.6 with.)
 // An MMA tile has eight columns: moe_up's are eight tokens, moe_down's four, each twice (below).  An expert of more tokens is listed, and read, once for every
 // eight or four of them; L2 serves the further readings.
 //
 // Weights stream through a ring of cp.async stages that belongs to one warp: 16 rows x 128 bytes and their scales, no CTA-wide wait.  They become
 // fp16 without a rounding: 4-bit codes as subnormals in the bits of a half, e4m3 by conversion; products by mma.sync.m16n8k16, sums in fp32, times
-// the scales after each group.  Experts of 2048 x 1536 in 4 bits, 4 of 32 a token: 18.0 us for one token, of which 3.3 are the bytes' and the rest latency; 54 for 32 (25.6); in e4m3, 8 of
-// 64 of 2048 x 768, 4 tokens: 38.5 (19).  What bounds the stream of many tokens is less HBM than the number of instructions a stage takes: B fragments are made once
+// the scales after each group.  Experts of 2048 x 1536 in 4 bits and groups of 64, 4 of 32 a token: 18.5 us for one token, of which 3.3 are the bytes' and the rest latency; 61 to 64 for 32 (25.6); in
+// groups of 32 20 and 77 (3.6 and 28.4); in e4m3, 8 of 64 of 2048 x 768, 4 tokens: 39 to 40 (19).  What bounds the stream of many tokens is less HBM than the number of instructions a stage takes: B fragments are made once
 // a CTA and expert (moe_up) or once for several row tiles (moe_down), a row of activations has one power of two.
 // Activations, x and silu(g) * u, are fp16 times a power of two per row that puts its largest into [2^14, 2^15): bf16 x is not rounded down to
 // 2^-27 of that largest (4 bits) or 2^-31.  silu(g) * u, fp32, is a pair of fp16, a value and what it has beyond that, in two columns of one tile: 2^-22 of a value at most, where one
-// fp16 would be off by 2^-11.
+// fp16 would be off by 2^-11 and the result by 3e-4 of its size (now 4e-6 in 4 bits, 4e-7 in e4m3).  It costs a second reading where an expert has more than four tokens: 55 us for 32 tokens
+// with one fp16, 61 to 64 with the pair; one token 18.0 and 18.5.
 #pragma once
 #include "common.cuh"
 
