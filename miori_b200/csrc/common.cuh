@@ -193,12 +193,12 @@ __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
 }
 // What a wait orders.  OWN: what threads of this CTA, or its copies, have written.  CLUSTER: what other CTAs have.  TENSOR: nothing of memory; tensor memory that other
 // CTAs have read or written, with tcgen05.fence on either side of the barrier (by acquire and release, 1024 x 2048 x 8192 took 65.6 us for 23.4).
-enum Order { OWN, CLUSTER, TENSOR };
-template <Order O = OWN>
+enum class Order { OWN, CLUSTER, TENSOR };
+template <Order O = Order::OWN>
 __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
     uint32_t ok;
-    static_assert(O != CLUSTER, "by mbar_try_long");
-    if constexpr (O == TENSOR)
+    static_assert(O != Order::CLUSTER, "by mbar_try_long");
+    if constexpr (O == Order::TENSOR)
         asm volatile(
             "{\n\t.reg .pred p;\n\t"
             "mbarrier.try_wait.parity.relaxed.cluster.shared::cta.b64 p, [%1], %2;\n\t"
@@ -231,11 +231,11 @@ __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
 // The same, but the thread may sleep up to WAIT_SLEEP_NS in the instruction before it comes back false:
 // a waiting warp then takes no issue slots from the working ones.
 constexpr uint32_t WAIT_SLEEP_NS = 1000000u;
-template <Order O = OWN>
+template <Order O = Order::OWN>
 __device__ __forceinline__ bool mbar_try_long(uint32_t bar, uint32_t parity) {
     uint32_t ok;
-    static_assert(O != TENSOR, "by mbar_try");
-    if constexpr (O == CLUSTER)
+    static_assert(O != Order::TENSOR, "by mbar_try");
+    if constexpr (O == Order::CLUSTER)
         asm volatile(
             "{\n\t.reg .pred p;\n\t"
             "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
@@ -258,7 +258,7 @@ __device__ __forceinline__ bool mbar_try_long(uint32_t bar, uint32_t parity) {
 // SLEEP: wait inside the instruction.  Right where a few threads wait beside working ones (the GEMMs: 1024 x
 // 3072 14.3 us against 15.9 with short tries); where every warp of a CTA waits for the same barrier the short
 // ones wake up sooner (gemv_cache.cuh).
-template <bool SLEEP = true, Order O = OWN>
+template <bool SLEEP = true, Order O = Order::OWN>
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile uint32_t* abort,
                                           uint32_t where) {
     auto attempt = [&] {

@@ -108,7 +108,7 @@ __device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
     return v;
 }
 // mbar_wait by a whole warp, with one answer for it.  (By one lane, that tells the others: 100 cycles more a wait.)
-template <Order O = OWN>
+template <Order O = Order::OWN>
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile uint32_t* abort, uint32_t where) {
     if (__all_sync(0xFFFFFFFFu, mbar_try<O>(bar, parity))) return true;
     return __all_sync(0xFFFFFFFFu, mbar_wait<false, O>(bar, parity, abort, where));
@@ -235,7 +235,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_con
             bool ok = true;
             for (uint32_t t = pair; t < tiles && ok; t += pairs) {
                 for (uint32_t kb = 0; kb < k_blocks; ++kb) {
-                    if (!(ok = warp_wait<TENSOR>(taken(b), b_parity, &abort_flag, 0x72))) break;
+                    if (!(ok = warp_wait<Order::TENSOR>(taken(b), b_parity, &abort_flag, 0x72))) break;
                     if (!(ok = warp_wait(full(s), parity, &abort_flag, 0x73))) break;
                     fence_after();
                     if (elect_one()) {

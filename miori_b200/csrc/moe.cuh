@@ -956,7 +956,7 @@ moe_down_kernel(const Args a) {
         // No CTA leaves, or sends a next pass's sums, before all have come this far; on the last pass that is said before they are waited for.
         if (last >= r1) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
         if (mine_now) {
-            const bool ok = mbar_wait<true, miori_b200::CLUSTER>(smem_addr(&arrived), parity, &abort_flag, 0x81);
+            const bool ok = mbar_wait<true, Order::CLUSTER>(smem_addr(&arrived), parity, &abort_flag, 0x81);
             for (uint32_t i = threadIdx.x; ok && i < mine_now * a.tokens * 16u; i += THREADS) {
                 const uint32_t rest = i >> 4, q = a.by_tokens(rest), token = rest - q * a.tokens;
                 float v = 0.0f;

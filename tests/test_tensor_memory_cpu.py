@@ -48,11 +48,11 @@ def test_hand_overs_between_ctas():
     assert remote and all("mbarrier.arrive.relaxed.cluster" in a for a in remote)
     relay = fp8[:fp8.index("arrive_leader(taken(b))")].rsplit("mbar_wait(taken(b)", 1)[1]
     assert relay.index("fence_after();") < relay.index("fence_before();")
-    leader = fp8[fp8.index("warp_wait<TENSOR>(taken(b)"):]
+    leader = fp8[fp8.index("warp_wait<Order::TENSOR>(taken(b)"):]
     assert leader.index("fence_after();") < leader.index("umma_e4m3<2>")
     wait = code(os.path.join(CSRC, "common.cuh"))
     assert wait.count("mbarrier.try_wait.parity.relaxed.cluster") == 1 and wait.count("mbarrier.try_wait.parity.acquire.cluster") == 1
-    assert "mbar_wait<true, miori_b200::CLUSTER>(smem_addr(&arrived)" in code(os.path.join(CSRC, "moe.cuh"))
+    assert "mbar_wait<true, Order::CLUSTER>(smem_addr(&arrived)" in code(os.path.join(CSRC, "moe.cuh"))
 
 
 def test_whole_warps_come_to_barriers_of_whole_warps():
